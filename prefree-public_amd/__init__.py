@@ -2,6 +2,7 @@
 
 ctypes over the C ABI of ``lib/libprefree.so`` (include/prefree_c.h) and, for
 index-level tests, ``lib/libprefree_kernels.so`` (include/prefree_kernels.h).
+The operators of expert layers (include/prefree_moe.h) are in ``moe.py``.
 Device buffers are passed as raw pointers; anything with ``data_ptr()`` (a
 torch tensor on the GPU) is accepted.  Streams are HIP stream handles (torch's
 ``stream.cuda_stream``); ``None`` is the null stream.
@@ -27,10 +28,11 @@ LIB_PATH = os.path.join(LIB_DIR, "libprefree.so")
 KLIB_PATH = os.path.join(LIB_DIR, "libprefree_kernels.so")
 
 F64, F32, F16 = 0, 1, 2
+BF16 = 3  # the expert-layer operators only (moe.py)
 AUTO, PREFREE, ADAPTIVE, FLAT = 0, 1, 2, 3
 VARIANTS = {"auto": AUTO, "prefree": PREFREE, "adaptive": ADAPTIVE, "flat": FLAT}
 VARIANT_NAMES = {v: k for k, v in VARIANTS.items()}
-DTYPES = {"f64": F64, "f32": F32, "f16": F16}
+DTYPES = {"f64": F64, "f32": F32, "f16": F16, "bf16": BF16}
 STATUS = {0: "PF_OK", 1: "PF_ERR_INVALID", 2: "PF_ERR_ALIGN", 3: "PF_ERR_HIP", 4: "PF_ERR_NOMEM",
           5: "PF_ERR_UNSUPPORTED", 6: "PF_ERR_CSR", 7: "PF_ERR_KERNEL", 8: "PF_ERR_IO"}
 
@@ -188,6 +190,7 @@ def lib() -> ctypes.CDLL:
         _sig(L.pf_memcpy_h2d, [_vp, _vp, ctypes.c_size_t, _vp])
         _sig(L.pf_memcpy_d2h, [_vp, _vp, ctypes.c_size_t, _vp])
         _sig(L.pf_stream_synchronize, [_vp])
+        moe._signatures(L)
         _lib = L
     return _lib
 
@@ -255,6 +258,8 @@ def dtype_code(d) -> int:
         return F64
     if "float32" in name or name == "float":
         return F32
+    if "bfloat16" in name:
+        return BF16
     if "float16" in name or name == "half":
         return F16
     raise ValueError(f"unsupported dtype {d}")
@@ -533,3 +538,9 @@ def synth_x(cfg, n, seed=1, vals=0, dtypes=("f64",)):
 
 def version() -> int:
     return int(lib().pf_version())
+
+
+# ---- expert-layer operators ----------------------------------------------------
+
+from . import moe  # noqa: E402  (uses the names above)
+from .moe import *  # noqa: E402,F401,F403

@@ -1,0 +1,139 @@
+// moe_mx4.hip — 4-bit blocks on gfx950 (include/prefree_moe.h): blocks of 32 elements e2m1 with one scale byte e8m0.
+#include "moe_common.hpp"
+#include "moe_launch.hpp"
+#include "prefree_moe_kernels.h"
+
+namespace {
+
+using namespace pfmoe;
+
+// Eight elements as fp32 from `at` of a row.
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void load8(const T *p, float v[8])
+{
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const i32x4 b = VECTOR ? *(const i32x4 *)(p + 4 * h) : load16_any(p + 4 * h);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * h + i] = __int_as_float(b[i]);
+        }
+    } else {
+        typedef typename vec<T>::x8 x8;
+        const x8 b = __builtin_bit_cast(x8, VECTOR ? *(const i32x4 *)p : load16_any(p));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)b[i];
+    }
+}
+
+// A lane takes eight elements, four lanes a block of 32.  The block's scale exponent is its largest magnitude's
+// exponent less 2, so that magnitude / scale lies in [4, 8); dividing by a power of two is exact, and the conversion
+// instruction rounds to nearest even and saturates at 6, with scale 1.
+template <typename T, bool VECTOR>
+__global__ __launch_bounds__(256) void k_quantize(const T *x, long long ld, long long units, int per_row, unsigned *codes,
+                                                  unsigned char *scales)
+{
+    const long long unit = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (unit >= units) return;   // units come in fours
+    const long long r = unit / per_row;
+    float v[8];
+    load8<T, VECTOR>(x + ld * r + (unit - r * per_row) * 8, v);
+    unsigned most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const unsigned b = __float_as_uint(v[i]) & 0x7fffffffu;
+        most = b > most ? b : most;
+    }
+    unsigned o = pfdev::dpp<pfdev::kDppXor1>(most);
+    most = o > most ? o : most;
+    o = pfdev::dpp<pfdev::kDppXor2>(most);
+    most = o > most ? o : most;
+    const int e = (int)(most >> 23);                      // 255: an infinity or a NaN
+    const int scale = e == 255 ? 255 : e < 2 ? 0 : e - 2;  // exponent + 127; 2^-127 at the least
+    unsigned code = 0;
+    if (e != 255) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = ldexpf(v[i], 127 - scale);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[0], v[1], 1.0f, 0);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[2], v[3], 1.0f, 1);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[4], v[5], 1.0f, 2);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[6], v[7], 1.0f, 3);
+    }
+    codes[unit] = code;
+    if ((threadIdx.x & 3) == 0) scales[unit >> 2] = (unsigned char)scale;
+}
+
+__device__ __forceinline__ float value_of(unsigned code)
+{
+    const int e = code >> 1 & 3, m = code & 1;
+    const float v = e ? ldexpf(1.0f + 0.5f * m, e - 1) : 0.5f * m;
+    return code & 8 ? -v : v;
+}
+
+template <typename T, bool VECTOR>
+__global__ __launch_bounds__(256) void k_dequantize(const unsigned *codes, const unsigned char *scales, long long units,
+                                                    int per_row, T *y, long long ld)
+{
+    const long long unit = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (unit >= units) return;
+    const long long r = unit / per_row;
+    const unsigned code = codes[unit];
+    const int scale = scales[unit >> 2];
+    T *out = y + ld * r + (unit - r * per_row) * 8;
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        v[i] = (T)(scale == 255 ? __builtin_nanf("") : ldexpf(value_of(code >> 4 * i & 15), scale - 127));
+    if constexpr (VECTOR) {
+#pragma unroll
+        for (unsigned i = 0; i < sizeof(v) / 16; ++i) {
+            i32x4 b;
+            __builtin_memcpy(&b, (const char *)v + 16 * i, 16);
+            *(i32x4 *)((char *)out + 16 * i) = b;
+        }
+    } else {
+        __builtin_memcpy(out, v, sizeof(v));
+    }
+}
+
+template <typename T>
+int quantize(const void *x, long long ld, int rows, int k, void *codes, void *scales, hipStream_t s)
+{
+    const long long units = (long long)rows * (k / 8), grid = (units + 255) / 256;
+    if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "4-bit blocks: too many elements");
+    const bool vector = (uintptr_t)x % 16 == 0 && ld * sizeof(T) % 16 == 0;
+    if (vector) k_quantize<T, true><<<dim3((unsigned)grid), dim3(256), 0, s>>>((const T *)x, ld, units, k / 8, (unsigned *)codes, (unsigned char *)scales);
+    else k_quantize<T, false><<<dim3((unsigned)grid), dim3(256), 0, s>>>((const T *)x, ld, units, k / 8, (unsigned *)codes, (unsigned char *)scales);
+    return pfk_internal_launched("k_quantize");
+}
+
+template <typename T>
+int dequantize(const void *codes, const void *scales, int rows, int k, void *y, long long ld, hipStream_t s)
+{
+    const long long units = (long long)rows * (k / 8), grid = (units + 255) / 256;
+    if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "4-bit blocks: too many elements");
+    const bool vector = (uintptr_t)y % 16 == 0 && ld * sizeof(T) % 16 == 0;
+    if (vector) k_dequantize<T, true><<<dim3((unsigned)grid), dim3(256), 0, s>>>((const unsigned *)codes, (const unsigned char *)scales, units, k / 8, (T *)y, ld);
+    else k_dequantize<T, false><<<dim3((unsigned)grid), dim3(256), 0, s>>>((const unsigned *)codes, (const unsigned char *)scales, units, k / 8, (T *)y, ld);
+    return pfk_internal_launched("k_dequantize");
+}
+
+}  // namespace
+
+extern "C" {
+
+int pfk_mx4_quantize(const void *x, long long ld_x, int dtype, int rows, int k, void *codes, void *scales, void *stream)
+{
+    hipStream_t s = (hipStream_t)stream;
+    return dtype == PF_F32 ? quantize<float>(x, ld_x, rows, k, codes, scales, s)
+         : dtype == PF_F16 ? quantize<f16>(x, ld_x, rows, k, codes, scales, s) : quantize<bf16>(x, ld_x, rows, k, codes, scales, s);
+}
+
+int pfk_mx4_dequantize(const void *codes, const void *scales, int rows, int k, int dtype, void *y, long long ld_y, void *stream)
+{
+    hipStream_t s = (hipStream_t)stream;
+    return dtype == PF_F32 ? dequantize<float>(codes, scales, rows, k, y, ld_y, s)
+         : dtype == PF_F16 ? dequantize<f16>(codes, scales, rows, k, y, ld_y, s) : dequantize<bf16>(codes, scales, rows, k, y, ld_y, s);
+}
+
+}  // extern "C"

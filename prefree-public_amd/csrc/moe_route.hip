@@ -1,0 +1,536 @@
+// moe_route.hip — routing of an expert layer on gfx950 (include/prefree_moe.h): the choice of experts and their order,
+// the weighted sum of the experts' rows, and the gradients of both.
+#include "moe_common.hpp"
+#include "moe_launch.hpp"
+#include "prefree_moe_kernels.h"
+
+namespace {
+
+using namespace pfmoe;
+
+constexpr int kBlock = PFK_MOE_ROUTE_BLOCK;  // tokens a workgroup: one bit each in a 64-bit mask of an expert
+static_assert(kBlock == 64, "masks of 64 tokens");
+constexpr int kDirect = 1024;                // blocks up to which each workgroup sums the counts before it itself
+constexpr int kSuper = 64;                   // blocks whose counts are summed beforehand above that
+
+template <typename T>
+__device__ __forceinline__ float as_float(T v) { return (float)v; }
+
+// Order-preserving key of a logit: 0 for -infinity (never chosen), the largest for NaN, -0 and 0 alike.
+__device__ __forceinline__ unsigned key_of(float z)
+{
+    if (z != z) return 0xffffffffu;
+    if (z == 0.0f) z = 0.0f;
+    const unsigned b = __float_as_uint(z);
+    if (b == 0xff800000u) return 0;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+struct MaxU { __device__ unsigned operator()(unsigned a, unsigned b) const { return a > b ? a : b; } };
+
+struct Route {
+    const void *logits;
+    long long ld;
+    int tokens, experts, top_k, normalise, blocks;
+    int *choice;
+    float *weight;
+    int *offsets, *order, *slot;
+    unsigned char *counts;  // [blocks][experts]
+    int *super;             // [blocks / kSuper][experts], behind the counts
+};
+
+// One wave takes a token at a time: lane l has logits l*PER .. l*PER + PER-1.  The k-th choice is the largest key
+// of the wave; the first lane that has it owns the lowest index.
+template <typename T, int PER>
+__device__ __forceinline__ void choose(const Route &a, int t, unsigned long long *mask)
+{
+    const int lane = threadIdx.x & (kWave - 1), local = t & (kBlock - 1);
+    const T *row = (const T *)a.logits + a.ld * t;
+    float z[PER];
+    unsigned key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int e = lane * PER + i;
+        z[i] = e < a.experts ? as_float(row[e]) : -INFINITY;
+        key[i] = key_of(z[i]);
+    }
+    float mine = 0, top = 0;   // lane j: the logit of choice j; the row's largest
+    int expert = -1;
+    for (int j = 0; j < a.top_k; ++j) {
+        unsigned best = 0;
+        int at = 0;
+#pragma unroll
+        for (int i = PER - 1; i >= 0; --i)
+            if (key[i] >= best) { best = key[i]; at = i; }
+        const unsigned most = pfdev::wave_reduce_u32(best, MaxU());
+        if (most == 0) break;
+        const int winner = __builtin_ctzll(__ballot(best == most));
+        const int i = __builtin_amdgcn_readlane(at, winner), e = winner * PER + i;
+        float v = 0;
+#pragma unroll
+        for (int c = 0; c < PER; ++c)
+            if (c == i) { v = z[c]; if (lane == winner) key[c] = 0; }
+        v = pfdev::readlane(v, winner);
+        if (j == 0) top = v;
+        if (lane == j) { mine = v; expert = e; }
+    }
+    const float part = expert >= 0 ? expf(mine - top) : 0.0f;
+    float total = part;
+    if (!a.normalise) {
+        total = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) total += expf(z[i] - top);
+    }
+    total = pfdev::wave_sum(total);
+    if (lane < a.top_k) {
+        const long long at = (long long)t * a.top_k + lane;
+        a.choice[at] = expert;
+        a.weight[at] = expert >= 0 ? part / total : 0.0f;
+        if (expert >= 0) atomicOr(mask + expert, 1ull << local);
+    }
+}
+
+// Places the entries of block `block`: mask[e] has a bit for each of its tokens that chose expert e (a token chooses an
+// expert once, so the bits below its own count the entries before it), first[e] is the slot of the first of them.
+__device__ __forceinline__ void place(const Route &a, int block, const unsigned long long *mask, const int *first,
+                                      int used)
+{
+    const int begin = block * kBlock, entries = min(kBlock, a.tokens - begin) * a.top_k;
+    for (int i = threadIdx.x; i < entries; i += blockDim.x) {
+        const int f = begin * a.top_k + i, e = a.choice[f], local = i / a.top_k;
+        int s = -1;
+        if (e >= 0) {
+            s = first[e] + __popcll(mask[e] & ((1ull << local) - 1));
+            a.order[s] = f;
+        }
+        a.slot[f] = s;
+    }
+    // slots that no entry takes
+    for (long long s = used + (long long)block * blockDim.x + threadIdx.x; s < (long long)a.tokens * a.top_k;
+         s += (long long)a.blocks * blockDim.x)
+        a.order[s] = -1;
+}
+
+// Exclusive sums over the experts of total[e] into first[e] (in LDS); returns the sum.  One wave.
+__device__ __forceinline__ int scan_experts(const int *total, int *first, int experts)
+{
+    const int lane = threadIdx.x & (kWave - 1);
+    int before = 0;
+    for (int base = 0; base < experts; base += kWave) {
+        const int v = base + lane < experts ? total[base + lane] : 0;
+        const int incl = scan_wave(v);
+        if (base + lane < experts) first[base + lane] = before + incl - v;
+        before += __builtin_amdgcn_readlane(incl, kWave - 1);
+    }
+    return before;
+}
+
+// Choice and weights; with one block also offsets and order, else the block's counts.
+template <typename T, int PER>
+__global__ __launch_bounds__(512) void k_route(const Route a)
+{
+    __shared__ unsigned long long mask[PER * 64];
+    __shared__ int total[PER * 64], first[PER * 64], used;
+    const int block = blockIdx.x, wave = threadIdx.x >> 6;
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) mask[e] = 0;
+    __syncthreads();
+    for (int t = block * kBlock + wave; t < min(a.tokens, (block + 1) * kBlock); t += 8) choose<T, PER>(a, t, mask);
+    __syncthreads();
+    if (a.blocks > 1) {
+        for (int e = threadIdx.x; e < a.experts; e += blockDim.x)
+            a.counts[(long long)block * a.experts + e] = (unsigned char)__popcll(mask[e]);
+        return;
+    }
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) total[e] = __popcll(mask[e]);
+    __syncthreads();
+    if (wave == 0) {
+        const int n = scan_experts(total, first, a.experts);
+        if (threadIdx.x == 0) used = n;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) a.offsets[e] = first[e];
+    if (threadIdx.x == 0) a.offsets[a.experts] = used;
+    place(a, block, mask, first, used);
+}
+
+// Sums of kSuper blocks' counts each, for many blocks.
+__global__ __launch_bounds__(256) void k_route_super(const Route a)
+{
+    const int begin = blockIdx.x * kSuper, end = min(a.blocks, begin + kSuper);
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
+        int n = 0;
+        for (int b = begin; b < end; ++b) n += a.counts[(long long)b * a.experts + e];
+        a.super[(long long)blockIdx.x * a.experts + e] = n;
+    }
+}
+
+// Offsets and order from the counts: each workgroup sums all blocks' counts, and those before its own.
+__global__ __launch_bounds__(512) void k_route_place(const Route a)
+{
+    extern __shared__ unsigned long long lds[];
+    unsigned long long *mask = lds;
+    int *total = (int *)(lds + a.experts), *before = total + a.experts, *first = before + a.experts, *used = first + a.experts;
+    const int block = blockIdx.x;
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
+        mask[e] = 0;
+        total[e] = before[e] = 0;
+    }
+    __syncthreads();
+    const int begin = block * kBlock, entries = min(kBlock, a.tokens - begin) * a.top_k;
+    for (int i = threadIdx.x; i < entries; i += blockDim.x) {
+        const int e = a.choice[begin * a.top_k + i];
+        if (e >= 0) atomicOr(mask + e, 1ull << (i / a.top_k));
+    }
+    // thread groups of `wide` experts share the blocks out; integer sums, so their order does not matter
+    const int wide = a.experts < (int)blockDim.x ? a.experts : (int)blockDim.x, groups = blockDim.x / wide;
+    const int group = threadIdx.x / wide;
+    if (group < groups) {
+        const int supers = a.super ? a.blocks / kSuper : 0, own = block / kSuper;
+        for (int e = threadIdx.x % wide; e < a.experts; e += wide) {
+            int all = 0, prior = 0;
+            for (int i = group; i < supers; i += groups) {
+                const int n = a.super[(long long)i * a.experts + e];
+                all += n;
+                if (i < own) prior += n;
+            }
+            for (int b = supers * kSuper + group; b < a.blocks; b += groups) {
+                const int n = a.counts[(long long)b * a.experts + e];
+                all += n;
+                if (b < block) prior += n;
+            }
+            if (own < supers)
+                for (int b = own * kSuper + group; b < block; b += groups) prior += a.counts[(long long)b * a.experts + e];
+            atomicAdd(total + e, all);
+            atomicAdd(before + e, prior);
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < kWave) {
+        const int n = scan_experts(total, first, a.experts);
+        if (threadIdx.x == 0) *used = n;
+    }
+    __syncthreads();
+    if (block == 0) {
+        for (int e = threadIdx.x; e < a.experts; e += blockDim.x) a.offsets[e] = first[e];
+        if (threadIdx.x == 0) a.offsets[a.experts] = *used;
+        __syncthreads();
+    }
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) first[e] += before[e];
+    __syncthreads();
+    place(a, block, mask, first, *used);
+}
+
+// dz = w (g - sum w g) at the chosen under `normalise`, else [chosen] w g - p sum w g.  One wave a token.
+template <typename T, int PER>
+__global__ __launch_bounds__(256) void k_route_backward(const T *logits, long long ld, int tokens, int experts, int top_k,
+                                                        int normalise, const int *choice, const float *weight,
+                                                        const float *dweight, T *dlogits, long long ld_d)
+{
+    const int lane = threadIdx.x & (kWave - 1), t = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (t >= tokens) return;
+    int e = -1;
+    float w = 0, g = 0;
+    if (lane < top_k) {
+        const long long at = (long long)t * top_k + lane;
+        e = choice[at];
+        if (e >= 0) { w = weight[at]; g = dweight[at]; }
+    }
+    const float inner = pfdev::wave_sum(w * g);
+    const float grad = normalise ? w * (g - inner) : w * g;
+    float p[PER], d[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) p[i] = d[i] = 0;
+    if (!normalise) {
+        float most = -INFINITY, sum = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = lane * PER + i;
+            p[i] = c < experts ? as_float(logits[ld * t + c]) : -INFINITY;
+            most = fmaxf(most, p[i]);
+        }
+        for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+        const float base = most > -INFINITY ? most : 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) sum += p[i] = expf(p[i] - base);
+        sum = pfdev::wave_sum(sum);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) d[i] = p[i] == 0.0f ? 0.0f : -p[i] / sum * inner;
+    }
+    for (int j = 0; j < top_k; ++j) {
+        const int ej = __builtin_amdgcn_readlane(e, j);
+        const float gj = pfdev::readlane(grad, j);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (ej == lane * PER + i) d[i] += gj;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int c = lane * PER + i;
+        if (c < experts) dlogits[ld_d * t + c] = (T)d[i];
+    }
+}
+
+// Eight elements of a row from `at`, those behind its end as zeros; VECTOR: rows of whole 16-byte pieces.
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void load8(const T *row, int at, int have, float v[8])
+{
+    if (VECTOR || at + 8 <= have) {
+        typedef typename vec<T>::x8 x8;
+        const x8 h = VECTOR ? *(const x8 *)(row + at) : __builtin_bit_cast(x8, load16_any(row + at));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = at + i < have ? (float)row[at + i] : 0.0f;
+    }
+}
+
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void store8(T *row, int at, int have, const float v[8])
+{
+    if (VECTOR || at + 8 <= have) {
+        typename vec<T>::x8 h;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = (T)v[i];
+        if (VECTOR) *(typename vec<T>::x8 *)(row + at) = h;
+        else __builtin_memcpy(row + at, &h, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (at + i < have) row[at + i] = (T)v[i];
+    }
+}
+
+// out[t] = sum of w y[slot]: a wave takes 512 columns of a token, so that a few tokens already fill many waves.
+template <typename T, bool VECTOR>
+__global__ __launch_bounds__(256) void k_combine(const T *y, long long ld_y, int slots, const int *slot, const float *weight,
+                                                 int tokens, int top_k, int width, T *out, long long ld_out, int parts)
+{
+    const int lane = threadIdx.x & (kWave - 1);
+    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (unit >= (long long)tokens * parts) return;
+    const int t = (int)(unit / parts), at = (int)(unit % parts) * 512 + lane * 8;
+    int s = -1;
+    float w = 0;
+    if (lane < top_k) {
+        s = slot[(long long)t * top_k + lane];
+        if ((unsigned)s >= (unsigned)slots) s = -1;
+        w = s < 0 ? 0.0f : weight ? weight[(long long)t * top_k + lane] : 1.0f;
+    }
+    float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int j = 0; j < top_k; ++j) {
+        const int sj = __builtin_amdgcn_readlane(s, j);
+        const float wj = pfdev::readlane(w, j);
+        if (sj < 0 || at >= width) continue;
+        float v[8];
+        load8<T, VECTOR>(y + ld_y * sj, at, width, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] = __builtin_fmaf(wj, v[i], sum[i]);
+    }
+    if (at < width) store8<T, VECTOR>(out + ld_out * t, at, width, sum);
+}
+
+// dy[slot] = w dout[t], dweight = <dout[t], y[slot]>: a workgroup a token, which reads dout[t] once for all its slots.
+template <typename T, bool VECTOR>
+__global__ __launch_bounds__(256) void k_combine_backward(const T *dout, long long ld_dout, const T *y, long long ld_y,
+                                                          int slots, const int *slot, const float *weight, int top_k,
+                                                          int width, T *dy, long long ld_dy, float *dweight)
+{
+    __shared__ float part[4][PF_MOE_MAX_TOP_K];
+    const int t = blockIdx.x, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+    int s = -1;
+    float w = 0;
+    if (lane < top_k) {
+        s = slot[(long long)t * top_k + lane];
+        if ((unsigned)s >= (unsigned)slots) s = -1;
+        w = s < 0 ? 0.0f : weight ? weight[(long long)t * top_k + lane] : 1.0f;
+    }
+    float dot[PF_MOE_MAX_TOP_K];
+#pragma unroll
+    for (int j = 0; j < PF_MOE_MAX_TOP_K; ++j) dot[j] = 0;
+    for (int begin = 0; begin < width; begin += 2048) {
+        const int at = begin + threadIdx.x * 8;
+        const bool in = at < width;
+        float g[8];
+        if (in) load8<T, VECTOR>(dout + ld_dout * t, at, width, g);
+#pragma unroll
+        for (int j = 0; j < PF_MOE_MAX_TOP_K; ++j) {
+            const int sj = __builtin_amdgcn_readlane(s, j);
+            const float wj = pfdev::readlane(w, j);
+            if (sj >= 0 && in) {
+                float v[8], d[8];
+                load8<T, VECTOR>(y + ld_y * sj, at, width, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    dot[j] = __builtin_fmaf(g[i], v[i], dot[j]);
+                    d[i] = wj * g[i];
+                }
+                store8<T, VECTOR>(dy + ld_dy * sj, at, width, d);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < PF_MOE_MAX_TOP_K; ++j) {
+        const float sum = pfdev::wave_sum(dot[j]);
+        if (lane == 0) part[wave][j] = sum;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < top_k)
+        dweight[(long long)t * top_k + threadIdx.x] =
+            (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+}
+
+// h = silu(g) u: dg = dh u s (1 + g (1 - s)), du = dh g s, with s = 1 / (1 + exp(-g)).
+template <typename T, bool VECTOR>
+__global__ __launch_bounds__(256) void k_swiglu_backward(const T *dh, long long ld_dh, const T *pre, long long ld_pre, int rows,
+                                                         int n, T *dpre, long long ld_dpre, int parts)
+{
+    const long long unit = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (unit >= (long long)rows * parts) return;
+    const long long r = unit / parts;
+    const int at = (int)(unit % parts) * 8;
+    float d[8], g[8], u[8], dg[8], du[8];
+    load8<T, VECTOR>(dh + ld_dh * r, at, n, d);
+    load8<T, VECTOR>(pre + ld_pre * r, at, n, g);
+    load8<T, VECTOR>(pre + ld_pre * r + n, at, n, u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float s = 1.0f / (1.0f + __expf(-g[i]));
+        dg[i] = d[i] * u[i] * s * (1.0f + g[i] * (1.0f - s));
+        du[i] = d[i] * g[i] * s;
+    }
+    store8<T, VECTOR>(dpre + ld_dpre * r, at, n, dg);
+    store8<T, VECTOR>(dpre + ld_dpre * r + n, at, n, du);
+}
+
+template <typename T>
+int route(const Route &a, hipStream_t s)
+{
+    const dim3 grid(a.blocks), block(512);
+    if (a.experts <= 64) k_route<T, 1><<<grid, block, 0, s>>>(a);
+    else if (a.experts <= 128) k_route<T, 2><<<grid, block, 0, s>>>(a);
+    else if (a.experts <= 256) k_route<T, 4><<<grid, block, 0, s>>>(a);
+    else if (a.experts <= 512) k_route<T, 8><<<grid, block, 0, s>>>(a);
+    else k_route<T, 16><<<grid, block, 0, s>>>(a);
+    if (a.blocks > 1) {
+        const size_t lds = (size_t)a.experts * 20 + 8;
+        if (a.super) k_route_super<<<dim3(a.blocks / kSuper), dim3(256), 0, s>>>(a);
+        k_route_place<<<grid, block, lds, s>>>(a);
+    }
+    return pfk_internal_launched("k_route");
+}
+
+template <typename T>
+int route_backward(const void *logits, long long ld, int tokens, int experts, int top_k, int normalise, const int *choice,
+                   const float *weight, const float *dweight, void *dlogits, long long ld_d, hipStream_t s)
+{
+    const dim3 grid((tokens + 3) / 4), block(256);
+    const T *z = (const T *)logits;
+    T *dz = (T *)dlogits;
+#define PFK_BACKWARD(PER) \
+    k_route_backward<T, PER><<<grid, block, 0, s>>>(z, ld, tokens, experts, top_k, normalise, choice, weight, dweight, dz, ld_d)
+    if (experts <= 64) PFK_BACKWARD(1);
+    else if (experts <= 128) PFK_BACKWARD(2);
+    else if (experts <= 256) PFK_BACKWARD(4);
+    else if (experts <= 512) PFK_BACKWARD(8);
+    else PFK_BACKWARD(16);
+#undef PFK_BACKWARD
+    return pfk_internal_launched("k_route_backward");
+}
+
+// whether rows of 16-bit elements start at, and hold, whole 16-byte pieces
+bool whole(const void *p, long long ld, int width) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && width % 8 == 0; }
+
+template <typename T>
+int combine(const void *y, long long ld_y, int slots, const int *slot, const float *weight, int tokens, int top_k, int width,
+            void *out, long long ld_out, hipStream_t s)
+{
+    const int parts = (width + 511) / 512;
+    const dim3 grid((unsigned)(((long long)tokens * parts + 3) / 4)), block(256);
+    if (whole(y, ld_y, width) && whole(out, ld_out, width))
+        k_combine<T, true><<<grid, block, 0, s>>>((const T *)y, ld_y, slots, slot, weight, tokens, top_k, width, (T *)out, ld_out, parts);
+    else
+        k_combine<T, false><<<grid, block, 0, s>>>((const T *)y, ld_y, slots, slot, weight, tokens, top_k, width, (T *)out, ld_out, parts);
+    return pfk_internal_launched("k_combine");
+}
+
+template <typename T>
+int combine_backward(const void *dout, long long ld_dout, const void *y, long long ld_y, int slots, const int *slot,
+                     const float *weight, int tokens, int top_k, int width, void *dy, long long ld_dy, float *dweight,
+                     hipStream_t s)
+{
+    const dim3 grid(tokens), block(256);
+    if (whole(dout, ld_dout, width) && whole(y, ld_y, width) && whole(dy, ld_dy, width))
+        k_combine_backward<T, true><<<grid, block, 0, s>>>((const T *)dout, ld_dout, (const T *)y, ld_y, slots, slot, weight, top_k, width, (T *)dy, ld_dy, dweight);
+    else
+        k_combine_backward<T, false><<<grid, block, 0, s>>>((const T *)dout, ld_dout, (const T *)y, ld_y, slots, slot, weight, top_k, width, (T *)dy, ld_dy, dweight);
+    return pfk_internal_launched("k_combine_backward");
+}
+
+template <typename T>
+int swiglu_backward(const void *dh, long long ld_dh, const void *pre, long long ld_pre, int rows, int n, void *dpre,
+                    long long ld_dpre, hipStream_t s)
+{
+    const int parts = (n + 7) / 8;
+    const long long grid = ((long long)rows * parts + 255) / 256;
+    if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "activation's gradient: too many elements");
+    if (whole(dh, ld_dh, n) && whole(pre, ld_pre, n) && whole(dpre, ld_dpre, n))
+        k_swiglu_backward<T, true><<<dim3((unsigned)grid), dim3(256), 0, s>>>((const T *)dh, ld_dh, (const T *)pre, ld_pre, rows, n, (T *)dpre, ld_dpre, parts);
+    else
+        k_swiglu_backward<T, false><<<dim3((unsigned)grid), dim3(256), 0, s>>>((const T *)dh, ld_dh, (const T *)pre, ld_pre, rows, n, (T *)dpre, ld_dpre, parts);
+    return pfk_internal_launched("k_swiglu_backward");
+}
+
+}  // namespace
+
+extern "C" {
+
+int pfk_moe_route(const void *logits, long long ld, int dtype, int tokens, int experts, int top_k, int normalise,
+                  int *choice, float *weight, int *offsets, int *order, int *slot, int *counts, void *stream)
+{
+    Route a = {logits, ld, tokens, experts, top_k, normalise, (tokens + kBlock - 1) / kBlock, choice, weight, offsets, order, slot, nullptr, nullptr};
+    if (a.blocks < 1) a.blocks = 1;
+    if (a.blocks > 1) a.counts = (unsigned char *)counts;
+    if (a.blocks > kDirect)  // the bytes of the counts, rounded up to whole ints, then the sums
+        a.super = counts + ((long long)a.blocks * experts + 3) / 4;
+    hipStream_t s = (hipStream_t)stream;
+    return dtype == PF_F32 ? route<float>(a, s) : dtype == PF_F16 ? route<f16>(a, s) : route<bf16>(a, s);
+}
+
+int pfk_moe_route_backward(const void *logits, long long ld, int dtype, int tokens, int experts, int top_k, int normalise,
+                           const int *choice, const float *weight, const float *dweight, void *dlogits, long long ld_d,
+                           void *stream)
+{
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == PF_F32) return route_backward<float>(logits, ld, tokens, experts, top_k, normalise, choice, weight, dweight, dlogits, ld_d, s);
+    if (dtype == PF_F16) return route_backward<f16>(logits, ld, tokens, experts, top_k, normalise, choice, weight, dweight, dlogits, ld_d, s);
+    return route_backward<bf16>(logits, ld, tokens, experts, top_k, normalise, choice, weight, dweight, dlogits, ld_d, s);
+}
+
+int pfk_moe_combine(const void *y, long long ld_y, int dtype, int slots, const int *slot, const float *weight, int tokens,
+                    int top_k, int width, void *out, long long ld_out, void *stream)
+{
+    hipStream_t s = (hipStream_t)stream;
+    return dtype == PF_F16 ? combine<f16>(y, ld_y, slots, slot, weight, tokens, top_k, width, out, ld_out, s)
+                           : combine<bf16>(y, ld_y, slots, slot, weight, tokens, top_k, width, out, ld_out, s);
+}
+
+int pfk_moe_combine_backward(const void *dout, long long ld_dout, const void *y, long long ld_y, int dtype, int slots,
+                             const int *slot, const float *weight, int tokens, int top_k, int width, void *dy,
+                             long long ld_dy, float *dweight, void *stream)
+{
+    hipStream_t s = (hipStream_t)stream;
+    return dtype == PF_F16
+               ? combine_backward<f16>(dout, ld_dout, y, ld_y, slots, slot, weight, tokens, top_k, width, dy, ld_dy, dweight, s)
+               : combine_backward<bf16>(dout, ld_dout, y, ld_y, slots, slot, weight, tokens, top_k, width, dy, ld_dy, dweight, s);
+}
+
+int pfk_swiglu_backward(const void *dh, long long ld_dh, const void *pre, long long ld_pre, int dtype, int rows, int n,
+                        void *dpre, long long ld_dpre, void *stream)
+{
+    hipStream_t s = (hipStream_t)stream;
+    return dtype == PF_F16 ? swiglu_backward<f16>(dh, ld_dh, pre, ld_pre, rows, n, dpre, ld_dpre, s)
+                           : swiglu_backward<bf16>(dh, ld_dh, pre, ld_pre, rows, n, dpre, ld_dpre, s);
+}
+
+}  // extern "C"

@@ -56,6 +56,7 @@
 #include "../../include/prefree_c.h"
 #include "../../include/prefree_kernels.h"
 #include "device_common.hpp"
+#include "moe_launch.hpp"
 
 #include <hip/hip_runtime.h>
 #include <stdio.h>
@@ -5375,3 +5376,15 @@ int pfk_scratch(void **ptr, size_t *bytes)
 const char *pfk_last_error(void) { return g_err; }
 
 }  // extern "C"
+
+int pfk_internal_fail(int status, const char *what)
+{
+    snprintf(g_err, sizeof g_err, "%s", what);
+    return status;
+}
+
+int pfk_internal_launched(const char *what)
+{
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? PF_OK : hip_fail(e, what);
+}

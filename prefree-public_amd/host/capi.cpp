@@ -3,6 +3,7 @@
 // through the thin HIP layer of include/prefree_kernels.h.
 #include "prefree_c.h"
 #include "prefree_kernels.h"
+#include "error.h"
 
 #include <algorithm>
 #include <cstdint>
@@ -2174,3 +2175,5 @@ int pf_memcpy_d2h(void *dst, const void *src, size_t bytes, void *stream)
 int pf_stream_synchronize(void *stream) { return from_kernel_layer(pfk_stream_sync(stream), "synchronise"); }
 
 }  // extern "C"
+
+int pf_internal_fail(int status, const std::string &msg) { return fail(status, msg); }
