@@ -9,7 +9,7 @@ namespace {
 using namespace pfmoe;
 
 // What the three products have in common: C[m][n] = sum over k of P[m][k] Q[n][k], tile by tile.  Both operands
-// are staged through LDS in tiles of 128 bytes of k per row (64 elements of 16 bits, 256 of 4 bits).
+// are staged through LDS in tiles of 64 bytes of k per row (32 elements of 16 bits, 128 of 4 bits).
 //   forward    m: slots of an expert (P: x, gathered)   n: rows of w                k: x's columns, both row by row
 //   kDx        m: slots of an expert (P: dy)            n: columns of w             k: rows of w: Q lies across
 //   kDw        m: columns of dy                         n: columns of x (gathered)  k: slots of an expert: both across
@@ -26,14 +26,22 @@ struct Args {
     char *out, *pre;
 };
 
-// 16 zero bytes in global memory: what a lane loads whose k lies behind the operand's end.  (Loads that go straight
-// to LDS cannot be masked per lane without leaving old bytes there.)
-__device__ const i32x4 g_zero = {0, 0, 0, 0};
+// Loads straight to LDS go through buffer descriptors: 32-bit offsets from a base in scalar registers, and a lane whose
+// offset lies behind the operand writes zeros, which is how k is cut off at its end.  (The other form, global_load_lds,
+// counts as a flat access: the compiler then waits for every LDS read under way wherever it waits for one.)
+typedef __amdgpu_buffer_rsrc_t Buffer;
+constexpr unsigned kOutside = 0xffffffffu;       // an offset behind every operand
+constexpr unsigned long long kBufferMax = 0xfffff000ull;
 
-__device__ __forceinline__ void to_lds16(const char *src, char *dst)
+__device__ __forceinline__ Buffer buffer_of(const char *base, unsigned long long bytes)
 {
-    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)src,
-                                     (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+    return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)(unsigned)(bytes < kBufferMax ? bytes : kBufferMax), 0x00020000);
+}
+
+__device__ __forceinline__ void to_lds16(Buffer from, unsigned lane_offset, unsigned offset, char *dst)
+{
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)dst, 16, (int)lane_offset,
+                                             (int)offset, 0, 0);
 }
 
 template <typename T>
@@ -114,38 +122,43 @@ __device__ __forceinline__ i32x4 load8_any(const char *row, int at, int have)
     return v;
 }
 
-// An operand whose k lies along its rows: a tile is ROWS rows of 128 bytes.  The 16-byte piece c of row r lies at
-// place c ^ ((r >> 1) & 7) of the row, so that the 16 lanes that read one piece of 16 rows touch each bank once.
+// An operand whose k lies along its rows: a tile is ROWS rows of 64 bytes.  The 16-byte piece c of row r lies at place
+// c ^ ((r >> 1) & 3) of the row, so that eight lanes that read one piece of eight rows touch each bank of 128 bytes once.
 template <int ROWS, int THREADS, bool ALIGNED>
 struct Along {
-    static constexpr int kBytes = ROWS * 128;
-    static constexpr int kLoads = ROWS * 8 / THREADS;
-    const char *row[kLoads];
+    static constexpr int kBytes = ROWS * 64;
+    static constexpr int kLoads = ROWS * 4 / THREADS;
+    Buffer from;                          // ALIGNED: the operand, and this thread's pieces of its rows in the first tile
+    unsigned at[ALIGNED ? kLoads : 1];
+    const char *row[ALIGNED ? 1 : kLoads];
     int piece;          // this thread's piece of its rows (the same for all its loads)
     int k_pieces, k;
     i32x4 held[ALIGNED ? 1 : kLoads];
 
-    static __device__ __forceinline__ int tile_row(int i) { return i * (THREADS / 8) + (int)(threadIdx.x >> 3); }
+    static __device__ __forceinline__ int tile_row(int i) { return i * (THREADS / 4) + (int)(threadIdx.x >> 2); }
 
-    __device__ __forceinline__ void init(int k_, int per_piece)
+    // row_of(r): the operand's row for row r of the tile
+    template <typename F>
+    __device__ __forceinline__ void init(const char *base, unsigned long long bytes, long long ld, F row_of, int k_, int per_piece)
     {
-        piece = (threadIdx.x & 7) ^ ((threadIdx.x >> 4) & 7);
+        piece = (threadIdx.x & 3) ^ ((threadIdx.x >> 3) & 3);
         k = k_;
         k_pieces = k_ / per_piece;
-    }
-    __device__ __forceinline__ void issue(int t, char *lds)
-    {
-        const int at = t * 8 + piece;
-        if constexpr (ALIGNED) {
-            const bool in = at < k_pieces;
+        if constexpr (ALIGNED) from = buffer_of(base, bytes);
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i)
-                to_lds16(in ? row[i] + 16LL * at : (const char *)&g_zero,
-                         lds + i * THREADS * 16 + (threadIdx.x & ~(kWave - 1)) * 16);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) held[i] = load8_any(row[i], at * 8, k);
+        for (int i = 0; i < kLoads; ++i) {
+            const long long r = ld * row_of(tile_row(i));
+            if constexpr (ALIGNED) at[i] = (unsigned)r + piece * 16;
+            else row[i] = base + r;
         }
+    }
+    __device__ __forceinline__ void issue(int i, int t, char *lds)
+    {
+        const int c = t * 4 + piece;
+        if constexpr (ALIGNED)
+            to_lds16(from, c < k_pieces ? at[i] : kOutside, t * 64, lds + i * THREADS * 16 + (threadIdx.x & ~(kWave - 1)) * 16);
+        else
+            held[i] = load8_any(row[i], c * 8, k);
     }
     __device__ __forceinline__ void commit(char *lds)
     {
@@ -154,27 +167,29 @@ struct Along {
             for (int i = 0; i < kLoads; ++i) *(i32x4 *)(lds + i * THREADS * 16 + threadIdx.x * 16) = held[i];
         }
     }
-    // 16 rows from r0 (a multiple of 16), step kk of 4 pieces: lane l has row l % 16, piece 4 kk + l / 16
-    static __device__ __forceinline__ i32x4 fragment(const char *lds, int r0, int kk)
+    // 16 rows from r0 (a multiple of 16): lane l has row l % 16, piece l / 16
+    static __device__ __forceinline__ i32x4 fragment(const char *lds, int r0)
     {
         const int l = threadIdx.x & (kWave - 1);
-        return *(const i32x4 *)(lds + r0 * 128 + (l & 15) * 128 + (((kk * 4 + (l >> 4)) ^ ((l >> 1) & 7)) * 16));
+        return *(const i32x4 *)(lds + r0 * 64 + (l & 15) * 64 + (((l >> 4) ^ ((l >> 1) & 3)) * 16));
     }
 };
 
-// An operand whose k lies across its rows: a tile is 64 rows of COLS columns (16 bits), read with the transposing LDS
+// An operand whose k lies across its rows: a tile is 32 rows of COLS columns (16 bits), read with the transposing LDS
 // read, which hands a group of 16 lanes a block of 4 rows x 16 columns by columns.  The 32-byte unit u of row r lies
 // at place u ^ f(r), f of bits 0, 1 and 3 of r, so that the eight rows which half a wave reads lie in other banks.
 template <int COLS, int THREADS, bool ALIGNED>
 struct Across {
-    static constexpr int kBytes = COLS * 128;
-    static constexpr int kLoads = COLS * 8 / THREADS;
+    static constexpr int kBytes = COLS * 64;
+    static constexpr int kLoads = COLS * 4 / THREADS;
     static constexpr int kPieces = COLS / 8;             // 16-byte pieces a row
     static constexpr int kStride = THREADS / kPieces;    // rows a load of all threads covers
-    static_assert(kPieces >= 16 && kStride % 16 == 0, "the swizzle repeats every 16 rows");
+    static constexpr int kWaveRows = kWave / kPieces;    // and of one wave
+    static_assert(kPieces >= 16 && kPieces <= 32 && kStride % 8 == 0, "see f");
+    Buffer from;         // ALIGNED
     const char *base;
     long long ld;
-    int col, cols;       // this thread's first column, and the columns there are
+    int col[2], cols;    // this thread's first column in loads of even and odd number, and the columns there are
     int k;
     i32x4 held[ALIGNED ? 1 : kLoads];
 
@@ -182,32 +197,40 @@ struct Across {
     static __device__ __forceinline__ int tile_row(int i) { return i * kStride + (int)threadIdx.x / kPieces; }
 
     // columns from c0 of rows of `cols_` columns
-    __device__ __forceinline__ void init(const char *base_, long long ld_, int c0, int cols_, int k_)
+    __device__ __forceinline__ void init(const char *base_, unsigned long long bytes, long long ld_, int c0, int cols_, int k_)
     {
+        if constexpr (ALIGNED) from = buffer_of(base_, bytes);
         const int place = threadIdx.x % kPieces, r = threadIdx.x / kPieces;
-        col = c0 + (((place >> 1) ^ f(r)) * 2 + (place & 1)) * 8;
         cols = cols_;
-        if (ALIGNED && col >= cols) col = 0;   // columns behind the end: any, their results are not stored
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            col[i] = c0 + (((place >> 1) ^ f(i * kStride + r)) * 2 + (place & 1)) * 8;
+            if (ALIGNED && col[i] >= cols) col[i] = 0;   // columns behind the end: any, their results are not stored
+        }
         base = base_;
         ld = ld_;
         k = k_;
     }
-    // row_of(r): the operand's row for k = r < k
-    template <typename F>
-    __device__ __forceinline__ void issue(int t, char *lds, F row_of)
+    // Load i of tile t; with GATHER its rows are numbered by `rows` (see lookup), else by k itself.
+    template <bool GATHER>
+    __device__ __forceinline__ void issue(int i, int t, char *lds, int rows)
     {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int r = t * 64 + tile_row(i);
-            if constexpr (ALIGNED) {
-                const char *src = (const char *)&g_zero;
-                if (r < k) src = base + ld * row_of(r) + 2LL * col;
-                to_lds16(src, lds + i * THREADS * 16 + (threadIdx.x & ~(kWave - 1)) * 16);
-            } else {
-                held[i] = i32x4{0, 0, 0, 0};
-                if (r < k && col < cols) held[i] = load8_any(base + ld * row_of(r), col, cols);
-            }
+        const int r = t * 32 + tile_row(i);
+        const int at = GATHER ? __shfl(rows, i * kWaveRows + (int)(threadIdx.x & (kWave - 1)) / kPieces) : r;
+        if constexpr (ALIGNED) {
+            const unsigned first = GATHER ? (unsigned)at * (unsigned)ld : (unsigned)tile_row(i) * (unsigned)ld;
+            to_lds16(from, r < k ? first + 2 * col[i & 1] : kOutside, GATHER ? 0 : (unsigned)(t * 32) * (unsigned)ld,
+                     lds + i * THREADS * 16 + (threadIdx.x & ~(kWave - 1)) * 16);
+        } else {
+            held[i] = i32x4{0, 0, 0, 0};
+            if (r < k && col[i & 1] < cols) held[i] = load8_any(base + ld * at, col[i & 1], cols);
         }
+    }
+    // The k of tile t whose row lane l looks up for its wave: load l / kWaveRows, row l % kWaveRows of the wave's.
+    static __device__ __forceinline__ int lookup(int t)
+    {
+        const int l = (threadIdx.x & (kWave - 1)) % (kLoads * kWaveRows), w = threadIdx.x / kWave;
+        return t * 32 + l / kWaveRows * kStride + w * kWaveRows + l % kWaveRows;
     }
     __device__ __forceinline__ void commit(char *lds)
     {
@@ -216,12 +239,12 @@ struct Across {
             for (int i = 0; i < kLoads; ++i) *(i32x4 *)(lds + i * THREADS * 16 + threadIdx.x * 16) = held[i];
         }
     }
-    // 16 columns from c0 (a multiple of 16), step kk of 32 rows: lane l has column l % 16, rows 32 kk + 8 (l / 16) ..+7
-    static __device__ __forceinline__ i32x4 fragment(const char *lds, int c0, int kk)
+    // 16 columns from c0 (a multiple of 16): lane l has column l % 16, rows 8 (l / 16) .. +7
+    static __device__ __forceinline__ i32x4 fragment(const char *lds, int c0)
     {
         const int l = threadIdx.x & (kWave - 1), g = l >> 4, q = (l >> 2) & 3, part = l & 3;
         const int unit = (c0 / 16) ^ (q | ((g & 1) << 2));
-        const char *at = lds + (kk * 32 + g * 8 + q) * (COLS * 2) + unit * 32 + part * 8;
+        const char *at = lds + (g * 8 + q) * (COLS * 2) + unit * 32 + part * 8;
         typedef __attribute__((address_space(3))) s16x4 lds4;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)at);
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(at + 4 * COLS * 2));
@@ -267,6 +290,40 @@ __device__ __forceinline__ int row_of_slot(const Args &a, int s)
     return (unsigned)r < (unsigned)a.p_rows ? r : 0;
 }
 
+// The four scale bytes of each row of a tile of either operand, by way of registers (scale rows have any alignment):
+// thread r takes row r, those of the rows operand first.
+struct Scales {
+    const unsigned char *row;
+    unsigned held;
+
+    // whether tile t has all its scales, and loading them is one load
+    static __device__ __forceinline__ bool whole(int t, int blocks) { return t * 4 + 4 <= blocks; }
+    __device__ __forceinline__ void issue(int t, int blocks)
+    {
+        if (whole(t, blocks)) {
+            __builtin_memcpy(&held, row + t * 4, 4);
+        } else {
+            held = 0x7f7f7f7fu;   // 1 where the codes are zeros behind the row's end
+            for (int b = 0; t * 4 + b < blocks; ++b) held = (held & ~(0xffu << 8 * b)) | (unsigned)row[t * 4 + b] << 8 * b;
+        }
+    }
+    __device__ __forceinline__ void commit(char *lds) { *(unsigned *)(lds + threadIdx.x * 4) = held; }
+    // the scale of this lane's row of 16 from r0 and piece
+    static __device__ __forceinline__ int fragment(const char *lds, int r0)
+    {
+        const int l = threadIdx.x & (kWave - 1);
+        return *(const unsigned char *)(lds + (r0 + (l & 15)) * 4 + (l >> 4));
+    }
+};
+
+// Waits until at most LOADS of this wave's loads to LDS are under way and all its LDS reads are done, then for the
+// other waves.  (__syncthreads() would wait for every load.)
+template <int LOADS>
+__device__ __forceinline__ void wait_and_meet()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+}
+
 // T: f16 or bf16 of the results; FP4: 4-bit operands
 template <typename T, bool FP4, int MODE, int ACT, int BM, int BN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
@@ -275,7 +332,10 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
     constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
     typedef typename std::conditional<MODE == kDw, Across<BM, THREADS, ALIGNED>, Along<BM, THREADS, ALIGNED>>::type P;
     typedef typename std::conditional<MODE == kFwd, Along<BN, THREADS, ALIGNED>, Across<BN, THREADS, ALIGNED>>::type Q;
-    __shared__ __align__(1024) char lds[2][P::kBytes + Q::kBytes];
+    constexpr int SCALES = P::kBytes + Q::kBytes;   // where a tile's scales lie
+    constexpr int SLOT = SCALES + (FP4 ? (BM + BN) * 4 : 0);
+    static_assert(!FP4 || BM + BN == THREADS, "see Scales");
+    __shared__ __align__(1024) char lds[4][SLOT];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
     constexpr int OUT_N = ACT ? BN / 2 : BN;   // results of a tile's row
@@ -294,60 +354,61 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
     }
 
     const int k = MODE == kDw ? t.end - t.begin : a.k;
-    const int steps = FP4 ? (k + 255) / 256 : (k + 63) / 64;
+    const int steps = FP4 ? (k + 127) / 128 : (k + 31) / 32;
+    const int m0 = t.m * BM, count = t.end - t.begin;
+    // Row of w that row r of the tile stands for.  Under SwiGLU rows of the gate and of the rest take turns of 16, so
+    // that a wave holds both.
+    const auto weight_row = [&](int r) {
+        if constexpr (ACT) return min(t.n * OUT_N + r / 32 * 16 + r % 16, a.n - 1) + (r / 16 % 2) * a.n;
+        else return min(t.n * BN + r, a.n - 1);
+    };
+    const auto slot_row = [&](int r) { return row_of_slot(a, t.begin + min(m0 + r, count - 1)); };
     P p;
     Q q;
-    const int m0 = t.m * BM, count = t.end - t.begin;
+    Scales scales;
+    int rows = 0;   // kDw: x's rows of the next tile to be loaded
     if constexpr (MODE == kDw) {
-        p.init(a.p + a.ld_p * t.begin, a.ld_p, m0, a.m, k);
-        q.init(a.q, a.ld_q, t.n * BN, a.n, k);
+        p.init(a.p + a.ld_p * t.begin, a.ld_p * k, a.ld_p, m0, a.m, k);
+        q.init(a.q, a.ld_q * a.p_rows, a.ld_q, t.n * BN, a.n, k);
+        if (k > 0) rows = row_of_slot(a, t.begin + min(Q::lookup(0), k - 1));
     } else {
-        p.init(k, FP4 ? 32 : 8);
-#pragma unroll
-        for (int i = 0; i < P::kLoads; ++i)
-            p.row[i] = a.p + a.ld_p * row_of_slot(a, t.begin + min(m0 + P::tile_row(i), count - 1));
-        if constexpr (MODE == kFwd) {
-            q.init(k, FP4 ? 32 : 8);
-#pragma unroll
-            for (int i = 0; i < Q::kLoads; ++i) {
-                const int r = Q::tile_row(i);
-                int n;
-                if constexpr (ACT) {  // rows of the gate and of the rest by turns of 16, so that a wave holds both
-                    n = min(t.n * OUT_N + r / 32 * 16 + r % 16, a.n - 1) + (r / 16 % 2) * a.n;
-                } else {
-                    n = min(t.n * BN + r, a.n - 1);
-                }
-                q.row[i] = a.q + a.q_expert * t.e + a.ld_q * n;
-            }
-        } else {
-            q.init(a.q + a.q_expert * t.e, a.ld_q, t.n * BN, a.n, k);
-        }
+        p.init(a.p, a.ld_p * a.p_rows, a.ld_p, slot_row, k, FP4 ? 32 : 8);
+        if constexpr (MODE == kFwd) q.init(a.q + a.q_expert * t.e, a.q_expert, a.ld_q, weight_row, k, FP4 ? 32 : 8);
+        else q.init(a.q + a.q_expert * t.e, a.q_expert, a.ld_q, t.n * BN, a.n, k);
     }
-    const auto own_row = [&](int r) { return (long long)r; };
-    const auto slot_row = [&](int r) { return (long long)row_of_slot(a, t.begin + r); };
-    const auto issue = [&](int s, char *to) {
-        if constexpr (MODE == kDw) p.issue(s, to, own_row); else p.issue(s, to);
-        if constexpr (MODE == kFwd) q.issue(s, to + P::kBytes);
-        else if constexpr (MODE == kDx) q.issue(s, to + P::kBytes, own_row);
-        else q.issue(s, to + P::kBytes, slot_row);
-    };
-
-    // 4-bit operands: the scale rows of this lane's fragments' rows
-    const unsigned char *ps[FP4 ? FM : 1], *qs[FP4 ? FN : 1];
     if constexpr (FP4) {
         const long long blocks = k / 32;
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-            ps[i] = a.p_scales + blocks * row_of_slot(a, t.begin + min(m0 + (wm * FM + i) * 16 + (lane & 15), count - 1));
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int r = (wn * FN + j) * 16 + (lane & 15);
-            int n;
-            if constexpr (ACT) n = min(t.n * OUT_N + r / 32 * 16 + r % 16, a.n - 1) + (r / 16 % 2) * a.n;
-            else n = min(t.n * BN + r, a.n - 1);
-            qs[j] = a.q_scales + blocks * ((ACT ? 2LL : 1LL) * a.n * t.e + n);
-        }
+        if (tid < BM) scales.row = a.p_scales + blocks * slot_row(tid);
+        else scales.row = a.q_scales + blocks * ((ACT ? 2LL : 1LL) * a.n * t.e + weight_row(tid - BM));
     }
+    constexpr int LOADS = P::kLoads + Q::kLoads;   // of a tile, by each thread
+    int now = 0;
+    // load i of tile s
+    const auto issue = [&](int i, int s, char *to) {
+        if (i == 0) {
+            if constexpr (MODE == kDw) {   // looked up before the loads, so that waiting for it does not wait for them
+                now = rows;
+                rows = row_of_slot(a, t.begin + min(Q::lookup(s + 1), k - 1));
+            }
+        }
+        if (i < P::kLoads) {
+            if constexpr (MODE == kDw) p.template issue<false>(i, s, to, 0);
+            else p.issue(i, s, to);
+        } else {
+            if constexpr (MODE == kFwd) q.issue(i - P::kLoads, s, to + P::kBytes);
+            else q.template issue<MODE == kDw>(i - P::kLoads, s, to + P::kBytes, now);
+        }
+    };
+    const auto commit = [&](char *to) {   // what came by way of registers
+        p.commit(to);
+        q.commit(to + P::kBytes);
+    };
+
+    // A wave's rows are every WM-th block of 16 of the tile, its columns FN blocks side by side.
+    const auto read_x = [&](const char *from, int i) { return P::fragment(from, (i * WM + wm) * 16); };
+    const auto read_w = [&](const char *from, int j) { return Q::fragment(from + P::kBytes, (wn * FN + j) * 16); };
+    const auto scale_x = [&](const char *from, int i) { return FP4 ? Scales::fragment(from + SCALES, (i * WM + wm) * 16) : 0; };
+    const auto scale_w = [&](const char *from, int j) { return FP4 ? Scales::fragment(from + SCALES, BM + (wn * FN + j) * 16) : 0; };
 
     f32x4 acc[FM][FN];
 #pragma unroll
@@ -355,55 +416,92 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
+    // Four tiles of k in LDS.  While tile s is multiplied its rows' fragments are read two ahead and the columns'
+    // fragments of tile s+1 beside them, so that the matrix cores find their operands in registers; tile s+3 is on its
+    // way into the place of tile s-1, which every wave has left.  Two tiles of loads may be under way at the meeting
+    // of the waves, which only waits for tile s+2.  (The places are told apart as restricted pointers: otherwise the
+    // compiler waits for all loads to LDS before each transposing read.)
+    i32x4 x[4], w[FN], w_next[FN];
+    int xs[4], ws[FN], ws_next[FN];
+    const auto step = [&](int s, char *__restrict__ fill, const char *__restrict__ here, const char *__restrict__ next) {
+        if constexpr (FP4) {   // a tile further ahead, since their loads end in a register
+            scales.commit(fill + SCALES);
+            scales.issue(s + 4, k / 32);
+        }
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+#pragma unroll
+            for (int l = i * LOADS / FM; l < (i + 1) * LOADS / FM; ++l) issue(l, s + 3, fill);
+            const char *from = i + 2 < FM ? here : next;
+            x[(i + 2) % 4] = read_x(from, (i + 2) % FM);
+            xs[(i + 2) % 4] = scale_x(from, (i + 2) % FM);
+#pragma unroll
+            for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j) {
+                w_next[j] = read_w(next, j);
+                ws_next[j] = scale_w(next, j);
+            }
+            // reads and loads stay ahead of these products (mask: only address arithmetic may pass; it
+            // would let the scaled products pass too)
+            __builtin_amdgcn_sched_barrier(FP4 ? 0 : 0x6);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                if constexpr (FP4) {
+                    const i32x8 A = {w[j][0], w[j][1], w[j][2], w[j][3], 0, 0, 0, 0};
+                    const i32x8 B = {x[i % 4][0], x[i % 4][1], x[i % 4][2], x[i % 4][3], 0, 0, 0, 0};
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc[i][j], 4, 4, 0, ws[j], 0, xs[i % 4]);
+                } else {
+                    acc[i][j] = mfma<T>(w[j], x[i % 4], acc[i][j]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(FP4 ? 0 : 0x6);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        commit(fill);
+        if (FP4 && Scales::whole(s + 4, k / 32)) wait_and_meet<LOADS + 1>();   // the scales' load as well
+        else wait_and_meet<ALIGNED ? LOADS : 0>();
+        __builtin_amdgcn_sched_barrier(0);
+    };
     if (steps > 0) {
-        issue(0, lds[0]);
-        p.commit(lds[0]);
-        q.commit(lds[0] + P::kBytes);
-    }
-    for (int s = 0; s < steps; ++s) {
-        __syncthreads();
-        char *now = lds[s & 1], *next = lds[(s & 1) ^ 1];
-        if (s + 1 < steps) issue(s + 1, next);
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            i32x4 x[FM], w[FN];
+        for (int s = 0; s < 3; ++s) {
 #pragma unroll
-            for (int i = 0; i < FM; ++i) x[i] = P::fragment(now, (wm * FM + i) * 16, kk);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) w[j] = Q::fragment(now + P::kBytes, (wn * FN + j) * 16, kk);
+            for (int i = 0; i < LOADS; ++i) issue(i, s, lds[s]);
+            commit(lds[s]);
             if constexpr (FP4) {
-                const int block = s * 8 + kk * 4 + (lane >> 4), blocks = k / 32;
-                int xs[FM], ws[FN];
-#pragma unroll
-                for (int i = 0; i < FM; ++i) xs[i] = block < blocks ? ps[i][block] : 127;
-#pragma unroll
-                for (int j = 0; j < FN; ++j) ws[j] = block < blocks ? qs[j][block] : 127;
-#pragma unroll
-                for (int i = 0; i < FM; ++i)
-#pragma unroll
-                    for (int j = 0; j < FN; ++j) {
-                        const i32x8 A = {w[j][0], w[j][1], w[j][2], w[j][3], 0, 0, 0, 0};
-                        const i32x8 B = {x[i][0], x[i][1], x[i][2], x[i][3], 0, 0, 0, 0};
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc[i][j], 4, 4, 0, ws[j], 0, xs[i]);
-                    }
-            } else {
-#pragma unroll
-                for (int i = 0; i < FM; ++i)
-#pragma unroll
-                    for (int j = 0; j < FN; ++j) acc[i][j] = mfma<T>(w[j], x[i], acc[i][j]);
+                scales.issue(s, k / 32);
+                scales.commit(lds[s] + SCALES);
             }
         }
-        if (s + 1 < steps) {
-            p.commit(next);
-            q.commit(next + P::kBytes);
+        if constexpr (FP4) scales.issue(3, k / 32);
+        wait_and_meet<ALIGNED ? LOADS : 0>();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[i] = read_x(lds[0], i);
+            xs[i] = scale_x(lds[0], i);
         }
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            w[j] = read_w(lds[0], j);
+            ws[j] = scale_w(lds[0], j);
+        }
+#pragma unroll 1
+        for (int s = 0; s < steps; ++s) {
+            step(s, lds[(s + 3) & 3], lds[s & 3], lds[(s + 1) & 3]);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                w[j] = w_next[j];
+                ws[j] = ws_next[j];
+            }
+        }
+        // nothing may still be on its way to LDS when the workgroup ends
+        wait_and_meet<0>();
     }
 
     // lane l holds row l % 16 of each block and four consecutive columns
     const int have = MODE == kDw ? a.m - m0 : count - m0;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-        const int r = (wm * FM + i) * 16 + (lane & 15);
+        const int r = (i * WM + wm) * 16 + (lane & 15);
         if (r >= have) continue;
         const long long at = MODE == kDw ? (long long)t.e * a.m + m0 + r : (long long)t.begin + m0 + r;
         char *out = a.out + a.ld_out * at;
@@ -453,6 +551,9 @@ int launch_size(const Args &a, hipStream_t stream)
     return launch<T, FP4, MODE, ACT, 256, 256, 2, 4, ALIGNED>(a, stream);
 }
 
+// whether `bytes` lie within the 32-bit offsets of a buffer descriptor
+bool fits(long long rows, long long ld) { return (unsigned long long)rows * ld < kBufferMax; }
+
 bool lies16(const void *p, long long ld) { return ((uintptr_t)p | (unsigned long long)ld) % 16 == 0; }
 
 template <int MODE, int ACT>
@@ -498,7 +599,7 @@ int pfk_moe_mm(const pfk_moe_mm_args *g, void *stream)
     const int each = g->act == PF_ACT_SWIGLU ? 2 : 1;
     a.q_expert = g->ld_q * g->n * each;
     a.wide = wide(g->out, g->ld_out, 2) && (!g->pre || (wide(g->pre, g->ld_pre, 2) && g->n % 4 == 0));
-    const bool aligned = lies16(g->p, g->ld_p) && lies16(g->q, g->ld_q) && g->k % 8 == 0;
+    const bool aligned = lies16(g->p, g->ld_p) && lies16(g->q, g->ld_q) && g->k % 8 == 0 && fits(g->p_rows, g->ld_p) && fits(1, a.q_expert);
     hipStream_t s = (hipStream_t)stream;
     return g->act == PF_ACT_SWIGLU ? run<kFwd, 1>(g, a, aligned, s) : run<kFwd, 0>(g, a, aligned, s);
 }
@@ -510,7 +611,8 @@ int pfk_moe_mm_dx(const pfk_moe_mm_args *g, void *stream)
     a.k = g->n;
     a.q_expert = g->ld_q * g->n;
     a.wide = wide(g->out, g->ld_out, 2);
-    const bool aligned = lies16(g->p, g->ld_p) && lies16(g->q, g->ld_q) && g->n % 8 == 0 && g->k % 8 == 0;
+    const bool aligned = lies16(g->p, g->ld_p) && lies16(g->q, g->ld_q) && g->n % 8 == 0 && g->k % 8 == 0 &&
+                         fits(g->slots, g->ld_p) && fits(1, a.q_expert);
     return run<kDx, 0>(g, a, aligned, (hipStream_t)stream);
 }
 
@@ -521,7 +623,8 @@ int pfk_moe_mm_dw(const pfk_moe_mm_args *g, void *stream)
     a.n = g->k;
     a.out_f32 = g->out_f32;
     a.wide = wide(g->out, g->ld_out, g->out_f32 ? 4 : 2);
-    const bool aligned = lies16(g->p, g->ld_p) && lies16(g->q, g->ld_q) && g->n % 8 == 0 && g->k % 8 == 0;
+    const bool aligned = lies16(g->p, g->ld_p) && lies16(g->q, g->ld_q) && g->n % 8 == 0 && g->k % 8 == 0 &&
+                         fits(g->slots, g->ld_p) && fits(g->p_rows, g->ld_q);
     return run<kDw, 0>(g, a, aligned, (hipStream_t)stream);
 }
 
