@@ -6,59 +6,6 @@ namespace {
 
 using namespace pfmoe;
 
-// The tile of workgroup `id`: expert, tile of rows, tile of columns.  The experts' tiles are counted from the offsets,
-// 64 experts at a time over the lanes, in every wave by itself.  Workgroups reach the 8 XCDs in turn, so each XCD is
-// given consecutive tiles (an eighth of those there are), whose operands then meet in its L2; inside an expert eight
-// tiles of rows go side by side over the columns.
-struct Tile {
-    int e, m, n, begin, end;
-};
-
-template <int BM>
-__device__ __forceinline__ bool find_tile(const Args &a, int nt, int id, Tile &t)
-{
-    const int lane = threadIdx.x & (kWave - 1);
-    int total = 0, mine = 0, incl = 0, b = 0, e = 0;
-    for (int base = 0; base < a.experts; base += kWave) {
-        mine = 0;
-        if (base + lane < a.experts) {
-            expert_rows(a.offsets, base + lane, a.slots, b, e);
-            mine = (e - b + BM - 1) / BM * nt;
-        }
-        incl = scan_wave(mine);
-        total += __builtin_amdgcn_readlane(incl, kWave - 1);
-    }
-    const int chunk = (total + kXcds - 1) / kXcds;
-    const int at = (id % kXcds) * chunk + id / kXcds;
-    if (id / kXcds >= chunk || at >= total) return false;
-    int before = 0;
-    for (int base = 0; base < a.experts; base += kWave) {
-        if (a.experts > kWave) {
-            mine = 0;
-            if (base + lane < a.experts) {
-                expert_rows(a.offsets, base + lane, a.slots, b, e);
-                mine = (e - b + BM - 1) / BM * nt;
-            }
-            incl = scan_wave(mine);
-        }
-        const unsigned long long past = __ballot(before + incl > at);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            t.e = base + l;
-            t.begin = __builtin_amdgcn_readlane(b, l);
-            t.end = __builtin_amdgcn_readlane(e, l);
-            const int tiles = __builtin_amdgcn_readlane(mine, l);
-            const int i = at - before - (__builtin_amdgcn_readlane(incl, l) - tiles);
-            const int mt = tiles / nt, group = i / (8 * nt), rows = min(8, mt - group * 8), j = i - group * 8 * nt;
-            t.m = group * 8 + j % rows;
-            t.n = j / rows;
-            return true;
-        }
-        before += __builtin_amdgcn_readlane(incl, kWave - 1);
-    }
-    return false;
-}
-
 // T: f16 or bf16 of the results; FP4: 4-bit operands
 template <typename T, bool FP4, int MODE, int ACT, int BM, int BN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
@@ -259,6 +206,9 @@ template <typename T, bool FP4, int MODE, int ACT, bool ALIGNED>
 int launch_size(const Args &a, hipStream_t stream)
 {
     const long long rows = a.experts > 0 ? a.slots / a.experts : 0;  // an expert's, on average
+    if constexpr (MODE == kFwd) {
+        if (rows <= 48) return launch_rows<T, FP4, ACT, ALIGNED>(a, rows, stream);
+    }
     if (!ALIGNED || rows < 128) return launch<T, FP4, MODE, ACT, 128, 128, 2, 2, ALIGNED>(a, stream);
     if constexpr (ALIGNED) return launch_stream<T, FP4, MODE, ACT>(a, stream);
 }

@@ -1,0 +1,180 @@
+// moe_mm_rows.hip — grouped products with few rows an expert (tokens of sequences that answer): bound by reading the
+// weights, which go straight from memory to the matrix cores' registers, once for up to 16 MT rows.
+#include "moe_tiles.hpp"
+
+namespace pfmoe {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kPieces = 4;   // 16-byte pieces of a row that a lane takes at a time; four lanes share a row
+
+// A workgroup computes 16 columns (and the 16 of the gate) of up to 16 MT rows.  Its waves share k out in blocks of
+// kPieces pieces a lane, the next block's weights on their way while one is multiplied, and add their sums in LDS in a
+// fixed order.  Lane l has row l % 16 of both operands and the k that group g = l / 16 takes: of 16-bit elements the
+// pieces g, 4 + g, ... of a block, of 4-bit ones 4 g to 4 g + 3, whose four scales are then one word.
+template <typename T, bool FP4, int ACT, int MT, bool ALIGNED>
+__global__ __launch_bounds__(kWaves * kWave) void k_mm_rows(const Args a)
+{
+    constexpr int NB = ACT ? 2 : 1;
+    __shared__ float sums[kWaves][NB * MT][256];
+    const int lane = threadIdx.x & (kWave - 1), wave = wave_id(), g = lane >> 4, r = lane & 15;
+    const int nt = (a.n + 15) / 16;
+    Tile t;
+    if (!find_tile<16 * MT>(a, nt, blockIdx.x, t)) return;
+    const int m0 = t.m * 16 * MT, count = t.end - t.begin, blocks32 = a.k / 32;
+
+    const char *x[MT], *w[NB];
+    const unsigned char *xs[FP4 ? MT : 1], *ws[FP4 ? NB : 1];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const long long row = row_of_slot(a, t.begin + min(m0 + i * 16 + r, count - 1));
+        x[i] = a.p + a.ld_p * row;
+        if constexpr (FP4) xs[i] = a.p_scales + blocks32 * row;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const long long row = min(t.n * 16 + r, a.n - 1) + (long long)b * a.n;
+        w[b] = a.q + a.q_expert * t.e + a.ld_q * row;
+        if constexpr (FP4) ws[b] = a.q_scales + blocks32 * ((long long)NB * a.n * t.e + row);
+    }
+
+    const int pieces = FP4 ? blocks32 : ALIGNED ? a.k / 8 : (a.k + 7) / 8;
+    const int blocks = (pieces + 4 * kPieces - 1) / (4 * kPieces);
+    const auto load = [&](const char *row, int b, i32x4 (&v)[kPieces]) {
+#pragma unroll
+        for (int u = 0; u < kPieces; ++u) {
+            const int at = b * 4 * kPieces + (FP4 ? kPieces * g + u : 4 * u + g);
+            if constexpr (ALIGNED) {
+                v[u] = i32x4{0, 0, 0, 0};
+                if (at < pieces) v[u] = *(const i32x4 *)(row + 16LL * at);
+            } else {
+                v[u] = load8_any(row, at * 8, a.k);
+            }
+        }
+    };
+    const auto load_scales = [&](const unsigned char *row, int b) {
+        const int at = b * 4 * kPieces + kPieces * g;
+        unsigned v = 0x7f7f7f7fu;   // 1 where the codes are zeros behind the row's end
+        if (at + 4 <= blocks32) {
+            __builtin_memcpy(&v, row + at, 4);
+        } else {
+            for (int i = 0; at + i < blocks32; ++i) v = (v & ~(0xffu << 8 * i)) | (unsigned)row[at + i] << 8 * i;
+        }
+        return (int)v;
+    };
+
+    f32x4 acc[NB][MT];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[b][i] = f32x4{0, 0, 0, 0};
+    i32x4 wv[2][NB][kPieces], xv[2][MT][kPieces];
+    int wsv[2][NB], xsv[2][MT];
+    const auto fetch = [&](int side, int b) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            load(w[j], b, wv[side][j]);
+            if constexpr (FP4) wsv[side][j] = load_scales(ws[j], b);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            load(x[i], b, xv[side][i]);
+            if constexpr (FP4) xsv[side][i] = load_scales(xs[i], b);
+        }
+    };
+    const auto piece = [&](int side, auto at) {
+        constexpr int u = decltype(at)::value;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                if constexpr (FP4) {
+                    const i32x4 &p = wv[side][j][u], &q = xv[side][i][u];
+                    const i32x8 A = {p[0], p[1], p[2], p[3], 0, 0, 0, 0}, B = {q[0], q[1], q[2], q[3], 0, 0, 0, 0};
+                    acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc[j][i], 4, 4, u, wsv[side][j], u, xsv[side][i]);
+                } else {
+                    acc[j][i] = mfma<T>(wv[side][j][u], xv[side][i][u], acc[j][i]);
+                }
+            }
+    };
+    const auto multiply = [&](int side) {
+        piece(side, std::integral_constant<int, 0>());
+        piece(side, std::integral_constant<int, 1>());
+        piece(side, std::integral_constant<int, 2>());
+        piece(side, std::integral_constant<int, 3>());
+    };
+    int b = wave;
+    if (b < blocks) fetch(0, b);
+    while (b < blocks) {
+        if (b + kWaves < blocks) fetch(1, b + kWaves);
+        multiply(0);
+        b += kWaves;
+        if (b >= blocks) break;
+        if (b + kWaves < blocks) fetch(0, b + kWaves);
+        multiply(1);
+        b += kWaves;
+    }
+
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) *(f32x4 *)&sums[wave][j * MT + i][r * 16 + g * 4] = acc[j][i];
+    __syncthreads();
+    const int row = threadIdx.x / 16, n = t.n * 16 + threadIdx.x % 16;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        float v[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            v[j] = (sums[0][j * MT + i][threadIdx.x] + sums[1][j * MT + i][threadIdx.x]) +
+                   (sums[2][j * MT + i][threadIdx.x] + sums[3][j * MT + i][threadIdx.x]);
+        const int s = m0 + i * 16 + row;
+        if (s >= count || n >= a.n) continue;
+        T *out = (T *)(a.out + a.ld_out * ((long long)t.begin + s)) + n;
+        if constexpr (ACT) {
+            *out = (T)(silu(v[0]) * v[1]);
+            if (a.pre) {
+                T *pre = (T *)(a.pre + a.ld_pre * ((long long)t.begin + s)) + n;
+                pre[0] = (T)v[0];
+                pre[a.n] = (T)v[1];
+            }
+        } else {
+            *out = (T)v[0];
+        }
+    }
+}
+
+template <typename T, bool FP4, int ACT, int MT, bool ALIGNED>
+int launch(const Args &a, hipStream_t stream)
+{
+    const long long tiles = ((long long)a.slots / (16 * MT) + (a.experts < a.slots ? a.experts : a.slots)) * ((a.n + 15) / 16);
+    const long long grid = (tiles + kXcds - 1) / kXcds * kXcds;
+    if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "grouped product: too many tiles");
+    k_mm_rows<T, FP4, ACT, MT, ALIGNED><<<dim3((unsigned)grid), dim3(kWaves * kWave), 0, stream>>>(a);
+    return pfk_internal_launched("k_mm_rows");
+}
+
+}  // namespace
+
+template <typename T, bool FP4, int ACT, bool ALIGNED>
+int launch_rows(const Args &a, long long rows, hipStream_t stream)
+{
+    if (rows <= 4) return launch<T, FP4, ACT, 1, ALIGNED>(a, stream);
+    if (rows <= 16) return launch<T, FP4, ACT, 2, ALIGNED>(a, stream);
+    return launch<T, FP4, ACT, 4, ALIGNED>(a, stream);
+}
+
+template int launch_rows<f16, false, 0, true>(const Args &, long long, hipStream_t);
+template int launch_rows<f16, false, 0, false>(const Args &, long long, hipStream_t);
+template int launch_rows<f16, false, 1, true>(const Args &, long long, hipStream_t);
+template int launch_rows<f16, false, 1, false>(const Args &, long long, hipStream_t);
+template int launch_rows<f16, true, 0, true>(const Args &, long long, hipStream_t);
+template int launch_rows<f16, true, 1, true>(const Args &, long long, hipStream_t);
+template int launch_rows<bf16, false, 0, true>(const Args &, long long, hipStream_t);
+template int launch_rows<bf16, false, 0, false>(const Args &, long long, hipStream_t);
+template int launch_rows<bf16, false, 1, true>(const Args &, long long, hipStream_t);
+template int launch_rows<bf16, false, 1, false>(const Args &, long long, hipStream_t);
+template int launch_rows<bf16, true, 0, true>(const Args &, long long, hipStream_t);
+template int launch_rows<bf16, true, 1, true>(const Args &, long long, hipStream_t);
+
+}  // namespace pfmoe

@@ -42,21 +42,38 @@ def _signatures(L):
     L.pf_moe_route_workspace.restype = ctypes.c_size_t
 
 
+# Type of a buffer, by what its `dtype` is: kept per type object, since these calls are a few microseconds long.
+_KINDS = {}
+
+
+def _kind(dtype):
+    text = str(dtype)
+    if text.endswith("int32") and "uint32" not in text:
+        return "i32"
+    if text.endswith("uint8"):
+        return "u8"
+    if any(w in text for w in ("int", "bool", "complex", "float8")):
+        return text
+    try:
+        return dtype_code(dtype)
+    except ValueError:
+        return text
+
+
 def _buf(obj, kind, name):
     """Raw pointer of `obj`, whose type (where it says one) has to be `kind`: a code of this package, "i32" or "u8"."""
-    got = getattr(obj, "dtype", None)
-    if got is not None:
-        text = str(got)
-        if kind in ("i32", "u8"):
-            ok = text.endswith("int32" if kind == "i32" else "uint8") and ("uint32" not in text)
-        else:
-            ok = not any(w in text for w in ("int", "bool", "complex", "float8")) and dtype_code(got) == kind
-        if not ok:
-            raise TypeError(f"{name} is {text}")
-    device = getattr(obj, "device", None)
-    if getattr(device, "type", "cuda") != "cuda":
-        raise TypeError(f"{name} is on {device}, not on the GPU")
-    return _p(obj)
+    if obj is None or isinstance(obj, int):
+        return obj
+    dtype = getattr(obj, "dtype", None)
+    if dtype is not None:
+        have = _KINDS.get(dtype)
+        if have is None:
+            have = _KINDS[dtype] = _kind(dtype)
+        if have != kind:
+            raise TypeError(f"{name} is {dtype}")
+    if not getattr(obj, "is_cuda", True):
+        raise TypeError(f"{name} is on {obj.device}, not on the GPU")
+    return obj.data_ptr()
 
 
 def _act(act):
