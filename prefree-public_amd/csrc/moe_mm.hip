@@ -51,11 +51,11 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
     S scales;
     int rows = 0;   // kDw: x's rows of the next tile to be loaded
     if constexpr (MODE == kDw) {
-        p.init(a.p + a.ld_p * t.begin, a.ld_p * k, a.ld_p, m0, a.m, k);
-        q.init(a.q, a.ld_q * a.p_rows, a.ld_q, t.n * BN, a.n, k);
+        p.init(a.p + a.ld_p * t.begin, span(a.ld_p, k, a.m), a.ld_p, m0, a.m, k);
+        q.init(a.q, span(a.ld_q, a.p_rows, a.n), a.ld_q, t.n * BN, a.n, k);
         if (k > 0) rows = row_of_slot(a, t.begin + min(Q::lookup(0), k - 1));
     } else {
-        p.init(a.p, a.ld_p * a.p_rows, a.ld_p, slot_row, k, FP4 ? 32 : 8);
+        p.init(a.p, FP4 ? a.ld_p * a.p_rows : span(a.ld_p, a.p_rows, k), a.ld_p, slot_row, k, FP4 ? 32 : 8);
         if constexpr (MODE == kFwd) q.init(a.q + a.q_expert * t.e, a.q_expert, a.ld_q, weight_row, k, FP4 ? 32 : 8);
         else q.init(a.q + a.q_expert * t.e, a.q_expert, a.ld_q, t.n * BN, a.n, k);
     }
@@ -115,6 +115,11 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
             scales.commit(fill + SCALES);
             scales.issue(s + 4, k / 32);
         }
+        if constexpr (!ALIGNED) {   // the same
+            commit(fill);
+#pragma unroll
+            for (int l = 0; l < LOADS; ++l) issue(l, s + 4, nullptr);
+        }
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             const char *from = i + 2 < FM ? here : next;
@@ -129,13 +134,15 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
                 if (j == 0) {
                     x[(i + 2) % 4] = read_x(from, (i + 2) % FM);
                     xs[(i + 2) % 4] = scale_x(from, (i + 2) % FM);
-                } else if (j == 1) {
+                }
+                if (j == 1) {
 #pragma unroll
                     for (int c = i * FN / FM; c < (i + 1) * FN / FM; ++c) {
                         w[1][c] = read_w(next, c);
                         ws[1][c] = scale_w(next, c);
                     }
-                } else if (j == 2) {
+                }
+                if (j == FN / 2 && ALIGNED) {
 #pragma unroll
                     for (int l = i * LOADS / FM; l < (i + 1) * LOADS / FM; ++l) issue(l, s + 3, fill);
                 }
@@ -143,9 +150,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        commit(fill);
         if (FP4 && S::whole(s + 4, k / 32)) wait_and_meet<LOADS + S::kLoads>();   // the scales' loads as well
-        else wait_and_meet<ALIGNED ? LOADS : 0>();
+        else wait_and_meet<ALIGNED ? LOADS : 63>();
         __builtin_amdgcn_sched_barrier(0);
     };
     if (steps > 0) {
@@ -160,7 +166,11 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
             }
         }
         if constexpr (FP4) scales.issue(3, k / 32);
-        wait_and_meet<ALIGNED ? LOADS : 0>();
+        if constexpr (!ALIGNED) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) issue(i, 3, nullptr);
+        }
+        wait_and_meet<ALIGNED ? LOADS : 63>();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             x[i] = read_x(lds[0], i);
@@ -179,6 +189,13 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
             for (int j = 0; j < FN; ++j) {
                 w[0][j] = w[1][j];
                 ws[0][j] = ws[1][j];
+            }
+            if constexpr (FM == 2) {   // read two ahead is a tile ahead
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    x[i] = x[i + 2];
+                    xs[i] = xs[i + 2];
+                }
             }
         }
         // nothing may still be on its way to LDS when the workgroup ends
@@ -205,9 +222,11 @@ int launch(const Args &a, hipStream_t stream)
 template <typename T, bool FP4, int MODE, int ACT, bool ALIGNED>
 int launch_size(const Args &a, hipStream_t stream)
 {
-    const long long rows = a.experts > 0 ? a.slots / a.experts : 0;  // an expert's, on average
+    const long long rows = a.experts > 0 ? a.slots / a.experts : 0;   // an expert's, on average
     if constexpr (MODE == kFwd) {
-        if (rows <= 48) return launch_rows<T, FP4, ACT, ALIGNED>(a, rows, stream);
+        const long long tiles = ((long long)a.slots / 128 + (a.experts < a.slots ? a.experts : a.slots)) * ((a.n * (ACT ? 2 : 1) + 127) / 128);
+        if (rows <= (ALIGNED ? 8 : 32) && (tiles < 512 || (ALIGNED && a.ld_q >= 4096))) return launch_rows<T, FP4, ACT, ALIGNED>(a, rows, stream);
+        if (!ALIGNED && tiles < 256) return launch<T, FP4, MODE, ACT, 64, 64, 2, 2, ALIGNED>(a, stream);
     }
     if (!ALIGNED || rows < 128) return launch<T, FP4, MODE, ACT, 128, 128, 2, 2, ALIGNED>(a, stream);
     if constexpr (ALIGNED) return launch_stream<T, FP4, MODE, ACT>(a, stream);

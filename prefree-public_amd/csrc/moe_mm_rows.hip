@@ -13,7 +13,7 @@ constexpr int kPieces = 4;   // 16-byte pieces of a row that a lane takes at a t
 // fixed order.  Lane l has row l % 16 of both operands and the k that group g = l / 16 takes: of 16-bit elements the
 // pieces g, 4 + g, ... of a block, of 4-bit ones 4 g to 4 g + 3, whose four scales are then one word.
 template <typename T, bool FP4, int ACT, int MT, bool ALIGNED>
-__global__ __launch_bounds__(kWaves * kWave) void k_mm_rows(const Args a)
+__global__ __launch_bounds__(kWaves * kWave, MT == 1 && ALIGNED ? (ACT ? 3 : 4) : 2) void k_mm_rows(const Args a)
 {
     constexpr int NB = ACT ? 2 : 1;
     __shared__ float sums[kWaves][NB * MT][256];
@@ -23,14 +23,9 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mm_rows(const Args a)
     if (!find_tile<16 * MT>(a, nt, blockIdx.x, t)) return;
     const int m0 = t.m * 16 * MT, count = t.end - t.begin, blocks32 = a.k / 32;
 
+    // The weights' addresses need the expert alone: their first loads go out before the rows are looked up.
     const char *x[MT], *w[NB];
     const unsigned char *xs[FP4 ? MT : 1], *ws[FP4 ? NB : 1];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const long long row = row_of_slot(a, t.begin + min(m0 + i * 16 + r, count - 1));
-        x[i] = a.p + a.ld_p * row;
-        if constexpr (FP4) xs[i] = a.p_scales + blocks32 * row;
-    }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const long long row = min(t.n * 16 + r, a.n - 1) + (long long)b * a.n;
@@ -40,7 +35,11 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mm_rows(const Args a)
 
     const int pieces = FP4 ? blocks32 : ALIGNED ? a.k / 8 : (a.k + 7) / 8;
     const int blocks = (pieces + 4 * kPieces - 1) / (4 * kPieces);
-    const auto load = [&](const char *row, int b, i32x4 (&v)[kPieces]) {
+    typedef typename std::conditional<ALIGNED, i32x4, Words>::type Piece;
+    const bool any = a.k > 0;
+    const char *x_end = any ? Words::end_of(a.p, a.ld_p * (a.p_rows - 1LL) + 2LL * a.k) : a.p;
+    const char *w_end = any ? Words::end_of(a.q + a.q_expert * t.e, a.q_expert) : a.q;
+    const auto load = [&](const char *row, int b, Piece (&v)[kPieces], const char *end) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < kPieces; ++u) {
             const int at = b * 4 * kPieces + (FP4 ? kPieces * g + u : 4 * u + g);
@@ -48,9 +47,13 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mm_rows(const Args a)
                 v[u] = i32x4{0, 0, 0, 0};
                 if (at < pieces) v[u] = *(const i32x4 *)(row + 16LL * at);
             } else {
-                v[u] = load8_any(row, at * 8, a.k);
+                v[u].load(row, at * 8, a.k, (b + 1) * 32 * kPieces <= a.k, end);
             }
         }
+    };
+    const auto settled = [](const Piece &v) {
+        if constexpr (ALIGNED) return v;
+        else return v.settle();
     };
     const auto load_scales = [&](const unsigned char *row, int b) {
         const int at = b * 4 * kPieces + kPieces * g;
@@ -68,21 +71,27 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mm_rows(const Args a)
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[b][i] = f32x4{0, 0, 0, 0};
-    i32x4 wv[2][NB][kPieces], xv[2][MT][kPieces];
+    Piece wv[2][NB][kPieces], xv[2][MT][kPieces];
     int wsv[2][NB], xsv[2][MT];
-    const auto fetch = [&](int side, int b) {
+    const auto fetch_w = [&](int side, int b) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            load(w[j], b, wv[side][j]);
+            load(w[j], b, wv[side][j], w_end);
             if constexpr (FP4) wsv[side][j] = load_scales(ws[j], b);
         }
+    };
+    const auto fetch_x = [&](int side, int b) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            load(x[i], b, xv[side][i]);
+            load(x[i], b, xv[side][i], x_end);
             if constexpr (FP4) xsv[side][i] = load_scales(xs[i], b);
         }
     };
-    const auto piece = [&](int side, auto at) {
+    const auto fetch = [&](int side, int b) __attribute__((always_inline)) {
+        fetch_w(side, b);
+        fetch_x(side, b);
+    };
+    const auto piece = [&](int side, auto at) __attribute__((always_inline)) {
         constexpr int u = decltype(at)::value;
 #pragma unroll
         for (int i = 0; i < MT; ++i)
@@ -93,18 +102,25 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mm_rows(const Args a)
                     const i32x8 A = {p[0], p[1], p[2], p[3], 0, 0, 0, 0}, B = {q[0], q[1], q[2], q[3], 0, 0, 0, 0};
                     acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc[j][i], 4, 4, u, wsv[side][j], u, xsv[side][i]);
                 } else {
-                    acc[j][i] = mfma<T>(wv[side][j][u], xv[side][i][u], acc[j][i]);
+                    acc[j][i] = mfma<T>(settled(wv[side][j][u]), settled(xv[side][i][u]), acc[j][i]);
                 }
             }
     };
-    const auto multiply = [&](int side) {
+    const auto multiply = [&](int side) __attribute__((always_inline)) {
         piece(side, std::integral_constant<int, 0>());
         piece(side, std::integral_constant<int, 1>());
         piece(side, std::integral_constant<int, 2>());
         piece(side, std::integral_constant<int, 3>());
     };
     int b = wave;
-    if (b < blocks) fetch(0, b);
+    if (b < blocks) fetch_w(0, b);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const long long row = row_of_slot(a, t.begin + min(m0 + i * 16 + r, count - 1));
+        x[i] = a.p + a.ld_p * row;
+        if constexpr (FP4) xs[i] = a.p_scales + blocks32 * row;
+    }
+    if (b < blocks) fetch_x(0, b);
     while (b < blocks) {
         if (b + kWaves < blocks) fetch(1, b + kWaves);
         multiply(0);
@@ -159,9 +175,8 @@ int launch(const Args &a, hipStream_t stream)
 template <typename T, bool FP4, int ACT, bool ALIGNED>
 int launch_rows(const Args &a, long long rows, hipStream_t stream)
 {
-    if (rows <= 4) return launch<T, FP4, ACT, 1, ALIGNED>(a, stream);
-    if (rows <= 16) return launch<T, FP4, ACT, 2, ALIGNED>(a, stream);
-    return launch<T, FP4, ACT, 4, ALIGNED>(a, stream);
+    if (ALIGNED || rows <= 16) return launch<T, FP4, ACT, 1, ALIGNED>(a, stream);
+    return launch<T, FP4, ACT, ALIGNED ? 1 : 2, ALIGNED>(a, stream);
 }
 
 template int launch_rows<f16, false, 0, true>(const Args &, long long, hipStream_t);

@@ -168,10 +168,10 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
         load_begin = w.begin;
         load_depth = depth(w);
         if constexpr (MODE == kDw) {
-            p.init(a.p + a.ld_p * w.begin, a.ld_p * load_depth, a.ld_p, w.m0, a.m, load_depth);
-            q.init(a.q, a.ld_q * a.p_rows, a.ld_q, w.n * kTile, a.n, load_depth);
+            p.init(a.p + a.ld_p * w.begin, span(a.ld_p, load_depth, a.m), a.ld_p, w.m0, a.m, load_depth);
+            q.init(a.q, span(a.ld_q, a.p_rows, a.n), a.ld_q, w.n * kTile, a.n, load_depth);
         } else {
-            p.from = buffer_of(a.p, a.ld_p * a.p_rows);
+            p.from = buffer_of(a.p, FP4 ? a.ld_p * a.p_rows : span(a.ld_p, a.p_rows, a.k));
             p.k_pieces = a.k / (FP4 ? 32 : 8);
 #pragma unroll
             for (int i = 0; i < P::kLoads; ++i) p.at[i] = (unsigned)row_of(w, side, P::tile_row(i)) * (unsigned)a.ld_p + p.piece * 16;

@@ -44,6 +44,12 @@ __device__ __forceinline__ Buffer buffer_of(const char *base, unsigned long long
     return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)(unsigned)(bytes < kBufferMax ? bytes : kBufferMax), 0x00020000);
 }
 
+// Bytes from the first to the last of `rows` rows of `columns` 16-bit elements, ld bytes apart.
+__device__ __forceinline__ unsigned long long span(long long ld, long long rows, long long columns)
+{
+    return rows > 0 ? (unsigned long long)(ld * (rows - 1) + 2 * columns) : 0;
+}
+
 __device__ __forceinline__ void to_lds16(Buffer from, unsigned lane_offset, unsigned offset, char *dst)
 {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)dst, 16, (int)lane_offset,
@@ -73,22 +79,6 @@ __device__ __forceinline__ f32x4 mfma_fp4(const i32x4 &a, const i32x4 &b, const 
 // Waits for all of this wave's loads.
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// Elements [at, at+8) of a row of `have` elements, zeros behind its end, from any alignment of two bytes.
-__device__ __forceinline__ i32x4 load8_any(const char *row, int at, int have)
-{
-    i32x4 v = {0, 0, 0, 0};
-    if (at + 8 <= have) {
-        v = load16_any(row + 2LL * at);
-    } else {
-        unsigned short h[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (at + i < have) h[i] = *(const unsigned short *)(row + 2LL * (at + i));
-        __builtin_memcpy(&v, h, 16);
-    }
-    return v;
-}
-
 // An operand whose k lies along its rows: a tile is ROWS rows of 64 bytes.  The 16-byte piece c of row r lies at place
 // c ^ ((r >> 1) & 3) of the row, so that eight lanes that read one piece of eight rows touch each bank of 128 bytes once.
 template <int ROWS, int THREADS, bool ALIGNED>
@@ -97,10 +87,10 @@ struct Along {
     static constexpr int kLoads = ROWS * 4 / THREADS;
     Buffer from;                          // ALIGNED: the operand, and this thread's pieces of its rows in the first tile
     unsigned at[ALIGNED ? kLoads : 1];
-    const char *row[ALIGNED ? 1 : kLoads];
+    const char *row[ALIGNED ? 1 : kLoads], *end;
     int piece;          // this thread's piece of its rows (the same for all its loads)
     int k_pieces, k;
-    i32x4 held[ALIGNED ? 1 : kLoads];
+    Words held[ALIGNED ? 1 : kLoads];
 
     static __device__ __forceinline__ int tile_row(int i) { return i * (THREADS / 4) + (int)(threadIdx.x >> 2); }
 
@@ -112,6 +102,7 @@ struct Along {
         k = k_;
         k_pieces = k_ / per_piece;
         if constexpr (ALIGNED) from = buffer_of(base, bytes);
+        else end = Words::end_of(base, bytes);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const long long r = ld * row_of(tile_row(i));
@@ -125,13 +116,13 @@ struct Along {
         if constexpr (ALIGNED)
             to_lds16(from, c < k_pieces ? at[i] : kOutside, t * 64, lds + i * THREADS * 16 + wave_id() * (kWave * 16));
         else
-            held[i] = load8_any(row[i], c * 8, k);
+            held[i].load(row[i], c * 8, k, t * 32 + 32 <= k, end);
     }
     __device__ __forceinline__ void commit(char *lds)
     {
         if constexpr (!ALIGNED) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) *(i32x4 *)(lds + i * THREADS * 16 + threadIdx.x * 16) = held[i];
+            for (int i = 0; i < kLoads; ++i) *(i32x4 *)(lds + i * THREADS * 16 + threadIdx.x * 16) = held[i].settle();
         }
     }
     // 16 rows from r0 (a multiple of 16): lane l has row l % 16, piece l / 16
@@ -154,11 +145,12 @@ struct Across {
     static constexpr int kWaveRows = kWave / kPieces;    // and of one wave
     static_assert(kPieces >= 16 && kPieces <= 32 && kStride % 8 == 0, "see f");
     Buffer from;         // ALIGNED
-    const char *base;
+    const char *base, *end;
     long long ld;
+    bool inside;         // all of the tile's columns are there
     int col[2], cols;    // this thread's first column in loads of even and odd number, and the columns there are
     int k;
-    i32x4 held[ALIGNED ? 1 : kLoads];
+    Words held[ALIGNED ? 1 : kLoads];
 
     static __device__ __forceinline__ int f(int r) { return (r & 3) | ((r >> 1) & 4); }
     static __device__ __forceinline__ int tile_row(int i) { return i * kStride + (int)threadIdx.x / kPieces; }
@@ -167,6 +159,8 @@ struct Across {
     __device__ __forceinline__ void init(const char *base_, unsigned long long bytes, long long ld_, int c0, int cols_, int k_)
     {
         if constexpr (ALIGNED) from = buffer_of(base_, bytes);
+        else end = Words::end_of(base_, bytes);
+        inside = c0 + COLS <= cols_;
         const int place = threadIdx.x % kPieces, r = threadIdx.x / kPieces;
         cols = cols_;
 #pragma unroll
@@ -189,8 +183,7 @@ struct Across {
             to_lds16(from, r < k ? first + 2 * col[i & 1] : kOutside, GATHER ? 0 : (unsigned)(t * 32) * (unsigned)ld,
                      lds + i * THREADS * 16 + wave_id() * (kWave * 16));
         } else {
-            held[i] = i32x4{0, 0, 0, 0};
-            if (r < k && col[i & 1] < cols) held[i] = load8_any(base + ld * at, col[i & 1], cols);
+            held[i].load(base + ld * at, col[i & 1], r < k ? cols : 0, inside && t * 32 + 32 <= k, end);
         }
     }
     // The k of tile t whose row lane l looks up for its wave: load l / kWaveRows, row l % kWaveRows of the wave's.
@@ -203,7 +196,7 @@ struct Across {
     {
         if constexpr (!ALIGNED) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) *(i32x4 *)(lds + i * THREADS * 16 + threadIdx.x * 16) = held[i];
+            for (int i = 0; i < kLoads; ++i) *(i32x4 *)(lds + i * THREADS * 16 + threadIdx.x * 16) = held[i].settle();
         }
     }
     // 16 columns from c0 (a multiple of 16): lane l has column l % 16, rows 8 (l / 16) .. +7
@@ -257,13 +250,13 @@ __device__ __forceinline__ void swap16(unsigned &a, unsigned &b)
 template <int N>
 __device__ __forceinline__ void gather_columns(unsigned (&v)[N][2])
 {
-    static_assert(N == 2 || N == 4, "blocks");
+    static_assert(N == 1 || N == 2 || N == 4, "blocks");
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) swap32(v[i][c], v[i + N / 2][c]);
 #pragma unroll
-        for (int i = 0; i < N; i += 2) swap16(v[i][c], v[i + 1][c]);
+        for (int i = 0; i + 1 < N; i += 2) swap16(v[i][c], v[i + 1][c]);
     }
 }
 
@@ -280,11 +273,12 @@ __device__ __forceinline__ void store_columns(char *row, bool is, int n0, int ha
     }
     gather_columns<N>(h);
     if (!is) return;
+    constexpr int EACH = N == 1 ? 1 : 2;   // blocks a store
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-        T x[8];
-        __builtin_memcpy(x, h[i], 16);
-        store<T, WHOLE, 8>(row, n0 + (lane >> 4) * 4 * N + 4 * i, have, x);
+    for (int i = 0; i < N; i += EACH) {
+        T x[4 * EACH];
+        __builtin_memcpy(x, h[i], 8 * EACH);
+        store<T, WHOLE, 4 * EACH>(row, n0 + (lane >> 4) * 4 * N + 4 * i, have, x);
     }
 }
 
@@ -347,7 +341,6 @@ __device__ __forceinline__ void wait_and_meet()
 template <typename T, int MODE, int ACT, bool WHOLE, int FMV, int FM, int FN, int WM>
 __device__ __forceinline__ void store_blocks(const Args &a, const f32x4 (&acc)[FM][FN], int wm, int wn, long long first, int have, int n0)
 {
-    static_assert(FN == 4, "see store_columns");
     int lane = threadIdx.x & (kWave - 1);
     asm volatile("" : "+v"(lane));   // addresses are formed here, not kept over the loop before
 #pragma unroll
@@ -358,16 +351,20 @@ __device__ __forceinline__ void store_blocks(const Args &a, const f32x4 (&acc)[F
         const bool is = r < have;
         char *out = a.out + a.ld_out * (first + r);
         if constexpr (ACT) {
-            f32x4 h[2];
+            f32x4 h[FN / 2], gate[FN / 2], rest[FN / 2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < FN / 2; ++j) {
+                gate[j] = acc[i][2 * j];
+                rest[j] = acc[i][2 * j + 1];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) h[j][c] = silu(acc[i][2 * j][c]) * acc[i][2 * j + 1][c];
-            store_columns<T, WHOLE, 2>(out, is, n0 + wn * 32, a.n, h, lane);
+                for (int c = 0; c < 4; ++c) h[j][c] = silu(gate[j][c]) * rest[j][c];
+            }
+            const int n = n0 + wn * FN * 8;
+            store_columns<T, WHOLE, FN / 2>(out, is, n, a.n, h, lane);
             if (a.pre) {
                 char *pre = a.pre + a.ld_pre * (first + r);
-                store_columns<T, WHOLE, 2>(pre, is, n0 + wn * 32, a.n, {acc[i][0], acc[i][2]}, lane);
-                store_columns<T, WHOLE, 2>(pre + 2LL * a.n, is, n0 + wn * 32, a.n, {acc[i][1], acc[i][3]}, lane);
+                store_columns<T, WHOLE, FN / 2>(pre, is, n, a.n, gate, lane);
+                store_columns<T, WHOLE, FN / 2>(pre + 2LL * a.n, is, n, a.n, rest, lane);
             }
         } else if (MODE == kDw && a.out_f32) {
 #pragma unroll
@@ -376,7 +373,7 @@ __device__ __forceinline__ void store_blocks(const Args &a, const f32x4 (&acc)[F
                 if (is) store<float, WHOLE, 4>(out, n0 + (wn * FN + j) * 16 + (lane >> 4) * 4, a.n, x);
             }
         } else {
-            store_columns<T, WHOLE, 4>(out, is, n0 + wn * 64, a.n, acc[i], lane);
+            store_columns<T, WHOLE, FN>(out, is, n0 + wn * FN * 16, a.n, acc[i], lane);
         }
     }
 }

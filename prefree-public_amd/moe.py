@@ -62,14 +62,22 @@ def _kind(dtype):
 
 def _buf(obj, kind, name):
     """Raw pointer of `obj`, whose type (where it says one) has to be `kind`: a code of this package, "i32" or "u8"."""
+    try:
+        if _KINDS[obj.dtype] == kind and obj.is_cuda:
+            return obj.data_ptr()
+    except (AttributeError, KeyError):
+        pass
+    return _buf_checked(obj, kind, name)
+
+
+def _buf_checked(obj, kind, name):
     if obj is None or isinstance(obj, int):
         return obj
     dtype = getattr(obj, "dtype", None)
     if dtype is not None:
-        have = _KINDS.get(dtype)
-        if have is None:
-            have = _KINDS[dtype] = _kind(dtype)
-        if have != kind:
+        if dtype not in _KINDS:
+            _KINDS[dtype] = _kind(dtype)
+        if _KINDS[dtype] != kind:
             raise TypeError(f"{name} is {dtype}")
     if not getattr(obj, "is_cuda", True):
         raise TypeError(f"{name} is on {obj.device}, not on the GPU")
