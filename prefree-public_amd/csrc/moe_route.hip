@@ -26,7 +26,12 @@ __device__ __forceinline__ unsigned key_of(float z)
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-struct MaxU { __device__ unsigned operator()(unsigned a, unsigned b) const { return a > b ? a : b; } };
+// and back: NaN for the largest key, -infinity for 0
+__device__ __forceinline__ float logit_of(unsigned key)
+{
+    if (key == 0) return -INFINITY;
+    return __uint_as_float(key & 0x80000000u && key != 0xffffffffu ? key & 0x7fffffffu : key == 0xffffffffu ? 0x7fc00000u : ~key);
+}
 
 struct Route {
     const void *logits;
@@ -35,26 +40,55 @@ struct Route {
     int *choice;
     float *weight;
     int *offsets, *order, *slot;
-    unsigned char *counts;  // [blocks][experts]
+    unsigned char *counts;  // [blocks][counts_ld(experts)]
     int *super;             // [blocks / kSuper][experts], behind the counts
 };
 
-// One wave takes a token at a time: lane l has logits l*PER .. l*PER + PER-1.  The k-th choice is the largest key
-// of the wave; the first lane that has it owns the lowest index.
-template <typename T, int PER>
-__device__ __forceinline__ void choose(const Route &a, int t, unsigned long long *mask)
+// Counts are read four experts a word: their rows are whole words, zeros behind the last expert.
+__device__ __host__ constexpr int counts_ld(int experts) { return (experts + 3) & ~3; }
+
+// The largest of v, and the smallest of i, over the G = 16 or 64 lanes of a token; every lane has it.
+template <int G>
+__device__ __forceinline__ unsigned most_of(unsigned v)
 {
-    const int lane = threadIdx.x & (kWave - 1), local = t & (kBlock - 1);
+    const auto op = [](unsigned a, unsigned b) { return a > b ? a : b; };
+    v = op(v, pfdev::dpp<pfdev::kDppXor1>(v));
+    v = op(v, pfdev::dpp<pfdev::kDppXor2>(v));
+    v = op(v, pfdev::dpp<pfdev::kDppHalfMirror>(v));
+    v = op(v, pfdev::dpp<pfdev::kDppMirror>(v));
+    if constexpr (G == 64) {
+        v = op(v, (unsigned)__builtin_amdgcn_ds_swizzle((int)v, pfdev::swizzle_xor_pattern<16>()));
+        v = op((unsigned)__builtin_amdgcn_readlane((int)v, 0), (unsigned)__builtin_amdgcn_readlane((int)v, 32));
+    }
+    return v;
+}
+template <int G>
+__device__ __forceinline__ int least_of(int i) { return (int)~most_of<G>(~(unsigned)i); }
+template <int G>
+__device__ __forceinline__ float sum_of(float v)
+{
+    if constexpr (G == 64) return pfdev::wave_sum(v);
+    else return pfdev::group_sum<16>(v);
+}
+
+// G lanes take a token: lane l of them has logits l*PER .. l*PER + PER-1 in registers, and each choice is the largest
+// key among them, at its lowest index.  With 16 lanes a token that takes shifts inside a row of lanes only, a block of 64
+// tokens at once (16384 tokens, 8 of 128: 21 us with a wave a token).
+template <typename T, int G, int PER>
+__device__ __forceinline__ void choose(const Route &a, int t, bool is, unsigned long long *mask)
+{
+    const int lane = threadIdx.x % G, local = t & (kBlock - 1);
     const T *row = (const T *)a.logits + a.ld * t;
     float z[PER];
     unsigned key[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int e = lane * PER + i;
-        z[i] = e < a.experts ? as_float(row[e]) : -INFINITY;
-        key[i] = key_of(z[i]);
+        z[i] = is && e < a.experts ? as_float(row[e]) : -INFINITY;
     }
-    float mine = 0, top = 0;   // lane j: the logit of choice j; the row's largest
+#pragma unroll
+    for (int i = 0; i < PER; ++i) key[i] = key_of(z[i]);
+    unsigned mine = 0, top = 0;   // lane j: the key of choice j; the row's largest
     int expert = -1;
     for (int j = 0; j < a.top_k; ++j) {
         unsigned best = 0;
@@ -62,27 +96,24 @@ __device__ __forceinline__ void choose(const Route &a, int t, unsigned long long
 #pragma unroll
         for (int i = PER - 1; i >= 0; --i)
             if (key[i] >= best) { best = key[i]; at = i; }
-        const unsigned most = pfdev::wave_reduce_u32(best, MaxU());
-        if (most == 0) break;
-        const int winner = __builtin_ctzll(__ballot(best == most));
-        const int i = __builtin_amdgcn_readlane(at, winner), e = winner * PER + i;
-        float v = 0;
+        const unsigned most = most_of<G>(best);
+        const int e = least_of<G>(best == most ? lane * PER + at : 0x7fffffff);
+        if (j == 0) top = most;
+        if (most != 0 && lane == j) { mine = most; expert = e; }
 #pragma unroll
-        for (int c = 0; c < PER; ++c)
-            if (c == i) { v = z[c]; if (lane == winner) key[c] = 0; }
-        v = pfdev::readlane(v, winner);
-        if (j == 0) top = v;
-        if (lane == j) { mine = v; expert = e; }
+        for (int i = 0; i < PER; ++i)
+            if (e == lane * PER + i) key[i] = 0;
     }
-    const float part = expert >= 0 ? expf(mine - top) : 0.0f;
+    const float best = logit_of(top);
+    const float part = expert >= 0 ? expf(logit_of(mine) - best) : 0.0f;
     float total = part;
     if (!a.normalise) {
         total = 0;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) total += expf(z[i] - top);
+        for (int i = 0; i < PER; ++i) total += expf(z[i] - best);
     }
-    total = pfdev::wave_sum(total);
-    if (lane < a.top_k) {
+    total = sum_of<G>(total);
+    if (is && lane < a.top_k) {
         const long long at = (long long)t * a.top_k + lane;
         a.choice[at] = expert;
         a.weight[at] = expert >= 0 ? part / total : 0.0f;
@@ -126,24 +157,28 @@ __device__ __forceinline__ int scan_experts(const int *total, int *first, int ex
 }
 
 // Choice and weights; with one block also offsets and order, else the block's counts.
-template <typename T, int PER>
-__global__ __launch_bounds__(512) void k_route(const Route a)
+template <typename T, int G, int PER>
+__global__ __launch_bounds__(1024) void k_route(const Route a)
 {
-    __shared__ unsigned long long mask[PER * 64];
-    __shared__ int total[PER * 64], first[PER * 64], used;
-    const int block = blockIdx.x, wave = threadIdx.x >> 6;
+    __shared__ unsigned long long mask[PER * G];
+    __shared__ int total[PER * G], first[PER * G], used;
+    const int block = blockIdx.x;
     for (int e = threadIdx.x; e < a.experts; e += blockDim.x) mask[e] = 0;
     __syncthreads();
-    for (int t = block * kBlock + wave; t < min(a.tokens, (block + 1) * kBlock); t += 8) choose<T, PER>(a, t, mask);
+    for (int i = threadIdx.x / G; i < kBlock; i += 1024 / G) {   // whole waves: each lane's group has a token or none
+        const int t = block * kBlock + i;
+        if (block * kBlock + (i & ~(kWave / G - 1)) < a.tokens) choose<T, G, PER>(a, t, t < a.tokens, mask);
+    }
     __syncthreads();
     if (a.blocks > 1) {
-        for (int e = threadIdx.x; e < a.experts; e += blockDim.x)
-            a.counts[(long long)block * a.experts + e] = (unsigned char)__popcll(mask[e]);
+        const int ld = counts_ld(a.experts);
+        for (int e = threadIdx.x; e < ld; e += blockDim.x)
+            a.counts[(long long)block * ld + e] = e < a.experts ? (unsigned char)__popcll(mask[e]) : 0;
         return;
     }
     for (int e = threadIdx.x; e < a.experts; e += blockDim.x) total[e] = __popcll(mask[e]);
     __syncthreads();
-    if (wave == 0) {
+    if (threadIdx.x < kWave) {
         const int n = scan_experts(total, first, a.experts);
         if (threadIdx.x == 0) used = n;
     }
@@ -156,16 +191,18 @@ __global__ __launch_bounds__(512) void k_route(const Route a)
 // Sums of kSuper blocks' counts each, for many blocks.
 __global__ __launch_bounds__(256) void k_route_super(const Route a)
 {
-    const int begin = blockIdx.x * kSuper, end = min(a.blocks, begin + kSuper);
+    const int begin = blockIdx.x * kSuper, end = min(a.blocks, begin + kSuper), ld = counts_ld(a.experts);
     for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
         int n = 0;
-        for (int b = begin; b < end; ++b) n += a.counts[(long long)b * a.experts + e];
+        for (int b = begin; b < end; ++b) n += a.counts[(long long)b * ld + e];
         a.super[(long long)blockIdx.x * a.experts + e] = n;
     }
 }
 
-// Offsets and order from the counts: each workgroup sums all blocks' counts, and those before its own.
-__global__ __launch_bounds__(512) void k_route_place(const Route a)
+// Offsets and order from the counts: each workgroup sums all blocks' counts, and those before its own.  A thread sums
+// words of four experts' counts, as two pairs of 16 bits: of at most 1024 blocks with 64 tokens each, shared out over
+// the groups of threads (at least four), that is less than 2^16.
+__global__ __launch_bounds__(1024) void k_route_place(const Route a)
 {
     extern __shared__ unsigned long long lds[];
     unsigned long long *mask = lds;
@@ -178,31 +215,47 @@ __global__ __launch_bounds__(512) void k_route_place(const Route a)
     __syncthreads();
     const int begin = block * kBlock, entries = min(kBlock, a.tokens - begin) * a.top_k;
     for (int i = threadIdx.x; i < entries; i += blockDim.x) {
-        const int e = a.choice[begin * a.top_k + i];
+        const int e = a.choice[(long long)begin * a.top_k + i];
         if (e >= 0) atomicOr(mask + e, 1ull << (i / a.top_k));
     }
-    // thread groups of `wide` experts share the blocks out; integer sums, so their order does not matter
-    const int wide = a.experts < (int)blockDim.x ? a.experts : (int)blockDim.x, groups = blockDim.x / wide;
-    const int group = threadIdx.x / wide;
+    // integer sums, so the order in which they are added does not matter
+    const int words = counts_ld(a.experts) / 4, groups = blockDim.x / words, group = threadIdx.x / words, word = threadIdx.x % words;
+    const int supers = a.super ? a.blocks / kSuper : 0, own = block / kSuper;
     if (group < groups) {
-        const int supers = a.super ? a.blocks / kSuper : 0, own = block / kSuper;
-        for (int e = threadIdx.x % wide; e < a.experts; e += wide) {
-            int all = 0, prior = 0;
-            for (int i = group; i < supers; i += groups) {
-                const int n = a.super[(long long)i * a.experts + e];
-                all += n;
-                if (i < own) prior += n;
-            }
-            for (int b = supers * kSuper + group; b < a.blocks; b += groups) {
-                const int n = a.counts[(long long)b * a.experts + e];
-                all += n;
-                if (b < block) prior += n;
-            }
-            if (own < supers)
-                for (int b = own * kSuper + group; b < block; b += groups) prior += a.counts[(long long)b * a.experts + e];
-            atomicAdd(total + e, all);
-            atomicAdd(before + e, prior);
+        unsigned all[2] = {0, 0}, prior[2] = {0, 0};
+        const unsigned *counts = (const unsigned *)a.counts + word;
+        const auto add = [](unsigned (&to)[2], unsigned v) {
+            to[0] += v & 0x00ff00ffu;
+            to[1] += v >> 8 & 0x00ff00ffu;
+        };
+#pragma unroll 8
+        for (int b = supers * kSuper + group; b < a.blocks; b += groups) {
+            const unsigned v = counts[(long long)b * words];
+            add(all, v);
+            add(prior, b < block ? v : 0);
         }
+        if (own < supers) {
+#pragma unroll 8
+            for (int b = own * kSuper + group; b < block; b += groups) add(prior, counts[(long long)b * words]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = word * 4 + i;
+            if (e >= a.experts) break;
+            atomicAdd(total + e, (int)(all[i & 1] >> (i & 2) * 8 & 0xffff));
+            atomicAdd(before + e, (int)(prior[i & 1] >> (i & 2) * 8 & 0xffff));
+        }
+    }
+    const int shares = blockDim.x / a.experts, share = threadIdx.x / a.experts, e = threadIdx.x % a.experts;
+    if (supers > 0 && share < shares) {
+        int all = 0, prior = 0;
+        for (int i = share; i < supers; i += shares) {
+            const int v = a.super[(long long)i * a.experts + e];
+            all += v;
+            if (i < own) prior += v;
+        }
+        atomicAdd(total + e, all);
+        atomicAdd(before + e, prior);
     }
     __syncthreads();
     if (threadIdx.x < kWave) {
@@ -406,12 +459,12 @@ __global__ __launch_bounds__(256) void k_swiglu_backward(const T *dh, long long 
 template <typename T>
 int route(const Route &a, hipStream_t s)
 {
-    const dim3 grid(a.blocks), block(512);
-    if (a.experts <= 64) k_route<T, 1><<<grid, block, 0, s>>>(a);
-    else if (a.experts <= 128) k_route<T, 2><<<grid, block, 0, s>>>(a);
-    else if (a.experts <= 256) k_route<T, 4><<<grid, block, 0, s>>>(a);
-    else if (a.experts <= 512) k_route<T, 8><<<grid, block, 0, s>>>(a);
-    else k_route<T, 16><<<grid, block, 0, s>>>(a);
+    const dim3 grid(a.blocks), block(1024);
+    if (a.experts <= 64) k_route<T, 16, 4><<<grid, block, 0, s>>>(a);
+    else if (a.experts <= 128) k_route<T, 16, 8><<<grid, block, 0, s>>>(a);
+    else if (a.experts <= 256) k_route<T, 16, 16><<<grid, block, 0, s>>>(a);
+    else if (a.experts <= 512) k_route<T, 64, 8><<<grid, block, 0, s>>>(a);
+    else k_route<T, 64, 16><<<grid, block, 0, s>>>(a);
     if (a.blocks > 1) {
         const size_t lds = (size_t)a.experts * 20 + 8;
         if (a.super) k_route_super<<<dim3(a.blocks / kSuper), dim3(256), 0, s>>>(a);
@@ -491,8 +544,7 @@ int pfk_moe_route(const void *logits, long long ld, int dtype, int tokens, int e
     Route a = {logits, ld, tokens, experts, top_k, normalise, (tokens + kBlock - 1) / kBlock, choice, weight, offsets, order, slot, nullptr, nullptr};
     if (a.blocks < 1) a.blocks = 1;
     if (a.blocks > 1) a.counts = (unsigned char *)counts;
-    if (a.blocks > kDirect)  // the bytes of the counts, rounded up to whole ints, then the sums
-        a.super = counts + ((long long)a.blocks * experts + 3) / 4;
+    if (a.blocks > kDirect) a.super = counts + (long long)a.blocks * (counts_ld(experts) / 4);
     hipStream_t s = (hipStream_t)stream;
     return dtype == PF_F32 ? route<float>(a, s) : dtype == PF_F16 ? route<f16>(a, s) : route<bf16>(a, s);
 }
