@@ -1,4 +1,6 @@
 // moe_mx4.hip — 4-bit blocks on gfx950 (include/prefree_moe.h): blocks of 32 elements e2m1 with one scale byte e8m0.
+#include <type_traits>
+
 #include "moe_common.hpp"
 #include "moe_launch.hpp"
 #include "prefree_moe_kernels.h"
@@ -26,80 +28,105 @@ __device__ __forceinline__ void load8(const T *p, float v[8])
     }
 }
 
-// A lane takes eight elements, four lanes a block of 32.  The block's scale exponent is its largest magnitude's
+constexpr int kUnits = 4;   // pieces a thread takes, a workgroup's width apart: their loads go out together
+
+// A lane takes eight elements at a time, four lanes a block of 32.  The block's scale exponent is its largest magnitude's
 // exponent less 2, so that magnitude / scale lies in [4, 8); dividing by a power of two is exact, and the conversion
 // instruction rounds to nearest even and saturates at 6, with scale 1.
 template <typename T, bool VECTOR>
 __global__ __launch_bounds__(256) void k_quantize(const T *x, long long ld, long long units, int per_row, unsigned *codes,
                                                   unsigned char *scales)
 {
-    const long long unit = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (unit >= units) return;   // units come in fours
-    const long long r = unit / per_row;
-    float v[8];
-    load8<T, VECTOR>(x + ld * r + (unit - r * per_row) * 8, v);
-    unsigned most = 0;
+    const long long first = (long long)blockIdx.x * 256 * kUnits + threadIdx.x;
+    float v[kUnits][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const unsigned b = __float_as_uint(v[i]) & 0x7fffffffu;
-        most = b > most ? b : most;
+    for (int j = 0; j < kUnits; ++j) {
+        const long long unit = first + j * 256;
+        if (unit >= units) break;   // units come in fours
+        const long long r = unit / per_row;
+        load8<T, VECTOR>(x + ld * r + (unit - r * per_row) * 8, v[j]);
     }
-    unsigned o = pfdev::dpp<pfdev::kDppXor1>(most);
-    most = o > most ? o : most;
-    o = pfdev::dpp<pfdev::kDppXor2>(most);
-    most = o > most ? o : most;
-    const int e = (int)(most >> 23);                      // 255: an infinity or a NaN
-    const int scale = e == 255 ? 255 : e < 2 ? 0 : e - 2;  // exponent + 127; 2^-127 at the least
-    unsigned code = 0;
-    if (e != 255) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = ldexpf(v[i], 127 - scale);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[0], v[1], 1.0f, 0);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[2], v[3], 1.0f, 1);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[4], v[5], 1.0f, 2);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[6], v[7], 1.0f, 3);
+    for (int j = 0; j < kUnits; ++j) {
+        const long long unit = first + j * 256;
+        if (unit >= units) break;
+        unsigned most = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const unsigned b = __float_as_uint(v[j][i]) & 0x7fffffffu;
+            most = b > most ? b : most;
+        }
+        unsigned o = pfdev::dpp<pfdev::kDppXor1>(most);
+        most = o > most ? o : most;
+        o = pfdev::dpp<pfdev::kDppXor2>(most);
+        most = o > most ? o : most;
+        const int e = (int)(most >> 23);                      // 255: an infinity or a NaN
+        const int scale = e == 255 ? 255 : e < 2 ? 0 : e - 2;  // exponent + 127; 2^-127 at the least
+        unsigned code = 0;
+        if (e != 255) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j][i] = ldexpf(v[j][i], 127 - scale);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[j][0], v[j][1], 1.0f, 0);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[j][2], v[j][3], 1.0f, 1);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[j][4], v[j][5], 1.0f, 2);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[j][6], v[j][7], 1.0f, 3);
+        }
+        codes[unit] = code;
+        if ((threadIdx.x & 3) == 0) scales[unit >> 2] = (unsigned char)scale;
     }
-    codes[unit] = code;
-    if ((threadIdx.x & 3) == 0) scales[unit >> 2] = (unsigned char)scale;
 }
 
-__device__ __forceinline__ float value_of(unsigned code)
-{
-    const int e = code >> 1 & 3, m = code & 1;
-    const float v = e ? ldexpf(1.0f + 0.5f * m, e - 1) : 0.5f * m;
-    return code & 8 ? -v : v;
-}
-
+// A lane writes 16 bytes at a time, next to its neighbours': four elements in fp32, eight in 16 bits.
 template <typename T, bool VECTOR>
-__global__ __launch_bounds__(256) void k_dequantize(const unsigned *codes, const unsigned char *scales, long long units,
+__global__ __launch_bounds__(256) void k_dequantize(const unsigned char *codes, const unsigned char *scales, long long units,
                                                     int per_row, T *y, long long ld)
 {
-    const long long unit = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (unit >= units) return;
-    const long long r = unit / per_row;
-    const unsigned code = codes[unit];
-    const int scale = scales[unit >> 2];
-    T *out = y + ld * r + (unit - r * per_row) * 8;
-    T v[8];
+    constexpr int EACH = 16 / sizeof(T);
+    typedef typename std::conditional<EACH == 8, unsigned, unsigned short>::type Codes;
+    const long long first = (long long)blockIdx.x * 256 * kUnits + threadIdx.x;
+    unsigned code[kUnits];
+    int scale[kUnits];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        v[i] = (T)(scale == 255 ? __builtin_nanf("") : ldexpf(value_of(code >> 4 * i & 15), scale - 127));
-    if constexpr (VECTOR) {
+    for (int j = 0; j < kUnits; ++j) {
+        const long long unit = first + j * 256;
+        if (unit >= units) break;
+        code[j] = ((const Codes *)codes)[unit];
+        scale[j] = scales[unit / (32 / EACH)];
+    }
 #pragma unroll
-        for (unsigned i = 0; i < sizeof(v) / 16; ++i) {
-            i32x4 b;
-            __builtin_memcpy(&b, (const char *)v + 16 * i, 16);
-            *(i32x4 *)((char *)out + 16 * i) = b;
+    for (int j = 0; j < kUnits; ++j) {
+        const long long unit = first + j * 256;
+        if (unit >= units) break;
+        T v[EACH];
+        const auto put = [&](auto at) {
+            constexpr int i = decltype(at)::value;
+            const auto two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[j], 1.0f, i);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                v[2 * i + c] = (T)(scale[j] == 255 ? __builtin_nanf("") : ldexpf(two[c], scale[j] - 127));
+        };
+        put(std::integral_constant<int, 0>());
+        put(std::integral_constant<int, 1>());
+        if constexpr (EACH == 8) {
+            put(std::integral_constant<int, 2>());
+            put(std::integral_constant<int, 3>());
         }
-    } else {
-        __builtin_memcpy(out, v, sizeof(v));
+        const long long r = unit / per_row;
+        T *out = y + ld * r + (unit - r * per_row) * EACH;
+        if constexpr (VECTOR) {
+            i32x4 b;
+            __builtin_memcpy(&b, v, 16);
+            *(i32x4 *)out = b;
+        } else {
+            __builtin_memcpy(out, v, 16);
+        }
     }
 }
 
 template <typename T>
 int quantize(const void *x, long long ld, int rows, int k, void *codes, void *scales, hipStream_t s)
 {
-    const long long units = (long long)rows * (k / 8), grid = (units + 255) / 256;
+    const long long units = (long long)rows * (k / 8), grid = (units + 256 * kUnits - 1) / (256 * kUnits);
     if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "4-bit blocks: too many elements");
     const bool vector = (uintptr_t)x % 16 == 0 && ld * sizeof(T) % 16 == 0;
     if (vector) k_quantize<T, true><<<dim3((unsigned)grid), dim3(256), 0, s>>>((const T *)x, ld, units, k / 8, (unsigned *)codes, (unsigned char *)scales);
@@ -110,11 +137,13 @@ int quantize(const void *x, long long ld, int rows, int k, void *codes, void *sc
 template <typename T>
 int dequantize(const void *codes, const void *scales, int rows, int k, void *y, long long ld, hipStream_t s)
 {
-    const long long units = (long long)rows * (k / 8), grid = (units + 255) / 256;
+    const int per_row = k / (16 / (int)sizeof(T));
+    const long long units = (long long)rows * per_row, grid = (units + 256 * kUnits - 1) / (256 * kUnits);
     if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "4-bit blocks: too many elements");
     const bool vector = (uintptr_t)y % 16 == 0 && ld * sizeof(T) % 16 == 0;
-    if (vector) k_dequantize<T, true><<<dim3((unsigned)grid), dim3(256), 0, s>>>((const unsigned *)codes, (const unsigned char *)scales, units, k / 8, (T *)y, ld);
-    else k_dequantize<T, false><<<dim3((unsigned)grid), dim3(256), 0, s>>>((const unsigned *)codes, (const unsigned char *)scales, units, k / 8, (T *)y, ld);
+    const unsigned char *c = (const unsigned char *)codes, *e = (const unsigned char *)scales;
+    if (vector) k_dequantize<T, true><<<dim3((unsigned)grid), dim3(256), 0, s>>>(c, e, units, per_row, (T *)y, ld);
+    else k_dequantize<T, false><<<dim3((unsigned)grid), dim3(256), 0, s>>>(c, e, units, per_row, (T *)y, ld);
     return pfk_internal_launched("k_dequantize");
 }
 
