@@ -17,7 +17,6 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
     typedef Scales<BM + BN, THREADS> S;
     constexpr int SCALES = P::kBytes + Q::kBytes;   // where a tile's scales lie
     constexpr int SLOT = SCALES + (FP4 ? S::kBytes : 0);
-    
     __shared__ __align__(1024) char lds[4][SLOT];
 
     const int tid = threadIdx.x, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
@@ -219,17 +218,41 @@ int launch(const Args &a, hipStream_t stream)
     return pfk_internal_launched("k_mm");
 }
 
+// Which kernel takes a product.  Figures in us with the weights not in cache, bf16 unless said otherwise; "rows" are an
+// expert's on average, n counts both halves under SwiGLU.
+//
+// Few rows: k_mm_rows, the weights straight to registers, against the 128 x 128 tiles: 64 experts, 2048 -> 2 x 1024, rows
+// 1: 94 against 115, 8: 104 / 128, 16: 137 / 128; 16 experts, 2048 -> 2048, rows 1: 26 / 37, 8: 32 / 38, 16: 48 / 38.  With
+// many tiles of short rows it loses: 128 experts, 1024 -> 2 x 512, rows 1: 60 / 52, 8: 74 / 56 (1024 tiles of 2 KB rows);
+// 64 experts in 4-bit blocks, rows 1: 40.5 / 40, 8: 48 / 42 (2048 tiles of 1 KB rows).  Operands that do not lie in 16
+// bytes cost the tiles more, and the rows' kernel then takes 32 rows a time: 12 experts, 1111 -> 717, rows 8: 17.5 / 38,
+// 24: 27 / 39, 32: 27 to 37 / 40, 64: 50 / 44.  Above that 64 x 64 tiles fill the chip where 128 x 128 do not: 8 experts,
+// 1000 -> 1111, rows 39: 30 / 43, 60: 31 / 46, 100: 36 / 48; 16 experts, 2047 -> 1023, rows 40: 61 / 78, 80: 65 / 83, 120:
+// 87 / 82.
+//
+// Many: k_mm_stream, 256 x 256 tiles, against 128 x 128.  It wins from a tile a CU on, whatever the rows, since its loads
+// run ahead of everything: dx of 64 experts, 2048 x 2048, rows 1: 91 / 94, 64: 104 / 120, 512: 334 / 409; dw of 16, rows
+// 64: 44 / 50, 512: 101 / 128, of 128, 1024 x 1024, rows 64: 82 / 116, 1: 81 / 76; forward, 32 experts, 2048 -> 2 x 2048,
+// rows 96: 129 / 141, 512: 343 / 412, in 4-bit blocks 51 / 65, 128 / 172.  With fewer tiles, half of them at least, it
+// still wins from 96 rows on, where a tile's half is full (16 experts, 2048 -> 2048, 96: 52 / 56, 256: 66 / 75, but 192:
+// 65 / 56; rows 64: 51 / 39), and loses under that (8 experts, 1024 -> 1024, 256: 26 / 19, 512: 27 / 24; dw 8 of 1024 x
+// 1024, 512: 30 / 21).
 template <typename T, bool FP4, int MODE, int ACT, bool ALIGNED>
 int launch_size(const Args &a, hipStream_t stream)
 {
-    const long long rows = a.experts > 0 ? a.slots / a.experts : 0;   // an expert's, on average
+    const long long rows = a.experts > 0 ? a.slots / a.experts : 0, used = a.experts < a.slots ? a.experts : a.slots;
+    const long long columns = (long long)a.n * (ACT ? 2 : 1);
     if constexpr (MODE == kFwd) {
-        const long long tiles = ((long long)a.slots / 128 + (a.experts < a.slots ? a.experts : a.slots)) * ((a.n * (ACT ? 2 : 1) + 127) / 128);
+        const long long tiles = (a.slots / 128 + used) * ((columns + 127) / 128);
         if (rows <= (ALIGNED ? 8 : 32) && (tiles < 512 || (ALIGNED && a.ld_q >= 4096))) return launch_rows<T, FP4, ACT, ALIGNED>(a, rows, stream);
         if (!ALIGNED && tiles < 256) return launch<T, FP4, MODE, ACT, 64, 64, 2, 2, ALIGNED>(a, stream);
     }
-    if (!ALIGNED || rows < 128) return launch<T, FP4, MODE, ACT, 128, 128, 2, 2, ALIGNED>(a, stream);
-    if constexpr (ALIGNED) return launch_stream<T, FP4, MODE, ACT>(a, stream);
+    if constexpr (ALIGNED) {
+        const long long down = MODE == kDw ? (long long)a.experts * ((a.m + 255) / 256) : a.slots / 256 + used;
+        const long long tiles = down * ((columns + 255) / 256);
+        if (tiles >= (MODE != kDw && rows >= 96 ? 128 : 256)) return launch_stream<T, FP4, MODE, ACT>(a, stream);
+    }
+    return launch<T, FP4, MODE, ACT, 128, 128, 2, 2, ALIGNED>(a, stream);
 }
 
 // whether `bytes` lie within the 32-bit offsets of a buffer descriptor

@@ -13,14 +13,17 @@ constexpr int kMinSteps = 4;    // tiles of k an output tile takes at least: the
 // One output tile.
 struct Work {
     int e, m0, n, begin, count;   // expert, first row, tile of columns; the expert's slots
+    int rows;                     // of the tile, at most
 };
 
 // The tiles of this workgroup, by number.  Each XCD has consecutive tiles, whose operands then meet in its L2: inside an
 // expert eight tiles of rows go side by side over the columns, its last one, with fewer rows, among them.  (With these
 // last ones kept for the end, to even out the workgroups' shares, the weights are read once more: 8192 tokens x 4 of 32
-// experts, 2048 -> 2 x 2048, in 606 us.)
+// experts, 2048 -> 2 x 2048, in 606 us, 545 so.)  Where at most half the workgroups have a tile in the last round, two
+// share each, by rows: 16 experts, 2048 -> 2048, 128 rows each in 53 us and not 63, 512 in 106 and not 120.
 struct Plan {
     const int *before, *begins, *counts;   // in LDS: tiles before each expert, its first slot, its slots
+    const int *ranked;                     // the weights' gradient: the experts by their slots, most first
     int experts, nt, mt;
     int tile0, tiles;                      // this XCD's
     int first, step;
@@ -35,7 +38,11 @@ struct Plan {
     }
     __device__ __forceinline__ bool get(int i, Work &w) const
     {
-        const int q = first + i * step;
+        int q = first + i * step, half = -1;
+        if (i == tiles / step && 2 * (tiles % step) <= step) {
+            q = i * step + first / 2;
+            half = first % 2;
+        }
         if (q >= tiles) return false;
         const int id = tile0 + q;
         w.e = expert_of(id);
@@ -45,22 +52,24 @@ struct Plan {
         const int group = at / (8 * nt), side = min(8, rows - group * 8), j = at - group * 8 * nt;
         w.m0 = (group * 8 + j % side) * kTile;
         w.n = j / side;
-        return true;
+        w.rows = half < 0 ? kTile : kTile / 2;
+        if (half > 0) w.m0 += kTile / 2;
+        return w.m0 < w.count;
     }
-    // the weights' gradient: each XCD takes its share of every expert's tiles, since experts differ in their slots
+    // The weights' gradient: each XCD takes its share of every expert's tiles, since experts differ in their slots; those
+    // with most come first, and the workgroups take them forth and back by turns, so that their sums of slots are alike.
     __device__ __forceinline__ bool get_dw(const Args &a, int i, Work &w) const
     {
-        const int q = first + i * step, each = mt * nt;
+        const int q = (i % 2 ? step - 1 - first : first) + i * step, each = mt * nt;
         const long long at = (long long)q * kXcds + tile0;   // tile0: the XCD
         if (at >= (long long)a.experts * each) return false;
-        w.e = (int)(at / each);
-        const int j = (int)(at - (long long)w.e * each);
+        w.e = __builtin_amdgcn_readfirstlane(ranked[(int)(at / each)]);
+        const int j = (int)(at % each);
         w.m0 = j % mt * kTile;
         w.n = j / mt;
-        int end;
-        expert_rows(a.offsets, w.e, a.slots, w.begin, end);
-        w.begin = __builtin_amdgcn_readfirstlane(w.begin);
-        w.count = __builtin_amdgcn_readfirstlane(end) - w.begin;
+        w.rows = kTile;
+        w.begin = __builtin_amdgcn_readfirstlane(begins[w.e]);
+        w.count = __builtin_amdgcn_readfirstlane(counts[w.e]);
         return true;
     }
 };
@@ -80,7 +89,7 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
     // One array for all: of several the compiler would tell accesses apart, but not the loads to LDS, and wait for those
     // before every read.  Four tiles of k; the experts' tables (Plan); rows of this output tile and of the next, as `rows`
     // has them.
-    constexpr int TABLE = MODE == kDw ? 0 : PF_MOE_MAX_EXPERTS + 1, IDS = MODE == kDw ? 0 : 2 * kTile;
+    constexpr int TABLE = PF_MOE_MAX_EXPERTS + 1, IDS = MODE == kDw ? 0 : 2 * kTile;
     __shared__ __align__(1024) char shared[4 * SLOT + 4 * (3 * TABLE + IDS)];
     const auto lds = [&](int place) { return shared + place * SLOT; };
     const auto table = [&](int i) { return (int *)(shared + 4 * SLOT) + i * TABLE; };
@@ -95,8 +104,28 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
     plan.first = blockIdx.x / kXcds;
     plan.step = gridDim.x / kXcds;
     const int xcd = blockIdx.x % kXcds;
+    plan.before = plan.ranked = table(0);
+    plan.begins = table(1);
+    plan.counts = table(2);
     if constexpr (MODE == kDw) {
         plan.tile0 = xcd;
+        for (int e = tid; e < a.experts; e += kThreads) {
+            int b, f;
+            expert_rows(a.offsets, e, a.slots, b, f);
+            table(1)[e] = b;
+            table(2)[e] = f - b;
+        }
+        __syncthreads();
+        for (int e = tid; e < a.experts; e += kThreads) {
+            const int mine = table(2)[e];
+            int rank = 0;
+            for (int i = 0; i < a.experts; ++i) {
+                const int other = table(2)[i];
+                rank += other > mine || (other == mine && i < e);
+            }
+            table(0)[rank] = e;
+        }
+        __syncthreads();
     } else {
         if (wave == 0) {
             int before = 0;
@@ -114,9 +143,6 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
             if (lane == 0) table(0)[0] = 0;
         }
         __syncthreads();
-        plan.before = table(0);
-        plan.begins = table(1);
-        plan.counts = table(2);
         const int all = __builtin_amdgcn_readfirstlane(table(0)[a.experts]), each = (all + kXcds - 1) / kXcds;
         plan.tile0 = min(xcd * each, all);
         plan.tiles = min(plan.tile0 + each, all) - plan.tile0;
@@ -331,7 +357,7 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
 
     int place = 0;   // of the current tile of k
     for (int i = 0;; ++i) {
-        const int steps = steps_of(now), have = (MODE == kDw ? a.m : now.count) - now.m0;
+        const int steps = steps_of(now), have = min((MODE == kDw ? a.m : now.count) - now.m0, now.rows);
 #pragma unroll
         for (int r = 0; r < FM; ++r)
 #pragma unroll
