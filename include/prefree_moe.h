@@ -7,7 +7,7 @@
  * pointers are device memory, `stream` is a hipStream_t as void*, every function returns a pf_status and
  * pf_last_error() says more.  All calls are asynchronous on `stream`: no allocation, no synchronisation, no host copy
  * of the offsets (each workgroup finds its expert and its rows by searching them), and they may be captured into a
- * graph.  Results do not depend on the order in which workgroups run: no atomics, same bits each time.
+ * graph.  Results do not depend on the order in which workgroups run: no atomics on floating-point numbers, same bits each time.
  *
  * Value types: PF_F16 and PF_BF16 (sums in fp32, each result rounded once, to nearest even), PF_F32 where noted.
  * Leading dimensions (ld*) count elements between rows; 0 stands for the row's length.  Any alignment that the

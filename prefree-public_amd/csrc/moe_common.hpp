@@ -86,9 +86,6 @@ __device__ __forceinline__ i32x4 load16_any(const void *p)
     return w.settle();
 }
 
-// sum over aligned groups of 16 lanes; every lane has it
-__device__ __forceinline__ float sum16(float v) { return pfdev::group_sum<16>(v); }
-
 // Inclusive sum over the lanes of a wave: inside the rows of 16 lanes by shifts, then the rows' last lanes are handed on
 // (row_bcast 15 to the odd rows, row_bcast 31 to the upper half).  Whole wave active.
 __device__ __forceinline__ int scan_wave(int v)

@@ -129,7 +129,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
                 } else {
                     acc[i][j] = mfma<T>(w[0][j], x[i % 4], acc[i][j]);
                 }
-                // a product keeps the matrix core busy for 16 cycles: what else there is to issue goes between them
+                // a product occupies the matrix core for 16 cycles: what else there is to issue goes between them
                 if (j == 0) {
                     x[(i + 2) % 4] = read_x(from, (i + 2) % FM);
                     xs[(i + 2) % 4] = scale_x(from, (i + 2) % FM);
@@ -268,6 +268,13 @@ int run(const pfk_moe_mm_args *g, Args a, bool aligned, hipStream_t stream)
     return aligned ? launch_size<bf16, false, MODE, ACT, true>(a, stream) : launch_size<bf16, false, MODE, ACT, false>(a, stream);
 }
 
+// Operands of 4-bit blocks lie in 16 bytes always; beyond the descriptors' offsets k_mm_rows has 64-bit addresses.
+template <typename T, int ACT>
+int run_mx4(const Args &a, bool fit, hipStream_t stream)
+{
+    return fit ? launch_size<T, true, kFwd, ACT, true>(a, stream) : launch_rows<T, true, ACT, true>(a, 0, stream);
+}
+
 Args common(const pfk_moe_mm_args *g)
 {
     Args a = {};
@@ -305,7 +312,8 @@ int pfk_moe_mm(const pfk_moe_mm_args *g, void *stream)
     const int each = g->act == PF_ACT_SWIGLU ? 2 : 1;
     a.q_expert = g->ld_q * g->n * each;
     a.wide = lies16(g->out, g->ld_out) && (!g->pre || (lies16(g->pre, g->ld_pre) && g->n % 8 == 0));
-    const bool aligned = lies16(g->p, g->ld_p) && lies16(g->q, g->ld_q) && g->k % 8 == 0 && fits(g->p_rows, g->ld_p) && fits(1, a.q_expert);
+    const bool aligned = lies16(g->p, g->ld_p) && lies16(g->q, g->ld_q) && g->k % 8 == 0 && fits(g->p_rows, g->ld_p) && fits(1, a.q_expert) &&
+                         fits(g->slots, 4);
     hipStream_t s = (hipStream_t)stream;
     return g->act == PF_ACT_SWIGLU ? run<kFwd, 1>(g, a, aligned, s) : run<kFwd, 0>(g, a, aligned, s);
 }
@@ -343,10 +351,10 @@ int pfk_moe_mm_mx4(const pfk_moe_mm_args *g, void *stream)
     a.q_scales = (const unsigned char *)g->q_scales;
     a.q_expert = g->ld_q * g->n * (g->act == PF_ACT_SWIGLU ? 2 : 1);
     a.wide = lies16(g->out, g->ld_out);
+    const bool fit = fits(g->p_rows, g->ld_p) && fits(1, a.q_expert) && fits(g->slots, 4);
     hipStream_t s = (hipStream_t)stream;
-    if (g->act == PF_ACT_SWIGLU)
-        return g->dtype == PF_F16 ? launch_size<f16, true, kFwd, 1, true>(a, s) : launch_size<bf16, true, kFwd, 1, true>(a, s);
-    return g->dtype == PF_F16 ? launch_size<f16, true, kFwd, 0, true>(a, s) : launch_size<bf16, true, kFwd, 0, true>(a, s);
+    if (g->act == PF_ACT_SWIGLU) return g->dtype == PF_F16 ? run_mx4<f16, 1>(a, fit, s) : run_mx4<bf16, 1>(a, fit, s);
+    return g->dtype == PF_F16 ? run_mx4<f16, 0>(a, fit, s) : run_mx4<bf16, 0>(a, fit, s);
 }
 
 }  // extern "C"

@@ -128,17 +128,18 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
         __syncthreads();
     } else {
         if (wave == 0) {
-            int before = 0;
+            int before = 0;   // held at kMost where offsets that decrease give the experts more slots than there are
+            constexpr int kMost = 1 << 30;
             for (int base = 0; base < a.experts; base += kWave) {
                 int b = 0, e = 0;
                 if (base + lane < a.experts) expert_rows(a.offsets, base + lane, a.slots, b, e);
                 const int sum = scan_wave((e - b + kTile - 1) / kTile * plan.nt);
                 if (base + lane < a.experts) {
-                    table(0)[base + lane + 1] = before + sum;
+                    table(0)[base + lane + 1] = min(before + sum, kMost);
                     table(1)[base + lane] = b;
                     table(2)[base + lane] = e - b;
                 }
-                before += __builtin_amdgcn_readlane(sum, kWave - 1);
+                before = min(before + __builtin_amdgcn_readlane(sum, kWave - 1), kMost);
             }
             if (lane == 0) table(0)[0] = 0;
         }
@@ -284,7 +285,7 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
             for (int j = 0; j < FN; ++j) {
                 if constexpr (FP4) acc[i][j] = mfma_fp4(w[0][j], x[i % 4], acc[i][j], ws[0][j], xs[i % 4]);
                 else acc[i][j] = mfma<T>(w[0][j], x[i % 4], acc[i][j]);
-                // a product keeps the matrix core busy for 16 cycles: what else there is to issue goes between them
+                // a product occupies the matrix core for 16 cycles: what else there is to issue goes between them
                 if (j == 0) {
                     x[(i + 2) % 4] = read_x(from, (i + 2) % FMV);
                     xs[(i + 2) % 4] = scale_x(from, (i + 2) % FMV);

@@ -23,7 +23,7 @@ struct Args {
     long long ld_p, ld_q, q_expert, ld_out, ld_pre;
     const int *rows, *offsets;
     int row_div, p_rows, experts, slots;
-    unsigned div_mul;    // floor(v / row_div) = (v * div_mul >> 32) >> div_shift for 0 <= v < 2^30
+    unsigned div_mul;    // floor(v / row_div) = (v * div_mul >> 32) >> div_shift for 0 <= v < 2^31
     int div_shift;
     int m, n, k;         // m only for kDw; n: results per row (the gate's half under SwiGLU)
     int out_f32, wide;   // wide: the output's rows take stores of 16 bytes
