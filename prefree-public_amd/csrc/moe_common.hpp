@@ -31,59 +31,62 @@ template <> struct vec<bf16> { typedef bf16x4 x4; typedef bf16x8 x8; };
 
 // Eight 16-bit elements on their way from rows of any alignment: as the whole words that hold them, which take half the
 // time of the hardware's own unaligned loads (rows of 2222 bytes out of the L2: 7.4 against 3.7 TB/s).  A word may hold
-// an element that lies outside of what is asked for, but never only such.  settle() shifts them into place and clears
-// what lies behind the row's end; it alone waits, and loading has no branch in which anything but loads happens, so that
-// several of them can be under way.
+// an element that lies outside of what is asked for, but never only such, so it lies in the operand's memory.  shifted()
+// puts them into place and kept() clears what lies behind the row's end; only these wait, and loading has no branch in
+// which anything but loads happens, so that several of them can be under way.
 struct Words {
     i32x4 v;
-    int last, valid;
-    bool odd;
+    int last;
 
-    // elements [at, at + 8) of a row of `have`; `whole`, the same for all lanes: the row has them; end: the operand's last word
-    __device__ __forceinline__ void load(const char *row, int at, int have, bool whole, const char *end)
+    // Said to be global memory: of pointers made of numbers the compiler does not know it, and its flat loads have to be
+    // waited for wherever an LDS read is (gradient of 32764 slots x 2049 from 1023, 32 experts: 681 us, 535 so).
+    typedef int words __attribute__((ext_vector_type(4), aligned(4)));
+    typedef const __attribute__((address_space(1))) words *Four;
+    typedef const __attribute__((address_space(1))) int *One;
+
+    static __device__ __forceinline__ uintptr_t word_of(uintptr_t p) { return p & ~(uintptr_t)3; }
+    static __device__ __forceinline__ unsigned shift_of(uintptr_t p) { return (unsigned)p & 2; }
+
+    // the words from p, and the one at `more`: p + 16, or anything where the shift is 0
+    __device__ __forceinline__ void load(uintptr_t p, uintptr_t more)
     {
-        typedef int words __attribute__((ext_vector_type(4), aligned(4)));
-        const char *p = row + 2LL * at;
-        odd = (uintptr_t)p & 2;
-        valid = have - at;
-        p = (const char *)((uintptr_t)p & ~(uintptr_t)3);
-        if (whole) {
-            v = *(const words *)p;
-            last = *(const int *)(odd ? p + 16 : p);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = *(const int *)(p + 4 * i < end ? p + 4 * i : end);
-            last = *(const int *)(p + 16 < end ? p + 16 : end);
-        }
+        v = *(Four)p;
+        last = *(One)more;
     }
-    __device__ __forceinline__ i32x4 settle() const
+    // those of them before `end`, the operand's last word
+    __device__ __forceinline__ void load_until(uintptr_t p, uintptr_t end)
     {
-        i32x4 r = v;
-        if (odd) {
-            r[0] = __builtin_amdgcn_alignbyte(v[1], v[0], 2);
-            r[1] = __builtin_amdgcn_alignbyte(v[2], v[1], 2);
-            r[2] = __builtin_amdgcn_alignbyte(v[3], v[2], 2);
-            r[3] = __builtin_amdgcn_alignbyte(last, v[3], 2);
-        }
-        if (valid < 8) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = 2 * i + 1 < valid ? r[i] : 2 * i < valid ? r[i] & 0xffff : 0;
-        }
+        for (int i = 0; i < 4; ++i) v[i] = *(One)(p + 4 * i < end ? p + 4 * i : end);
+        last = *(One)(p + 16 < end ? p + 16 : end);
+    }
+    __device__ __forceinline__ i32x4 shifted(unsigned shift) const
+    {
+        return i32x4{(int)__builtin_amdgcn_alignbyte(v[1], v[0], shift), (int)__builtin_amdgcn_alignbyte(v[2], v[1], shift),
+                     (int)__builtin_amdgcn_alignbyte(v[3], v[2], shift), (int)__builtin_amdgcn_alignbyte(last, v[3], shift)};
+    }
+    // the first `valid` of eight elements, zeros behind them
+    static __device__ __forceinline__ i32x4 kept(i32x4 r, int valid)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = 2 * i + 1 < valid ? r[i] : 2 * i < valid ? r[i] & 0xffff : 0;
         return r;
     }
     // the last word of an operand of `bytes` > 0
-    static __device__ __forceinline__ const char *end_of(const char *base, unsigned long long bytes)
+    static __device__ __forceinline__ uintptr_t end_of(const char *base, unsigned long long bytes)
     {
-        return (const char *)(((uintptr_t)base + bytes - 2) & ~(uintptr_t)3);
+        return word_of((uintptr_t)base + bytes - 2);
     }
 };
 
 // 16 bytes that are all there, from an address that is a multiple of two.
 __device__ __forceinline__ i32x4 load16_any(const void *p)
 {
+    const uintptr_t at = Words::word_of((uintptr_t)p);
+    const unsigned shift = Words::shift_of((uintptr_t)p);
     Words w;
-    w.load((const char *)p, 0, 8, true, nullptr);
-    return w.settle();
+    w.load(at, shift ? at + 16 : at);
+    return w.shifted(shift);
 }
 
 // Inclusive sum over the lanes of a wave: inside the rows of 16 lanes by shifts, then the rows' last lanes are handed on

@@ -6,6 +6,10 @@ namespace {
 
 using namespace pfmoe;
 
+// A workgroup a tile, two (128 x 128) or five (64 x 64) of them on a CU: for products too small for k_mm_stream, and, by
+// way of registers, for operands of any alignment.  8192 rows of 16 experts, 2048 -> 2048, in 114 us against its 106;
+// 311 tokens x 2 of 12, 1111 -> 717, in 23 us: there a step of k takes the CU's address units longest, which handle rows
+// that cross lines twice.
 // T: f16 or bf16 of the results; FP4: 4-bit operands
 template <typename T, bool FP4, int MODE, int ACT, int BM, int BN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
@@ -69,25 +73,40 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
     }
     constexpr int LOADS = P::kLoads + Q::kLoads;   // of a tile, by each thread
     int now = 0;
-    // load i of tile s
-    const auto issue = [&](int i, int s, char *to) {
-        if (i == 0) {
-            if constexpr (MODE == kDw) {   // looked up before the loads, so that waiting for it does not wait for them
-                now = rows;
-                rows = row_of_slot(a, t.begin + min(Q::lookup(s + 1), k - 1));
-            }
-        }
-        if (i < P::kLoads) {
-            if constexpr (MODE == kDw) p.template issue<false>(i, s, to, 0);
-            else p.issue(i, s, to);
-        } else {
-            if constexpr (MODE == kFwd) q.issue(i - P::kLoads, s, to + P::kBytes);
-            else q.template issue<MODE == kDw>(i - P::kLoads, s, to + P::kBytes, now);
+    const auto look_up = [&](int s) {   // before the loads, so that waiting for it does not wait for them
+        if constexpr (MODE == kDw) {
+            now = rows;
+            rows = row_of_slot(a, t.begin + min(Q::lookup(s + 1), k - 1));
         }
     };
-    const auto commit = [&](char *to) {   // what came by way of registers
-        p.commit(to);
-        q.commit(to + P::kBytes);
+    // load i of tile s, straight to LDS
+    const auto issue = [&](int i, int s, char *to) {
+        if constexpr (ALIGNED) {
+            if (i == 0) look_up(s);
+            if (i < P::kLoads) {
+                if constexpr (MODE == kDw) p.template issue<false>(i, s, to, 0);
+                else p.issue(i, s, to);
+            } else {
+                if constexpr (MODE == kFwd) q.issue(i - P::kLoads, s, to + P::kBytes);
+                else q.template issue<MODE == kDw>(i - P::kLoads, s, to + P::kBytes, now);
+            }
+        }
+    };
+    // tile s by way of registers, and from there to LDS
+    const auto fetch = [&](int s) {
+        if constexpr (!ALIGNED) {
+            look_up(s);
+            if constexpr (MODE == kDw) p.template fetch<false>(s, 0);
+            else p.fetch(s);
+            if constexpr (MODE == kFwd) q.fetch(s);
+            else q.template fetch<MODE == kDw>(s, now);
+        }
+    };
+    const auto commit = [&](char *to, int s) {
+        if constexpr (!ALIGNED) {
+            p.commit(to, s);
+            q.commit(to + P::kBytes, s);
+        }
     };
 
     // A wave's rows are every WM-th block of 16 of the tile, its columns FN blocks side by side.
@@ -115,9 +134,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
             scales.issue(s + 4, k / 32);
         }
         if constexpr (!ALIGNED) {   // the same
-            commit(fill);
-#pragma unroll
-            for (int l = 0; l < LOADS; ++l) issue(l, s + 4, nullptr);
+            commit(fill, s + 3);
+            fetch(s + 4);
         }
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
@@ -158,17 +176,15 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
         for (int s = 0; s < 3; ++s) {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) issue(i, s, lds[s]);
-            commit(lds[s]);
+            fetch(s);
+            commit(lds[s], s);
             if constexpr (FP4) {
                 scales.issue(s, k / 32);
                 scales.commit(lds[s] + SCALES);
             }
         }
         if constexpr (FP4) scales.issue(3, k / 32);
-        if constexpr (!ALIGNED) {
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i) issue(i, 3, nullptr);
-        }
+        fetch(3);
         wait_and_meet<ALIGNED ? LOADS : 63>();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -224,11 +240,7 @@ int launch(const Args &a, hipStream_t stream)
 // Few rows: k_mm_rows, the weights straight to registers, against the 128 x 128 tiles: 64 experts, 2048 -> 2 x 1024, rows
 // 1: 94 against 115, 8: 104 / 128, 16: 137 / 128; 16 experts, 2048 -> 2048, rows 1: 26 / 37, 8: 32 / 38, 16: 48 / 38.  With
 // many tiles of short rows it loses: 128 experts, 1024 -> 2 x 512, rows 1: 60 / 52, 8: 74 / 56 (1024 tiles of 2 KB rows);
-// 64 experts in 4-bit blocks, rows 1: 40.5 / 40, 8: 48 / 42 (2048 tiles of 1 KB rows).  Operands that do not lie in 16
-// bytes cost the tiles more, and the rows' kernel then takes 32 rows a time: 12 experts, 1111 -> 717, rows 8: 17.5 / 38,
-// 24: 27 / 39, 32: 27 to 37 / 40, 64: 50 / 44.  Above that 64 x 64 tiles fill the chip where 128 x 128 do not: 8 experts,
-// 1000 -> 1111, rows 39: 30 / 43, 60: 31 / 46, 100: 36 / 48; 16 experts, 2047 -> 1023, rows 40: 61 / 78, 80: 65 / 83, 120:
-// 87 / 82.
+// 64 experts in 4-bit blocks, rows 1: 40.5 / 40, 8: 48 / 42 (2048 tiles of 1 KB rows).
 //
 // Many: k_mm_stream, 256 x 256 tiles, against 128 x 128.  It wins from a tile a CU on, whatever the rows, since its loads
 // run ahead of everything: dx of 64 experts, 2048 x 2048, rows 1: 91 / 94, 64: 104 / 120, 512: 334 / 409; dw of 16, rows
@@ -237,20 +249,32 @@ int launch(const Args &a, hipStream_t stream)
 // still wins from 96 rows on, where a tile's half is full (16 experts, 2048 -> 2048, 96: 52 / 56, 256: 66 / 75, but 192:
 // 65 / 56; rows 64: 51 / 39), and loses under that (8 experts, 1024 -> 1024, 256: 26 / 19, 512: 27 / 24; dw 8 of 1024 x
 // 1024, 512: 30 / 21).
+//
+// Operands that do not lie in 16 bytes are bound by their loads' addresses, a row of which crosses lines.  Forward, the
+// rows' kernel against 64 x 64, 128 x 128 and 256 x 256 tiles: 12 experts, 1111 -> 717, rows 8: 14 / 28 / 35 / 56, 32: 25 /
+// 29 / 39 / 62, 64: 39 / 29 / 42 / 69, 200: 97 / 43 / 47 / 95; 16 experts, 2047 -> 2047, 8: 53 / 54 / 61 / 96, 16: 71 / 56 /
+// 63 / 98, 48: 148 / 96 / 69 / 107, 200: 513 / 198 / 170 / 147; 64 experts, 1025 -> 513, 8: 35 / 38 / 52 / 57, 48: 102 / 53 /
+// 70 / 66, 200: 346 / 121 / 122 / 98; 32 experts, 2047 -> 2 x 1023, 8: 85 / 98 / 99 / 107, 64: 318 / 190 / 138 / 125.
+// Gradients with 128 x 128 against 256 x 256: 32764 slots of 32 experts, 1023 x 2049, dx 522 / 450, dw 628 / 546; 8000 of
+// 16, 2047 x 2047, dx 253 / 270, dw 377 / 288; 2000 of 16, 1023 x 1025, dx 44 / 72, dw 90 / 91.
 template <typename T, bool FP4, int MODE, int ACT, bool ALIGNED>
 int launch_size(const Args &a, hipStream_t stream)
 {
     const long long rows = a.experts > 0 ? a.slots / a.experts : 0, used = a.experts < a.slots ? a.experts : a.slots;
-    const long long columns = (long long)a.n * (ACT ? 2 : 1);
+    const auto tiles = [&](long long side) {   // at most, of side x side results
+        return (MODE == kDw ? a.experts * ((a.m + side - 1) / side) : a.slots / side + used) * ((a.n * (ACT ? 2LL : 1LL) + side - 1) / side);
+    };
     if constexpr (MODE == kFwd) {
-        const long long tiles = (a.slots / 128 + used) * ((columns + 127) / 128);
-        if (rows <= (ALIGNED ? 8 : 32) && (tiles < 512 || (ALIGNED && a.ld_q >= 4096))) return launch_rows<T, FP4, ACT, ALIGNED>(a, rows, stream);
-        if (!ALIGNED && tiles < 256) return launch<T, FP4, MODE, ACT, 64, 64, 2, 2, ALIGNED>(a, stream);
+        if (rows <= 8 && (tiles(128) < 512 || a.ld_q >= 4000)) return launch_rows<T, FP4, ACT, ALIGNED>(a, stream);
+        if (!ALIGNED && rows <= 32 && tiles(128) < 128) return launch_rows<T, FP4, ACT, ALIGNED>(a, stream);
     }
     if constexpr (ALIGNED) {
-        const long long down = MODE == kDw ? (long long)a.experts * ((a.m + 255) / 256) : a.slots / 256 + used;
-        const long long tiles = down * ((columns + 255) / 256);
-        if (tiles >= (MODE != kDw && rows >= 96 ? 128 : 256)) return launch_stream<T, FP4, MODE, ACT>(a, stream);
+        if (tiles(256) >= (MODE != kDw && rows >= 96 ? 128 : 256)) return launch_stream<T, FP4, MODE, ACT>(a, stream);
+    } else {
+        if constexpr (MODE == kFwd)
+            if (tiles(64) < 800) return launch<T, FP4, MODE, ACT, 64, 64, 2, 2, ALIGNED>(a, stream);
+        if (MODE == kDx ? tiles(256) >= 512 && rows >= 256 : tiles(256) >= (MODE == kDw ? 256 : 192))
+            return launch<T, FP4, MODE, ACT, 256, 256, 2, 4, ALIGNED>(a, stream);
     }
     return launch<T, FP4, MODE, ACT, 128, 128, 2, 2, ALIGNED>(a, stream);
 }
@@ -272,7 +296,7 @@ int run(const pfk_moe_mm_args *g, Args a, bool aligned, hipStream_t stream)
 template <typename T, int ACT>
 int run_mx4(const Args &a, bool fit, hipStream_t stream)
 {
-    return fit ? launch_size<T, true, kFwd, ACT, true>(a, stream) : launch_rows<T, true, ACT, true>(a, 0, stream);
+    return fit ? launch_size<T, true, kFwd, ACT, true>(a, stream) : launch_rows<T, true, ACT, true>(a, stream);
 }
 
 Args common(const pfk_moe_mm_args *g)

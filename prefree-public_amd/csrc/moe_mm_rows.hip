@@ -1,5 +1,5 @@
 // moe_mm_rows.hip — grouped products with few rows an expert (tokens of sequences that answer): bound by reading the
-// weights, which go straight from memory to the matrix cores' registers, once for up to 16 MT rows.
+// weights, which go straight from memory to the matrix cores' registers, once for up to 16 rows.
 #include "moe_tiles.hpp"
 
 namespace pfmoe {
@@ -8,7 +8,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kPieces = 4;   // 16-byte pieces of a row that a lane takes at a time; four lanes share a row
 
-// A workgroup computes 16 columns (and the 16 of the gate) of up to 16 MT rows.  Its waves share k out in blocks of
+// A workgroup computes 16 columns (and the 16 of the gate) of up to 16 rows.  Its waves share k out in blocks of
 // kPieces pieces a lane, the next block's weights on their way while one is multiplied, and add their sums in LDS in a
 // fixed order.  Lane l has row l % 16 of both operands and the k that group g = l / 16 takes: of 16-bit elements the
 // pieces g, 4 + g, ... of a block, of 4-bit ones 4 g to 4 g + 3, whose four scales are then one word.
@@ -16,20 +16,20 @@ constexpr int kPieces = 4;   // 16-byte pieces of a row that a lane takes at a t
 // Measured with the weights not in cache: one token, 8 of 64 experts, 2048 -> 2 x 1024, 67 MB, in 13.6 us; 67 tokens, 537
 // MB in 109 us, 4.9 TB/s, a large copy's rate.  With the gate a wave has twice the loads on their way, and two waves a SIMD
 // with their registers do better than three with a spill (118 us); without it two to four are alike.
-template <typename T, bool FP4, int ACT, int MT, bool ALIGNED>
-__global__ __launch_bounds__(kWaves * kWave, MT == 1 && ALIGNED && !ACT ? 4 : 2) void k_mm_rows(const Args a)
+template <typename T, bool FP4, int ACT, bool ALIGNED>
+__global__ __launch_bounds__(kWaves * kWave, ALIGNED && !ACT ? 4 : 2) void k_mm_rows(const Args a)
 {
     constexpr int NB = ACT ? 2 : 1;
-    __shared__ float sums[kWaves][NB * MT][256];
+    __shared__ float sums[kWaves][NB][256];
     const int lane = threadIdx.x & (kWave - 1), wave = wave_id(), g = lane >> 4, r = lane & 15;
     const int nt = (a.n + 15) / 16;
     Tile t;
-    if (!find_tile<16 * MT>(a, nt, blockIdx.x, t)) return;
-    const int m0 = t.m * 16 * MT, count = t.end - t.begin, blocks32 = a.k / 32;
+    if (!find_tile<16>(a, nt, blockIdx.x, t)) return;
+    const int m0 = t.m * 16, count = t.end - t.begin, blocks32 = a.k / 32;
 
     // The weights' addresses need the expert alone: their first loads go out before the rows are looked up.
-    const char *x[MT], *w[NB];
-    const unsigned char *xs[FP4 ? MT : 1], *ws[FP4 ? NB : 1];
+    const char *x, *w[NB];
+    const unsigned char *xs, *ws[FP4 ? NB : 1];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const long long row = min(t.n * 16 + r, a.n - 1) + (long long)b * a.n;
@@ -41,9 +41,10 @@ __global__ __launch_bounds__(kWaves * kWave, MT == 1 && ALIGNED && !ACT ? 4 : 2)
     const int blocks = (pieces + 4 * kPieces - 1) / (4 * kPieces);
     typedef typename std::conditional<ALIGNED, i32x4, Words>::type Piece;
     const bool any = a.k > 0;
-    const char *x_end = any ? Words::end_of(a.p, a.ld_p * (a.p_rows - 1LL) + 2LL * a.k) : a.p;
-    const char *w_end = any ? Words::end_of(a.q + a.q_expert * t.e, a.q_expert) : a.q;
-    const auto load = [&](const char *row, int b, Piece (&v)[kPieces], const char *end) __attribute__((always_inline)) {
+    const uintptr_t x_end = any ? Words::end_of(a.p, a.ld_p * (a.p_rows - 1LL) + 2LL * a.k) : 0;
+    const uintptr_t w_end = any ? Words::end_of(a.q + a.q_expert * t.e, a.q_expert) : 0;
+    const auto whole = [&](int b) { return (b + 1) * 32 * kPieces <= a.k; };   // whether rows have all of block b
+    const auto load = [&](const char *row, int b, Piece (&v)[kPieces], uintptr_t end) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < kPieces; ++u) {
             const int at = b * 4 * kPieces + (FP4 ? kPieces * g + u : 4 * u + g);
@@ -51,13 +52,19 @@ __global__ __launch_bounds__(kWaves * kWave, MT == 1 && ALIGNED && !ACT ? 4 : 2)
                 v[u] = i32x4{0, 0, 0, 0};
                 if (at < pieces) v[u] = *(const i32x4 *)(row + 16LL * at);
             } else {
-                v[u].load(row, at * 8, a.k, (b + 1) * 32 * kPieces <= a.k, end);
+                const uintptr_t p = Words::word_of((uintptr_t)row + 16LL * at);
+                if (whole(b)) v[u].load(p, p + 8 * Words::shift_of((uintptr_t)row));
+                else v[u].load_until(p, end);
             }
         }
     };
-    const auto settled = [](const Piece &v) {
-        if constexpr (ALIGNED) return v;
-        else return v.settle();
+    const auto settled = [&](const Piece &v, const char *row, int b, int u) {
+        if constexpr (ALIGNED) {
+            return v;
+        } else {
+            const i32x4 r = v.shifted(Words::shift_of((uintptr_t)row));
+            return whole(b) ? r : Words::kept(r, a.k - (b * 4 * kPieces + 4 * u + g) * 8);
+        }
     };
     const auto load_scales = [&](const unsigned char *row, int b) {
         const int at = b * 4 * kPieces + kPieces * g;
@@ -70,13 +77,11 @@ __global__ __launch_bounds__(kWaves * kWave, MT == 1 && ALIGNED && !ACT ? 4 : 2)
         return (int)v;
     };
 
-    f32x4 acc[NB][MT];
+    f32x4 acc[NB];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[b][i] = f32x4{0, 0, 0, 0};
-    Piece wv[2][NB][kPieces], xv[2][MT][kPieces];
-    int wsv[2][NB], xsv[2][MT];
+    for (int b = 0; b < NB; ++b) acc[b] = f32x4{0, 0, 0, 0};
+    Piece wv[2][NB][kPieces], xv[2][kPieces];
+    int wsv[2][NB], xsv[2];
     const auto fetch_w = [&](int side, int b) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
@@ -85,115 +90,93 @@ __global__ __launch_bounds__(kWaves * kWave, MT == 1 && ALIGNED && !ACT ? 4 : 2)
         }
     };
     const auto fetch_x = [&](int side, int b) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            load(x[i], b, xv[side][i], x_end);
-            if constexpr (FP4) xsv[side][i] = load_scales(xs[i], b);
-        }
+        load(x, b, xv[side], x_end);
+        if constexpr (FP4) xsv[side] = load_scales(xs, b);
     };
     const auto fetch = [&](int side, int b) __attribute__((always_inline)) {
         fetch_w(side, b);
         fetch_x(side, b);
     };
-    const auto piece = [&](int side, auto at) __attribute__((always_inline)) {
+    const auto piece = [&](int side, int b, auto at) __attribute__((always_inline)) {
         constexpr int u = decltype(at)::value;
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                if constexpr (FP4) {
-                    const i32x4 &p = wv[side][j][u], &q = xv[side][i][u];
-                    const i32x8 A = {p[0], p[1], p[2], p[3], 0, 0, 0, 0}, B = {q[0], q[1], q[2], q[3], 0, 0, 0, 0};
-                    acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc[j][i], 4, 4, u, wsv[side][j], u, xsv[side][i]);
-                } else {
-                    acc[j][i] = mfma<T>(settled(wv[side][j][u]), settled(xv[side][i][u]), acc[j][i]);
-                }
+        for (int j = 0; j < NB; ++j) {
+            if constexpr (FP4) {
+                const i32x4 &p = wv[side][j][u], &q = xv[side][u];
+                const i32x8 A = {p[0], p[1], p[2], p[3], 0, 0, 0, 0}, B = {q[0], q[1], q[2], q[3], 0, 0, 0, 0};
+                acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc[j], 4, 4, u, wsv[side][j], u, xsv[side]);
+            } else {
+                acc[j] = mfma<T>(settled(wv[side][j][u], w[j], b, u), settled(xv[side][u], x, b, u), acc[j]);
             }
+        }
     };
-    const auto multiply = [&](int side) __attribute__((always_inline)) {
-        piece(side, std::integral_constant<int, 0>());
-        piece(side, std::integral_constant<int, 1>());
-        piece(side, std::integral_constant<int, 2>());
-        piece(side, std::integral_constant<int, 3>());
+    const auto multiply = [&](int side, int b) __attribute__((always_inline)) {
+        piece(side, b, std::integral_constant<int, 0>());
+        piece(side, b, std::integral_constant<int, 1>());
+        piece(side, b, std::integral_constant<int, 2>());
+        piece(side, b, std::integral_constant<int, 3>());
     };
     int b = wave;
     if (b < blocks) fetch_w(0, b);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const long long row = row_of_slot(a, t.begin + min(m0 + i * 16 + r, count - 1));
-        x[i] = a.p + a.ld_p * row;
-        if constexpr (FP4) xs[i] = a.p_scales + blocks32 * row;
-    }
+    const long long x_row = row_of_slot(a, t.begin + min(m0 + r, count - 1));
+    x = a.p + a.ld_p * x_row;
+    if constexpr (FP4) xs = a.p_scales + blocks32 * x_row;
     if (b < blocks) fetch_x(0, b);
     while (b < blocks) {
         if (b + kWaves < blocks) fetch(1, b + kWaves);
-        multiply(0);
+        multiply(0, b);
         b += kWaves;
         if (b >= blocks) break;
         if (b + kWaves < blocks) fetch(0, b + kWaves);
-        multiply(1);
+        multiply(1, b);
         b += kWaves;
     }
 
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) *(f32x4 *)&sums[wave][j * MT + i][r * 16 + g * 4] = acc[j][i];
+    for (int j = 0; j < NB; ++j) *(f32x4 *)&sums[wave][j][r * 16 + g * 4] = acc[j];
     __syncthreads();
-    const int row = threadIdx.x / 16, n = t.n * 16 + threadIdx.x % 16;
+    const int s = m0 + threadIdx.x / 16, n = t.n * 16 + threadIdx.x % 16;
+    float v[NB];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        float v[NB];
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-            v[j] = (sums[0][j * MT + i][threadIdx.x] + sums[1][j * MT + i][threadIdx.x]) +
-                   (sums[2][j * MT + i][threadIdx.x] + sums[3][j * MT + i][threadIdx.x]);
-        const int s = m0 + i * 16 + row;
-        if (s >= count || n >= a.n) continue;
-        T *out = (T *)(a.out + a.ld_out * ((long long)t.begin + s)) + n;
-        if constexpr (ACT) {
-            *out = (T)(silu(v[0]) * v[1]);
-            if (a.pre) {
-                T *pre = (T *)(a.pre + a.ld_pre * ((long long)t.begin + s)) + n;
-                pre[0] = (T)v[0];
-                pre[a.n] = (T)v[1];
-            }
-        } else {
-            *out = (T)v[0];
+    for (int j = 0; j < NB; ++j)
+        v[j] = (sums[0][j][threadIdx.x] + sums[1][j][threadIdx.x]) + (sums[2][j][threadIdx.x] + sums[3][j][threadIdx.x]);
+    if (s >= count || n >= a.n) return;
+    T *out = (T *)(a.out + a.ld_out * ((long long)t.begin + s)) + n;
+    if constexpr (ACT) {
+        *out = (T)(silu(v[0]) * v[1]);
+        if (a.pre) {
+            T *pre = (T *)(a.pre + a.ld_pre * ((long long)t.begin + s)) + n;
+            pre[0] = (T)v[0];
+            pre[a.n] = (T)v[1];
         }
+    } else {
+        *out = (T)v[0];
     }
-}
-
-template <typename T, bool FP4, int ACT, int MT, bool ALIGNED>
-int launch(const Args &a, hipStream_t stream)
-{
-    const long long tiles = ((long long)a.slots / (16 * MT) + (a.experts < a.slots ? a.experts : a.slots)) * ((a.n + 15) / 16);
-    const long long grid = (tiles + kXcds - 1) / kXcds * kXcds;
-    if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "grouped product: too many tiles");
-    k_mm_rows<T, FP4, ACT, MT, ALIGNED><<<dim3((unsigned)grid), dim3(kWaves * kWave), 0, stream>>>(a);
-    return pfk_internal_launched("k_mm_rows");
 }
 
 }  // namespace
 
 template <typename T, bool FP4, int ACT, bool ALIGNED>
-int launch_rows(const Args &a, long long rows, hipStream_t stream)
+int launch_rows(const Args &a, hipStream_t stream)
 {
-    if (ALIGNED || rows <= 16) return launch<T, FP4, ACT, 1, ALIGNED>(a, stream);
-    return launch<T, FP4, ACT, ALIGNED ? 1 : 2, ALIGNED>(a, stream);
+    const long long tiles = ((long long)a.slots / 16 + (a.experts < a.slots ? a.experts : a.slots)) * ((a.n + 15) / 16);
+    const long long grid = (tiles + kXcds - 1) / kXcds * kXcds;
+    if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "grouped product: too many tiles");
+    k_mm_rows<T, FP4, ACT, ALIGNED><<<dim3((unsigned)grid), dim3(kWaves * kWave), 0, stream>>>(a);
+    return pfk_internal_launched("k_mm_rows");
 }
 
-template int launch_rows<f16, false, 0, true>(const Args &, long long, hipStream_t);
-template int launch_rows<f16, false, 0, false>(const Args &, long long, hipStream_t);
-template int launch_rows<f16, false, 1, true>(const Args &, long long, hipStream_t);
-template int launch_rows<f16, false, 1, false>(const Args &, long long, hipStream_t);
-template int launch_rows<f16, true, 0, true>(const Args &, long long, hipStream_t);
-template int launch_rows<f16, true, 1, true>(const Args &, long long, hipStream_t);
-template int launch_rows<bf16, false, 0, true>(const Args &, long long, hipStream_t);
-template int launch_rows<bf16, false, 0, false>(const Args &, long long, hipStream_t);
-template int launch_rows<bf16, false, 1, true>(const Args &, long long, hipStream_t);
-template int launch_rows<bf16, false, 1, false>(const Args &, long long, hipStream_t);
-template int launch_rows<bf16, true, 0, true>(const Args &, long long, hipStream_t);
-template int launch_rows<bf16, true, 1, true>(const Args &, long long, hipStream_t);
+template int launch_rows<f16, false, 0, true>(const Args &, hipStream_t);
+template int launch_rows<f16, false, 0, false>(const Args &, hipStream_t);
+template int launch_rows<f16, false, 1, true>(const Args &, hipStream_t);
+template int launch_rows<f16, false, 1, false>(const Args &, hipStream_t);
+template int launch_rows<f16, true, 0, true>(const Args &, hipStream_t);
+template int launch_rows<f16, true, 1, true>(const Args &, hipStream_t);
+template int launch_rows<bf16, false, 0, true>(const Args &, hipStream_t);
+template int launch_rows<bf16, false, 0, false>(const Args &, hipStream_t);
+template int launch_rows<bf16, false, 1, true>(const Args &, hipStream_t);
+template int launch_rows<bf16, false, 1, false>(const Args &, hipStream_t);
+template int launch_rows<bf16, true, 0, true>(const Args &, hipStream_t);
+template int launch_rows<bf16, true, 1, true>(const Args &, hipStream_t);
 
 }  // namespace pfmoe

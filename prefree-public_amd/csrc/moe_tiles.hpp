@@ -85,11 +85,12 @@ template <int ROWS, int THREADS, bool ALIGNED>
 struct Along {
     static constexpr int kBytes = ROWS * 64;
     static constexpr int kLoads = ROWS * 4 / THREADS;
-    Buffer from;                          // ALIGNED: the operand, and this thread's pieces of its rows in the first tile
-    unsigned at[ALIGNED ? kLoads : 1];
-    const char *row[ALIGNED ? 1 : kLoads], *end;
     int piece;          // this thread's piece of its rows (the same for all its loads)
     int k_pieces, k;
+    Buffer from;                          // ALIGNED: the operand, and this thread's pieces of its rows in the first tile
+    unsigned at[ALIGNED ? kLoads : 1];
+    uintptr_t word[ALIGNED ? 1 : kLoads], end;   // else the words that hold them, and by how much they are shifted
+    unsigned shift[ALIGNED ? 1 : kLoads];
     Words held[ALIGNED ? 1 : kLoads];
 
     static __device__ __forceinline__ int tile_row(int i) { return i * (THREADS / 4) + (int)(threadIdx.x >> 2); }
@@ -106,23 +107,38 @@ struct Along {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const long long r = ld * row_of(tile_row(i));
-            if constexpr (ALIGNED) at[i] = (unsigned)r + piece * 16;
-            else row[i] = base + r;
+            if constexpr (ALIGNED) {
+                at[i] = (unsigned)r + piece * 16;
+            } else {
+                const uintptr_t p = (uintptr_t)(base + r) + piece * 16;
+                word[i] = Words::word_of(p);
+                shift[i] = Words::shift_of(p);
+            }
         }
     }
     __device__ __forceinline__ void issue(int i, int t, char *lds)
     {
-        const int c = t * 4 + piece;
-        if constexpr (ALIGNED)
-            to_lds16(from, c < k_pieces ? at[i] : kOutside, t * 64, lds + i * THREADS * 16 + wave_id() * (kWave * 16));
-        else
-            held[i].load(row[i], c * 8, k, t * 32 + 32 <= k, end);
+        to_lds16(from, t * 4 + piece < k_pieces ? at[i] : kOutside, t * 64, lds + i * THREADS * 16 + wave_id() * (kWave * 16));
     }
-    __device__ __forceinline__ void commit(char *lds)
+    // whether the rows have all of tile t and the word behind it
+    __device__ __forceinline__ bool whole(int t) const { return t * 32 + 34 <= k; }
+    __device__ __forceinline__ void fetch(int t)
     {
-        if constexpr (!ALIGNED) {
+        if (whole(t)) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) *(i32x4 *)(lds + i * THREADS * 16 + threadIdx.x * 16) = held[i].settle();
+            for (int i = 0; i < kLoads; ++i) held[i].load(word[i] + 64LL * t, word[i] + 64LL * t + 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) held[i].load_until(word[i] + 64LL * t, end);
+        }
+    }
+    __device__ __forceinline__ void commit(char *lds, int t)
+    {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            i32x4 v = held[i].shifted(shift[i]);
+            if (!whole(t)) v = Words::kept(v, k - (t * 4 + piece) * 8);
+            *(i32x4 *)(lds + i * THREADS * 16 + threadIdx.x * 16) = v;
         }
     }
     // 16 rows from r0 (a multiple of 16): lane l has row l % 16, piece l / 16
@@ -145,11 +161,12 @@ struct Across {
     static constexpr int kWaveRows = kWave / kPieces;    // and of one wave
     static_assert(kPieces >= 16 && kPieces <= 32 && kStride % 8 == 0, "see f");
     Buffer from;         // ALIGNED
-    const char *base, *end;
+    uintptr_t base, end;
     long long ld;
     bool inside;         // all of the tile's columns are there
     int col[2], cols;    // this thread's first column in loads of even and odd number, and the columns there are
     int k;
+    unsigned shift[ALIGNED ? 1 : kLoads];
     Words held[ALIGNED ? 1 : kLoads];
 
     static __device__ __forceinline__ int f(int r) { return (r & 3) | ((r >> 1) & 4); }
@@ -168,7 +185,7 @@ struct Across {
             col[i] = c0 + (((place >> 1) ^ f(i * kStride + r)) * 2 + (place & 1)) * 8;
             if (ALIGNED && col[i] >= cols) col[i] = 0;   // columns behind the end: any, their results are not stored
         }
-        base = base_;
+        base = (uintptr_t)base_;
         ld = ld_;
         k = k_;
     }
@@ -177,13 +194,40 @@ struct Across {
     __device__ __forceinline__ void issue(int i, int t, char *lds, int rows)
     {
         const int r = t * 32 + tile_row(i);
-        const int at = GATHER ? __shfl(rows, i * kWaveRows + (int)(threadIdx.x & (kWave - 1)) / kPieces) : r;
-        if constexpr (ALIGNED) {
-            const unsigned first = GATHER ? (unsigned)at * (unsigned)ld : (unsigned)tile_row(i) * (unsigned)ld;
-            to_lds16(from, r < k ? first + 2 * col[i & 1] : kOutside, GATHER ? 0 : (unsigned)(t * 32) * (unsigned)ld,
-                     lds + i * THREADS * 16 + wave_id() * (kWave * 16));
+        const unsigned first = (unsigned)(GATHER ? given(rows, i) : tile_row(i)) * (unsigned)ld;
+        to_lds16(from, r < k ? first + 2 * col[i & 1] : kOutside, GATHER ? 0 : (unsigned)(t * 32) * (unsigned)ld,
+                 lds + i * THREADS * 16 + wave_id() * (kWave * 16));
+    }
+    static __device__ __forceinline__ int given(int rows, int i)
+    {
+        return __shfl(rows, i * kWaveRows + (int)(threadIdx.x & (kWave - 1)) / kPieces);
+    }
+    __device__ __forceinline__ bool whole(int t) const { return inside && t * 32 + 32 <= k; }
+    template <bool GATHER>
+    __device__ __forceinline__ void fetch(int t, int rows)
+    {
+        uintptr_t p[kLoads];
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            p[i] = base + ld * (GATHER ? given(rows, i) : t * 32 + tile_row(i)) + 2LL * col[i & 1];
+            shift[i] = Words::shift_of(p[i]);
+            p[i] = Words::word_of(p[i]);
+        }
+        if (whole(t)) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) held[i].load(p[i], p[i] + 8 * shift[i]);
         } else {
-            held[i].load(base + ld * at, col[i & 1], r < k ? cols : 0, inside && t * 32 + 32 <= k, end);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) held[i].load_until(p[i], end);
+        }
+    }
+    __device__ __forceinline__ void commit(char *lds, int t)
+    {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            i32x4 v = held[i].shifted(shift[i]);
+            if (!whole(t)) v = Words::kept(v, t * 32 + tile_row(i) < k ? cols - col[i & 1] : 0);
+            *(i32x4 *)(lds + i * THREADS * 16 + threadIdx.x * 16) = v;
         }
     }
     // The k of tile t whose row lane l looks up for its wave: load l / kWaveRows, row l % kWaveRows of the wave's.
@@ -191,13 +235,6 @@ struct Across {
     {
         const int l = (threadIdx.x & (kWave - 1)) % (kLoads * kWaveRows), w = threadIdx.x / kWave;
         return t * 32 + l / kWaveRows * kStride + w * kWaveRows + l % kWaveRows;
-    }
-    __device__ __forceinline__ void commit(char *lds)
-    {
-        if constexpr (!ALIGNED) {
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) *(i32x4 *)(lds + i * THREADS * 16 + threadIdx.x * 16) = held[i].settle();
-        }
     }
     // 16 columns from c0 (a multiple of 16): lane l has column l % 16, rows 8 (l / 16) .. +7
     static __device__ __forceinline__ i32x4 fragment(const char *lds, int c0)
@@ -442,8 +479,8 @@ __device__ __forceinline__ bool find_tile(const Args &a, int nt, int id, Tile &t
 template <typename T, bool FP4, int MODE, int ACT>
 int launch_stream(const Args &a, hipStream_t stream);
 
-// moe_mm_rows.hip; rows: of an expert on average
+// moe_mm_rows.hip
 template <typename T, bool FP4, int ACT, bool ALIGNED>
-int launch_rows(const Args &a, long long rows, hipStream_t stream);
+int launch_rows(const Args &a, hipStream_t stream);
 
 }  // namespace pfmoe
