@@ -29,36 +29,40 @@ template <typename T> struct vec { };
 template <> struct vec<f16> { typedef f16x4 x4; typedef f16x8 x8; };
 template <> struct vec<bf16> { typedef bf16x4 x4; typedef bf16x8 x8; };
 
-// Eight 16-bit elements on their way from rows of any alignment: as the whole words that hold them, which take half the
-// time of the hardware's own unaligned loads (rows of 2222 bytes out of the L2: 7.4 against 3.7 TB/s).  A word may hold
-// an element that lies outside of what is asked for, but never only such, so it lies in the operand's memory.  shifted()
-// puts them into place and kept() clears what lies behind the row's end; only these wait, and loading has no branch in
-// which anything but loads happens, so that several of them can be under way.
+// Rows of any alignment are loaded by the whole words that hold them, the elements then shifted into place (rows of 2222
+// bytes out of the L2: 7.4 TB/s, 3.7 with the hardware's unaligned loads).  A word may hold an element that lies outside
+// of what is asked for, but never only such, so it lies in the operand's memory.
+//
+// The words are said to be global memory: of pointers made of numbers the compiler does not know it, and its flat loads
+// have to be waited for wherever an LDS read is (gradient of 32764 slots x 2049 from 1023, 32 experts: 681 us, 535 so).
+__device__ __forceinline__ uintptr_t word_of(uintptr_t p) { return p & ~(uintptr_t)3; }
+__device__ __forceinline__ unsigned load_word(uintptr_t p) { return *(const __attribute__((address_space(1))) unsigned *)p; }
+// the last word of an operand of `bytes` > 0
+__device__ __forceinline__ uintptr_t end_of(const char *base, unsigned long long bytes) { return word_of((uintptr_t)base + bytes - 2); }
+// the first `valid` of a word's two elements, zeros behind them
+__device__ __forceinline__ unsigned kept_word(unsigned v, int valid) { return valid >= 2 ? v : valid == 1 ? v & 0xffff : 0; }
+
+// Eight elements of a row.  shifted() puts them into place and kept() clears what lies behind the row's end; only these
+// wait, and loading has no branch in which anything but loads happens, so that several of them can be under way.
 struct Words {
     i32x4 v;
     int last;
 
-    // Said to be global memory: of pointers made of numbers the compiler does not know it, and its flat loads have to be
-    // waited for wherever an LDS read is (gradient of 32764 slots x 2049 from 1023, 32 experts: 681 us, 535 so).
-    typedef int words __attribute__((ext_vector_type(4), aligned(4)));
-    typedef const __attribute__((address_space(1))) words *Four;
-    typedef const __attribute__((address_space(1))) int *One;
-
-    static __device__ __forceinline__ uintptr_t word_of(uintptr_t p) { return p & ~(uintptr_t)3; }
     static __device__ __forceinline__ unsigned shift_of(uintptr_t p) { return (unsigned)p & 2; }
 
     // the words from p, and the one at `more`: p + 16, or anything where the shift is 0
     __device__ __forceinline__ void load(uintptr_t p, uintptr_t more)
     {
-        v = *(Four)p;
-        last = *(One)more;
+        typedef int words __attribute__((ext_vector_type(4), aligned(4)));
+        v = *(const __attribute__((address_space(1))) words *)p;
+        last = (int)load_word(more);
     }
     // those of them before `end`, the operand's last word
     __device__ __forceinline__ void load_until(uintptr_t p, uintptr_t end)
     {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = *(One)(p + 4 * i < end ? p + 4 * i : end);
-        last = *(One)(p + 16 < end ? p + 16 : end);
+        for (int i = 0; i < 4; ++i) v[i] = (int)load_word(p + 4 * i < end ? p + 4 * i : end);
+        last = (int)load_word(p + 16 < end ? p + 16 : end);
     }
     __device__ __forceinline__ i32x4 shifted(unsigned shift) const
     {
@@ -69,20 +73,15 @@ struct Words {
     static __device__ __forceinline__ i32x4 kept(i32x4 r, int valid)
     {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = 2 * i + 1 < valid ? r[i] : 2 * i < valid ? r[i] & 0xffff : 0;
+        for (int i = 0; i < 4; ++i) r[i] = (int)kept_word((unsigned)r[i], valid - 2 * i);
         return r;
-    }
-    // the last word of an operand of `bytes` > 0
-    static __device__ __forceinline__ uintptr_t end_of(const char *base, unsigned long long bytes)
-    {
-        return word_of((uintptr_t)base + bytes - 2);
     }
 };
 
 // 16 bytes that are all there, from an address that is a multiple of two.
 __device__ __forceinline__ i32x4 load16_any(const void *p)
 {
-    const uintptr_t at = Words::word_of((uintptr_t)p);
+    const uintptr_t at = word_of((uintptr_t)p);
     const unsigned shift = Words::shift_of((uintptr_t)p);
     Words w;
     w.load(at, shift ? at + 16 : at);

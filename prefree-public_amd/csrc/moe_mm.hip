@@ -6,18 +6,22 @@ namespace {
 
 using namespace pfmoe;
 
-// A workgroup a tile, two (128 x 128) or five (64 x 64) of them on a CU: for products too small for k_mm_stream, and, by
-// way of registers, for operands of any alignment.  8192 rows of 16 experts, 2048 -> 2048, in 114 us against its 106;
-// 311 tokens x 2 of 12, 1111 -> 717, in 23 us: there a step of k takes the CU's address units longest, which handle rows
-// that cross lines twice.
+// A workgroup a tile, for products too small for k_mm_stream and, by way of registers, for operands of any alignment.  8192
+// rows of 16 experts, 2048 -> 2048, in 114 us against its 106; 311 tokens x 2 of 12, 1111 -> 717, in 22.6 us.  There one
+// workgroup a CU waits for its loads: four tiles of k under way in registers (with two 25.7, with three 23.5); larger tiles
+// have no registers for that.  An operand along k is loaded by single words, sixteen lanes a row, since the L1 takes one
+// lane a cycle of wider loads that do not lie in their width (32764 slots of 32 experts, 2049 -> 1023, 128 x 128 tiles: 503
+// with 16 bytes a lane, 435 so); an operand across k, with longer rows, by 16 bytes a lane (dw 540, by words 778).
 // T: f16 or bf16 of the results; FP4: 4-bit operands
 template <typename T, bool FP4, int MODE, int ACT, int BM, int BN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
 {
     constexpr int THREADS = WM * WN * 64;
     constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-    typedef typename std::conditional<MODE == kDw, Across<BM, THREADS, ALIGNED>, Along<BM, THREADS, ALIGNED>>::type P;
-    typedef typename std::conditional<MODE == kFwd, Along<BN, THREADS, ALIGNED>, Across<BN, THREADS, ALIGNED>>::type Q;
+    constexpr int RING = ALIGNED || MODE == kDw ? 1 : BM == 64 ? 4 : 2;   // tiles under way in registers
+    constexpr int BODIES = BM == 64 ? RING : 1;   // of the loop; with one the ring's tiles move on from place to place
+    typedef typename std::conditional<MODE == kDw, Across<BM, THREADS, ALIGNED>, Along<BM, THREADS, ALIGNED, RING>>::type P;
+    typedef typename std::conditional<MODE == kFwd, Along<BN, THREADS, ALIGNED, RING>, Across<BN, THREADS, ALIGNED>>::type Q;
     typedef Scales<BM + BN, THREADS> S;
     constexpr int SCALES = P::kBytes + Q::kBytes;   // where a tile's scales lie
     constexpr int SLOT = SCALES + (FP4 ? S::kBytes : 0);
@@ -92,20 +96,23 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
             }
         }
     };
-    // tile s by way of registers, and from there to LDS
-    const auto fetch = [&](int s) {
+    // By way of registers: tile s to LDS, and then what comes into its place, of an operand along k tile s + RING and of
+    // one across it tile s + 1.
+    const auto refill = [&](int s, int place) {
         if constexpr (!ALIGNED) {
-            look_up(s);
-            if constexpr (MODE == kDw) p.template fetch<false>(s, 0);
-            else p.fetch(s);
-            if constexpr (MODE == kFwd) q.fetch(s);
-            else q.template fetch<MODE == kDw>(s, now);
+            look_up(s + 1);
+            if constexpr (MODE == kDw) p.template fetch<false>(s + 1, 0);
+            else p.fetch(s + RING, p.freed(BODIES, place));
+            if constexpr (MODE == kFwd) q.fetch(s + RING, q.freed(BODIES, place));
+            else q.template fetch<MODE == kDw>(s + 1, now);
         }
     };
-    const auto commit = [&](char *to, int s) {
+    const auto commit = [&](char *to, int s, int place) {
         if constexpr (!ALIGNED) {
-            p.commit(to, s);
-            q.commit(to + P::kBytes, s);
+            if constexpr (MODE == kDw) p.commit(to, s);
+            else p.commit(to, s, place);
+            if constexpr (MODE == kFwd) q.commit(to + P::kBytes, s, place);
+            else q.commit(to + P::kBytes, s);
         }
     };
 
@@ -128,14 +135,14 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
     // compiler waits for all loads to LDS before each transposing read.)
     i32x4 x[4], w[2][FN];
     int xs[4], ws[2][FN];
-    const auto step = [&](int s, char *__restrict__ fill, const char *__restrict__ here, const char *__restrict__ next) {
+    const auto step = [&](int s, int place, char *__restrict__ fill, const char *__restrict__ here, const char *__restrict__ next) {
         if constexpr (FP4) {   // a tile further ahead, since their loads end in a register
             scales.commit(fill + SCALES);
             scales.issue(s + 4, k / 32);
         }
         if constexpr (!ALIGNED) {   // the same
-            commit(fill, s + 3);
-            fetch(s + 4);
+            commit(fill, s + 3, place);
+            refill(s + 3, place);
         }
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
@@ -172,19 +179,28 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
         __builtin_amdgcn_sched_barrier(0);
     };
     if (steps > 0) {
+        if constexpr (!ALIGNED) {
+#pragma unroll
+            for (int r = 0; r < RING; ++r) {
+                if constexpr (MODE != kDw) p.fetch(r, r);
+                if constexpr (MODE == kFwd) q.fetch(r, r);
+            }
+            look_up(0);
+            if constexpr (MODE == kDw) p.template fetch<false>(0, 0);
+            if constexpr (MODE != kFwd) q.template fetch<MODE == kDw>(0, now);
+        }
 #pragma unroll
         for (int s = 0; s < 3; ++s) {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) issue(i, s, lds[s]);
-            fetch(s);
-            commit(lds[s], s);
+            commit(lds[s], s, s % BODIES);
+            refill(s, s % BODIES);
             if constexpr (FP4) {
                 scales.issue(s, k / 32);
                 scales.commit(lds[s] + SCALES);
             }
         }
         if constexpr (FP4) scales.issue(3, k / 32);
-        fetch(3);
         wait_and_meet<ALIGNED ? LOADS : 63>();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -196,20 +212,25 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
             w[0][j] = read_w(lds[0], j);
             ws[0][j] = scale_w(lds[0], j);
         }
-        // one body a tile: the pointers of two would not be told apart
+        // With loads to LDS one body a tile: the pointers of two would not be told apart.
 #pragma unroll 1
-        for (int s = 0; s < steps; ++s) {
-            step(s, lds[(s + 3) & 3], lds[s & 3], lds[(s + 1) & 3]);
+        for (int s0 = 0; s0 < steps; s0 += BODIES) {
 #pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                w[0][j] = w[1][j];
-                ws[0][j] = ws[1][j];
-            }
-            if constexpr (FM == 2) {   // read two ahead is a tile ahead
+            for (int r = 0; r < BODIES; ++r) {
+                const int s = s0 + r;
+                if (r > 0 && s >= steps) break;
+                step(s, (r + 3) % BODIES, lds[(s + 3) & 3], lds[s & 3], lds[(s + 1) & 3]);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    x[i] = x[i + 2];
-                    xs[i] = xs[i + 2];
+                for (int j = 0; j < FN; ++j) {
+                    w[0][j] = w[1][j];
+                    ws[0][j] = ws[1][j];
+                }
+                if constexpr (FM == 2) {   // read two ahead is a tile ahead
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        x[i] = x[i + 2];
+                        xs[i] = xs[i + 2];
+                    }
                 }
             }
         }
@@ -250,13 +271,13 @@ int launch(const Args &a, hipStream_t stream)
 // 65 / 56; rows 64: 51 / 39), and loses under that (8 experts, 1024 -> 1024, 256: 26 / 19, 512: 27 / 24; dw 8 of 1024 x
 // 1024, 512: 30 / 21).
 //
-// Operands that do not lie in 16 bytes are bound by their loads' addresses, a row of which crosses lines.  Forward, the
-// rows' kernel against 64 x 64, 128 x 128 and 256 x 256 tiles: 12 experts, 1111 -> 717, rows 8: 14 / 28 / 35 / 56, 32: 25 /
-// 29 / 39 / 62, 64: 39 / 29 / 42 / 69, 200: 97 / 43 / 47 / 95; 16 experts, 2047 -> 2047, 8: 53 / 54 / 61 / 96, 16: 71 / 56 /
-// 63 / 98, 48: 148 / 96 / 69 / 107, 200: 513 / 198 / 170 / 147; 64 experts, 1025 -> 513, 8: 35 / 38 / 52 / 57, 48: 102 / 53 /
-// 70 / 66, 200: 346 / 121 / 122 / 98; 32 experts, 2047 -> 2 x 1023, 8: 85 / 98 / 99 / 107, 64: 318 / 190 / 138 / 125.
-// Gradients with 128 x 128 against 256 x 256: 32764 slots of 32 experts, 1023 x 2049, dx 522 / 450, dw 628 / 546; 8000 of
-// 16, 2047 x 2047, dx 253 / 270, dw 377 / 288; 2000 of 16, 1023 x 1025, dx 44 / 72, dw 90 / 91.
+// Operands that do not lie in 16 bytes come by way of registers, which favours many small workgroups.  Forward, the rows'
+// kernel against 64 x 64 and 128 x 128 tiles: 12 experts, 1111 -> 717, rows 8: 15 / 23 / 42, 32: 25 / 24 / 43, 400: 179 /
+// 55 / 61; 16 experts, 2047 -> 2047, 4: 48 / 45 / 74, 64: 189 / 78 / 81, 100: 277 / 105 / 105, 200: 518 / 151 / 113; 64
+// experts, 1025 -> 513, 8: 35 / 34 / 48, 64: 129 / 55 / 59, 400: 661 / 163 / 148; 32 experts, 2047 -> 2 x 1023, 4: 82 / 89 /
+// 98, 16: 120 / 93 / 96, 64: 317 / 136 / 107.  Gradients with 128 x 128 against 256 x 256: 32764 slots of 32 experts, 1023 x
+// 2049, dx 522 / 423, dw 628 / 540; 8000 of 16, 2047 x 2047, dx 243 / 270, dw 377 / 287; 2000 of 16, 1023 x 1025, dx 45 /
+// 72, dw 90 / 91.
 template <typename T, bool FP4, int MODE, int ACT, bool ALIGNED>
 int launch_size(const Args &a, hipStream_t stream)
 {
@@ -265,16 +286,15 @@ int launch_size(const Args &a, hipStream_t stream)
         return (MODE == kDw ? a.experts * ((a.m + side - 1) / side) : a.slots / side + used) * ((a.n * (ACT ? 2LL : 1LL) + side - 1) / side);
     };
     if constexpr (MODE == kFwd) {
-        if (rows <= 8 && (tiles(128) < 512 || a.ld_q >= 4000)) return launch_rows<T, FP4, ACT, ALIGNED>(a, stream);
-        if (!ALIGNED && rows <= 32 && tiles(128) < 128) return launch_rows<T, FP4, ACT, ALIGNED>(a, stream);
+        const bool few = ALIGNED ? rows <= 8 && (tiles(128) < 512 || a.ld_q >= 4000) : rows <= (tiles(128) < 128 ? 24 : 4);
+        if (few) return launch_rows<T, FP4, ACT, ALIGNED>(a, stream);
     }
     if constexpr (ALIGNED) {
         if (tiles(256) >= (MODE != kDw && rows >= 96 ? 128 : 256)) return launch_stream<T, FP4, MODE, ACT>(a, stream);
+    } else if constexpr (MODE == kFwd) {
+        if (tiles(64) < 1300) return launch<T, FP4, MODE, ACT, 64, 64, 2, 2, ALIGNED>(a, stream);
     } else {
-        if constexpr (MODE == kFwd)
-            if (tiles(64) < 800) return launch<T, FP4, MODE, ACT, 64, 64, 2, 2, ALIGNED>(a, stream);
-        if (MODE == kDx ? tiles(256) >= 512 && rows >= 256 : tiles(256) >= (MODE == kDw ? 256 : 192))
-            return launch<T, FP4, MODE, ACT, 256, 256, 2, 4, ALIGNED>(a, stream);
+        if (MODE == kDw ? tiles(256) >= 256 : tiles(256) >= 512 && rows >= 256) return launch<T, FP4, MODE, ACT, 256, 256, 2, 4, ALIGNED>(a, stream);
     }
     return launch<T, FP4, MODE, ACT, 128, 128, 2, 2, ALIGNED>(a, stream);
 }

@@ -41,8 +41,8 @@ __global__ __launch_bounds__(kWaves * kWave, ALIGNED && !ACT ? 4 : 2) void k_mm_
     const int blocks = (pieces + 4 * kPieces - 1) / (4 * kPieces);
     typedef typename std::conditional<ALIGNED, i32x4, Words>::type Piece;
     const bool any = a.k > 0;
-    const uintptr_t x_end = any ? Words::end_of(a.p, a.ld_p * (a.p_rows - 1LL) + 2LL * a.k) : 0;
-    const uintptr_t w_end = any ? Words::end_of(a.q + a.q_expert * t.e, a.q_expert) : 0;
+    const uintptr_t x_end = any ? end_of(a.p, a.ld_p * (a.p_rows - 1LL) + 2LL * a.k) : 0;
+    const uintptr_t w_end = any ? end_of(a.q + a.q_expert * t.e, a.q_expert) : 0;
     const auto whole = [&](int b) { return (b + 1) * 32 * kPieces <= a.k; };   // whether rows have all of block b
     const auto load = [&](const char *row, int b, Piece (&v)[kPieces], uintptr_t end) __attribute__((always_inline)) {
 #pragma unroll
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(kWaves * kWave, ALIGNED && !ACT ? 4 : 2) void k_mm_
                 v[u] = i32x4{0, 0, 0, 0};
                 if (at < pieces) v[u] = *(const i32x4 *)(row + 16LL * at);
             } else {
-                const uintptr_t p = Words::word_of((uintptr_t)row + 16LL * at);
+                const uintptr_t p = word_of((uintptr_t)row + 16LL * at);
                 if (whole(b)) v[u].load(p, p + 8 * Words::shift_of((uintptr_t)row));
                 else v[u].load_until(p, end);
             }

@@ -81,7 +81,7 @@ __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)"
 
 // An operand whose k lies along its rows: a tile is ROWS rows of 64 bytes.  The 16-byte piece c of row r lies at place
 // c ^ ((r >> 1) & 3) of the row, so that eight lanes that read one piece of eight rows touch each bank of 128 bytes once.
-template <int ROWS, int THREADS, bool ALIGNED>
+template <int ROWS, int THREADS, bool ALIGNED, int RING = 2>
 struct Along {
     static constexpr int kBytes = ROWS * 64;
     static constexpr int kLoads = ROWS * 4 / THREADS;
@@ -89,9 +89,11 @@ struct Along {
     int k_pieces, k;
     Buffer from;                          // ALIGNED: the operand, and this thread's pieces of its rows in the first tile
     unsigned at[ALIGNED ? kLoads : 1];
-    uintptr_t word[ALIGNED ? 1 : kLoads], end;   // else the words that hold them, and by how much they are shifted
-    unsigned shift[ALIGNED ? 1 : kLoads];
-    Words held[ALIGNED ? 1 : kLoads];
+    // else words: sixteen lanes share a row of the tile, whose elements may start in the middle of one
+    static constexpr int kWords = ALIGNED ? 1 : ROWS * 16 / THREADS;
+    uintptr_t word[kWords], end;          // this thread's of the first tile; the operand's last
+    unsigned shift[kWords];               // 2: by two bytes
+    unsigned held[ALIGNED ? 1 : RING][kWords];   // of tile t at place t % RING
 
     static __device__ __forceinline__ int tile_row(int i) { return i * (THREADS / 4) + (int)(threadIdx.x >> 2); }
 
@@ -103,16 +105,16 @@ struct Along {
         k = k_;
         k_pieces = k_ / per_piece;
         if constexpr (ALIGNED) from = buffer_of(base, bytes);
-        else end = Words::end_of(base, bytes);
+        else end = end_of(base, bytes);
+        if constexpr (ALIGNED) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const long long r = ld * row_of(tile_row(i));
-            if constexpr (ALIGNED) {
-                at[i] = (unsigned)r + piece * 16;
-            } else {
-                const uintptr_t p = (uintptr_t)(base + r) + piece * 16;
-                word[i] = Words::word_of(p);
-                shift[i] = Words::shift_of(p);
+            for (int i = 0; i < kLoads; ++i) at[i] = (unsigned)(ld * row_of(tile_row(i))) + piece * 16;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                const uintptr_t p = (uintptr_t)(base + ld * row_of(word_row(i)));
+                word[i] = word_of(p) + (threadIdx.x & 15) * 4;
+                shift[i] = (unsigned)p & 2;
             }
         }
     }
@@ -120,25 +122,41 @@ struct Along {
     {
         to_lds16(from, t * 4 + piece < k_pieces ? at[i] : kOutside, t * 64, lds + i * THREADS * 16 + wave_id() * (kWave * 16));
     }
-    // whether the rows have all of tile t and the word behind it
-    __device__ __forceinline__ bool whole(int t) const { return t * 32 + 34 <= k; }
-    __device__ __forceinline__ void fetch(int t)
+    static __device__ __forceinline__ int word_row(int i) { return i * (THREADS / 16) + (int)(threadIdx.x >> 4); }
+    __device__ __forceinline__ bool whole(int t) const { return t * 32 + 32 <= k; }   // whether the rows have all of tile t
+    __device__ __forceinline__ void fetch(int t, int place)
     {
         if (whole(t)) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) held[i].load(word[i] + 64LL * t, word[i] + 64LL * t + 16);
+            for (int i = 0; i < kWords; ++i) held[place][i] = load_word(word[i] + 64LL * t);
         } else {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) held[i].load_until(word[i] + 64LL * t, end);
+            for (int i = 0; i < kWords; ++i) held[place][i] = load_word(word[i] + 64LL * t < end ? word[i] + 64LL * t : end);
         }
     }
-    __device__ __forceinline__ void commit(char *lds, int t)
+    // With one body of the loop all tiles move on a place, and the last one is free; else the stored tile's place is.
+    __device__ __forceinline__ int freed(int bodies, int place)
     {
+        if (bodies > 1) return place;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            i32x4 v = held[i].shifted(shift[i]);
-            if (!whole(t)) v = Words::kept(v, k - (t * 4 + piece) * 8);
-            *(i32x4 *)(lds + i * THREADS * 16 + threadIdx.x * 16) = v;
+        for (int r = 0; r + 1 < RING; ++r)
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) held[r][i] = held[r + 1][i];
+        return RING - 1;
+    }
+    // A tile is stored when the first words of the one behind it are there.
+    __device__ __forceinline__ void commit(char *lds, int t, int place)
+    {
+        const int j = threadIdx.x & 15, row = threadIdx.x >> 4;   // rows of the other words: multiples of 8 further
+        char *to = lds + row * 64 + (((j >> 2) ^ ((row >> 1) & 3)) * 16) + (j & 3) * 4;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            // the next word: the next lane's, and of the last lane the first of the tile behind
+            unsigned next = __builtin_amdgcn_update_dpp(0, held[place][i], 0x101, 0xf, 0xf, true);     // row_shl 1
+            next = __builtin_amdgcn_update_dpp(next, held[(place + 1) % RING][i], 0x11f, 0xf, 0xf, false);         // row_shr 15
+            unsigned v = __builtin_amdgcn_alignbyte(next, held[place][i], shift[i]);
+            if (!whole(t)) v = kept_word(v, k - t * 32 - j * 2);
+            *(unsigned *)(to + i * (THREADS / 16) * 64) = v;
         }
     }
     // 16 rows from r0 (a multiple of 16): lane l has row l % 16, piece l / 16
@@ -176,7 +194,7 @@ struct Across {
     __device__ __forceinline__ void init(const char *base_, unsigned long long bytes, long long ld_, int c0, int cols_, int k_)
     {
         if constexpr (ALIGNED) from = buffer_of(base_, bytes);
-        else end = Words::end_of(base_, bytes);
+        else end = end_of(base_, bytes);
         inside = c0 + COLS <= cols_;
         const int place = threadIdx.x % kPieces, r = threadIdx.x / kPieces;
         cols = cols_;
@@ -211,7 +229,7 @@ struct Across {
         for (int i = 0; i < kLoads; ++i) {
             p[i] = base + ld * (GATHER ? given(rows, i) : t * 32 + tile_row(i)) + 2LL * col[i & 1];
             shift[i] = Words::shift_of(p[i]);
-            p[i] = Words::word_of(p[i]);
+            p[i] = word_of(p[i]);
         }
         if (whole(t)) {
 #pragma unroll

@@ -136,6 +136,49 @@ def test_mm_around_the_rows_where_another_kernel_takes_over(mean, n, k, shift):
             close(y[b:f], z, slack, dtype, f"expert {i}")
 
 
+@pytest.mark.parametrize("experts", [5, 150])
+@pytest.mark.parametrize("mean", [3, 4, 5, 23, 24, 25, 300])
+def test_mm_unaligned_around_the_rows_where_another_kernel_takes_over(mean, experts):
+    g, dtype, n, k = gen(mean), "f16", 70, 331
+    counts = [mean] * experts
+    counts[1], counts[3], counts[4] = 0, 2 * mean - 1, 1
+    slots = mean * experts
+    x = torch.randn(slots, k, generator=g, device=DEV).to(TORCH[dtype])
+    for act in (0, 1):
+        w = (torch.randn(experts, (1 + act) * n, k, generator=g, device=DEV) * k ** -0.5).to(TORCH[dtype])
+        y, ld_y = strided(torch.full((slots, n), 7.0, dtype=TORCH[dtype], device=DEV), n, 1)
+        pf.moe_mm(x, slots, None, 1, w, offsets_of(counts), experts, slots, n, k, y, dtype=dtype, act="swiglu" if act else "none", ld_y=ld_y)
+        for i, b, f in groups(counts):
+            if b == f:
+                continue
+            z, slack = product(x[b:f], w[i])
+            if act:
+                z, slack = swiglu(z[:, :n], z[:, n:], slack[:, :n], slack[:, n:])
+            close(y[b:f], z, slack, dtype, f"expert {i}")
+
+
+def test_mm_values_behind_unaligned_rows_do_not_matter():
+    """Rows of odd length that start at odd elements, with NaN around them: the words that are loaded hold some of it."""
+    g, dtype = gen(8), "bf16"
+    for experts, mean, n, k in ((5, 3, 9, 31), (5, 40, 67, 33), (40, 200, 70, 97), (3, 700, 33, 1)):
+        counts = [mean] * experts
+        slots = mean * experts
+        x, ld_x = strided(torch.randn(slots, k, generator=g, device=DEV).to(TORCH[dtype]), k + 2, 1)
+        flat = torch.full((experts * n * k + 9,), NAN, dtype=TORCH[dtype], device=DEV)
+        w = flat[3:3 + experts * n * k].view(experts, n, k)
+        w.copy_(torch.randn(experts, n, k, generator=g, device=DEV) * k ** -0.5)
+        dy, ld_dy = strided(torch.randn(slots, n, generator=g, device=DEV).to(TORCH[dtype]), n + 2, 1)
+        y, dx, dw = (torch.empty(*s, dtype=t, device=DEV) for s, t in (((slots, n), TORCH[dtype]), ((slots, k), TORCH[dtype]), ((experts, n, k), torch.float32)))
+        off = offsets_of(counts)
+        pf.moe_mm(x, slots, None, 1, w, off, experts, slots, n, k, y, dtype=dtype, ld_x=ld_x)
+        pf.moe_mm_dx(dy, w, off, experts, slots, n, k, dx, dtype=dtype, ld_dy=ld_dy)
+        pf.moe_mm_dw(dy, x, slots, None, 1, off, experts, slots, n, k, dw, dtype=dtype, dw_dtype="f32", ld_dy=ld_dy, ld_x=ld_x)
+        for i, b, f in groups(counts):
+            close(y[b:f], *product(x[b:f], w[i]), dtype, "y")
+            close(dx[b:f], *product(dy[b:f], w[i].t()), dtype, "dx")
+            close(dw[i], *product(dy[b:f].t(), x[b:f].t()), "f32", "dw")
+
+
 def test_same_bits_each_time():
     g, counts, slots, rows, x, w = operands(300, 60, 264, 136, "bf16", 1, True, 5)
     off = offsets_of(counts)
