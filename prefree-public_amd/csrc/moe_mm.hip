@@ -173,6 +173,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        if constexpr (FP4) formed<FM>(acc);
         __builtin_amdgcn_sched_barrier(0);
         if (FP4 && S::whole(s + 4, k / 32)) wait_and_meet<LOADS + S::kLoads>();   // the scales' loads as well
         else wait_and_meet<ALIGNED ? LOADS : 63>();

@@ -1,11 +1,11 @@
 // moe_mm_stream.hip — grouped products with many rows an expert: one workgroup a CU takes tile after tile, its loads
 // running ahead of the products across the tiles' ends.
 //
-// 8192 tokens x 4 of 32 experts, 2048 -> 2 x 2048, SwiGLU, bf16: 545 us, 1.01 PFLOP/s; a library's product of the same
+// 8192 tokens x 4 of 32 experts, 2048 -> 2 x 2048, SwiGLU, bf16: 526 us, 1.05 PFLOP/s; a library's product of the same
 // size in one piece 366 to 400.  In one piece this kernel takes 503: its loads and LDS reads cost power, and the clock
 // falls to 1.75 GHz (all-zero operands 402; without loads to LDS 440, without LDS reads 443, without either 340; without
 // the meetings of the waves no less).  Ragged rows add 7% of rows that are not there and a tenth round of tiles where
-// 9.2 would do.  With 4-bit operands 237 us, 2.3 PFLOP/s; gradients of 16384 slots of 16 experts, 2048 x 2048, 168 us (dx)
+// 9.2 would do.  With 4-bit operands 216 us, 2.5 PFLOP/s; gradients of 16384 slots of 16 experts, 2048 x 2048, 168 us (dx)
 // and 180 us (dw, fp32).
 #include "moe_tiles.hpp"
 
@@ -314,6 +314,7 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        if constexpr (FP4) formed<FMV>(acc);
         rows = looked_up(rows_next);
         // The tile after the next has to be there: this step's loads may still be on their way, and after an output
         // tile's end, where all before them are there, stores besides.
