@@ -335,8 +335,12 @@ __device__ __forceinline__ void store_columns(char *row, bool is, int n0, int ha
     unsigned h[N][2];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const T x[4] = {(T)v[i][0], (T)v[i][1], (T)v[i][2], (T)v[i][3]};
-        __builtin_memcpy(h[i], x, 8);
+        // by pairs: one conversion instruction a pair to bf16, rather than one a value and two to join them
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        typedef T t2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+            h[i][c] = __builtin_bit_cast(unsigned, __builtin_convertvector((f2{v[i][2 * c], v[i][2 * c + 1]}), t2));
     }
     gather_columns<N>(h);
     if (!is) return;
