@@ -1,7 +1,7 @@
 // moe_mm_stream.hip — grouped products with many rows an expert: one workgroup a CU takes tile after tile, its loads
 // running ahead of the products across the tiles' ends.
 //
-// 8192 tokens x 4 of 32 experts, 2048 -> 2 x 2048, SwiGLU, bf16: 526 us, 1.05 PFLOP/s; a library's product of the same
+// 8192 tokens x 4 of 32 experts, 2048 -> 2 x 2048, SwiGLU, bf16: 526 us (to 554 on a warm card), 1.05 PFLOP/s; a library's product of the same
 // size in one piece 366 to 400.  In one piece this kernel takes 503: its loads and LDS reads cost power, and the clock
 // falls to 1.75 GHz (all-zero operands 402; without loads to LDS 440, without LDS reads 443, without either 340; without
 // the meetings of the waves no less).  Ragged rows add 7% of rows that are not there and a tenth round of tiles where
