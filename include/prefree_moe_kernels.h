@@ -16,8 +16,19 @@
 extern "C" {
 #endif
 
-/* Tokens per workgroup of the routing kernels: one count of each expert per such block in the workspace. */
+/* Workspace of the routing kernels.  With one block of PFK_MOE_ROUTE_BLOCK tokens there is none.  Else it holds the counts,
+ * a row of bytes a block, each row as many whole words as hold a byte an expert; and behind them, for more than
+ * PFK_MOE_ROUTE_DIRECT blocks, the sums of each PFK_MOE_ROUTE_SUPER whole blocks, a word an expert.  The library that
+ * says how large it is and the one that fills it both take it from here. */
 #define PFK_MOE_ROUTE_BLOCK 64
+#define PFK_MOE_ROUTE_DIRECT 1024
+#define PFK_MOE_ROUTE_SUPER 64
+#define PFK_MOE_ROUTE_BLOCKS(tokens) (((long long)(tokens) + PFK_MOE_ROUTE_BLOCK - 1) / PFK_MOE_ROUTE_BLOCK)
+#define PFK_MOE_ROUTE_ROW_WORDS(experts) (((experts) + 3) / 4)
+/* words of the counts, and of the sums behind them */
+#define PFK_MOE_ROUTE_COUNT_WORDS(blocks, experts) ((long long)(blocks) * PFK_MOE_ROUTE_ROW_WORDS(experts))
+#define PFK_MOE_ROUTE_SUPER_WORDS(blocks, experts) \
+    ((blocks) > PFK_MOE_ROUTE_DIRECT ? (long long)(blocks) / PFK_MOE_ROUTE_SUPER * (experts) : 0LL)
 
 int pfk_moe_route(const void *logits, long long ld, int dtype, int tokens, int experts, int top_k, int normalise,
                   int *choice, float *weight, int *offsets, int *order, int *slot, int *counts, void *stream);

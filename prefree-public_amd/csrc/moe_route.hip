@@ -10,8 +10,7 @@ using namespace pfmoe;
 
 constexpr int kBlock = PFK_MOE_ROUTE_BLOCK;  // tokens a workgroup: one bit each in a 64-bit mask of an expert
 static_assert(kBlock == 64, "masks of 64 tokens");
-constexpr int kDirect = 1024;                // blocks up to which each workgroup sums the counts before it itself
-constexpr int kSuper = 64;                   // blocks whose counts are summed beforehand above that
+constexpr int kSuper = PFK_MOE_ROUTE_SUPER;  // blocks whose counts are summed beforehand, where each workgroup does not sum all
 
 template <typename T>
 __device__ __forceinline__ float as_float(T v) { return (float)v; }
@@ -45,7 +44,7 @@ struct Route {
 };
 
 // Counts are read four experts a word: their rows are whole words, zeros behind the last expert.
-__device__ __host__ constexpr int counts_ld(int experts) { return (experts + 3) & ~3; }
+__device__ constexpr int counts_ld(int experts) { return 4 * PFK_MOE_ROUTE_ROW_WORDS(experts); }
 
 // The largest of v, and the smallest of i, over the G = 16 or 64 lanes of a token; every lane has it.
 template <int G>
@@ -545,10 +544,10 @@ extern "C" {
 int pfk_moe_route(const void *logits, long long ld, int dtype, int tokens, int experts, int top_k, int normalise,
                   int *choice, float *weight, int *offsets, int *order, int *slot, int *counts, void *stream)
 {
-    Route a = {logits, ld, tokens, experts, top_k, normalise, (tokens + kBlock - 1) / kBlock, choice, weight, offsets, order, slot, nullptr, nullptr};
+    Route a = {logits, ld, tokens, experts, top_k, normalise, (int)PFK_MOE_ROUTE_BLOCKS(tokens), choice, weight, offsets, order, slot, nullptr, nullptr};
     if (a.blocks < 1) a.blocks = 1;
     if (a.blocks > 1) a.counts = (unsigned char *)counts;
-    if (a.blocks > kDirect) a.super = counts + (long long)a.blocks * (counts_ld(experts) / 4);
+    if (PFK_MOE_ROUTE_SUPER_WORDS(a.blocks, experts) > 0) a.super = counts + PFK_MOE_ROUTE_COUNT_WORDS(a.blocks, experts);
     hipStream_t s = (hipStream_t)stream;
     return dtype == PF_F32 ? route<float>(a, s) : dtype == PF_F16 ? route<f16>(a, s) : route<bf16>(a, s);
 }

@@ -4,6 +4,7 @@
 #include "prefree_kernels.h"
 #include "prefree_moe_kernels.h"
 
+#include <algorithm>
 #include <climits>
 #include <cstdint>
 #include <string>
@@ -62,7 +63,11 @@ extern "C" {
 size_t pf_moe_route_workspace(int tokens, int experts)
 {
     if (tokens < 1 || experts < 1) return 0;
-    return (size_t)4 * experts * (((size_t)tokens + PFK_MOE_ROUTE_BLOCK - 1) / PFK_MOE_ROUTE_BLOCK);
+    const long long blocks = PFK_MOE_ROUTE_BLOCKS(tokens);
+    const long long words = PFK_MOE_ROUTE_COUNT_WORDS(blocks, experts) + PFK_MOE_ROUTE_SUPER_WORDS(blocks, experts);
+    // A word for each expert of a block holds both, but for one expert above 1024 blocks.  It stays the least that is
+    // asked for, so that a caller's reservation does not depend on how counts are packed.
+    return 4 * (size_t)std::max(words, blocks * experts);
 }
 
 int pf_moe_route(const void *logits, long long ld_logits, int dtype, int tokens, int experts, int top_k, int normalise,
