@@ -126,14 +126,20 @@ __global__ __launch_bounds__(256) void k_dequantize(const unsigned char *codes, 
     }
 }
 
+// rows that one launch takes
+long long most_rows(int per_row) { return most_workgroups(256) * 256 * kUnits / per_row; }
+unsigned workgroups(long long units) { return (unsigned)((units + 256 * kUnits - 1) / (256 * kUnits)); }
+
 template <typename T>
 int quantize(const void *x, long long ld, int rows, int k, void *codes, void *scales, hipStream_t s)
 {
-    const long long units = (long long)rows * (k / 8), grid = (units + 256 * kUnits - 1) / (256 * kUnits);
-    if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "4-bit blocks: too many elements");
     const bool vector = (uintptr_t)x % 16 == 0 && ld * sizeof(T) % 16 == 0;
-    if (vector) k_quantize<T, true><<<dim3((unsigned)grid), dim3(256), 0, s>>>((const T *)x, ld, units, k / 8, (unsigned *)codes, (unsigned char *)scales);
-    else k_quantize<T, false><<<dim3((unsigned)grid), dim3(256), 0, s>>>((const T *)x, ld, units, k / 8, (unsigned *)codes, (unsigned char *)scales);
+    const auto kernel = vector ? k_quantize<T, true> : k_quantize<T, false>;
+    in_launches(rows, most_rows(k / 8), [&](long long first, long long count) {
+        const long long units = count * (k / 8);
+        kernel<<<dim3(workgroups(units)), dim3(256), 0, s>>>((const T *)x + ld * first, ld, units, k / 8,
+                                                             (unsigned *)codes + first * (k / 8), (unsigned char *)scales + first * (k / 32));
+    });
     return pfk_internal_launched("k_quantize");
 }
 
@@ -141,12 +147,14 @@ template <typename T>
 int dequantize(const void *codes, const void *scales, int rows, int k, void *y, long long ld, hipStream_t s)
 {
     const int per_row = k / (16 / (int)sizeof(T));
-    const long long units = (long long)rows * per_row, grid = (units + 256 * kUnits - 1) / (256 * kUnits);
-    if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "4-bit blocks: too many elements");
     const bool vector = (uintptr_t)y % 16 == 0 && ld * sizeof(T) % 16 == 0;
-    const unsigned char *c = (const unsigned char *)codes, *e = (const unsigned char *)scales;
-    if (vector) k_dequantize<T, true><<<dim3((unsigned)grid), dim3(256), 0, s>>>(c, e, units, per_row, (T *)y, ld);
-    else k_dequantize<T, false><<<dim3((unsigned)grid), dim3(256), 0, s>>>(c, e, units, per_row, (T *)y, ld);
+    const auto kernel = vector ? k_dequantize<T, true> : k_dequantize<T, false>;
+    in_launches(rows, most_rows(per_row), [&](long long first, long long count) {
+        const long long units = count * per_row;
+        kernel<<<dim3(workgroups(units)), dim3(256), 0, s>>>((const unsigned char *)codes + first * (k / 2),
+                                                             (const unsigned char *)scales + first * (k / 32), units, per_row,
+                                                             (T *)y + ld * first, ld);
+    });
     return pfk_internal_launched("k_dequantize");
 }
 

@@ -41,6 +41,7 @@ struct Route {
     int *offsets, *order, *slot;
     unsigned char *counts;  // [blocks][counts_ld(experts)]
     int *super;             // [blocks / kSuper][experts], behind the counts
+    int first;              // block of the launch's first workgroup
 };
 
 // Counts are read four experts a word: their rows are whole words, zeros behind the last expert.
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(1024) void k_route(const Route a)
 {
     __shared__ unsigned long long mask[PER * G];
     __shared__ int total[PER * G], first[PER * G], used;
-    const int block = blockIdx.x;
+    const int block = a.first + blockIdx.x;
     for (int e = threadIdx.x; e < a.experts; e += blockDim.x) mask[e] = 0;
     __syncthreads();
     for (int i = threadIdx.x / G; i < kBlock; i += 1024 / G) {   // whole waves: each lane's group has a token or none
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(1024) void k_route_place(const Route a)
     extern __shared__ unsigned long long lds[];
     unsigned long long *mask = lds;
     int *total = (int *)(lds + a.experts), *before = total + a.experts, *first = before + a.experts, *used = first + a.experts;
-    const int block = blockIdx.x;
+    const int block = a.first + blockIdx.x;
     for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
         mask[e] = 0;
         total[e] = before[e] = 0;
@@ -460,18 +461,25 @@ __global__ __launch_bounds__(256) void k_swiglu_backward(const T *dh, long long 
 }
 
 template <typename T>
-int route(const Route &a, hipStream_t s)
+int route(Route a, hipStream_t s)
 {
-    const dim3 grid(a.blocks), block(1024);
-    if (a.experts <= 64) k_route<T, 16, 4><<<grid, block, 0, s>>>(a);
-    else if (a.experts <= 128) k_route<T, 16, 8><<<grid, block, 0, s>>>(a);
-    else if (a.experts <= 256) k_route<T, 16, 16><<<grid, block, 0, s>>>(a);
-    else if (a.experts <= 512) k_route<T, 64, 8><<<grid, block, 0, s>>>(a);
-    else k_route<T, 64, 16><<<grid, block, 0, s>>>(a);
+    constexpr int kThreads = 1024;
+    in_launches(a.blocks, most_workgroups(kThreads), [&](long long first, long long count) {
+        const dim3 grid((unsigned)count), block(kThreads);
+        a.first = (int)first;
+        if (a.experts <= 64) k_route<T, 16, 4><<<grid, block, 0, s>>>(a);
+        else if (a.experts <= 128) k_route<T, 16, 8><<<grid, block, 0, s>>>(a);
+        else if (a.experts <= 256) k_route<T, 16, 16><<<grid, block, 0, s>>>(a);
+        else if (a.experts <= 512) k_route<T, 64, 8><<<grid, block, 0, s>>>(a);
+        else k_route<T, 64, 16><<<grid, block, 0, s>>>(a);
+    });
     if (a.blocks > 1) {
         const size_t lds = (size_t)a.experts * 20 + 8;
         if (a.super) k_route_super<<<dim3(a.blocks / kSuper), dim3(256), 0, s>>>(a);
-        k_route_place<<<grid, block, lds, s>>>(a);
+        in_launches(a.blocks, most_workgroups(kThreads), [&](long long first, long long count) {
+            a.first = (int)first;
+            k_route_place<<<dim3((unsigned)count), dim3(kThreads), lds, s>>>(a);
+        });
     }
     return pfk_internal_launched("k_route");
 }
@@ -480,17 +488,21 @@ template <typename T>
 int route_backward(const void *logits, long long ld, int tokens, int experts, int top_k, int normalise, const int *choice,
                    const float *weight, const float *dweight, void *dlogits, long long ld_d, hipStream_t s)
 {
-    const dim3 grid((tokens + 3) / 4), block(256);
-    const T *z = (const T *)logits;
-    T *dz = (T *)dlogits;
-#define PFK_BACKWARD(PER) \
-    k_route_backward<T, PER><<<grid, block, 0, s>>>(z, ld, tokens, experts, top_k, normalise, choice, weight, dweight, dz, ld_d)
-    if (experts <= 64) PFK_BACKWARD(1);
-    else if (experts <= 128) PFK_BACKWARD(2);
-    else if (experts <= 256) PFK_BACKWARD(4);
-    else if (experts <= 512) PFK_BACKWARD(8);
-    else PFK_BACKWARD(16);
+    in_launches(tokens, most_workgroups(256) * 4, [&](long long first, long long count) {
+        const dim3 grid((unsigned)((count + 3) / 4)), block(256);
+        const T *z = (const T *)logits + ld * first;
+        T *dz = (T *)dlogits + ld_d * first;
+        const long long at = first * top_k;
+#define PFK_BACKWARD(PER)                                                                                                  \
+    k_route_backward<T, PER><<<grid, block, 0, s>>>(z, ld, (int)count, experts, top_k, normalise, choice + at, weight + at, \
+                                                    dweight + at, dz, ld_d)
+        if (experts <= 64) PFK_BACKWARD(1);
+        else if (experts <= 128) PFK_BACKWARD(2);
+        else if (experts <= 256) PFK_BACKWARD(4);
+        else if (experts <= 512) PFK_BACKWARD(8);
+        else PFK_BACKWARD(16);
 #undef PFK_BACKWARD
+    });
     return pfk_internal_launched("k_route_backward");
 }
 
@@ -502,11 +514,12 @@ int combine(const void *y, long long ld_y, int slots, const int *slot, const flo
             void *out, long long ld_out, hipStream_t s)
 {
     const int parts = (width + 511) / 512;
-    const dim3 grid((unsigned)(((long long)tokens * parts + 3) / 4)), block(256);
-    if (whole(y, ld_y, width) && whole(out, ld_out, width))
-        k_combine<T, true><<<grid, block, 0, s>>>((const T *)y, ld_y, slots, slot, weight, tokens, top_k, width, (T *)out, ld_out, parts);
-    else
-        k_combine<T, false><<<grid, block, 0, s>>>((const T *)y, ld_y, slots, slot, weight, tokens, top_k, width, (T *)out, ld_out, parts);
+    const auto kernel = whole(y, ld_y, width) && whole(out, ld_out, width) ? k_combine<T, true> : k_combine<T, false>;
+    in_launches(tokens, most_workgroups(256) * 4 / parts, [&](long long first, long long count) {
+        kernel<<<dim3((unsigned)((count * parts + 3) / 4)), dim3(256), 0, s>>>(
+            (const T *)y, ld_y, slots, slot + first * top_k, weight ? weight + first * top_k : nullptr, (int)count, top_k, width,
+            (T *)out + ld_out * first, ld_out, parts);
+    });
     return pfk_internal_launched("k_combine");
 }
 
@@ -515,11 +528,13 @@ int combine_backward(const void *dout, long long ld_dout, const void *y, long lo
                      const float *weight, int tokens, int top_k, int width, void *dy, long long ld_dy, float *dweight,
                      hipStream_t s)
 {
-    const dim3 grid(tokens), block(256);
-    if (whole(dout, ld_dout, width) && whole(y, ld_y, width) && whole(dy, ld_dy, width))
-        k_combine_backward<T, true><<<grid, block, 0, s>>>((const T *)dout, ld_dout, (const T *)y, ld_y, slots, slot, weight, top_k, width, (T *)dy, ld_dy, dweight);
-    else
-        k_combine_backward<T, false><<<grid, block, 0, s>>>((const T *)dout, ld_dout, (const T *)y, ld_y, slots, slot, weight, top_k, width, (T *)dy, ld_dy, dweight);
+    const bool vector = whole(dout, ld_dout, width) && whole(y, ld_y, width) && whole(dy, ld_dy, width);
+    const auto kernel = vector ? k_combine_backward<T, true> : k_combine_backward<T, false>;
+    in_launches(tokens, most_workgroups(256), [&](long long first, long long count) {
+        kernel<<<dim3((unsigned)count), dim3(256), 0, s>>>(
+            (const T *)dout + ld_dout * first, ld_dout, (const T *)y, ld_y, slots, slot + first * top_k,
+            weight ? weight + first * top_k : nullptr, top_k, width, (T *)dy, ld_dy, dweight + first * top_k);
+    });
     return pfk_internal_launched("k_combine_backward");
 }
 
@@ -528,12 +543,13 @@ int swiglu_backward(const void *dh, long long ld_dh, const void *pre, long long 
                     long long ld_dpre, hipStream_t s)
 {
     const int parts = (n + 7) / 8;
-    const long long grid = ((long long)rows * parts + 255) / 256;
-    if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "activation's gradient: too many elements");
-    if (whole(dh, ld_dh, n) && whole(pre, ld_pre, n) && whole(dpre, ld_dpre, n))
-        k_swiglu_backward<T, true><<<dim3((unsigned)grid), dim3(256), 0, s>>>((const T *)dh, ld_dh, (const T *)pre, ld_pre, rows, n, (T *)dpre, ld_dpre, parts);
-    else
-        k_swiglu_backward<T, false><<<dim3((unsigned)grid), dim3(256), 0, s>>>((const T *)dh, ld_dh, (const T *)pre, ld_pre, rows, n, (T *)dpre, ld_dpre, parts);
+    const bool vector = whole(dh, ld_dh, n) && whole(pre, ld_pre, n) && whole(dpre, ld_dpre, n);
+    const auto kernel = vector ? k_swiglu_backward<T, true> : k_swiglu_backward<T, false>;
+    in_launches(rows, most_workgroups(256) * 256 / parts, [&](long long first, long long count) {
+        kernel<<<dim3((unsigned)((count * parts + 255) / 256)), dim3(256), 0, s>>>(
+            (const T *)dh + ld_dh * first, ld_dh, (const T *)pre + ld_pre * first, ld_pre, (int)count, n,
+            (T *)dpre + ld_dpre * first, ld_dpre, parts);
+    });
     return pfk_internal_launched("k_swiglu_backward");
 }
 
@@ -544,7 +560,7 @@ extern "C" {
 int pfk_moe_route(const void *logits, long long ld, int dtype, int tokens, int experts, int top_k, int normalise,
                   int *choice, float *weight, int *offsets, int *order, int *slot, int *counts, void *stream)
 {
-    Route a = {logits, ld, tokens, experts, top_k, normalise, (int)PFK_MOE_ROUTE_BLOCKS(tokens), choice, weight, offsets, order, slot, nullptr, nullptr};
+    Route a = {logits, ld, tokens, experts, top_k, normalise, (int)PFK_MOE_ROUTE_BLOCKS(tokens), choice, weight, offsets, order, slot, nullptr, nullptr, 0};
     if (a.blocks < 1) a.blocks = 1;
     if (a.blocks > 1) a.counts = (unsigned char *)counts;
     if (PFK_MOE_ROUTE_SUPER_WORDS(a.blocks, experts) > 0) a.super = counts + PFK_MOE_ROUTE_COUNT_WORDS(a.blocks, experts);

@@ -38,3 +38,84 @@ def test_route_stays_inside_its_workspace(tokens, experts):
     ref = dict(zip(("choice", "weight", "offsets", "order", "slot"), route_reference(z.double().cpu().numpy(), top_k, True)))
     for name in ("choice", "offsets", "order", "slot"):
         assert np.array_equal(got[name].cpu().numpy(), ref[name].reshape(-1)), name
+
+
+# ---- more work items than one launch has (2^32) -------------------------------------------------------------------
+
+@pytest.fixture(autouse=True)
+def give_back_memory():
+    yield
+    torch.cuda.empty_cache()
+
+
+def test_route_past_a_launch():
+    """1024 work items take 64 tokens: one launch ends at 2^28 tokens."""
+    tokens, experts = (1 << 28) + 65, 2
+    g = torch.Generator(device=DEV)
+    g.manual_seed(1)
+    z = torch.empty(tokens, experts, dtype=torch.float16, device=DEV).normal_(generator=g)
+    z[3::16] = -float("inf")
+    got = routed(z, 1, "f16")
+    best = (z[:, 1] > z[:, 0]).int()
+    best[z[:, 0] == -float("inf")] = -1          # in rows of which both are
+    assert torch.equal(got["choice"], best)
+    assert torch.equal(got["weight"], (best >= 0).float())
+    del z
+    which = [torch.nonzero(best == e)[:, 0].int() for e in range(experts)]
+    counts = [w.numel() for w in which]
+    used = sum(counts)
+    assert got["offsets"].tolist() == [0, counts[0], used]
+    assert torch.equal(got["order"][:used], torch.cat(which)) and (got["order"][used:] == -1).all()
+    slot = torch.full((tokens,), -1, dtype=torch.int32, device=DEV)
+    slot[got["order"][:used].long()] = torch.arange(used, dtype=torch.int32, device=DEV)
+    assert torch.equal(got["slot"], slot)
+
+
+def test_route_backward_past_a_launch():
+    """A wave a token: one launch ends at 2^26 tokens."""
+    tokens, experts = (1 << 26) + 5, 2
+    g = torch.Generator(device=DEV)
+    g.manual_seed(2)
+    z = torch.randn(tokens, experts, generator=g, device=DEV)
+    choice = (z[:, 1] > z[:, 0]).int()
+    weight = torch.sigmoid((z[:, 1] - z[:, 0]).abs())          # of the larger, over both
+    dweight = torch.randn(tokens, generator=g, device=DEV)
+    dz = torch.full_like(z, NAN)
+    pf.moe_route_backward(z, tokens, experts, 1, choice, weight, dweight, dz, normalise=False)
+    # d weight / d z = w (1 - w) for the chosen and the opposite for the other.  A dozen fp32 roundings of numbers of up to
+    # |dweight|, and of an exponential of up to 20: (12 + 20) 2^-23.
+    want = weight.double() * (1 - weight.double()) * dweight.double()
+    want = torch.where(choice == 1, want, -want)
+    room = 32 * 2.0 ** -23 * dweight.double().abs() + 2.0 ** -126
+    for column, sign in ((1, 1), (0, -1)):
+        assert ((dz[:, column].double() - sign * want).abs() <= room).all()
+
+
+def test_combine_past_a_launch():
+    """A wave a token of up to 512 columns: one launch ends at 2^26 tokens."""
+    tokens = (1 << 26) + 5
+    g = torch.Generator(device=DEV)
+    g.manual_seed(3)
+    y = torch.empty(tokens, 1, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    weight = torch.randn(tokens, generator=g, device=DEV)
+    slot = torch.arange(tokens - 1, -1, -1, dtype=torch.int32, device=DEV)
+    slot[::1000] = -1
+    out = torch.full((tokens, 1), 7.0, dtype=torch.bfloat16, device=DEV)
+    pf.moe_combine(y, slot, weight, tokens, 1, 1, out)
+    want = torch.where(slot >= 0, weight * y.flip(0)[:, 0].float(), 0.0).bfloat16()   # one product, rounded to fp32 and to bf16
+    assert torch.equal(out[:, 0], want)
+
+
+def test_combine_backward_past_a_launch():
+    """A workgroup a token: one launch ends at 2^24 tokens."""
+    tokens, width = (1 << 24) + 9, 3
+    g = torch.Generator(device=DEV)
+    g.manual_seed(4)
+    y, dout = (torch.empty(tokens, width, dtype=torch.float16, device=DEV).normal_(generator=g) for _ in range(2))
+    weight = torch.randn(tokens, generator=g, device=DEV)
+    slot = torch.arange(tokens - 1, -1, -1, dtype=torch.int32, device=DEV)
+    dy, dweight = torch.full_like(y, 7.0), torch.full((tokens,), NAN, device=DEV)
+    pf.moe_combine_backward(dout, y, slot, weight, tokens, 1, width, dy, dweight, dtype="f16")
+    assert torch.equal(dy, (weight[:, None] * dout.float()).half().flip(0))
+    terms = dout.double() * y.flip(0).double()
+    assert ((dweight.double() - terms.sum(1)).abs() <= (width + 2) * 2.0 ** -23 * terms.abs().sum(1)).all()
