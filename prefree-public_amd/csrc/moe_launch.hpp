@@ -1,7 +1,8 @@
 // moe_launch.hpp — error reporting and launch limits that the kernel files of libprefree_kernels.so share.
 #pragma once
 
-// Workgroups of `threads` that one launch may have, since HIP counts a grid's work items in 32 bits; a multiple of the XCDs.
+// Workgroups of `threads` that one launch may have: a grid's work items are counted in 32 bits, and a launch of more reports
+// success and leaves out all but the remainder.  A multiple of the XCDs.
 constexpr long long most_workgroups(int threads) { return 0xffffffffLL / threads / 8 * 8; }
 
 // launch(first, count) over [0, total), no more than `most` at a time.

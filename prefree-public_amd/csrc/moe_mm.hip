@@ -30,17 +30,18 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
     const int tid = threadIdx.x, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
     constexpr int OUT_N = ACT ? BN / 2 : BN;   // results of a tile's row
     const int nt = (a.n + OUT_N - 1) / OUT_N;
+    const int id = a.first + blockIdx.x;
     Tile t;
     if constexpr (MODE == kDw) {
         const int mt = (a.m + BM - 1) / BM, all = a.experts * mt * nt, chunk = (all + kXcds - 1) / kXcds;
-        const int at = (blockIdx.x % kXcds) * chunk + blockIdx.x / kXcds;
-        if ((int)blockIdx.x / kXcds >= chunk || at >= all) return;
+        const int at = id % kXcds * chunk + id / kXcds;
+        if (id / kXcds >= chunk || at >= all) return;
         t.e = at / (mt * nt);
         t.m = at % (mt * nt) % mt;
         t.n = at % (mt * nt) / mt;
         expert_rows(a.offsets, t.e, a.slots, t.begin, t.end);
     } else {
-        if (!find_tile<BM>(a, nt, blockIdx.x, t)) return;
+        if (!find_tile<BM>(a, nt, id, t)) return;
     }
 
     const int k = MODE == kDw ? t.end - t.begin : a.k;
@@ -250,10 +251,7 @@ int launch(const Args &a, hipStream_t stream)
     long long tiles;
     if (MODE == kDw) tiles = (long long)a.experts * ((a.m + BM - 1) / BM) * nt;
     else tiles = ((long long)a.slots / BM + (a.experts < a.slots ? a.experts : a.slots)) * nt;
-    const long long grid = (tiles + kXcds - 1) / kXcds * kXcds;
-    if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "grouped product: too many tiles");
-    k_mm<T, FP4, MODE, ACT, BM, BN, WM, WN, ALIGNED><<<dim3((unsigned)grid), dim3(WM * WN * 64), 0, stream>>>(a);
-    return pfk_internal_launched("k_mm");
+    return launch_tiles(k_mm<T, FP4, MODE, ACT, BM, BN, WM, WN, ALIGNED>, a, tiles, WM * WN * 64, stream, "k_mm");
 }
 
 // Which kernel takes a product.  Figures in us with the weights not in cache, bf16 unless said otherwise; "rows" are an

@@ -24,7 +24,7 @@ __global__ __launch_bounds__(kWaves * kWave, ALIGNED && !ACT ? 4 : 2) void k_mm_
     const int lane = threadIdx.x & (kWave - 1), wave = wave_id(), g = lane >> 4, r = lane & 15;
     const int nt = (a.n + 15) / 16;
     Tile t;
-    if (!find_tile<16>(a, nt, blockIdx.x, t)) return;
+    if (!find_tile<16>(a, nt, a.first + blockIdx.x, t)) return;
     const int m0 = t.m * 16, count = t.end - t.begin, blocks32 = a.k / 32;
 
     // The weights' addresses need the expert alone: their first loads go out before the rows are looked up.
@@ -160,10 +160,7 @@ template <typename T, bool FP4, int ACT, bool ALIGNED>
 int launch_rows(const Args &a, hipStream_t stream)
 {
     const long long tiles = ((long long)a.slots / 16 + (a.experts < a.slots ? a.experts : a.slots)) * ((a.n + 15) / 16);
-    const long long grid = (tiles + kXcds - 1) / kXcds * kXcds;
-    if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "grouped product: too many tiles");
-    k_mm_rows<T, FP4, ACT, ALIGNED><<<dim3((unsigned)grid), dim3(kWaves * kWave), 0, stream>>>(a);
-    return pfk_internal_launched("k_mm_rows");
+    return launch_tiles(k_mm_rows<T, FP4, ACT, ALIGNED>, a, tiles, kWaves * kWave, stream, "k_mm_rows");
 }
 
 template int launch_rows<f16, false, 0, true>(const Args &, hipStream_t);

@@ -23,6 +23,7 @@ struct Args {
     long long ld_p, ld_q, q_expert, ld_out, ld_pre;
     const int *rows, *offsets;
     int row_div, p_rows, experts, slots;
+    int first;           // number of the launch's first workgroup (k_mm, k_mm_rows)
     unsigned div_mul;    // floor(v / row_div) = (v * div_mul >> 32) >> div_shift for 0 <= v < 2^31
     int div_shift;
     int m, n, k;         // m only for kDw; n: results per row (the gate's half under SwiGLU)
@@ -509,6 +510,19 @@ __device__ __forceinline__ bool find_tile(const Args &a, int nt, int id, Tile &t
         before += __builtin_amdgcn_readlane(incl, kWave - 1);
     }
     return false;
+}
+
+// Launches kernel(args) for all `tiles`, whose workgroups number themselves from args.first on; they reach the XCDs in turn.
+template <typename K>
+int launch_tiles(K kernel, Args a, long long tiles, int threads, hipStream_t stream, const char *what)
+{
+    const long long grid = (tiles + kXcds - 1) / kXcds * kXcds;
+    if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "grouped product: too many tiles");   // 32-bit numbers
+    in_launches(grid, most_workgroups(threads), [&](long long first, long long count) {
+        a.first = (int)first;
+        kernel<<<dim3((unsigned)count), dim3(threads), 0, stream>>>(a);
+    });
+    return pfk_internal_launched(what);
 }
 
 // moe_mm_stream.hip

@@ -119,3 +119,71 @@ def test_combine_backward_past_a_launch():
     assert torch.equal(dy, (weight[:, None] * dout.float()).half().flip(0))
     terms = dout.double() * y.flip(0).double()
     assert ((dweight.double() - terms.sum(1)).abs() <= (width + 2) * 2.0 ** -23 * terms.abs().sum(1)).all()
+
+
+# With k = 1 a product of 16-bit numbers has one term, which fp32 holds exactly: it is rounded once, as torch rounds it.
+
+def outer(x, w, out, rows):
+    """Whether out [experts * rows, n] is x [experts * rows] times w [experts, n] of its expert."""
+    for e in range(w.shape[0]):
+        at = slice(e * rows, (e + 1) * rows)
+        if not torch.equal(out[at], x[at, None] * w[e][None]):
+            return False
+    return True
+
+
+@pytest.mark.parametrize("rows,n", [(2, (1 << 18) + 5), (5, (1 << 21) + 9)])
+def test_mm_past_a_launch(rows, n):
+    """16 x 16 tiles (two rows an expert) and 128 x 128 tiles (five) of 256 work items: one launch ends at 2^24 tiles."""
+    experts, dtype = 1024, torch.bfloat16
+    assert experts * -(-n // (16 if rows == 2 else 128)) > 1 << 24
+    g = torch.Generator(device=DEV)
+    g.manual_seed(5)
+    x = torch.empty(experts * rows, 1, dtype=dtype, device=DEV).normal_(generator=g)
+    w = torch.empty(experts, n, 1, dtype=dtype, device=DEV).normal_(generator=g)
+    y = torch.full((experts * rows, n), 7.0, dtype=dtype, device=DEV)
+    off = torch.arange(0, experts * rows + 1, rows, dtype=torch.int32, device=DEV)
+    pf.moe_mm(x, experts * rows, None, 1, w, off, experts, experts * rows, n, 1, y)
+    assert outer(x[:, 0], w[:, :, 0], y, rows)
+
+
+def test_mm_dw_past_a_launch():
+    """256 x 256 tiles of 512 work items: one launch ends at 2^23 tiles."""
+    experts, n, dtype = 1024, (1 << 21) + 300, torch.bfloat16
+    assert experts * -(-n // 256) > 1 << 23
+    g = torch.Generator(device=DEV)
+    g.manual_seed(6)
+    x = torch.empty(experts, 1, dtype=dtype, device=DEV).normal_(generator=g)
+    dy = torch.empty(experts, n, dtype=dtype, device=DEV).normal_(generator=g)
+    dw = torch.full((experts, n, 1), 7.0, dtype=dtype, device=DEV)
+    off = torch.arange(experts + 1, dtype=torch.int32, device=DEV)
+    pf.moe_mm_dw(dy, x, experts, None, 1, off, experts, experts, n, 1, dw)
+    assert outer(x[:, 0], dy, dw[:, :, 0], 1)
+
+
+def test_mm_mx4_past_a_launch():
+    """4-bit operands behind 4 GiB, by 16 x 16 tiles of 256 work items: one launch ends at 2^32 results."""
+    k, n, slots, experts = 64, 2064, 1 << 21, 3
+    x_rows = (1 << 27) + 100
+    g = torch.Generator(device=DEV)
+    g.manual_seed(7)
+    codes = torch.randint(0, 256, (x_rows, k // 2), generator=g, device=DEV, dtype=torch.uint8)
+    w_codes = torch.randint(0, 256, (experts * n, k // 2), generator=g, device=DEV, dtype=torch.uint8)
+    scales, w_scales = (torch.full((v, k // 32), 127, dtype=torch.uint8, device=DEV) for v in (x_rows, experts * n))
+    rows = torch.randint(0, x_rows, (slots,), generator=g, device=DEV).int()
+    rows[::2] = x_rows - 1 - rows[::2] % 1000
+    bounds = [0, 700001, 700001, slots]
+    y = torch.full((slots, n), 7.0, dtype=torch.bfloat16, device=DEV)
+    off = torch.tensor(bounds, dtype=torch.int32, device=DEV)
+    pf.moe_mm_mx4(codes, scales, x_rows, rows, 1, w_codes, w_scales, off, experts, slots, n, k, y)
+    w = torch.empty(experts * n, k, device=DEV)
+    pf.mx4_dequantize(w_codes, w_scales, experts * n, k, w)
+    w = w.view(experts, n, k)
+    # all products are multiples of 1/4 of at most 36, so that fp32 holds their sums exactly in any order
+    for e in range(experts):
+        for b in range(bounds[e], bounds[e + 1], 1 << 18):
+            f = min(b + (1 << 18), bounds[e + 1])
+            at = rows[b:f].long()
+            x = torch.empty(f - b, k, device=DEV)
+            pf.mx4_dequantize(codes[at], scales[at], f - b, k, x)
+            assert torch.equal(y[b:f], (x @ w[e].t()).bfloat16()), (e, b)
