@@ -4605,10 +4605,9 @@ template <typename T>
 int launch_vector(const pfk_spmv_args *a, void *stream)
 {
     const Args<T> r = make_args<T>(a);
-    const long long grid = ((long long)a->m * a->tile + kBS - 1) / kBS;
-    if (grid < 1 || grid > 0x7FFFFFFFLL) {
-        snprintf(g_err, sizeof g_err, "row groups: %lld workgroups", grid);
-        return PF_ERR_UNSUPPORTED;
+    if (a->m < 1) {
+        snprintf(g_err, sizeof g_err, "row groups: %d rows", a->m);
+        return PF_ERR_INVALID;
     }
     if (a->n_dense > 0) {  // long rows beside the row groups
         if (a->tile != PFK_VECTOR_LONG_LANES || !a->dense_rows) {
@@ -4624,14 +4623,22 @@ int launch_vector(const pfk_spmv_args *a, void *stream)
         PFK_LAUNCHED("k_vector_long");
         return PF_OK;
     }
+    void (*kernel)(Args<T>) = nullptr;
     switch (a->tile) {
-    case 2: hipLaunchKernelGGL((k_vector<T, 2>), dim3((unsigned)grid), dim3(kBS), 0, S(stream), r); break;
-    case 4: hipLaunchKernelGGL((k_vector<T, 4>), dim3((unsigned)grid), dim3(kBS), 0, S(stream), r); break;
-    case 8: hipLaunchKernelGGL((k_vector<T, 8>), dim3((unsigned)grid), dim3(kBS), 0, S(stream), r); break;
-    case 16: hipLaunchKernelGGL((k_vector<T, 16>), dim3((unsigned)grid), dim3(kBS), 0, S(stream), r); break;
-    case 32: hipLaunchKernelGGL((k_vector<T, 32>), dim3((unsigned)grid), dim3(kBS), 0, S(stream), r); break;
+    case 2: kernel = k_vector<T, 2>; break;
+    case 4: kernel = k_vector<T, 4>; break;
+    case 8: kernel = k_vector<T, 8>; break;
+    case 16: kernel = k_vector<T, 16>; break;
+    case 32: kernel = k_vector<T, 32>; break;
     default: return PF_ERR_INVALID;
     }
+    in_launches(a->m, most_workgroups(kBS) * (kBS / a->tile), [&](long long first, long long count) {
+        Args<T> piece = r;
+        piece.rp += first;
+        piece.y += first;
+        piece.m = (int)count;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((count * a->tile + kBS - 1) / kBS)), dim3(kBS), 0, S(stream), piece);
+    });
     PFK_LAUNCHED("k_vector");
     return PF_OK;
 }
