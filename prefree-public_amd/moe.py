@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 
-from . import BF16, F16, F32, _check, _p, _s, dtype_code, lib
+from . import BF16, F16, F32, _check, _s, dtype_code, lib
 
 ACTIVATIONS = {"none": 0, "swiglu": 1}
 
@@ -71,10 +71,11 @@ def _buf(obj, kind, name):
 
 
 def _buf_checked(obj, kind, name):
+    """_buf for what it has not seen; kind None: of any type."""
     if obj is None or isinstance(obj, int):
         return obj
     dtype = getattr(obj, "dtype", None)
-    if dtype is not None:
+    if dtype is not None and kind is not None:
         if dtype not in _KINDS:
             _KINDS[dtype] = _kind(dtype)
         if _KINDS[dtype] != kind:
@@ -102,7 +103,7 @@ def moe_route(logits, tokens, experts, top_k, choice, weight, offsets, order, sl
     _check(lib().pf_moe_route(_buf(logits, d, "logits"), ld_logits, d, int(tokens), int(experts), int(top_k),
                               int(bool(normalise)), _buf(choice, "i32", "choice"), _buf(weight, F32, "weight"),
                               _buf(offsets, "i32", "offsets"), _buf(order, "i32", "order"), _buf(slot, "i32", "slot"),
-                              _p(workspace), int(workspace_bytes), _s(stream)), "pf_moe_route")
+                              _buf_checked(workspace, None, "workspace"), int(workspace_bytes), _s(stream)), "pf_moe_route")
 
 
 def moe_route_backward(logits, tokens, experts, top_k, choice, weight, dweight, dlogits, dtype="f32", normalise=True,

@@ -23,3 +23,14 @@ def test_routing_workspace_holds_what_routing_writes(tokens):
 def test_routing_workspace_stays_as_it_was_for_two_experts_and_more(tokens):
     for experts in (2, 3, 4, 5, 8, 33, 128, 1024):
         assert pf.moe_route_workspace(tokens, experts) == 4 * experts * -(-tokens // BLOCK)
+
+
+def test_a_workspace_on_the_host_is_refused_in_python():
+    torch = pytest.importorskip("torch")
+    P = 4096   # a pointer that is never followed
+    for dtype in (torch.uint8, torch.int32):
+        work = torch.zeros(1 << 20, dtype=dtype)
+        with pytest.raises(TypeError):
+            pf.moe_route(P, 100, 8, 2, P, P, P, P, P, work)
+        with pytest.raises(TypeError):
+            pf.moe_route(P, 100, 8, 2, P, P, P, P, P, work, workspace_bytes=1 << 20)
