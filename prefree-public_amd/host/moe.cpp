@@ -38,6 +38,15 @@ long long lead(long long ld, long long width) { return ld == 0 ? width : ld < wi
         if (!aligned(p, bytes)) return pf_internal_fail(PF_ERR_ALIGN, std::string(what) + ": " why); \
     } while (0)
 
+// whether arrays of 32-bit numbers lie on words (NULL does)
+template <typename... P>
+bool on_words(const P *...p) { return (aligned(p, 4) && ...); }
+
+#define PF_CHECK_WORDS(...)                                                                                              \
+    do {                                                                                                                 \
+        if (!on_words(__VA_ARGS__)) return pf_internal_fail(PF_ERR_ALIGN, std::string(what) + ": " #__VA_ARGS__ ": not 4-byte aligned"); \
+    } while (0)
+
 const char *routing(int tokens, int experts, int top_k)
 {
     if (tokens < 0) return "negative number of tokens";
@@ -82,6 +91,7 @@ int pf_moe_route(const void *logits, long long ld_logits, int dtype, int tokens,
     const long long ld = lead(ld_logits, experts);
     PF_CHECK(ld >= 0, "leading dimension under the row's length");
     PF_CHECK_ALIGN(logits, bytes_of(dtype), "logits not aligned to their elements");
+    PF_CHECK_WORDS(choice, weight, offsets, order, slot);
     const size_t need = tokens > PFK_MOE_ROUTE_BLOCK ? pf_moe_route_workspace(tokens, experts) : 0;
     PF_CHECK(need == 0 || (workspace && workspace_bytes >= need), "workspace smaller than pf_moe_route_workspace()");
     PF_CHECK_ALIGN(workspace, 4, "workspace not 4-byte aligned");
@@ -102,6 +112,7 @@ int pf_moe_route_backward(const void *logits, long long ld_logits, int dtype, in
     PF_CHECK(ld >= 0 && ld_d >= 0, "leading dimension under the row's length");
     PF_CHECK_ALIGN(logits, bytes_of(dtype), "logits not aligned to their elements");
     PF_CHECK_ALIGN(dlogits, bytes_of(dtype), "dlogits not aligned to their elements");
+    PF_CHECK_WORDS(choice, weight, dweight);
     return from_kernels(pfk_moe_route_backward(logits, ld, dtype, tokens, experts, top_k, normalise != 0, choice, weight,
                                                dweight, dlogits, ld_d, stream), what);
 }
@@ -119,6 +130,7 @@ int pf_moe_combine(const void *y, long long ld_y, int dtype, int slots, const in
     PF_CHECK(ly >= 0 && lo >= 0, "leading dimension under the row's length");
     PF_CHECK_ALIGN(y, 2, "y not aligned to its elements");
     PF_CHECK_ALIGN(out, 2, "out not aligned to its elements");
+    PF_CHECK_WORDS(slot, weight);
     return from_kernels(pfk_moe_combine(y, ly, dtype, slots, slot, weight, tokens, top_k, width, out, lo, stream), what);
 }
 
@@ -137,6 +149,7 @@ int pf_moe_combine_backward(const void *dout, long long ld_dout, const void *y, 
     PF_CHECK_ALIGN(dout, 2, "dout not aligned to its elements");
     PF_CHECK_ALIGN(y, 2, "y not aligned to its elements");
     PF_CHECK_ALIGN(dy, 2, "dy not aligned to its elements");
+    PF_CHECK_WORDS(slot, weight, dweight);
     return from_kernels(pfk_moe_combine_backward(dout, lo, y, ly, dtype, slots, slot, weight, tokens, top_k, width, dy, ld,
                                                  dweight, stream), what);
 }
@@ -160,6 +173,7 @@ int pf_moe_mm(const void *x, long long ld_x, int x_rows, const int *rows, int ro
     PF_CHECK_ALIGN(w, 2, "w not aligned to its elements");
     PF_CHECK_ALIGN(y, 2, "y not aligned to its elements");
     PF_CHECK_ALIGN(pre, 2, "pre not aligned to its elements");
+    PF_CHECK_WORDS(rows, offsets);
     pfk_moe_mm_args a = {};
     a.p = x; a.ld_p = 2 * lx; a.p_rows = x_rows; a.rows = rows; a.row_div = row_div;
     a.q = w; a.ld_q = 2LL * k; a.offsets = offsets; a.experts = experts; a.slots = slots; a.n = n; a.k = k;
@@ -180,6 +194,7 @@ int pf_moe_mm_dx(const void *dy, long long ld_dy, const void *w, const int *offs
     PF_CHECK_ALIGN(dy, 2, "dy not aligned to its elements");
     PF_CHECK_ALIGN(w, 2, "w not aligned to its elements");
     PF_CHECK_ALIGN(dx, 2, "dx not aligned to its elements");
+    PF_CHECK_WORDS(offsets);
     pfk_moe_mm_args a = {};
     a.p = dy; a.ld_p = 2 * ly; a.p_rows = slots; a.q = w; a.ld_q = 2LL * k;
     a.offsets = offsets; a.experts = experts; a.slots = slots; a.n = n; a.k = k;
@@ -203,6 +218,7 @@ int pf_moe_mm_dw(const void *dy, long long ld_dy, const void *x, long long ld_x,
     PF_CHECK_ALIGN(dy, 2, "dy not aligned to its elements");
     PF_CHECK_ALIGN(x, 2, "x not aligned to its elements");
     PF_CHECK_ALIGN(dw, bytes_of(dw_dtype), "dw not aligned to its elements");
+    PF_CHECK_WORDS(rows, offsets);
     pfk_moe_mm_args a = {};
     a.p = dy; a.ld_p = 2 * ly; a.p_rows = x_rows; a.q = x; a.ld_q = 2 * lx; a.rows = rows; a.row_div = row_div;
     a.offsets = offsets; a.experts = experts; a.slots = slots; a.n = n; a.k = k;
@@ -274,6 +290,7 @@ int pf_moe_mm_mx4(const void *x_codes, const void *x_scales, int x_rows, const i
     PF_CHECK_ALIGN(x_codes, 16, "codes not 16-byte aligned");
     PF_CHECK_ALIGN(w_codes, 16, "codes not 16-byte aligned");
     PF_CHECK_ALIGN(y, 2, "y not aligned to its elements");
+    PF_CHECK_WORDS(rows, offsets);
     pfk_moe_mm_args a = {};
     a.p = x_codes; a.ld_p = k / 2; a.p_scales = x_scales; a.p_rows = x_rows; a.rows = rows; a.row_div = row_div;
     a.q = w_codes; a.ld_q = k / 2; a.q_scales = w_scales; a.offsets = offsets; a.experts = experts; a.slots = slots;

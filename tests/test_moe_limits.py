@@ -34,3 +34,25 @@ def test_a_workspace_on_the_host_is_refused_in_python():
             pf.moe_route(P, 100, 8, 2, P, P, P, P, P, work)
         with pytest.raises(TypeError):
             pf.moe_route(P, 100, 8, 2, P, P, P, P, P, work, workspace_bytes=1 << 20)
+
+
+def test_arrays_of_words_that_do_not_lie_on_words_are_refused():
+    """choice, weight, offsets, order, slot, rows and dweight hold 32-bit numbers.  (No call here is launched.)"""
+    P = 4096
+    odd = P + 2
+
+    def each(call, names):
+        for name in names:
+            with pytest.raises(pf.PrefreeError) as e:
+                call(**{name: odd})
+            assert e.value.status == 2, name        # PF_ERR_ALIGN
+
+    each(lambda choice=P, weight=P, offsets=P, order=P, slot=P: pf.moe_route(
+        P, 100, 8, 2, choice, weight, offsets, order, slot, P, workspace_bytes=1 << 20), ("choice", "weight", "offsets", "order", "slot"))
+    each(lambda choice=P, weight=P, dweight=P: pf.moe_route_backward(P, 4, 8, 2, choice, weight, dweight, P), ("choice", "weight", "dweight"))
+    each(lambda slot=P, weight=P: pf.moe_combine(P, slot, weight, 4, 2, 64, P), ("slot", "weight"))
+    each(lambda slot=P, weight=P, dweight=P: pf.moe_combine_backward(P, P, slot, weight, 4, 2, 64, P, dweight), ("slot", "weight", "dweight"))
+    each(lambda rows=P, offsets=P: pf.moe_mm(P, 10, rows, 1, P, offsets, 4, 10, 64, 64, P), ("rows", "offsets"))
+    each(lambda offsets=P: pf.moe_mm_dx(P, P, offsets, 4, 10, 64, 64, P), ("offsets",))
+    each(lambda rows=P, offsets=P: pf.moe_mm_dw(P, P, 10, rows, 1, offsets, 4, 10, 64, 64, P), ("rows", "offsets"))
+    each(lambda rows=P, offsets=P: pf.moe_mm_mx4(P, P, 10, rows, 1, P, P, offsets, 4, 10, 64, 64, P), ("rows", "offsets"))
