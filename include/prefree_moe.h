@@ -72,8 +72,9 @@ int pf_moe_combine_backward(const void *dout, long long ld_dout, const void *y, 
  *   y[s] = act(x[rows ? rows[s] / row_div : s] w[e]^T)
  * x [x_rows][k], w [experts][n or 2n][k] without gaps, y [slots][n].  With rows = order and row_div = top_k of
  * pf_moe_route the tokens are gathered on the way in.  pre (PF_ACT_SWIGLU only, may be NULL): [slots][2n], what
- * the activation was applied to, for pf_swiglu_backward.  Slots from offsets[experts] on are not written.  A row index
- * outside [0, x_rows) gives an unspecified row (nothing outside x is read); so do offsets that decrease. */
+ * the activation was applied to, for pf_swiglu_backward.  SwiGLU is formed in
+ * fp32 from the sums and then rounded: silu(g) within (8 + |g|) 2^-23 of itself and within 2^-134 at the least, also where
+ * sigmoid(g) is no normal number any more.  Slots from offsets[experts] on are not written.  A row index outside [0, x_rows) gives an unspecified row (nothing outside x is read); so do offsets that decrease. */
 int pf_moe_mm(const void *x, long long ld_x, int x_rows, const int *rows, int row_div, const void *w,
               const int *offsets, int experts, int slots, int n, int k, int dtype, int act, void *y, long long ld_y,
               void *pre, long long ld_pre, void *stream);

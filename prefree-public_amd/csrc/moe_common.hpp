@@ -88,6 +88,13 @@ __device__ __forceinline__ i32x4 load16_any(const void *p)
     return w.shifted(shift);
 }
 
+// 1 / sigmoid(g), times kUnder.  As 1 + exp(-g) it would be infinite for gates under -88.7, and its reciprocal no normal number
+// under -87.3, where silu(g) of bf16 still is one; scaled, both have room down to -98, where silu(g) is under 2^-134, half of
+// the smallest bf16.  The scale is in the exponent (g / ln 2 rounded at up to 32: the exponential is off by 2^-20 of itself
+// at the most, near g = 0) and of 16-bit gates times kUnder nothing is lost.
+constexpr float kUnder = 0x1p-16f;
+__device__ __forceinline__ float inverse_sigmoid(float g) { return kUnder + __builtin_amdgcn_exp2f(__builtin_fmaf(g, -0x1.715476p+0f, -16.0f)); }
+
 // Inclusive sum over the lanes of a wave: inside the rows of 16 lanes by shifts, then the rows' last lanes are handed on
 // (row_bcast 15 to the odd rows, row_bcast 31 to the upper half).  Whole wave active.
 __device__ __forceinline__ int scan_wave(int v)

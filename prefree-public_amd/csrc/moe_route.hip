@@ -437,7 +437,7 @@ __global__ __launch_bounds__(256) void k_combine_backward(const T *dout, long lo
             (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
 }
 
-// h = silu(g) u: dg = dh u s (1 + g (1 - s)), du = dh g s, with s = 1 / (1 + exp(-g)).
+// h = silu(g) u: dg = dh u s (1 + g (1 - s)), du = dh g s, with s = sigmoid(g).
 template <typename T, bool VECTOR>
 __global__ __launch_bounds__(256) void k_swiglu_backward(const T *dh, long long ld_dh, const T *pre, long long ld_pre, int rows,
                                                          int n, T *dpre, long long ld_dpre, int parts)
@@ -452,9 +452,9 @@ __global__ __launch_bounds__(256) void k_swiglu_backward(const T *dh, long long 
     load8<T, VECTOR>(pre + ld_pre * r + n, at, n, u);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float s = 1.0f / (1.0f + __expf(-g[i]));
-        dg[i] = d[i] * u[i] * s * (1.0f + g[i] * (1.0f - s));
-        du[i] = d[i] * g[i] * s;
+        const float s = 1.0f / inverse_sigmoid(g[i]);   // over kUnder
+        dg[i] = d[i] * u[i] * kUnder * s * (1.0f + g[i] * (1.0f - kUnder * s));
+        du[i] = d[i] * (g[i] * kUnder) * s;
     }
     store8<T, VECTOR>(dpre + ld_dpre * r, at, n, dg);
     store8<T, VECTOR>(dpre + ld_dpre * r + n, at, n, du);

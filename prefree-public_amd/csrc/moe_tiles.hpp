@@ -355,8 +355,8 @@ __device__ __forceinline__ void store_columns(char *row, bool is, int n0, int ha
 }
 
 // The reciprocal instruction is within one unit in the last place, where the result is rounded to 16 bits; a division takes
-// eight more instructions for each of a tile's results.  (It gives 0 where it would be below 2^-126: gates under -87.)
-__device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
+// eight more instructions for each of a tile's results.
+__device__ __forceinline__ float silu(float g) { return g * kUnder * __builtin_amdgcn_rcpf(inverse_sigmoid(g)); }
 
 __device__ __forceinline__ int row_of_slot(const Args &a, int s)
 {
