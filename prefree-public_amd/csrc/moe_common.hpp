@@ -10,9 +10,7 @@ namespace pfmoe {
 
 typedef _Float16 f16;
 typedef __bf16 bf16;
-typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
-typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -20,14 +18,12 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-struct fp4 {};  // tag: e2m1 codes, two a byte, one e8m0 scale byte per 32
-
 constexpr int kWave = 64;
 constexpr int kXcds = 8;
 
 template <typename T> struct vec { };
-template <> struct vec<f16> { typedef f16x4 x4; typedef f16x8 x8; };
-template <> struct vec<bf16> { typedef bf16x4 x4; typedef bf16x8 x8; };
+template <> struct vec<f16> { typedef f16x8 x8; };
+template <> struct vec<bf16> { typedef bf16x8 x8; };
 
 // Rows of any alignment are loaded by the whole words that hold them, the elements then shifted into place (rows of 2222
 // bytes out of the L2: 7.4 TB/s, 3.7 with the hardware's unaligned loads).  A word may hold an element that lies outside
