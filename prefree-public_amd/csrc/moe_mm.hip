@@ -259,8 +259,10 @@ int launch(const Args &a, hipStream_t stream)
 //
 // Few rows: k_mm_rows, the weights straight to registers, against the 128 x 128 tiles: 64 experts, 2048 -> 2 x 1024, rows
 // 1: 94 against 115, 8: 104 / 128, 16: 137 / 128; 16 experts, 2048 -> 2048, rows 1: 26 / 37, 8: 32 / 38, 16: 48 / 38.  With
-// many tiles of short rows it loses: 128 experts, 1024 -> 2 x 512, rows 1: 60 / 52, 8: 74 / 56 (1024 tiles of 2 KB rows);
-// 64 experts in 4-bit blocks, rows 1: 40.5 / 40, 8: 48 / 42 (2048 tiles of 1 KB rows).
+// many tiles (512 and more of 128 x 128, which go to k_mm_stream) it depends on the weights' rows.  128 experts, k -> 2 x 512,
+// rows 1, 4, 8 against k_mm_stream: of 1 KB 42, 46, 48 / 32, 33, 33; 2 KB 57, 67, 69 / 54, 57, 57; 3 KB 78, 87, 91 / 82, 85, 86;
+// 3.5 KB 84, 94, 97 / 93, 97, 96; 4 KB 93, 102, 105 / 121, 130, 131; 5 KB 113, 127, 132 / 137, 142, 142.  In 4-bit blocks, of
+// 1 KB 36, 42, 44 / 37, 39, 39; 2 KB 58, 67, 72 / 67, 69, 70; 3 KB 83, 92, 102 / 103, 107, 108; 4 KB 103, 118, 131 / 138, 145, 146.
 //
 // Many: k_mm_stream, 256 x 256 tiles, against 128 x 128.  It wins from a tile a CU on, whatever the rows, since its loads
 // run ahead of everything: dx of 64 experts, 2048 x 2048, rows 1: 91 / 94, 64: 104 / 120, 512: 334 / 409; dw of 16, rows
@@ -274,9 +276,14 @@ int launch(const Args &a, hipStream_t stream)
 // kernel against 64 x 64 and 128 x 128 tiles: 12 experts, 1111 -> 717, rows 8: 15 / 23 / 42, 32: 25 / 24 / 43, 400: 179 /
 // 55 / 61; 16 experts, 2047 -> 2047, 4: 48 / 45 / 74, 64: 189 / 78 / 81, 100: 277 / 105 / 105, 200: 518 / 151 / 113; 64
 // experts, 1025 -> 513, 8: 35 / 34 / 48, 64: 129 / 55 / 59, 400: 661 / 163 / 148; 32 experts, 2047 -> 2 x 1023, 4: 82 / 89 /
-// 98, 16: 120 / 93 / 96, 64: 317 / 136 / 107.  Gradients with 128 x 128 against 256 x 256: 32764 slots of 32 experts, 1023 x
-// 2049, dx 522 / 423, dw 628 / 540; 8000 of 16, 2047 x 2047, dx 243 / 270, dw 377 / 287; 2000 of 16, 1023 x 1025, dx 45 /
-// 72, dw 90 / 91.
+// 98, 16: 120 / 93 / 96, 64: 317 / 136 / 107.  Of the 64 x 64 tiles five go to a CU at a time, 1280 to all: up to about there
+// they win, with 1152 of them (64 experts, 1025 -> 513, rows 64) 55 / 59, (32, 2047 -> 2 x 1023, 8) 90 / 94, with 1280 (the same,
+// 16) 91 / 94, and behind that lose, with 1312 (16, 2047 -> 2047, 100) 105 / 101, (32, 2047 -> 2 x 511, 100) 100 / 96, 1456 (16,
+// 1025 -> 1023, 300) 67 / 63, 1536 (32, 2047 -> 2 x 1023, 32) 104 / 97.  It costs up to 16% where the 128 x 128 tiles, two a CU,
+// just fit a round, with 1024 (32, 2047 -> 2 x 511, 64) 89 / 77, or just do not, with 2112 (16, 2047 -> 2047, 200) 156 / 173.
+//
+// Gradients with 128 x 128 against 256 x 256: 32764 slots of 32 experts, 1023 x 2049, dx 522 / 423, dw 628 / 540; 8000 of 16,
+// 2047 x 2047, dx 243 / 270, dw 377 / 287; 2000 of 16, 1023 x 1025, dx 45 / 72, dw 90 / 91.
 template <typename T, bool FP4, int MODE, int ACT, bool ALIGNED>
 int launch_size(const Args &a, hipStream_t stream)
 {

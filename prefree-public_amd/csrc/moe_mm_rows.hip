@@ -13,8 +13,8 @@ constexpr int kPieces = 4;   // 16-byte pieces of a row that a lane takes at a t
 // fixed order.  Lane l has row l % 16 of both operands and the k that group g = l / 16 takes: of 16-bit elements the
 // pieces g, 4 + g, ... of a block, of 4-bit ones 4 g to 4 g + 3, whose four scales are then one word.
 //
-// Measured with the weights not in cache: one token, 8 of 64 experts, 2048 -> 2 x 1024, 67 MB, in 13.6 us; 67 tokens, 537
-// MB in 109 us, 4.9 TB/s, a large copy's rate.  With the gate a wave has twice the loads on their way, and two waves a SIMD
+// Measured with the weights not in cache: one token, 8 of 64 experts, 2048 -> 2 x 1024, 67 MB, in 12.9 us; 67 tokens, 537
+// MB in 107 to 109 us, 5.0 TB/s (a stream that only reads: 6.2, with non-temporal loads 7.0).  With the gate a wave has twice the loads on their way, and two waves a SIMD
 // with their registers do better than three with a spill (118 us); without it two to four are alike.
 template <typename T, bool FP4, int ACT, bool ALIGNED>
 __global__ __launch_bounds__(kWaves * kWave, ALIGNED && !ACT ? 4 : 2) void k_mm_rows(const Args a)

@@ -1,12 +1,14 @@
 // moe_mm_stream.hip — grouped products with many rows an expert: one workgroup a CU takes tile after tile, its loads
 // running ahead of the products across the tiles' ends.
 //
-// 8192 tokens x 4 of 32 experts, 2048 -> 2 x 2048, SwiGLU, bf16: 526 us (to 554 on a warm card), 1.05 PFLOP/s; a library's product of the same
-// size in one piece 366 to 400.  In one piece this kernel takes 503: its loads and LDS reads cost power, and the clock
-// falls to 1.75 GHz (all-zero operands 402; without loads to LDS 440, without LDS reads 443, without either 340; without
-// the meetings of the waves no less).  Ragged rows add 7% of rows that are not there and a tenth round of tiles where
-// 9.2 would do.  With 4-bit operands 216 us, 2.5 PFLOP/s; gradients of 16384 slots of 16 experts, 2048 x 2048, 168 us (dx)
-// and 180 us (dw, fp32).
+// 8192 tokens x 4 of 32 experts, 2048 -> 2 x 2048, SwiGLU, bf16: 524 to 563 us by the card and how long it has run, 1.0
+// PFLOP/s (with the pre-activations, 268 MB more to write, 565 to 573); a library's product of the same size in one piece 366
+// to 400.  In one piece this kernel takes 503.  The clock falls to 1.75 GHz with random operands, and what is left out then
+// counts by its power: all-zero operands 402; without loads to LDS 440, without LDS reads 443, without either 340; without the
+// meetings of the waves no less.  So what a product costs in LDS reads is the bound, and that follows from the tiling: a wave
+// of 128 x 64 results reads 12 fragments for 32 products.  Ragged rows add 7% of rows that are not there and a tenth round of
+// tiles where 9.2 would do.  With 4-bit operands 215 to 227 us, 2.5 PFLOP/s; gradients of 16384 slots of 16 experts, 2048 x
+// 2048, 166 us (dx) and 177 to 188 us (dw, fp32).
 #include "moe_tiles.hpp"
 
 namespace pfmoe {

@@ -32,8 +32,8 @@ constexpr int kUnits = 4;   // pieces a thread takes, a workgroup's width apart:
 
 // A lane takes eight elements at a time, four lanes a block of 32.  The block's scale exponent is its largest magnitude's
 // exponent less 2, so that magnitude / scale lies in [4, 8); dividing by a power of two is exact, and the conversion
-// instruction rounds to nearest even and saturates at 6, with scale 1.  65536 x 2048 of bf16 (339 MB) in 75 us with the
-// input partly in cache, 93 without: a copy's rate.  (Scales gathered in LDS and written as words: no difference; eight
+// instruction rounds to nearest even and saturates at 6, with scale 1.  65536 x 2048 of bf16, 268 MB read and 71 written, in
+// 61 us, 5.6 TB/s (75 to 93 behind a fp32 result of 537 MB that is still being written back).  (Scales gathered in LDS and written as words: no difference; eight
 // pieces a thread: 15% slower.)
 template <typename T, bool VECTOR>
 __global__ __launch_bounds__(256) void k_quantize(const T *x, long long ld, long long units, int per_row, unsigned *codes,
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void k_quantize(const T *x, long long ld, long
 }
 
 // A lane writes 16 bytes at a time, next to its neighbours': four elements in fp32, eight in 16 bits.  65536 x 2048 to
-// fp32, 608 MB, in 97 us, 6.3 TB/s, near the rate of a large fill.
+// fp32, 608 MB, in 97 us with the codes in cache, 108 without, 5.6 TB/s; a large fill writes 6.9.
 template <typename T, bool VECTOR>
 __global__ __launch_bounds__(256) void k_dequantize(const unsigned char *codes, const unsigned char *scales, long long units,
                                                     int per_row, T *y, long long ld)

@@ -357,7 +357,7 @@ __device__ __forceinline__ void store8(T *row, int at, int have, const float v[8
 }
 
 // out[t] = sum of w y[slot]: a wave takes 512 columns of a token, so that a few tokens already fill many waves.  Bound by
-// reading y: 8191 tokens x 4, 2048 columns, 168 MB in 26.5 us with part of it in cache.
+// reading y: 8191 tokens x 4, 2048 columns, 168 MB in 26.5 us with part of it in cache, 35.5 without.
 template <typename T, bool VECTOR>
 __global__ __launch_bounds__(256) void k_combine(const T *y, long long ld_y, int slots, const int *slot, const float *weight,
                                                  int tokens, int top_k, int width, T *out, long long ld_out, int parts)
@@ -387,7 +387,7 @@ __global__ __launch_bounds__(256) void k_combine(const T *y, long long ld_y, int
 }
 
 // dy[slot] = w dout[t], dweight = <dout[t], y[slot]>: a workgroup a token, which reads dout[t] once for all its slots.
-// Bound by y and dy: 8191 tokens x 4, 2048 columns, 302 MB in 49 us.
+// Bound by y and dy: 8191 tokens x 4, 2048 columns, 302 MB in 49 us with part of it in cache, 60 without.
 template <typename T, bool VECTOR>
 __global__ __launch_bounds__(256) void k_combine_backward(const T *dout, long long ld_dout, const T *y, long long ld_y,
                                                           int slots, const int *slot, const float *weight, int top_k,
@@ -437,7 +437,8 @@ __global__ __launch_bounds__(256) void k_combine_backward(const T *dout, long lo
             (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
 }
 
-// h = silu(g) u: dg = dh u s (1 + g (1 - s)), du = dh g s, with s = sigmoid(g).
+// h = silu(g) u: dg = dh u s (1 + g (1 - s)), du = dh g s, with s = sigmoid(g).  32768 x 2048, 403
+// MB read and 268 written, in 116 us, 5.8 TB/s; rows that do not lie in 16 bytes (32764 x 1023) at 3.6 TB/s.
 template <typename T, bool VECTOR>
 __global__ __launch_bounds__(256) void k_swiglu_backward(const T *dh, long long ld_dh, const T *pre, long long ld_pre, int rows,
                                                          int n, T *dpre, long long ld_dpre, int parts)
