@@ -11,7 +11,11 @@
  *
  * Value types: PF_F16 and PF_BF16 (sums in fp32, each result rounded once, to nearest even), PF_F32 where noted.
  * Leading dimensions (ld*) count elements between rows; 0 stands for the row's length.  Any alignment that the
- * element type has is accepted; rows that all start at multiples of 16 bytes are read faster.
+ * element type has is accepted, less is refused (PF_ERR_ALIGN); rows that all start at multiples of 16 bytes are read
+ * faster.  Sizes: up to 1024 experts, 16 experts a token, 2^30 entries (tokens * top_k), 2^24 columns; offsets pass 32 bits.
+ * Products have a second limit that only costs time: 4 GiB of x or dy, or of one expert's weights.  From there on they
+ * are formed as unaligned ones are (2^20 slots of 16 experts, 2048 x 2048: 1.4 to 2.3 times as long), and 4-bit ones
+ * as those with few rows an expert are (32768 slots of 16 experts, 4096 -> 2048: 9 times as long).
  * No output may overlap an input.  The reference has no counterpart of any of these.
  */
 #ifndef PREFREE_MOE_H
@@ -45,7 +49,7 @@ enum pf_act {
  *   order [tokens*top_k]   slot s holds entry order[s] = token*top_k + j; by expert, then by entry; -1 from
  *                          offsets[experts] on
  *   slot [tokens*top_k]    the inverse: the slot of each entry, -1 where there is none
- * workspace: pf_moe_route_workspace() bytes, 4-byte aligned; what it holds before and after does not matter. */
+ * workspace: pf_moe_route_workspace() bytes, 4-byte aligned (none up to 64 tokens); what it holds before and after does not matter. */
 size_t pf_moe_route_workspace(int tokens, int experts);
 int pf_moe_route(const void *logits, long long ld_logits, int dtype, int tokens, int experts, int top_k, int normalise,
                  int *choice, float *weight, int *offsets, int *order, int *slot, void *workspace,
