@@ -110,6 +110,22 @@ int pf_moe_mm_mx4(const void *x_codes, const void *x_scales, int x_rows, const i
                   const void *w_codes, const void *w_scales, const int *offsets, int experts, int slots, int n, int k,
                   int dtype, int act, void *y, long long ld_y, void *stream);
 
+/* ---- 8-bit integers with a scale a row --------------------------------------------
+ * A row of x: scale = largest magnitude / 127 (the largest magnitude at least 2^-100); integers from -127 to 127, the nearest
+ * to 127 x / largest magnitude, ties to even.  A row that holds an infinity or a NaN has the scale NaN and zeros.
+ *   x [rows][k] (f32, f16, bf16), 1 <= k <= 2^24;
+ *   codes [rows][PF_I8_ROW(k)]: k signed bytes, zeros behind them, 16-byte aligned;  scales [rows], f32. */
+#define PF_I8_ROW(k) (((long long)(k) + 15) / 16 * 16)
+int pf_i8_quantize(const void *x, long long ld_x, int dtype, int rows, int k, void *codes, float *scales, void *stream);
+/* Integer times scale, formed in f32 and rounded to dtype. */
+int pf_i8_dequantize(const void *codes, const float *scales, int rows, int k, int dtype, void *y, long long ld_y, void *stream);
+/* pf_moe_mm of such rows: x (x_codes, x_scales) [x_rows][k], w (w_codes, w_scales) [experts][n or 2n][k], a scale for each
+ * token and each row of w; y in dtype (f16, bf16).  Sums are exact (k at most 131056); they are scaled, and the activation
+ * formed, in f32.  Codes behind a row's k elements are zeros, as pf_i8_quantize writes them; -128 is allowed. */
+int pf_moe_mm_i8(const void *x_codes, const float *x_scales, int x_rows, const int *rows, int row_div, const void *w_codes,
+                 const float *w_scales, const int *offsets, int experts, int slots, int n, int k, int dtype, int act, void *y,
+                 long long ld_y, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

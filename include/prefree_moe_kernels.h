@@ -46,12 +46,14 @@ int pfk_mx4_quantize(const void *x, long long ld_x, int dtype, int rows, int k, 
                      void *stream);
 int pfk_mx4_dequantize(const void *codes, const void *scales, int rows, int k, int dtype, void *y, long long ld_y,
                        void *stream);
+int pfk_i8_quantize(const void *x, long long ld_x, int dtype, int rows, int k, void *codes, float *scales, void *stream);
+int pfk_i8_dequantize(const void *codes, const float *scales, int rows, int k, int dtype, void *y, long long ld_y, void *stream);
 
 /* One grouped product.  Sizes in elements, strides in bytes. */
 typedef struct pfk_moe_mm_args {
     const void *p;          /* rows operand: x or dy */
     long long ld_p;
-    const void *p_scales;   /* 4-bit operands: [p_rows][k / 32] */
+    const void *p_scales;   /* 4-bit operands: [p_rows][k / 32]; 8-bit integers: [p_rows] */
     int p_rows;             /* rows behind p when it is gathered */
     const void *q;          /* the weights, or x for the weights' gradient (then gathered) */
     long long ld_q;
@@ -72,6 +74,7 @@ int pfk_moe_mm(const pfk_moe_mm_args *a, void *stream);
 int pfk_moe_mm_dx(const pfk_moe_mm_args *a, void *stream);
 int pfk_moe_mm_dw(const pfk_moe_mm_args *a, void *stream);
 int pfk_moe_mm_mx4(const pfk_moe_mm_args *a, void *stream);
+int pfk_moe_mm_i8(const pfk_moe_mm_args *a, void *stream);
 
 #ifdef __cplusplus
 }

@@ -12,10 +12,11 @@ using namespace pfmoe;
 // have no registers for that.  An operand along k is loaded by single words, sixteen lanes a row, since the L1 takes one
 // lane a cycle of wider loads that do not lie in their width (32764 slots of 32 experts, 2049 -> 1023, 128 x 128 tiles: 503
 // with 16 bytes a lane, 435 so); an operand across k, with longer rows, by 16 bytes a lane (dw 540, by words 778).
-// T: f16 or bf16 of the results; FP4: 4-bit operands
-template <typename T, bool FP4, int MODE, int ACT, int BM, int BN, int WM, int WN, bool ALIGNED>
+// T: f16 or bf16 of the results; FORM: what the operands hold
+template <typename T, int FORM, int MODE, int ACT, int BM, int BN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
 {
+    constexpr bool FP4 = FORM == kMx4;
     constexpr int THREADS = WM * WN * 64;
     constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
     constexpr int RING = ALIGNED || MODE == kDw ? 1 : BM == 64 ? 4 : 2;   // tiles under way in registers
@@ -45,7 +46,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
     }
 
     const int k = MODE == kDw ? t.end - t.begin : a.k;
-    const int steps = FP4 ? (k + 127) / 128 : (k + 31) / 32;
+    const int steps = (k + kPerTile<FORM> - 1) / kPerTile<FORM>;
     const int m0 = t.m * BM, count = t.end - t.begin;
     // Row of w that row r of the tile stands for.  Under SwiGLU rows of the gate and of the rest take turns of 16, so
     // that a wave holds both.
@@ -63,8 +64,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
         q.init(a.q, span(a.ld_q, a.p_rows, a.n), a.ld_q, t.n * BN, a.n, k);
         if (k > 0) rows = row_of_slot(a, t.begin + min(Q::lookup(0), k - 1));
     } else {
-        p.init(a.p, FP4 ? a.ld_p * a.p_rows : span(a.ld_p, a.p_rows, k), a.ld_p, slot_row, k, FP4 ? 32 : 8);
-        if constexpr (MODE == kFwd) q.init(a.q + a.q_expert * t.e, a.q_expert, a.ld_q, weight_row, k, FP4 ? 32 : 8);
+        p.init(a.p, FORM != kHalf ? a.ld_p * a.p_rows : span(a.ld_p, a.p_rows, k), a.ld_p, slot_row, k, kPerPiece<FORM>);
+        if constexpr (MODE == kFwd) q.init(a.q + a.q_expert * t.e, a.q_expert, a.ld_q, weight_row, k, kPerPiece<FORM>);
         else q.init(a.q + a.q_expert * t.e, a.q_expert, a.ld_q, t.n * BN, a.n, k);
     }
     if constexpr (FP4) {
@@ -123,11 +124,12 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
     const auto scale_x = [&](const char *from, int i) { return FP4 ? S::fragment(from + SCALES, (i * WM + wm) * 16) : 0; };
     const auto scale_w = [&](const char *from, int j) { return FP4 ? S::fragment(from + SCALES, BM + (wn * FN + j) * 16) : 0; };
 
-    f32x4 acc[FM][FN];
+    typedef typename sums_of<FORM>::type SUM;
+    SUM acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+        for (int j = 0; j < FN; ++j) acc[i][j] = SUM{0, 0, 0, 0};
 
     // Four tiles of k in LDS.  While tile s is multiplied its rows' fragments are read two ahead and the columns'
     // fragments of tile s+1 beside them, so that the matrix cores find their operands in registers; tile s+3 is on its
@@ -152,6 +154,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
             for (int j = 0; j < FN; ++j) {
                 if constexpr (FP4) {
                     acc[i][j] = mfma_fp4(w[0][j], x[i % 4], acc[i][j], ws[0][j], xs[i % 4]);
+                } else if constexpr (FORM == kI8) {
+                    acc[i][j] = mfma_i8(w[0][j], x[i % 4], acc[i][j]);
                 } else {
                     acc[i][j] = mfma<T>(w[0][j], x[i % 4], acc[i][j]);
                 }
@@ -240,18 +244,22 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
         wait_and_meet<0>();
     }
 
+    const auto units = [&]() {
+        if constexpr (FORM == kI8) return Units<ACT, FN>{&a, a.q_unit + (ACT ? 2LL : 1LL) * a.n * t.e, (long long)t.begin + m0, wn, t.n * OUT_N};
+        else return NoUnits{};
+    };
     store_results<T, MODE, ACT, FM, FM, FN, WM, OUT_N>(a, acc, wm, wn, MODE == kDw ? (long long)t.e * a.m + m0 : (long long)t.begin + m0,
-                                                MODE == kDw ? a.m - m0 : count - m0, t.n * OUT_N);
+                                                MODE == kDw ? a.m - m0 : count - m0, t.n * OUT_N, units());
 }
 
-template <typename T, bool FP4, int MODE, int ACT, int BM, int BN, int WM, int WN, bool ALIGNED>
+template <typename T, int FORM, int MODE, int ACT, int BM, int BN, int WM, int WN, bool ALIGNED>
 int launch(const Args &a, hipStream_t stream)
 {
     const long long out_n = ACT ? BN / 2 : BN, nt = (a.n + out_n - 1) / out_n;
     long long tiles;
     if (MODE == kDw) tiles = (long long)a.experts * ((a.m + BM - 1) / BM) * nt;
     else tiles = ((long long)a.slots / BM + (a.experts < a.slots ? a.experts : a.slots)) * nt;
-    return launch_tiles(k_mm<T, FP4, MODE, ACT, BM, BN, WM, WN, ALIGNED>, a, tiles, WM * WN * 64, stream, "k_mm");
+    return launch_tiles(k_mm<T, FORM, MODE, ACT, BM, BN, WM, WN, ALIGNED>, a, tiles, WM * WN * 64, stream, "k_mm");
 }
 
 // Which kernel takes a product.  Figures in us with the weights not in cache, bf16 unless said otherwise; "rows" are an
@@ -284,7 +292,7 @@ int launch(const Args &a, hipStream_t stream)
 //
 // Gradients with 128 x 128 against 256 x 256: 32764 slots of 32 experts, 1023 x 2049, dx 522 / 423, dw 628 / 540; 8000 of 16,
 // 2047 x 2047, dx 243 / 270, dw 377 / 287; 2000 of 16, 1023 x 1025, dx 45 / 72, dw 90 / 91.
-template <typename T, bool FP4, int MODE, int ACT, bool ALIGNED>
+template <typename T, int FORM, int MODE, int ACT, bool ALIGNED>
 int launch_size(const Args &a, hipStream_t stream)
 {
     const long long rows = a.experts > 0 ? a.slots / a.experts : 0, used = a.experts < a.slots ? a.experts : a.slots;
@@ -293,16 +301,16 @@ int launch_size(const Args &a, hipStream_t stream)
     };
     if constexpr (MODE == kFwd) {
         const bool few = ALIGNED ? rows <= 8 && (tiles(128) < 512 || a.ld_q >= 4000) : rows <= (tiles(128) < 128 ? 24 : 4);
-        if (few) return launch_rows<T, FP4, ACT, ALIGNED>(a, stream);
+        if (few) return launch_rows<T, FORM, ACT, ALIGNED>(a, stream);
     }
     if constexpr (ALIGNED) {
-        if (tiles(256) >= (MODE != kDw && rows >= 96 ? 128 : 256)) return launch_stream<T, FP4, MODE, ACT>(a, stream);
+        if (tiles(256) >= (MODE != kDw && rows >= 96 ? 128 : 256)) return launch_stream<T, FORM, MODE, ACT>(a, stream);
     } else if constexpr (MODE == kFwd) {
-        if (tiles(64) < 1300) return launch<T, FP4, MODE, ACT, 64, 64, 2, 2, ALIGNED>(a, stream);
+        if (tiles(64) < 1300) return launch<T, FORM, MODE, ACT, 64, 64, 2, 2, ALIGNED>(a, stream);
     } else {
-        if (MODE == kDw ? tiles(256) >= 256 : tiles(256) >= 512 && rows >= 256) return launch<T, FP4, MODE, ACT, 256, 256, 2, 4, ALIGNED>(a, stream);
+        if (MODE == kDw ? tiles(256) >= 256 : tiles(256) >= 512 && rows >= 256) return launch<T, FORM, MODE, ACT, 256, 256, 2, 4, ALIGNED>(a, stream);
     }
-    return launch<T, FP4, MODE, ACT, 128, 128, 2, 2, ALIGNED>(a, stream);
+    return launch<T, FORM, MODE, ACT, 128, 128, 2, 2, ALIGNED>(a, stream);
 }
 
 // whether `bytes` lie within the 32-bit offsets of a buffer descriptor
@@ -314,15 +322,27 @@ template <int MODE, int ACT>
 int run(const pfk_moe_mm_args *g, Args a, bool aligned, hipStream_t stream)
 {
     if (g->dtype == PF_F16)
-        return aligned ? launch_size<f16, false, MODE, ACT, true>(a, stream) : launch_size<f16, false, MODE, ACT, false>(a, stream);
-    return aligned ? launch_size<bf16, false, MODE, ACT, true>(a, stream) : launch_size<bf16, false, MODE, ACT, false>(a, stream);
+        return aligned ? launch_size<f16, kHalf, MODE, ACT, true>(a, stream) : launch_size<f16, kHalf, MODE, ACT, false>(a, stream);
+    return aligned ? launch_size<bf16, kHalf, MODE, ACT, true>(a, stream) : launch_size<bf16, kHalf, MODE, ACT, false>(a, stream);
 }
 
-// Operands of 4-bit blocks lie in 16 bytes always; beyond the descriptors' offsets k_mm_rows has 64-bit addresses.
-template <typename T, int ACT>
-int run_mx4(const Args &a, bool fit, hipStream_t stream)
+// Operands of 4-bit blocks and of 8-bit integers lie in 16 bytes always; beyond the descriptors' offsets k_mm_rows has
+// 64-bit addresses.
+template <int FORM, typename T, int ACT>
+int run_type(const Args &a, bool fit, hipStream_t stream)
 {
-    return fit ? launch_size<T, true, kFwd, ACT, true>(a, stream) : launch_rows<T, true, ACT, true>(a, stream);
+    return fit ? launch_size<T, FORM, kFwd, ACT, true>(a, stream) : launch_rows<T, FORM, ACT, true>(a, stream);
+}
+
+template <int FORM>
+int run_codes(const pfk_moe_mm_args *g, Args a, hipStream_t s)
+{
+    a.n = g->n;
+    a.q_expert = g->ld_q * g->n * (g->act == PF_ACT_SWIGLU ? 2 : 1);
+    a.wide = lies16(g->out, g->ld_out);
+    const bool fit = fits(g->p_rows, g->ld_p) && fits(1, a.q_expert) && fits(g->slots, 4);
+    if (g->act == PF_ACT_SWIGLU) return g->dtype == PF_F16 ? run_type<FORM, f16, 1>(a, fit, s) : run_type<FORM, bf16, 1>(a, fit, s);
+    return g->dtype == PF_F16 ? run_type<FORM, f16, 0>(a, fit, s) : run_type<FORM, bf16, 0>(a, fit, s);
 }
 
 Args common(const pfk_moe_mm_args *g)
@@ -395,16 +415,19 @@ int pfk_moe_mm_dw(const pfk_moe_mm_args *g, void *stream)
 int pfk_moe_mm_mx4(const pfk_moe_mm_args *g, void *stream)
 {
     Args a = common(g);
-    a.n = g->n;
     a.k = g->k;
     a.p_scales = (const unsigned char *)g->p_scales;
     a.q_scales = (const unsigned char *)g->q_scales;
-    a.q_expert = g->ld_q * g->n * (g->act == PF_ACT_SWIGLU ? 2 : 1);
-    a.wide = lies16(g->out, g->ld_out);
-    const bool fit = fits(g->p_rows, g->ld_p) && fits(1, a.q_expert) && fits(g->slots, 4);
-    hipStream_t s = (hipStream_t)stream;
-    if (g->act == PF_ACT_SWIGLU) return g->dtype == PF_F16 ? run_mx4<f16, 1>(a, fit, s) : run_mx4<bf16, 1>(a, fit, s);
-    return g->dtype == PF_F16 ? run_mx4<f16, 0>(a, fit, s) : run_mx4<bf16, 0>(a, fit, s);
+    return run_codes<kMx4>(g, a, (hipStream_t)stream);
+}
+
+int pfk_moe_mm_i8(const pfk_moe_mm_args *g, void *stream)
+{
+    Args a = common(g);
+    a.k = (int)g->ld_q;   // zeros behind the elements there are
+    a.p_unit = (const float *)g->p_scales;
+    a.q_unit = (const float *)g->q_scales;
+    return run_codes<kI8>(g, a, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -16,11 +16,14 @@ constexpr int kPieces = 4;   // 16-byte pieces of a row that a lane takes at a t
 // Measured with the weights not in cache: one token, 8 of 64 experts, 2048 -> 2 x 1024, 67 MB, in 12.9 us; 67 tokens, 537
 // MB in 107 to 109 us, 5.0 TB/s (a stream that only reads: 6.2, with non-temporal loads 7.0).  With the gate a wave has twice the loads on their way, and two waves a SIMD
 // with their registers do better than three with a spill (118 us); without it two to four are alike.
-template <typename T, bool FP4, int ACT, bool ALIGNED>
+template <typename T, int FORM, int ACT, bool ALIGNED>
 __global__ __launch_bounds__(kWaves * kWave, ALIGNED && !ACT ? 4 : 2) void k_mm_rows(const Args a)
 {
+    constexpr bool FP4 = FORM == kMx4;
     constexpr int NB = ACT ? 2 : 1;
-    __shared__ float sums[kWaves][NB][256];
+    typedef typename sums_of<FORM>::type SUM;
+    typedef typename std::conditional<FORM == kI8, int, float>::type Sum;
+    __shared__ Sum sums[kWaves][NB][256];
     const int lane = threadIdx.x & (kWave - 1), wave = wave_id(), g = lane >> 4, r = lane & 15;
     const int nt = (a.n + 15) / 16;
     Tile t;
@@ -37,7 +40,7 @@ __global__ __launch_bounds__(kWaves * kWave, ALIGNED && !ACT ? 4 : 2) void k_mm_
         if constexpr (FP4) ws[b] = a.q_scales + blocks32 * ((long long)NB * a.n * t.e + row);
     }
 
-    const int pieces = FP4 ? blocks32 : ALIGNED ? a.k / 8 : (a.k + 7) / 8;
+    const int pieces = ALIGNED ? a.k / kPerPiece<FORM> : (a.k + 7) / 8;
     const int blocks = (pieces + 4 * kPieces - 1) / (4 * kPieces);
     typedef typename std::conditional<ALIGNED, i32x4, Words>::type Piece;
     const bool any = a.k > 0;
@@ -77,9 +80,9 @@ __global__ __launch_bounds__(kWaves * kWave, ALIGNED && !ACT ? 4 : 2) void k_mm_
         return (int)v;
     };
 
-    f32x4 acc[NB];
+    SUM acc[NB];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) acc[b] = f32x4{0, 0, 0, 0};
+    for (int b = 0; b < NB; ++b) acc[b] = SUM{0, 0, 0, 0};
     Piece wv[2][NB][kPieces], xv[2][kPieces];
     int wsv[2][NB], xsv[2];
     const auto fetch_w = [&](int side, int b) __attribute__((always_inline)) {
@@ -105,6 +108,8 @@ __global__ __launch_bounds__(kWaves * kWave, ALIGNED && !ACT ? 4 : 2) void k_mm_
                 const i32x4 &p = wv[side][j][u], &q = xv[side][u];
                 const i32x8 A = {p[0], p[1], p[2], p[3], 0, 0, 0, 0}, B = {q[0], q[1], q[2], q[3], 0, 0, 0, 0};
                 acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc[j], 4, 4, u, wsv[side][j], u, xsv[side]);
+            } else if constexpr (FORM == kI8) {
+                acc[j] = mfma_i8(wv[side][j][u], xv[side][u], acc[j]);
             } else {
                 acc[j] = mfma<T>(settled(wv[side][j][u], w[j], b, u), settled(xv[side][u], x, b, u), acc[j]);
             }
@@ -133,14 +138,19 @@ __global__ __launch_bounds__(kWaves * kWave, ALIGNED && !ACT ? 4 : 2) void k_mm_
     }
 
 #pragma unroll
-    for (int j = 0; j < NB; ++j) *(f32x4 *)&sums[wave][j][r * 16 + g * 4] = acc[j];
+    for (int j = 0; j < NB; ++j) *(SUM *)&sums[wave][j][r * 16 + g * 4] = acc[j];
     __syncthreads();
     const int s = m0 + threadIdx.x / 16, n = t.n * 16 + threadIdx.x % 16;
     float v[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j)
-        v[j] = (sums[0][j][threadIdx.x] + sums[1][j][threadIdx.x]) + (sums[2][j][threadIdx.x] + sums[3][j][threadIdx.x]);
+        v[j] = (float)((sums[0][j][threadIdx.x] + sums[1][j][threadIdx.x]) + (sums[2][j][threadIdx.x] + sums[3][j][threadIdx.x]));
     if (s >= count || n >= a.n) return;
+    if constexpr (FORM == kI8) {
+        const float mine = a.p_unit[row_of_slot(a, t.begin + s)];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) v[j] *= mine * a.q_unit[(long long)NB * a.n * t.e + (long long)j * a.n + n];
+    }
     T *out = (T *)(a.out + a.ld_out * ((long long)t.begin + s)) + n;
     if constexpr (ACT) {
         *out = (T)(silu(v[0]) * v[1]);
@@ -156,24 +166,28 @@ __global__ __launch_bounds__(kWaves * kWave, ALIGNED && !ACT ? 4 : 2) void k_mm_
 
 }  // namespace
 
-template <typename T, bool FP4, int ACT, bool ALIGNED>
+template <typename T, int FORM, int ACT, bool ALIGNED>
 int launch_rows(const Args &a, hipStream_t stream)
 {
     const long long tiles = ((long long)a.slots / 16 + (a.experts < a.slots ? a.experts : a.slots)) * ((a.n + 15) / 16);
-    return launch_tiles(k_mm_rows<T, FP4, ACT, ALIGNED>, a, tiles, kWaves * kWave, stream, "k_mm_rows");
+    return launch_tiles(k_mm_rows<T, FORM, ACT, ALIGNED>, a, tiles, kWaves * kWave, stream, "k_mm_rows");
 }
 
-template int launch_rows<f16, false, 0, true>(const Args &, hipStream_t);
-template int launch_rows<f16, false, 0, false>(const Args &, hipStream_t);
-template int launch_rows<f16, false, 1, true>(const Args &, hipStream_t);
-template int launch_rows<f16, false, 1, false>(const Args &, hipStream_t);
-template int launch_rows<f16, true, 0, true>(const Args &, hipStream_t);
-template int launch_rows<f16, true, 1, true>(const Args &, hipStream_t);
-template int launch_rows<bf16, false, 0, true>(const Args &, hipStream_t);
-template int launch_rows<bf16, false, 0, false>(const Args &, hipStream_t);
-template int launch_rows<bf16, false, 1, true>(const Args &, hipStream_t);
-template int launch_rows<bf16, false, 1, false>(const Args &, hipStream_t);
-template int launch_rows<bf16, true, 0, true>(const Args &, hipStream_t);
-template int launch_rows<bf16, true, 1, true>(const Args &, hipStream_t);
+template int launch_rows<f16, kHalf, 0, true>(const Args &, hipStream_t);
+template int launch_rows<f16, kHalf, 0, false>(const Args &, hipStream_t);
+template int launch_rows<f16, kHalf, 1, true>(const Args &, hipStream_t);
+template int launch_rows<f16, kHalf, 1, false>(const Args &, hipStream_t);
+template int launch_rows<f16, kMx4, 0, true>(const Args &, hipStream_t);
+template int launch_rows<f16, kI8, 0, true>(const Args &, hipStream_t);
+template int launch_rows<f16, kMx4, 1, true>(const Args &, hipStream_t);
+template int launch_rows<f16, kI8, 1, true>(const Args &, hipStream_t);
+template int launch_rows<bf16, kHalf, 0, true>(const Args &, hipStream_t);
+template int launch_rows<bf16, kHalf, 0, false>(const Args &, hipStream_t);
+template int launch_rows<bf16, kHalf, 1, true>(const Args &, hipStream_t);
+template int launch_rows<bf16, kHalf, 1, false>(const Args &, hipStream_t);
+template int launch_rows<bf16, kMx4, 0, true>(const Args &, hipStream_t);
+template int launch_rows<bf16, kI8, 0, true>(const Args &, hipStream_t);
+template int launch_rows<bf16, kMx4, 1, true>(const Args &, hipStream_t);
+template int launch_rows<bf16, kI8, 1, true>(const Args &, hipStream_t);
 
 }  // namespace pfmoe

@@ -86,9 +86,10 @@ struct Plan {
 // floor(v / d) of 0 <= v < 2^31 by multiplication
 __device__ __forceinline__ unsigned divide(unsigned v, unsigned mul, int shift) { return (unsigned)(((unsigned long long)v * mul) >> 32) >> shift; }
 
-template <typename T, bool FP4, int MODE, int ACT>
+template <typename T, int FORM, int MODE, int ACT>
 __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
 {
+    constexpr bool FP4 = FORM == kMx4;
     constexpr int WM = 2, WN = 4, FM = kTile / WM / 16, FN = kTile / WN / 16;
     typedef typename std::conditional<MODE == kDw, Across<kTile, kThreads, true>, Along<kTile, kThreads, true>>::type P;
     typedef typename std::conditional<MODE == kFwd, Along<kTile, kThreads, true>, Across<kTile, kThreads, true>>::type Q;
@@ -163,7 +164,7 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
     };
     const auto depth = [&](const Work &w) { return MODE == kDw ? w.count : a.k; };
     const auto steps_of = [&](const Work &w) {   // tiles of k; zeros behind k
-        const int steps = FP4 ? (depth(w) + 127) / 128 : (depth(w) + 31) / 32;
+        const int steps = (depth(w) + kPerTile<FORM> - 1) / kPerTile<FORM>;
         return steps < kMinSteps ? kMinSteps : steps;
     };
     const auto weight_row = [&](const Work &w, int r) {
@@ -207,8 +208,8 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
             p.init(a.p + a.ld_p * w.begin, span(a.ld_p, load_depth, a.m), a.ld_p, w.m0, a.m, load_depth);
             q.init(a.q, span(a.ld_q, a.p_rows, a.n), a.ld_q, w.n * kTile, a.n, load_depth);
         } else {
-            p.from = buffer_of(a.p, FP4 ? a.ld_p * a.p_rows : span(a.ld_p, a.p_rows, a.k));
-            p.k_pieces = a.k / (FP4 ? 32 : 8);
+            p.from = buffer_of(a.p, FORM != kHalf ? a.ld_p * a.p_rows : span(a.ld_p, a.p_rows, a.k));
+            p.k_pieces = a.k / kPerPiece<FORM>;
 #pragma unroll
             for (int i = 0; i < P::kLoads; ++i) p.at[i] = (unsigned)row_of(w, side, P::tile_row(i)) * (unsigned)a.ld_p + p.piece * 16;
             if constexpr (MODE == kFwd) {
@@ -264,7 +265,8 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
     const auto read_w = [&](const char *from, int j) { return Q::fragment(from + P::kBytes, (wn * FN + j) * 16); };
     const auto scale_x = [&](const char *from, int i) { return FP4 ? S::fragment(from + SCALES, (i * WM + wm) * 16) : 0; };
     const auto scale_w = [&](const char *from, int j) { return FP4 ? S::fragment(from + SCALES, kTile + (wn * FN + j) * 16) : 0; };
-    f32x4 acc[FM][FN];
+    typedef typename sums_of<FORM>::type SUM;
+    SUM acc[FM][FN];
     i32x4 x[4], w[2][FN];
     int xs[4], ws[2][FN];
 
@@ -293,6 +295,7 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
                 if constexpr (FP4) acc[i][j] = mfma_fp4(w[0][j], x[i % 4], acc[i][j], ws[0][j], xs[i % 4]);
+                else if constexpr (FORM == kI8) acc[i][j] = mfma_i8(w[0][j], x[i % 4], acc[i][j]);
                 else acc[i][j] = mfma<T>(w[0][j], x[i % 4], acc[i][j]);
                 // a product occupies the matrix core for 16 cycles: what else there is to issue goes between them
                 if (j == 0) {
@@ -372,7 +375,7 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
 #pragma unroll
         for (int r = 0; r < FM; ++r)
 #pragma unroll
-            for (int c = 0; c < FN; ++c) acc[r][c] = f32x4{0, 0, 0, 0};
+            for (int c = 0; c < FN; ++c) acc[r][c] = SUM{0, 0, 0, 0};
         Work after;
         bool more_after = false;
         const auto all = [&](auto blocks) {
@@ -389,8 +392,13 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
             // Of the next output tile three tiles of k are on their way.  Stores would end behind them in no order that a
             // counted wait could use, so they have to be there first.
             wait_loads();
+            const auto units = [&]() {
+                if constexpr (FORM == kI8)
+                    return Units<ACT, FN>{&a, a.q_unit + (ACT ? 2LL : 1LL) * a.n * now.e, (long long)now.begin + now.m0, wn, now.n * OUT_N};
+                else return NoUnits{};
+            };
             store_results<T, MODE, ACT, decltype(blocks)::value, FM, FN, WM, OUT_N>(
-                a, acc, wm, wn, MODE == kDw ? (long long)now.e * a.m + now.m0 : (long long)now.begin + now.m0, have, now.n * OUT_N);
+                a, acc, wm, wn, MODE == kDw ? (long long)now.e * a.m + now.m0 : (long long)now.begin + now.m0, have, now.n * OUT_N, units());
         };
         if (have > kTile / 2) all(std::integral_constant<int, FM>());
         else all(std::integral_constant<int, FM / 2>());   // half the rows: half the products
@@ -404,24 +412,28 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
 
 }  // namespace
 
-template <typename T, bool FP4, int MODE, int ACT>
+template <typename T, int FORM, int MODE, int ACT>
 int launch_stream(const Args &a, hipStream_t stream)
 {
-    k_mm_stream<T, FP4, MODE, ACT><<<dim3(kCus), dim3(kThreads), 0, stream>>>(a);
+    k_mm_stream<T, FORM, MODE, ACT><<<dim3(kCus), dim3(kThreads), 0, stream>>>(a);
     return pfk_internal_launched("k_mm_stream");
 }
 
-template int launch_stream<f16, false, kFwd, 0>(const Args &, hipStream_t);
-template int launch_stream<f16, false, kFwd, 1>(const Args &, hipStream_t);
-template int launch_stream<f16, false, kDx, 0>(const Args &, hipStream_t);
-template int launch_stream<f16, false, kDw, 0>(const Args &, hipStream_t);
-template int launch_stream<f16, true, kFwd, 0>(const Args &, hipStream_t);
-template int launch_stream<f16, true, kFwd, 1>(const Args &, hipStream_t);
-template int launch_stream<bf16, false, kFwd, 0>(const Args &, hipStream_t);
-template int launch_stream<bf16, false, kFwd, 1>(const Args &, hipStream_t);
-template int launch_stream<bf16, false, kDx, 0>(const Args &, hipStream_t);
-template int launch_stream<bf16, false, kDw, 0>(const Args &, hipStream_t);
-template int launch_stream<bf16, true, kFwd, 0>(const Args &, hipStream_t);
-template int launch_stream<bf16, true, kFwd, 1>(const Args &, hipStream_t);
+template int launch_stream<f16, kHalf, kFwd, 0>(const Args &, hipStream_t);
+template int launch_stream<f16, kHalf, kFwd, 1>(const Args &, hipStream_t);
+template int launch_stream<f16, kHalf, kDx, 0>(const Args &, hipStream_t);
+template int launch_stream<f16, kHalf, kDw, 0>(const Args &, hipStream_t);
+template int launch_stream<f16, kMx4, kFwd, 0>(const Args &, hipStream_t);
+template int launch_stream<f16, kI8, kFwd, 0>(const Args &, hipStream_t);
+template int launch_stream<f16, kMx4, kFwd, 1>(const Args &, hipStream_t);
+template int launch_stream<f16, kI8, kFwd, 1>(const Args &, hipStream_t);
+template int launch_stream<bf16, kHalf, kFwd, 0>(const Args &, hipStream_t);
+template int launch_stream<bf16, kHalf, kFwd, 1>(const Args &, hipStream_t);
+template int launch_stream<bf16, kHalf, kDx, 0>(const Args &, hipStream_t);
+template int launch_stream<bf16, kHalf, kDw, 0>(const Args &, hipStream_t);
+template int launch_stream<bf16, kMx4, kFwd, 0>(const Args &, hipStream_t);
+template int launch_stream<bf16, kI8, kFwd, 0>(const Args &, hipStream_t);
+template int launch_stream<bf16, kMx4, kFwd, 1>(const Args &, hipStream_t);
+template int launch_stream<bf16, kI8, kFwd, 1>(const Args &, hipStream_t);
 
 }  // namespace pfmoe

@@ -11,15 +11,26 @@
 namespace pfmoe {
 
 // What the three products have in common: C[m][n] = sum over k of P[m][k] Q[n][k], tile by tile.  Both operands
-// are staged through LDS in tiles of 64 bytes of k per row (32 elements of 16 bits, 128 of 4 bits).
+// are staged through LDS in tiles of 64 bytes of k per row (32 elements of 16 bits, 64 of 8 bits, 128 of 4 bits).
 //   forward    m: slots of an expert (P: x, gathered)   n: rows of w                k: x's columns, both row by row
 //   kDx        m: slots of an expert (P: dy)            n: columns of w             k: rows of w: Q lies across
 //   kDw        m: columns of dy                         n: columns of x (gathered)  k: slots of an expert: both across
 enum { kFwd = 0, kDx = 1, kDw = 2 };
 
+// What the operands hold: f16 or bf16 (the results' type), 4-bit blocks, or 8-bit integers with a scale a row.
+enum { kHalf = 0, kMx4 = 1, kI8 = 2 };
+
+// elements in 16 bytes, and in a tile's 64 bytes of a row
+template <int FORM> constexpr int kPerPiece = FORM == kHalf ? 8 : FORM == kI8 ? 16 : 32;
+template <int FORM> constexpr int kPerTile = 4 * kPerPiece<FORM>;
+// Sums: of 8-bit integers exact ones.
+template <int FORM> struct sums_of { typedef f32x4 type; };
+template <> struct sums_of<kI8> { typedef i32x4 type; };
+
 struct Args {
     const char *p, *q;
     const unsigned char *p_scales, *q_scales;
+    const float *p_unit, *q_unit;   // kI8: what 1 of a row of either operand stands for
     long long ld_p, ld_q, q_expert, ld_out, ld_pre;
     const int *rows, *offsets;
     int row_div, p_rows, experts, slots;
@@ -71,6 +82,11 @@ __device__ __forceinline__ f32x4 mfma(const i32x4 &a, const i32x4 &b, const f32x
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+__device__ __forceinline__ i32x4 mfma_i8(const i32x4 &a, const i32x4 &b, const i32x4 &c)
+{
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+
 __device__ __forceinline__ f32x4 mfma_fp4(const i32x4 &a, const i32x4 &b, const f32x4 &c, int a_scale, int b_scale)
 {
     const i32x8 A = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, B = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
@@ -80,8 +96,8 @@ __device__ __forceinline__ f32x4 mfma_fp4(const i32x4 &a, const i32x4 &b, const 
 // Has the sums formed here: without it the compiler moves products of 4-bit blocks down past the meeting of the waves,
 // since nothing before it uses them, where no LDS reads are left to go beside them (8192 tokens x 4 of 32 experts, 2048 ->
 // 2 x 2048: 223 us, 216 so).
-template <int ROWS, int FM, int FN>
-__device__ __forceinline__ void formed(f32x4 (&acc)[FM][FN])
+template <int ROWS, int FM, int FN, typename SUM>
+__device__ __forceinline__ void formed(SUM (&acc)[FM][FN])
 {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
@@ -412,11 +428,17 @@ __device__ __forceinline__ void wait_and_meet()
 
 // Stores a wave's results: FMV of its FM blocks of 16 rows (every WM-th of the tile's, of which `have` rows exist),
 // FN blocks of 16 columns.  first: the tile's first row of the output, n0 its first column.
-template <typename T, int MODE, int ACT, bool WHOLE, int FMV, int FM, int FN, int WM>
-__device__ __forceinline__ void store_blocks(const Args &a, const f32x4 (&acc)[FM][FN], int wm, int wn, long long first, int have, int n0)
+template <typename T, int MODE, int ACT, bool WHOLE, int FMV, int FM, int FN, int WM, typename SUM, typename U>
+__device__ __forceinline__ void store_blocks(const Args &a, const SUM (&sums)[FM][FN], int wm, int wn, long long first, int have, int n0, const U &units)
 {
     int lane = threadIdx.x & (kWave - 1);
     asm volatile("" : "+v"(lane));   // addresses are formed here, not kept over the loop before
+    constexpr bool SCALED = std::is_same<SUM, i32x4>::value;
+    f32x4 unit[SCALED ? FN : 1];
+    if constexpr (SCALED) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j) unit[j] = units.columns(j, lane);
+    }
 #pragma unroll
     for (int i = 0; i < FMV; ++i) {
         __builtin_amdgcn_sched_barrier(0);   // one block's results at a time
@@ -424,12 +446,23 @@ __device__ __forceinline__ void store_blocks(const Args &a, const f32x4 (&acc)[F
         const int r = (i * WM + wm) * 16 + (lane & 15);
         const bool is = r < have;
         char *out = a.out + a.ld_out * (first + r);
+        f32x4 acc[1][FN];
+        if constexpr (SCALED) {
+            const float mine = units.row(r, is);
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[0][j][c] = (float)sums[i][j][c] * (mine * unit[j][c]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[0][j] = sums[i][j];
+        }
         if constexpr (ACT) {
             f32x4 h[FN / 2], gate[FN / 2], rest[FN / 2];
 #pragma unroll
             for (int j = 0; j < FN / 2; ++j) {
-                gate[j] = acc[i][2 * j];
-                rest[j] = acc[i][2 * j + 1];
+                gate[j] = acc[0][2 * j];
+                rest[j] = acc[0][2 * j + 1];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) h[j][c] = silu(gate[j][c]) * rest[j][c];
             }
@@ -443,21 +476,43 @@ __device__ __forceinline__ void store_blocks(const Args &a, const f32x4 (&acc)[F
         } else if (MODE == kDw && a.out_f32) {
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
-                const float x[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                const float x[4] = {acc[0][j][0], acc[0][j][1], acc[0][j][2], acc[0][j][3]};
                 if (is) store<float, WHOLE, 4>(out, n0 + (wn * FN + j) * 16 + (lane >> 4) * 4, a.n, x);
             }
         } else {
-            store_columns<T, WHOLE, FN>(out, is, n0 + wn * FN * 16, a.n, acc[i], lane);
+            store_columns<T, WHOLE, FN>(out, is, n0 + wn * FN * 16, a.n, acc[0], lane);
         }
     }
 }
 
-template <typename T, int MODE, int ACT, int FMV, int FM, int FN, int WM, int OUT_N>
-__device__ __forceinline__ void store_results(const Args &a, const f32x4 (&acc)[FM][FN], int wm, int wn, long long first, int have, int n0)
+template <typename T, int MODE, int ACT, int FMV, int FM, int FN, int WM, int OUT_N, typename SUM, typename U>
+__device__ __forceinline__ void store_results(const Args &a, const SUM (&acc)[FM][FN], int wm, int wn, long long first, int have, int n0, const U &units)
 {
-    if (a.wide && n0 + OUT_N <= a.n) store_blocks<T, MODE, ACT, true, FMV, FM, FN, WM>(a, acc, wm, wn, first, have, n0);
-    else store_blocks<T, MODE, ACT, false, FMV, FM, FN, WM>(a, acc, wm, wn, first, have, n0);
+    if (a.wide && n0 + OUT_N <= a.n) store_blocks<T, MODE, ACT, true, FMV, FM, FN, WM>(a, acc, wm, wn, first, have, n0, units);
+    else store_blocks<T, MODE, ACT, false, FMV, FM, FN, WM>(a, acc, wm, wn, first, have, n0, units);
 }
+
+// What 1 of a tile's rows and of its columns stands for, of 8-bit integers; for other operands nothing.
+template <int ACT, int FN>
+struct Units {
+    const Args *a;
+    const float *q;        // the expert's
+    long long first;       // slot of the tile's first row
+    int wn, n0;
+
+    // four columns of block j of this wave: those that lane's results are
+    __device__ __forceinline__ f32x4 columns(int j, int lane) const
+    {
+        const int n = ACT ? n0 + (wn * FN + j) / 2 * 16 + (lane >> 4) * 4 : n0 + (wn * FN + j) * 16 + (lane >> 4) * 4;
+        const float *from = q + (ACT && j % 2 ? a->n : 0);
+        f32x4 v;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = from[n + c < a->n ? n + c : a->n - 1];
+        return v;
+    }
+    __device__ __forceinline__ float row(int r, bool is) const { return is ? a->p_unit[row_of_slot(*a, (int)(first + r))] : 0.0f; }
+};
+struct NoUnits { };
 
 // The tile of workgroup `id`: expert, tile of rows, tile of columns.  The experts' tiles are counted from the offsets,
 // 64 experts at a time over the lanes, in every wave by itself.  Workgroups reach the 8 XCDs in turn, so each XCD is
@@ -526,11 +581,11 @@ int launch_tiles(K kernel, Args a, long long tiles, int threads, hipStream_t str
 }
 
 // moe_mm_stream.hip
-template <typename T, bool FP4, int MODE, int ACT>
+template <typename T, int FORM, int MODE, int ACT>
 int launch_stream(const Args &a, hipStream_t stream);
 
 // moe_mm_rows.hip
-template <typename T, bool FP4, int ACT, bool ALIGNED>
+template <typename T, int FORM, int ACT, bool ALIGNED>
 int launch_rows(const Args &a, hipStream_t stream);
 
 }  // namespace pfmoe

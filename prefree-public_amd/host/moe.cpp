@@ -298,4 +298,60 @@ int pf_moe_mm_mx4(const void *x_codes, const void *x_scales, int x_rows, const i
     return from_kernels(pfk_moe_mm_mx4(&a, stream), what);
 }
 
+int pf_i8_quantize(const void *x, long long ld_x, int dtype, int rows, int k, void *codes, float *scales, void *stream)
+{
+    const char *what = "pf_i8_quantize";
+    PF_CHECK(bytes_of(dtype), "values are f32, f16 or bf16");
+    PF_CHECK(rows >= 0 && k >= 1 && k <= (1 << 24), "negative, zero or too large size");
+    if (rows == 0) return PF_OK;
+    PF_CHECK(x && codes && scales, "NULL pointer");
+    const long long lx = lead(ld_x, k);
+    PF_CHECK(lx >= 0, "leading dimension under the row's length");
+    PF_CHECK_ALIGN(x, bytes_of(dtype), "x not aligned to its elements");
+    PF_CHECK_ALIGN(codes, 16, "codes not 16-byte aligned");
+    PF_CHECK_WORDS(scales);
+    return from_kernels(pfk_i8_quantize(x, lx, dtype, rows, k, codes, scales, stream), what);
+}
+
+int pf_i8_dequantize(const void *codes, const float *scales, int rows, int k, int dtype, void *y, long long ld_y, void *stream)
+{
+    const char *what = "pf_i8_dequantize";
+    PF_CHECK(bytes_of(dtype), "values are f32, f16 or bf16");
+    PF_CHECK(rows >= 0 && k >= 1 && k <= (1 << 24), "negative, zero or too large size");
+    if (rows == 0) return PF_OK;
+    PF_CHECK(codes && scales && y, "NULL pointer");
+    const long long ly = lead(ld_y, k);
+    PF_CHECK(ly >= 0, "leading dimension under the row's length");
+    PF_CHECK_ALIGN(y, bytes_of(dtype), "y not aligned to its elements");
+    PF_CHECK_ALIGN(codes, 16, "codes not 16-byte aligned");
+    PF_CHECK_WORDS(scales);
+    return from_kernels(pfk_i8_dequantize(codes, scales, rows, k, dtype, y, ly, stream), what);
+}
+
+int pf_moe_mm_i8(const void *x_codes, const float *x_scales, int x_rows, const int *rows, int row_div, const void *w_codes,
+                 const float *w_scales, const int *offsets, int experts, int slots, int n, int k, int dtype, int act, void *y,
+                 long long ld_y, void *stream)
+{
+    const char *what = "pf_moe_mm_i8", *why = grouped(offsets, experts, slots, n, k);
+    PF_CHECK(!why, why);
+    PF_CHECK(half_type(dtype), "results are f16 or bf16");
+    PF_CHECK(act == PF_ACT_NONE || act == PF_ACT_SWIGLU, "unknown activation");
+    PF_CHECK(k <= 131056, "k: at most 131056, so that sums of products hold in 32 bits");
+    PF_CHECK(!rows || row_div >= 1, "row_div: at least 1");
+    PF_CHECK(x_rows >= 0 && (slots == 0 || x_rows >= (rows ? 1 : slots)), "x has too few rows");
+    if (slots == 0 || n == 0) return PF_OK;
+    PF_CHECK(y && x_scales && w_scales && (k == 0 || (x_codes && w_codes)), "NULL pointer");
+    const long long ly = lead(ld_y, n);
+    PF_CHECK(ly >= 0, "leading dimension under the row's length");
+    PF_CHECK_ALIGN(x_codes, 16, "codes not 16-byte aligned");
+    PF_CHECK_ALIGN(w_codes, 16, "codes not 16-byte aligned");
+    PF_CHECK_ALIGN(y, 2, "y not aligned to its elements");
+    PF_CHECK_WORDS(rows, offsets, x_scales, w_scales);
+    pfk_moe_mm_args a = {};
+    a.p = x_codes; a.ld_p = PF_I8_ROW(k); a.p_scales = x_scales; a.p_rows = x_rows; a.rows = rows; a.row_div = row_div;
+    a.q = w_codes; a.ld_q = PF_I8_ROW(k); a.q_scales = w_scales; a.offsets = offsets; a.experts = experts; a.slots = slots;
+    a.n = n; a.k = k; a.dtype = dtype; a.act = act; a.out = y; a.ld_out = 2 * ly;
+    return from_kernels(pfk_moe_mm_i8(&a, stream), what);
+}
+
 }  // extern "C"

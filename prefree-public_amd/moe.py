@@ -30,6 +30,9 @@ _SIGNATURES = {
     "pf_mx4_quantize": [_vp, _ll, _i, _i, _i, _vp, _vp, _vp],
     "pf_mx4_dequantize": [_vp, _vp, _i, _i, _i, _vp, _ll, _vp],
     "pf_moe_mm_mx4": [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _ll, _vp],
+    "pf_i8_quantize": [_vp, _ll, _i, _i, _i, _vp, _vp, _vp],
+    "pf_i8_dequantize": [_vp, _vp, _i, _i, _i, _vp, _ll, _vp],
+    "pf_moe_mm_i8": [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _ll, _vp],
 }
 
 
@@ -52,6 +55,8 @@ def _kind(dtype):
         return "i32"
     if text.endswith("uint8"):
         return "u8"
+    if text.endswith("int8"):
+        return "i8"
     if any(w in text for w in ("int", "bool", "complex", "float8")):
         return text
     try:
@@ -61,7 +66,7 @@ def _kind(dtype):
 
 
 def _buf(obj, kind, name):
-    """Raw pointer of `obj`, whose type (where it says one) has to be `kind`: a code of this package, "i32" or "u8"."""
+    """Raw pointer of `obj`, whose type (where it says one) has to be `kind`: a code of this package, "i32", "u8" or "i8"."""
     try:
         if _KINDS[obj.dtype] == kind and obj.is_cuda:
             return obj.data_ptr()
@@ -194,6 +199,35 @@ def moe_mm_mx4(x_codes, x_scales, x_rows, rows, row_div, w_codes, w_scales, offs
            "pf_moe_mm_mx4")
 
 
+def i8_row(k) -> int:
+    """Bytes of a row of k 8-bit integers: whole pieces of 16, zeros behind the k."""
+    return (int(k) + 15) // 16 * 16
+
+
+def i8_quantize(x, rows, k, codes, scales, dtype="bf16", ld_x=0, stream=None):
+    """x [rows, k] to integers from -127 to 127, codes [rows, i8_row(k)] (int8), and scales [rows] (float32)."""
+    d = dtype_code(dtype)
+    _check(lib().pf_i8_quantize(_buf(x, d, "x"), ld_x, d, int(rows), int(k), _buf(codes, "i8", "codes"),
+                                _buf(scales, F32, "scales"), _s(stream)), "pf_i8_quantize")
+
+
+def i8_dequantize(codes, scales, rows, k, y, dtype="f32", ld_y=0, stream=None):
+    """Integer times scale, in y [rows, k]."""
+    d = dtype_code(dtype)
+    _check(lib().pf_i8_dequantize(_buf(codes, "i8", "codes"), _buf(scales, F32, "scales"), int(rows), int(k), d,
+                                  _buf(y, d, "y"), ld_y, _s(stream)), "pf_i8_dequantize")
+
+
+def moe_mm_i8(x_codes, x_scales, x_rows, rows, row_div, w_codes, w_scales, offsets, experts, slots, n, k, y, dtype="bf16",
+              act="none", ld_y=0, stream=None):
+    """moe_mm of 8-bit integers with a scale a row; y in `dtype`."""
+    d = dtype_code(dtype)
+    _check(lib().pf_moe_mm_i8(_buf(x_codes, "i8", "x_codes"), _buf(x_scales, F32, "x_scales"), int(x_rows),
+                              _buf(rows, "i32", "rows"), int(row_div), _buf(w_codes, "i8", "w_codes"),
+                              _buf(w_scales, F32, "w_scales"), _buf(offsets, "i32", "offsets"), int(experts), int(slots),
+                              int(n), int(k), d, _act(act), _buf(y, d, "y"), ld_y, _s(stream)), "pf_moe_mm_i8")
+
+
 __all__ = ["BF16", "F16", "ACTIVATIONS", "moe_route_workspace", "moe_route", "moe_route_backward", "moe_combine",
            "moe_combine_backward", "moe_mm", "moe_mm_dx", "moe_mm_dw", "swiglu_backward", "mx4_quantize",
-           "mx4_dequantize", "moe_mm_mx4"]
+           "mx4_dequantize", "moe_mm_mx4", "i8_row", "i8_quantize", "i8_dequantize", "moe_mm_i8"]
