@@ -126,6 +126,22 @@ int pf_moe_mm_i8(const void *x_codes, const float *x_scales, int x_rows, const i
                  const float *w_scales, const int *offsets, int experts, int slots, int n, int k, int dtype, int act, void *y,
                  long long ld_y, void *stream);
 
+/* ---- orthogonal updates --------------------------------------------------------------
+ * out = the update of each of `batch` matrices g [rows][columns] (f32, f16, bf16) made nearly orthogonal by Newton-Schulz
+ * products: X = g / |g| (the root of its sum of squares), then for each of n_steps triples (a, b, c) of `steps`, which is host memory
+ * and read during the call, X <- a X + (b A + c A A) X with A = X X^T (of the transpose where rows > columns).  Every singular value x
+ * becomes a x + b x^3 + c x^5 in each step: with (3.4445, -4.7750, 2.0315) five times those from 0.01 of |g| on come out
+ * between 0.7 and 1.2.  out [rows][columns] (f16, bf16).  Matrices follow each other, rows * ld elements apart.
+ * Products are of f16 values with sums in f32, X held in two f16 pieces: within about 2^-8 of the formula, in the 2-norm over
+ * all elements.  Steps have to keep singular values of 1 and less under 4.  A matrix of zeros gives zeros, one that
+ * holds an infinity or a NaN gives NaN; others of the batch are not touched by it.
+ * rows, columns: 1 to 2^20, rows * columns at most 2^29; batch at most 1024; n_steps 1 to 64.
+ * workspace: pf_orthogonalize_workspace() bytes, 16-byte aligned; what it holds before and after does not matter. */
+size_t pf_orthogonalize_workspace(int batch, int rows, int columns);
+int pf_orthogonalize(const void *g, long long ld_g, int dtype, int batch, int rows, int columns, const float *steps,
+                     int n_steps, void *out, long long ld_out, int out_dtype, void *workspace, size_t workspace_bytes,
+                     void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -318,7 +318,7 @@ __device__ __forceinline__ void store(char *row, int n, int have, const T (&v)[N
 // Lane l holds, of its row l % 16, four consecutive columns of each of N blocks of 16: those from 4 (l / 16).  Stores of
 // these would cover 32 bytes of a row at a time.  The two lane-swapping instructions hand each group of 16 lanes 4 N
 // consecutive columns instead, those from 4 N (l / 16), so that a store covers whole lines (N = 4) or halves.
-// in: the blocks' four results each, as two registers of two; out: 4 N columns in order.
+// in: the blocks' four results each, as two registers of two or four of one; out: 4 N columns in order.
 __device__ __forceinline__ void swap32(unsigned &a, unsigned &b)
 {
     const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
@@ -331,12 +331,12 @@ __device__ __forceinline__ void swap16(unsigned &a, unsigned &b)
     a = r[0];
     b = r[1];
 }
-template <int N>
-__device__ __forceinline__ void gather_columns(unsigned (&v)[N][2])
+template <int N, int C>
+__device__ __forceinline__ void gather_columns(unsigned (&v)[N][C])
 {
     static_assert(N == 1 || N == 2 || N == 4, "blocks");
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < C; ++c) {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) swap32(v[i][c], v[i + N / 2][c]);
 #pragma unroll

@@ -354,4 +354,32 @@ int pf_moe_mm_i8(const void *x_codes, const float *x_scales, int x_rows, const i
     return from_kernels(pfk_moe_mm_i8(&a, stream), what);
 }
 
+size_t pf_orthogonalize_workspace(int batch, int rows, int columns)
+{
+    if (batch < 1 || rows < 1 || columns < 1) return 0;
+    const size_t m = PFK_ORTH_SIDE((size_t)std::min(rows, columns)), n = PFK_ORTH_SIDE((size_t)std::max(rows, columns));
+    return batch * (2 * m * (4 * n + 2 * m) + 8 * PFK_ORTH_PARTS);
+}
+
+int pf_orthogonalize(const void *g, long long ld_g, int dtype, int batch, int rows, int columns, const float *steps, int n_steps, void *out,
+                     long long ld_out, int out_dtype, void *workspace, size_t workspace_bytes, void *stream)
+{
+    const char *what = "pf_orthogonalize";
+    PF_CHECK(bytes_of(dtype), "matrices are f32, f16 or bf16");
+    PF_CHECK(half_type(out_dtype), "results are f16 or bf16");
+    PF_CHECK(batch >= 0 && batch <= PF_MOE_MAX_EXPERTS, "batch: at most 1024");
+    PF_CHECK(rows >= 0 && columns >= 0 && rows <= (1 << 20) && columns <= (1 << 20) && (long long)rows * columns <= (1 << 29),
+             "negative or too large size");
+    PF_CHECK(n_steps >= 1 && n_steps <= 64 && steps, "steps: 1 to 64 triples");
+    if (batch == 0 || rows == 0 || columns == 0) return PF_OK;
+    PF_CHECK(g && out, "NULL pointer");
+    const long long lg = lead(ld_g, columns), lo = lead(ld_out, columns);
+    PF_CHECK(lg >= 0 && lo >= 0, "leading dimension under the row's length");
+    PF_CHECK_ALIGN(g, bytes_of(dtype), "g not aligned to its elements");
+    PF_CHECK_ALIGN(out, 2, "out not aligned to its elements");
+    PF_CHECK(workspace && workspace_bytes >= pf_orthogonalize_workspace(batch, rows, columns), "workspace smaller than pf_orthogonalize_workspace()");
+    PF_CHECK_ALIGN(workspace, 16, "workspace not 16-byte aligned");
+    return from_kernels(pfk_orthogonalize(g, lg, dtype, batch, rows, columns, steps, n_steps, out, lo, out_dtype, workspace, stream), what);
+}
+
 }  // extern "C"

@@ -32,6 +32,7 @@ _SIGNATURES = {
     "pf_moe_mm_mx4": [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _ll, _vp],
     "pf_i8_quantize": [_vp, _ll, _i, _i, _i, _vp, _vp, _vp],
     "pf_i8_dequantize": [_vp, _vp, _i, _i, _i, _vp, _ll, _vp],
+    "pf_orthogonalize": [_vp, _ll, _i, _i, _i, _i, _vp, _i, _vp, _ll, _i, _vp, ctypes.c_size_t, _vp],
     "pf_moe_mm_i8": [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _ll, _vp],
 }
 
@@ -43,6 +44,8 @@ def _signatures(L):
         f.restype = _i
     L.pf_moe_route_workspace.argtypes = [_i, _i]
     L.pf_moe_route_workspace.restype = ctypes.c_size_t
+    L.pf_orthogonalize_workspace.argtypes = [_i, _i, _i]
+    L.pf_orthogonalize_workspace.restype = ctypes.c_size_t
 
 
 # Type of a buffer, by what its `dtype` is: kept per type object, since these calls are a few microseconds long.
@@ -228,6 +231,31 @@ def moe_mm_i8(x_codes, x_scales, x_rows, rows, row_div, w_codes, w_scales, offse
                               int(n), int(k), d, _act(act), _buf(y, d, "y"), ld_y, _s(stream)), "pf_moe_mm_i8")
 
 
+#: Triples that bring singular values from 0.01 to 1 to between 0.7 and 1.2.
+ORTHOGONAL_STEPS = ((3.4445, -4.7750, 2.0315),) * 5
+
+
+def orthogonalize_workspace(batch, rows, columns) -> int:
+    """Bytes of workspace that orthogonalize takes."""
+    return int(lib().pf_orthogonalize_workspace(int(batch), int(rows), int(columns)))
+
+
+def orthogonalize(g, batch, rows, columns, out, workspace, dtype="f32", out_dtype="bf16", steps=ORTHOGONAL_STEPS,
+                  workspace_bytes=None, ld_g=0, ld_out=0, stream=None):
+    """g [batch, rows, columns] made nearly orthogonal by Newton-Schulz products; steps: triples of numbers."""
+    d, out_d = dtype_code(dtype), dtype_code(out_dtype)
+    if workspace_bytes is None:
+        workspace_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    flat = [float(v) for step in steps for v in step]
+    if len(flat) != 3 * len(steps):
+        raise ValueError("steps are triples")
+    _check(lib().pf_orthogonalize(_buf(g, d, "g"), ld_g, d, int(batch), int(rows), int(columns),
+                                  (ctypes.c_float * len(flat))(*flat), len(steps), _buf(out, out_d, "out"), ld_out, out_d,
+                                  _buf_checked(workspace, None, "workspace"), int(workspace_bytes), _s(stream)),
+           "pf_orthogonalize")
+
+
 __all__ = ["BF16", "F16", "ACTIVATIONS", "moe_route_workspace", "moe_route", "moe_route_backward", "moe_combine",
            "moe_combine_backward", "moe_mm", "moe_mm_dx", "moe_mm_dw", "swiglu_backward", "mx4_quantize",
-           "mx4_dequantize", "moe_mm_mx4", "i8_row", "i8_quantize", "i8_dequantize", "moe_mm_i8"]
+           "mx4_dequantize", "moe_mm_mx4", "i8_row", "i8_quantize", "i8_dequantize", "moe_mm_i8", "ORTHOGONAL_STEPS",
+           "orthogonalize_workspace", "orthogonalize"]
