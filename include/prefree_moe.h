@@ -60,6 +60,32 @@ int pf_moe_route_backward(const void *logits, long long ld_logits, int dtype, in
                           int normalise, const int *choice, const float *weight, const float *dweight, void *dlogits,
                           long long ld_dlogits, void *stream);
 
+/* ---- routing by scores ----------------------------------------------------------
+ * As pf_moe_route, but the choice goes by scores plus a bias that balances the experts' load, inside the best groups of experts:
+ *   s = sigmoid(logit), or exp(logit) / sum of exp(logits) over all experts;  r = s + bias (f32 [experts], NULL: 0)
+ *   the experts form `groups` groups of equal size, side by side; a group counts the sum of its group_best (1 or 2) largest
+ *   r, as far as it has as many, and the groups_kept groups that count most are kept (of equal ones the lowest index)
+ *   choice: the top_k largest r of their experts (of equal ones the lowest index), best first, -1 where there is none
+ *   weight: scale * s / sum of the chosen s (normalise 1), or scale * s (normalise 0); the bias is not part of it
+ * A logit of -infinity and an r of -infinity are never chosen and count in no group.  A NaN counts as larger than any number.
+ * r is compared as of 64 bits (and as its logit, where there is no bias and groups count one score: scores that 64 bits
+ * do not tell apart are then in the order of their logits).  experts is a multiple of groups; groups: 1 to 16; scale: a positive number.
+ * offsets, order, slot, workspace: as of pf_moe_route. */
+enum pf_score { PF_SCORE_SOFTMAX = 0, PF_SCORE_SIGMOID = 1 };
+#define PF_MOE_MAX_GROUPS 16
+int pf_moe_route_scores(const void *logits, long long ld_logits, int dtype, int tokens, int experts, int top_k, int score,
+                        const float *bias, int groups, int groups_kept, int group_best, int normalise, float scale,
+                        int *choice, float *weight, int *offsets, int *order, int *slot, void *workspace,
+                        size_t workspace_bytes, void *stream);
+/* dlogits [tokens][experts] (the type of logits) from dweight [tokens*top_k], with choice and weight as
+ * pf_moe_route_scores wrote them; the choice itself, and so bias and groups, has no gradient.  Every element is written. */
+int pf_moe_route_scores_backward(const void *logits, long long ld_logits, int dtype, int tokens, int experts, int top_k,
+                                 int score, int normalise, float scale, const int *choice, const float *weight,
+                                 const float *dweight, void *dlogits, long long ld_dlogits, void *stream);
+/* The next bias from the experts' load: next[e] = bias[e] + rate where expert e has fewer slots than the mean of all, - rate
+ * where it has more.  offsets [experts+1] as the routing wrote them; next may be bias. */
+int pf_moe_balance(const int *offsets, int experts, float rate, const float *bias, float *next, void *stream);
+
 /* out[t] = sum over j of weight[t,j] * y[slot[t,j]]: y [slots][width], out [tokens][width] (f16, bf16).  Entries whose
  * slot is outside [0, slots) are left out, and their rows not read; a token without any gets zeros.  weight NULL:
  * all 1 (the gradient of the tokens from that of their slots). */

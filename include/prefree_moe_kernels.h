@@ -35,6 +35,13 @@ int pfk_moe_route(const void *logits, long long ld, int dtype, int tokens, int e
 int pfk_moe_route_backward(const void *logits, long long ld, int dtype, int tokens, int experts, int top_k,
                            int normalise, const int *choice, const float *weight, const float *dweight, void *dlogits,
                            long long ld_d, void *stream);
+int pfk_moe_route_scores(const void *logits, long long ld, int dtype, int tokens, int experts, int top_k, int score,
+                         const float *bias, int groups, int groups_kept, int group_best, int normalise, float scale,
+                         int *choice, float *weight, int *offsets, int *order, int *slot, int *counts, void *stream);
+int pfk_moe_route_scores_backward(const void *logits, long long ld, int dtype, int tokens, int experts, int top_k,
+                                  int score, int normalise, float scale, const int *choice, const float *weight,
+                                  const float *dweight, void *dlogits, long long ld_d, void *stream);
+int pfk_moe_balance(const int *offsets, int experts, float rate, const float *bias, float *next, void *stream);
 int pfk_moe_combine(const void *y, long long ld_y, int dtype, int slots, const int *slot, const float *weight,
                     int tokens, int top_k, int width, void *out, long long ld_out, void *stream);
 int pfk_moe_combine_backward(const void *dout, long long ld_dout, const void *y, long long ld_y, int dtype, int slots,

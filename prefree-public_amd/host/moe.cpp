@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdint>
 #include <string>
 
@@ -115,6 +116,60 @@ int pf_moe_route_backward(const void *logits, long long ld_logits, int dtype, in
     PF_CHECK_WORDS(choice, weight, dweight);
     return from_kernels(pfk_moe_route_backward(logits, ld, dtype, tokens, experts, top_k, normalise != 0, choice, weight,
                                                dweight, dlogits, ld_d, stream), what);
+}
+
+int pf_moe_route_scores(const void *logits, long long ld_logits, int dtype, int tokens, int experts, int top_k, int score,
+                        const float *bias, int groups, int groups_kept, int group_best, int normalise, float scale, int *choice,
+                        float *weight, int *offsets, int *order, int *slot, void *workspace, size_t workspace_bytes, void *stream)
+{
+    const char *what = "pf_moe_route_scores", *why = routing(tokens, experts, top_k);
+    PF_CHECK(!why, why);
+    PF_CHECK(bytes_of(dtype), "logits are f32, f16 or bf16");
+    PF_CHECK(score == PF_SCORE_SOFTMAX || score == PF_SCORE_SIGMOID, "unknown score");
+    PF_CHECK(groups >= 1 && groups <= PF_MOE_MAX_GROUPS && experts % groups == 0, "groups: 1 to 16, of equal size");
+    PF_CHECK(groups_kept >= 1 && groups_kept <= groups, "groups_kept: 1 to groups");
+    PF_CHECK(group_best == 1 || group_best == 2, "group_best: 1 or 2");
+    PF_CHECK(scale > 0 && std::isfinite(scale), "scale: a positive number");
+    PF_CHECK(offsets, "NULL pointer");
+    PF_CHECK(tokens == 0 || (logits && choice && weight && order && slot), "NULL pointer");
+    const long long ld = lead(ld_logits, experts);
+    PF_CHECK(ld >= 0, "leading dimension under the row's length");
+    PF_CHECK_ALIGN(logits, bytes_of(dtype), "logits not aligned to their elements");
+    PF_CHECK_WORDS(choice, weight, offsets, order, slot, bias);
+    const size_t need = tokens > PFK_MOE_ROUTE_BLOCK ? pf_moe_route_workspace(tokens, experts) : 0;
+    PF_CHECK(need == 0 || (workspace && workspace_bytes >= need), "workspace smaller than pf_moe_route_workspace()");
+    PF_CHECK_ALIGN(workspace, 4, "workspace not 4-byte aligned");
+    return from_kernels(pfk_moe_route_scores(logits, ld, dtype, tokens, experts, top_k, score, bias, groups, groups_kept, group_best,
+                                             normalise != 0, scale, choice, weight, offsets, order, slot, (int *)workspace, stream), what);
+}
+
+int pf_moe_route_scores_backward(const void *logits, long long ld_logits, int dtype, int tokens, int experts, int top_k, int score,
+                                 int normalise, float scale, const int *choice, const float *weight, const float *dweight,
+                                 void *dlogits, long long ld_dlogits, void *stream)
+{
+    const char *what = "pf_moe_route_scores_backward", *why = routing(tokens, experts, top_k);
+    PF_CHECK(!why, why);
+    PF_CHECK(bytes_of(dtype), "logits are f32, f16 or bf16");
+    PF_CHECK(score == PF_SCORE_SOFTMAX || score == PF_SCORE_SIGMOID, "unknown score");
+    PF_CHECK(scale > 0 && std::isfinite(scale), "scale: a positive number");
+    if (tokens == 0) return PF_OK;
+    PF_CHECK(logits && choice && weight && dweight && dlogits, "NULL pointer");
+    const long long ld = lead(ld_logits, experts), ld_d = lead(ld_dlogits, experts);
+    PF_CHECK(ld >= 0 && ld_d >= 0, "leading dimension under the row's length");
+    PF_CHECK_ALIGN(logits, bytes_of(dtype), "logits not aligned to their elements");
+    PF_CHECK_ALIGN(dlogits, bytes_of(dtype), "dlogits not aligned to their elements");
+    PF_CHECK_WORDS(choice, weight, dweight);
+    return from_kernels(pfk_moe_route_scores_backward(logits, ld, dtype, tokens, experts, top_k, score, normalise != 0, scale, choice,
+                                                      weight, dweight, dlogits, ld_d, stream), what);
+}
+
+int pf_moe_balance(const int *offsets, int experts, float rate, const float *bias, float *next, void *stream)
+{
+    const char *what = "pf_moe_balance";
+    PF_CHECK(experts >= 1 && experts <= PF_MOE_MAX_EXPERTS, "experts: 1 to 1024");
+    PF_CHECK(offsets && bias && next, "NULL pointer");
+    PF_CHECK_WORDS(offsets, bias, next);
+    return from_kernels(pfk_moe_balance(offsets, experts, rate, bias, next, stream), what);
 }
 
 int pf_moe_combine(const void *y, long long ld_y, int dtype, int slots, const int *slot, const float *weight, int tokens,

@@ -13,6 +13,7 @@ import ctypes
 from . import BF16, F16, F32, _check, _s, dtype_code, lib
 
 ACTIVATIONS = {"none": 0, "swiglu": 1}
+SCORES = {"softmax": 0, "sigmoid": 1}
 
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
@@ -21,6 +22,10 @@ _ll = ctypes.c_longlong
 _SIGNATURES = {
     "pf_moe_route": [_vp, _ll, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp],
     "pf_moe_route_backward": [_vp, _ll, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _ll, _vp],
+    "pf_moe_route_scores": [_vp, _ll, _i, _i, _i, _i, _i, _vp, _i, _i, _i, _i, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _vp,
+                            ctypes.c_size_t, _vp],
+    "pf_moe_route_scores_backward": [_vp, _ll, _i, _i, _i, _i, _i, _i, ctypes.c_float, _vp, _vp, _vp, _vp, _ll, _vp],
+    "pf_moe_balance": [_vp, _i, ctypes.c_float, _vp, _vp, _vp],
     "pf_moe_combine": [_vp, _ll, _i, _i, _vp, _vp, _i, _i, _i, _vp, _ll, _vp],
     "pf_moe_combine_backward": [_vp, _ll, _vp, _ll, _i, _i, _vp, _vp, _i, _i, _i, _vp, _ll, _vp, _vp],
     "pf_moe_mm": [_vp, _ll, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _ll, _vp, _ll, _vp],
@@ -97,6 +102,10 @@ def _act(act):
     return act if isinstance(act, int) else ACTIVATIONS[act]
 
 
+def _score(score):
+    return score if isinstance(score, int) else SCORES[score]
+
+
 def moe_route_workspace(tokens, experts) -> int:
     """Bytes of workspace that moe_route takes."""
     return int(lib().pf_moe_route_workspace(int(tokens), int(experts)))
@@ -122,6 +131,41 @@ def moe_route_backward(logits, tokens, experts, top_k, choice, weight, dweight, 
                                        int(bool(normalise)), _buf(choice, "i32", "choice"), _buf(weight, F32, "weight"),
                                        _buf(dweight, F32, "dweight"), _buf(dlogits, d, "dlogits"), ld_dlogits,
                                        _s(stream)), "pf_moe_route_backward")
+
+
+def moe_route_scores(logits, tokens, experts, top_k, choice, weight, offsets, order, slot, workspace, dtype="f32",
+                     score="sigmoid", bias=None, groups=1, groups_kept=None, group_best=2, normalise=True, scale=1.0,
+                     workspace_bytes=None, ld_logits=0, stream=None):
+    """moe_route by sigmoid or softmax scores: the choice by score + bias inside the groups_kept (None: all) best groups
+    of experts, the weights by the scores alone."""
+    d = dtype_code(dtype)
+    if workspace_bytes is None:
+        workspace_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    _check(lib().pf_moe_route_scores(_buf(logits, d, "logits"), ld_logits, d, int(tokens), int(experts), int(top_k),
+                                     _score(score), _buf(bias, F32, "bias"), int(groups),
+                                     int(groups if groups_kept is None else groups_kept), int(group_best),
+                                     int(bool(normalise)), scale, _buf(choice, "i32", "choice"),
+                                     _buf(weight, F32, "weight"), _buf(offsets, "i32", "offsets"),
+                                     _buf(order, "i32", "order"), _buf(slot, "i32", "slot"),
+                                     _buf_checked(workspace, None, "workspace"), int(workspace_bytes), _s(stream)),
+           "pf_moe_route_scores")
+
+
+def moe_route_scores_backward(logits, tokens, experts, top_k, choice, weight, dweight, dlogits, dtype="f32",
+                              score="sigmoid", normalise=True, scale=1.0, ld_logits=0, ld_dlogits=0, stream=None):
+    """dlogits from dweight, with the choice and the weights that moe_route_scores wrote."""
+    d = dtype_code(dtype)
+    _check(lib().pf_moe_route_scores_backward(_buf(logits, d, "logits"), ld_logits, d, int(tokens), int(experts),
+                                              int(top_k), _score(score), int(bool(normalise)), scale,
+                                              _buf(choice, "i32", "choice"), _buf(weight, F32, "weight"),
+                                              _buf(dweight, F32, "dweight"), _buf(dlogits, d, "dlogits"), ld_dlogits,
+                                              _s(stream)), "pf_moe_route_scores_backward")
+
+
+def moe_balance(offsets, experts, rate, bias, next_bias, stream=None):
+    """next_bias (may be bias): up by `rate` for experts with fewer slots than the mean, down for those with more."""
+    _check(lib().pf_moe_balance(_buf(offsets, "i32", "offsets"), int(experts), rate, _buf(bias, F32, "bias"),
+                                _buf(next_bias, F32, "next_bias"), _s(stream)), "pf_moe_balance")
 
 
 def moe_combine(y, slot, weight, tokens, top_k, width, out, dtype="bf16", slots=None, ld_y=0, ld_out=0, stream=None):
@@ -255,7 +299,8 @@ def orthogonalize(g, batch, rows, columns, out, workspace, dtype="f32", out_dtyp
            "pf_orthogonalize")
 
 
-__all__ = ["BF16", "F16", "ACTIVATIONS", "moe_route_workspace", "moe_route", "moe_route_backward", "moe_combine",
+__all__ = ["BF16", "F16", "ACTIVATIONS", "SCORES", "moe_route_workspace", "moe_route", "moe_route_backward",
+           "moe_route_scores", "moe_route_scores_backward", "moe_balance", "moe_combine",
            "moe_combine_backward", "moe_mm", "moe_mm_dx", "moe_mm_dw", "swiglu_backward", "mx4_quantize",
            "mx4_dequantize", "moe_mm_mx4", "i8_row", "i8_quantize", "i8_dequantize", "moe_mm_i8", "ORTHOGONAL_STEPS",
            "orthogonalize_workspace", "orthogonalize"]
