@@ -84,6 +84,29 @@ __device__ __forceinline__ i32x4 load16_any(const void *p)
     return w.shifted(shift);
 }
 
+// Eight elements as fp32 from `at` of a row of k; zeros behind its end.  VECTOR: rows start at multiples of 16 bytes.
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void load8_any(const T *row, int at, int k, float v[8])
+{
+    const T *p = row + at;
+    if (at + 8 > k) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = at + i < k ? (float)p[i] : 0.0f;
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const i32x4 b = VECTOR ? *(const i32x4 *)(p + 4 * h) : load16_any(p + 4 * h);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * h + i] = __int_as_float(b[i]);
+        }
+    } else {
+        typedef typename vec<T>::x8 x8;
+        const x8 b = __builtin_bit_cast(x8, VECTOR ? *(const i32x4 *)p : load16_any(p));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)b[i];
+    }
+}
+
 // 1 / sigmoid(g), times kUnder.  As 1 + exp(-g) it would be infinite for gates under -88.7, and its reciprocal no normal number
 // under -87.3, where silu(g) of bf16 still is one; scaled, both have room down to -98, where silu(g) is under 2^-134, half of
 // the smallest bf16.  The scale is in the exponent (g / ln 2 rounded at up to 32: the exponential is off by 2^-20 of itself

@@ -9,29 +9,6 @@ namespace {
 
 using namespace pfmoe;
 
-// Eight elements as fp32 from `at` of a row of k; zeros behind its end.
-template <typename T, bool VECTOR>
-__device__ __forceinline__ void load8(const T *row, int at, int k, float v[8])
-{
-    const T *p = row + at;
-    if (at + 8 > k) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = at + i < k ? (float)p[i] : 0.0f;
-    } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const i32x4 b = VECTOR ? *(const i32x4 *)(p + 4 * h) : load16_any(p + 4 * h);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * h + i] = __int_as_float(b[i]);
-        }
-    } else {
-        typedef typename vec<T>::x8 x8;
-        const x8 b = __builtin_bit_cast(x8, VECTOR ? *(const i32x4 *)p : load16_any(p));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)b[i];
-    }
-}
-
 // The nearest integer to 127 x / most, ties to even.  per = 127 / most to 53 bits and the sum that moves the point give
 // the quotient as a multiple of 2^-33, off by less than that.  A quotient of numbers of 24 bits, the one 127 times larger,
 // that is no half lies 2^-25 from any at least, so that halves come out as halves and nothing else does; the second sum
@@ -81,7 +58,7 @@ __global__ __launch_bounds__(256) void k_i8_quantize(const T *x, long long ld, i
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
         const int at = (lane + j * G) * 8;
-        if (lane + j * G < units) load8<T, VECTOR>(row, at, k, v[j]);
+        if (lane + j * G < units) load8_any<T, VECTOR>(row, at, k, v[j]);
         else
             for (int i = 0; i < 8; ++i) v[j][i] = 0;
     }
@@ -89,7 +66,7 @@ __global__ __launch_bounds__(256) void k_i8_quantize(const T *x, long long ld, i
     for (int j = 0; j < PIECES; ++j) take(v[j]);
     for (int u = lane + PIECES * G; u < units; u += G) {
         float w[8];
-        load8<T, VECTOR>(row, u * 8, k, w);
+        load8_any<T, VECTOR>(row, u * 8, k, w);
         take(w);
     }
     for (int o = 32; o > 0; o >>= 1) {
@@ -113,7 +90,7 @@ __global__ __launch_bounds__(256) void k_i8_quantize(const T *x, long long ld, i
         if (lane + j * G < units) put(lane + j * G, v[j]);
     for (int u = lane + PIECES * G; u < units; u += G) {
         float w[8];
-        load8<T, VECTOR>(row, u * 8, k, w);
+        load8_any<T, VECTOR>(row, u * 8, k, w);
         put(u, w);
     }
 }

@@ -1,12 +1,14 @@
 // moe_orth.hip — orthogonal updates on gfx950 (include/prefree_moe.h): X = G / |G|, then a few times
 // X <- a X + (b A + c A A) X with A = X X^T, in 16-bit products on the matrix cores.
 //
-// X is carried in two f16 pieces, of which the products take the first.  What a rounding of X puts where G has nothing
-// is multiplied by a in every step (3.4445^5 = 485), and so are G's small directions with it; in one piece the result of
-// a momentum of rank n / 8 came out 1.5 to 4% off in f16 and 11 to 30% in bf16, in two 0.05 to 0.2% (64 to 1024 rows).
-// With a X formed from both pieces the roundings of the first reach X by way of A and of B X alone, and there they are
-// small beside what X has in the same directions.  A and B = b A + c A A are one f16 piece.
+// X is carried in two pieces, f16 and what that leaves in 8 bits (e5m2), of which the products take the first.  What a
+// rounding of X puts where G has nothing is multiplied by a in every step (3.4445^5 = 485), and so are G's small directions
+// with it: in one f16 piece the result of a momentum of rank n / 8 came out 1.5 to 4% off (in bf16 11 to 30%), in two
+// 0.15 to 0.25% (64 to 1024 rows; with 16 bits for the second 0.13 to 0.16).  With a X formed from both pieces the roundings
+// of the first reach X by way of A and of B X alone, and there they are small beside what X has in the same directions.
+// A and B = b A + c A A are one f16 piece.
 #include <algorithm>
+#include <utility>
 
 #include "moe_tiles.hpp"
 
@@ -14,20 +16,28 @@ namespace {
 
 using namespace pfmoe;
 
-constexpr float kRest = 2048.0f;   // the second piece is held times this, where f16 has all its bits for it
+constexpr float kRest = 2048.0f;   // the second piece is held times this: about as large as the first, whose exponents it has
 
 // One product of all matrices of a batch; they lie one after the other, rows and columns padded with zeros to multiples of 32.
 struct Product {
-    const f16 *p, *q;       // rows operand, and columns operand
-    int m, n, k;            // of a matrix
+    const f16 *p, *q;           // rows operand, and columns operand
+    int m, n, k;                // of a matrix
     int batch, first;
-    float alpha, beta;      // results: alpha times the sums plus beta times what stands there
-    const f16 *old, *old_rest;
-    f16 *out, *rest;
+    int whole, parts;           // tiles in one piece; quarters of the others
+    float alpha, beta, gamma;
+    const f16 *old;             // kPoly: A
+    const unsigned char *old_rest;
+    f16 *out;
+    unsigned char *rest;
+    char *result;               // the last step's, instead of the pieces: [rows][columns], ld_result apart
+    long long ld_result;
+    int rows, columns, result_f16, wide;
 };
 
-// kSquare: out = alpha P P^T;  kPoly: out = alpha P P^T + beta old, P symmetric (both symmetric: the tiles on and under
-// the diagonal, stored twice);  kApply: X' = beta X + P X, X and X' in two pieces, X read across its rows
+// kSquare: A = alpha P P^T
+// kPoly: B = gamma I + beta P + alpha P P, P symmetric.  Both are symmetric: the tiles on and under the diagonal, stored twice.
+// kApply: X' = P X + beta rest(X): P is B with a on its diagonal, so that a X of the first piece is part of the product.
+//         X is read across its rows.
 enum { kSquare = 0, kPoly = 1, kApply = 2 };
 
 // Transposes 4 x 4 values of 16 bits in each four neighbouring lanes: lane r of them has four values of row r, and gets
@@ -51,47 +61,88 @@ __device__ __forceinline__ unsigned pair_of(float a, float b)
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f2{a, b}), h2));
 }
 
+// Four numbers as their first pieces, and what is left of them in 8 bits (e5m2) each.
+struct Pieces {
+    unsigned first[2], rest;
+    __device__ __forceinline__ explicit Pieces(const float v[4])
+    {
+        float left[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) left[i] = (v[i] - (float)(f16)v[i]) * kRest;
+        first[0] = pair_of(v[0], v[1]);
+        first[1] = pair_of(v[2], v[3]);
+        rest = __builtin_amdgcn_cvt_pk_bf8_f32(left[0], left[1], 0, false);
+        rest = __builtin_amdgcn_cvt_pk_bf8_f32(left[2], left[3], rest, true);
+    }
+};
+__device__ __forceinline__ void rest_of(unsigned held, float v[4])
+{
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_bf8(held, false), hi = __builtin_amdgcn_cvt_pk_f32_bf8(held, true);
+    v[0] = lo[0] * (1.0f / kRest);
+    v[1] = lo[1] * (1.0f / kRest);
+    v[2] = hi[0] * (1.0f / kRest);
+    v[3] = hi[1] * (1.0f / kRest);
+}
+
+// N results from column c of a row of the result
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T *row, int c, int columns, bool wide, const float v[N])
+{
+    T h[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) h[i] = (T)v[i];
+    if (wide && c + N <= columns) {
+#pragma unroll
+        for (int i = 0; i < N; i += 8) {
+            i32x4 b;
+            __builtin_memcpy(&b, h + i, 16);
+            *(i32x4 *)(row + c + i) = b;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (c + i < columns) row[c + i] = h[i];
+    }
+}
+
+// The tile from row m0 and column n0 of a matrix's product.
 template <int KIND, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void k_orth(const Product a)
+__device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, int n0, char *shared)
 {
     constexpr int THREADS = WM * WN * 64, FM = BM / WM / 16, FN = BN / WN / 16;
     typedef Along<BM, THREADS, true> P;
     typedef typename std::conditional<KIND == kApply, Across<BN, THREADS, true>, Along<BN, THREADS, true>>::type Q;
     constexpr int SLOT = P::kBytes + Q::kBytes, LOADS = P::kLoads + Q::kLoads;
-    __shared__ __align__(1024) char lds[4][SLOT];
-    static_assert(KIND == kApply || BM == BN, "tiles under the diagonal");
+    const int wave = wave_id(), wm = wave / WN, wn = wave % WN, k = a.k;
+    int lane = threadIdx.x & (kWave - 1);
+    const long long base = (long long)matrix * a.m * a.n;
 
-    const int wave = wave_id(), lane = threadIdx.x & (kWave - 1), wm = wave / WN, wn = wave % WN;
-    const int mt = (a.m + BM - 1) / BM, nt = (a.n + BN - 1) / BN, each = KIND == kApply ? mt * nt : mt * (mt + 1) / 2;
-    const int id = a.first + blockIdx.x, all = a.batch * each, chunk = (all + kXcds - 1) / kXcds;
-    const int at = id % kXcds * chunk + id / kXcds;
-    if (id / kXcds >= chunk || at >= all) return;
-    const int matrix = at / each, t = at % each;
-    int tm, tn;
+    // the second pieces of what this lane will store; they are long there when the products are
+    typedef unsigned Rest __attribute__((ext_vector_type(FN)));
+    Rest rest[KIND == kApply ? FM : 1];
     if constexpr (KIND == kApply) {
-        const int group = t / (8 * nt), side = min(8, mt - group * 8), j = t - group * 8 * nt;
-        tm = group * 8 + j % side;
-        tn = j / side;
-    } else {
-        tm = (int)((__builtin_sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
-        while ((tm + 1) * (tm + 2) / 2 <= t) ++tm;
-        while (tm * (tm + 1) / 2 > t) --tm;
-        tn = t - tm * (tm + 1) / 2;
+        const int c = n0 + wn * FN * 16 + (lane >> 4) * 4 * FN;   // 4 FN columns from here, there as a whole or not at all
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const int r = m0 + (i * WM + wm) * 16 + (lane & 15);
+            rest[i] = Rest{};
+            if (r < a.m && c < a.n) rest[i] = *(const Rest *)(a.old_rest + base + (long long)r * a.n + c);
+        }
     }
-    const int m0 = tm * BM, n0 = tn * BN, k = a.k;
+
     P p;
     Q q;
     {
-        const char *base = (const char *)(a.p + (long long)matrix * a.m * k);
-        p.init(base, 2ull * a.m * k, 2LL * k, [&](int r) { return min(m0 + r, a.m - 1); }, k, 8);
+        const char *from = (const char *)(a.p + (long long)matrix * a.m * k);
+        p.init(from, 2ull * a.m * k, 2LL * k, [&](int r) { return min(m0 + r, a.m - 1); }, k, 8);
     }
     if constexpr (KIND == kApply) {
-        const char *base = (const char *)(a.q + (long long)matrix * k * a.n);
-        q.init(base, 2ull * k * a.n, 2LL * a.n, n0, a.n, k);
+        q.init((const char *)(a.q + (long long)matrix * k * a.n), 2ull * k * a.n, 2LL * a.n, n0, a.n, k);
     } else {
-        const char *base = (const char *)(a.q + (long long)matrix * a.m * k);
-        q.init(base, 2ull * a.m * k, 2LL * k, [&](int r) { return min(n0 + r, a.m - 1); }, k, 8);
+        const char *from = (const char *)(a.q + (long long)matrix * a.m * k);
+        q.init(from, 2ull * a.m * k, 2LL * k, [&](int r) { return min(n0 + r, a.m - 1); }, k, 8);
     }
+    const auto lds = [&](int place) { return shared + place * SLOT; };
     const auto issue = [&](int i, int s, char *to) {
         if (i < P::kLoads) p.issue(i, s, to);
         else if constexpr (KIND == kApply) q.template issue<false>(i - P::kLoads, s, to + P::kBytes, 0);
@@ -134,27 +185,43 @@ __global__ __launch_bounds__(WM * WN * 64) void k_orth(const Product a)
 #pragma unroll
     for (int s = 0; s < 3; ++s)
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) issue(i, s, lds[s]);
+        for (int i = 0; i < LOADS; ++i) issue(i, s, lds(s));
     wait_and_meet<LOADS>();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) x[i] = read_x(lds[0], i);
+    for (int i = 0; i < 2; ++i) x[i] = read_x(lds(0), i);
 #pragma unroll
-    for (int j = 0; j < FN; ++j) w[0][j] = read_w(lds[0], j);
+    for (int j = 0; j < FN; ++j) w[0][j] = read_w(lds(0), j);
 #pragma unroll 1
     for (int s = 0; s < steps; ++s) {
-        step(s, lds[(s + 3) & 3], lds[s & 3], lds[(s + 1) & 3]);
+        step(s, lds((s + 3) & 3), lds(s & 3), lds((s + 1) & 3));
 #pragma unroll
         for (int j = 0; j < FN; ++j) w[0][j] = w[1][j];
     }
     wait_and_meet<0>();   // nothing may still be on its way to LDS when the workgroup ends
 
     // Rows and columns are multiples of 32: blocks of 16 x 16 are there as a whole or not at all.
-    const long long base = (long long)matrix * a.m * a.n;
+    asm volatile("" : "+v"(lane));   // addresses are formed here, not kept over the loop before
+    const int g = lane >> 4, c0 = n0 + wn * FN * 16;
+    typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+    f16x4 old[2][FN];   // kPoly: P's, a block of rows ahead
+    const auto read_old = [&](int i) {
+        if constexpr (KIND == kPoly) {
+            const int r = m0 + (i * WM + wm) * 16 + (lane & 15);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const int c = c0 + j * 16 + g * 4;
+                old[i % 2][j] = f16x4{0, 0, 0, 0};
+                if (r < a.m && c < a.n) old[i % 2][j] = *(const f16x4 *)(a.old + base + (long long)r * a.n + c);
+            }
+        }
+    };
+    read_old(0);
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-        const int r0 = m0 + (i * WM + wm) * 16, c0 = n0 + wn * FN * 16;
+        if (i + 1 < FM) read_old(i + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        const int r0 = m0 + (i * WM + wm) * 16, r = r0 + (lane & 15);
         if (r0 >= a.m) continue;
-        const int r = r0 + (lane & 15), g = lane >> 4;
         if constexpr (KIND == kApply) {
             unsigned v[FN][4];
 #pragma unroll
@@ -162,43 +229,51 @@ __global__ __launch_bounds__(WM * WN * 64) void k_orth(const Product a)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) v[j][c] = __float_as_uint(acc[i][j][c]);
             gather_columns<FN>(v);
-            const int c = c0 + g * 4 * FN;   // 4 FN columns from here, whole or not at all
+            const int c = c0 + g * 4 * FN;
             if (c >= a.n) continue;
+            float y[4 * FN];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                rest_of(rest[i][j], y + 4 * j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[4 * j + e] = __builtin_fmaf(a.beta, y[4 * j + e], __uint_as_float(v[j][e]));
+            }
+            if (a.result) {
+                if (r >= a.rows) continue;
+#pragma unroll
+                for (int e = 0; e < 4 * FN; ++e) y[e] *= a.alpha;
+                char *row = a.result + 2 * a.ld_result * ((long long)matrix * a.rows + r);
+                if (a.result_f16) store_row<f16, 4 * FN>((f16 *)row, c, a.columns, a.wide, y);
+                else store_row<bf16, 4 * FN>((bf16 *)row, c, a.columns, a.wide, y);
+                continue;
+            }
             const long long to = base + (long long)r * a.n + c;
+            Rest left;
 #pragma unroll
             for (int j = 0; j < FN; j += 2) {
-                const f16x8 h = *(const f16x8 *)(a.old + to + 4 * j), l = *(const f16x8 *)(a.old_rest + to + 4 * j);
-                f16x8 nh, nl;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float old = __builtin_fmaf((float)l[e], 1.0f / kRest, (float)h[e]);
-                    const float y = __builtin_fmaf(a.beta, old, __uint_as_float(v[j + e / 4][e % 4]));
-                    nh[e] = (f16)y;
-                    nl[e] = (f16)((y - (float)nh[e]) * kRest);
-                }
-                *(f16x8 *)(a.out + to + 4 * j) = nh;
-                *(f16x8 *)(a.rest + to + 4 * j) = nl;
+                const Pieces one(y + 4 * j), two(y + 4 * j + 4);
+                left[j] = one.rest;
+                left[j + 1] = two.rest;
+                *(i32x4 *)(a.out + to + 4 * j) = i32x4{(int)one.first[0], (int)one.first[1], (int)two.first[0], (int)two.first[1]};
             }
+            *(Rest *)(a.rest + to) = left;
         } else {
             unsigned h[FN][2];
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
                 f32x4 y = acc[i][j];
-                const int c = c0 + j * 16 + g * 4;
-                if constexpr (KIND == kPoly) {
-                    typedef f16 f16x4 __attribute__((ext_vector_type(4)));
-                    f16x4 o = f16x4{0, 0, 0, 0};
-                    if (c < a.n) o = *(const f16x4 *)(a.old + base + (long long)r * a.n + c);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(a.alpha, y[e], a.beta * (float)o[e]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] *= a.alpha;
+                for (int e = 0; e < 4; ++e) {
+                    y[e] *= a.alpha;
+                    if constexpr (KIND == kPoly) {
+                        y[e] = __builtin_fmaf(a.beta, (float)old[i % 2][j][e], y[e]);
+                        if (r == c0 + j * 16 + g * 4 + e) y[e] += a.gamma;
+                    }
                 }
                 h[j][0] = pair_of(y[0], y[1]);
                 h[j][1] = pair_of(y[2], y[3]);
             }
-            if (tm != tn) {
+            if (m0 != n0) {
 #pragma unroll
                 for (int j = 0; j < FN; ++j) {
                     unsigned z[2] = {h[j][0], h[j][1]};
@@ -218,103 +293,228 @@ __global__ __launch_bounds__(WM * WN * 64) void k_orth(const Product a)
     }
 }
 
+// Tile `at` of all matrices' tiles of side B.
+template <int KIND, int B>
+__device__ __forceinline__ void find_orth_tile(const Product &a, int at, int &matrix, int &m0, int &n0)
+{
+    const int mt = (a.m + B - 1) / B, nt = (a.n + B - 1) / B, each = KIND == kApply ? mt * nt : mt * (mt + 1) / 2;
+    matrix = at / each;
+    const int t = at - matrix * each;
+    if constexpr (KIND == kApply) {   // eight tiles of rows side by side over the columns
+        const int group = t / (8 * nt), side = min(8, mt - group * 8), j = t - group * 8 * nt;
+        m0 = (group * 8 + j % side) * B;
+        n0 = j / side * B;
+    } else {
+        int tm = (int)((__builtin_sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
+        while ((tm + 1) * (tm + 2) / 2 <= t) ++tm;
+        while (tm * (tm + 1) / 2 > t) --tm;
+        m0 = tm * B;
+        n0 = (t - tm * (tm + 1) / 2) * B;
+    }
+}
+
+template <int KIND>
+__global__ __launch_bounds__(256) void k_orth_small(const Product a)
+{
+    __shared__ __align__(1024) char lds[4 * 256 * 64];
+    const int id = a.first + blockIdx.x, chunk = (a.whole + kXcds - 1) / kXcds, at = id % kXcds * chunk + id / kXcds;
+    if (id / kXcds >= chunk || at >= a.whole) return;
+    int matrix, m0, n0;
+    find_orth_tile<KIND, 128>(a, at, matrix, m0, n0);
+    orth_tile<KIND, 128, 128, 2, 2>(a, matrix, m0, n0, lds);
+}
+
+template <int KIND>
+__global__ __launch_bounds__(512) void k_orth(const Product a)
+{
+    __shared__ __align__(1024) char lds[4 * 512 * 64];
+    const int id = a.first + blockIdx.x;
+    int matrix, m0, n0;
+    const int big = (a.whole + kXcds - 1) / kXcds * kXcds;
+    if (id < big) {
+        const int at = id % kXcds * (big / kXcds) + id / kXcds;
+        if (at >= a.whole) return;
+        find_orth_tile<KIND, 256>(a, at, matrix, m0, n0);
+        orth_tile<KIND, 256, 256, 2, 4>(a, matrix, m0, n0, lds);
+        return;
+    }
+    if (id - big >= a.parts) return;
+    find_orth_tile<KIND, 256>(a, a.whole + (id - big) / 4, matrix, m0, n0);
+    const bool diagonal = KIND != kApply && m0 == n0;
+    m0 += (id - big) / 2 % 2 * 128;
+    n0 += (id - big) % 2 * 128;
+    if (m0 >= a.m || n0 >= a.n || (diagonal && n0 > m0)) return;
+    orth_tile<KIND, 128, 128, 2, 4>(a, matrix, m0, n0, lds);
+}
+
 // ---- into the two pieces, and out of them --------------------------------------------------------------------------
 
+constexpr int kCus = 256;                // compute units of the card
 constexpr int kParts = PFK_ORTH_PARTS;   // sums of squares of a matrix, at most
 
 // Sums of squares of `per` rows each, in 64 bits: no element is too large or too small for its square.
-template <typename T>
+template <typename T, bool VECTOR>
 __global__ __launch_bounds__(256) void k_orth_norm(const T *g, long long ld, int rows, int columns, int per, double *sums)
 {
     __shared__ double part[4];
-    const int begin = blockIdx.x * per, end = min(rows, begin + per);
-    const T *from = g + (long long)blockIdx.y * rows * ld;
+    const int begin = blockIdx.x * per, have = min(rows - begin, per);
+    const T *from = g + ((long long)blockIdx.y * rows + begin) * ld;
+    const int pieces = (columns + 7) / 8, units = have * pieces;
     double sum = 0;
-    for (int r = begin; r < end; ++r)
-        for (int c = threadIdx.x; c < columns; c += 256) {
-            const double v = (double)(float)from[ld * r + c];
-            sum = __builtin_fma(v, v, sum);
+    for (int u0 = threadIdx.x; u0 < units; u0 += 256 * 4) {
+        float v[4][8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {   // their loads go out together
+            const int u = u0 + 256 * j, r = u / pieces;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j][i] = 0;
+            if (u < units) load8_any<T, VECTOR>(from + ld * r, (u - r * pieces) * 8, columns, v[j]);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = __builtin_fma((double)v[j][i], (double)v[j][i], sum);
+    }
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
     if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = sum;
     __syncthreads();
     if (threadIdx.x == 0) sums[(long long)blockIdx.y * gridDim.x + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// The pieces of scale G / |G|, or of its transpose, in [m][n] with zeros behind the matrix; 64 x 64 elements a workgroup.
-template <typename T>
-__global__ __launch_bounds__(256) void k_orth_pieces(const T *g, long long ld, int rows, int columns, int transposed, const double *sums, int parts,
-                                                     float scale, int m, int n, f16 *x, f16 *rest)
+// scale / |G|; no number for a matrix that holds none, and 0 for one of zeros
+__device__ __forceinline__ double over_norm(const double *sums, int parts, float scale)
+{
+    const int lane = threadIdx.x & (kWave - 1);
+    double sum = lane < parts ? sums[lane] : 0;
+    static_assert(kParts <= kWave, "a lane each");
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    return !(sum < INFINITY) ? (double)NAN : sum > 0 ? scale / __builtin_sqrt(sum) : 0.0;
+}
+
+__device__ __forceinline__ void store_pieces(const float v[8], f16 *x, unsigned char *rest)
+{
+    const Pieces one(v), two(v + 4);
+    *(i32x4 *)x = i32x4{(int)one.first[0], (int)one.first[1], (int)two.first[0], (int)two.first[1]};
+    *(u32x2 *)rest = u32x2{one.rest, two.rest};
+}
+
+// The pieces of scale G / |G|, in [m][n] with zeros behind the matrix.
+template <typename T, bool VECTOR>
+__global__ __launch_bounds__(256) void k_orth_pieces(const T *g, long long ld, int rows, int columns, const double *sums, int parts, float scale, int m,
+                                                     int n, f16 *x, unsigned char *rest)
+{
+    const double by = over_norm(sums + (long long)blockIdx.y * parts, parts, scale);
+    const T *from = g + (long long)blockIdx.y * rows * ld;
+    const int pieces = n / 8, units = m * pieces, first = blockIdx.x * 1024 + threadIdx.x;
+    float v[4][8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int u = first + 256 * j, r = u / pieces, c = (u - r * pieces) * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j][i] = 0;
+        if (u < units && r < rows && c < columns) load8_any<T, VECTOR>(from + ld * r, c, columns, v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int u = first + 256 * j, r = u / pieces, c = (u - r * pieces) * 8;
+        if (u >= units) break;
+        // what lies behind the matrix stays zero, whatever the factor
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j][i] = r < rows && c + i < columns ? (float)((double)v[j][i] * by) : 0.0f;
+        const long long to = (long long)blockIdx.y * m * n + (long long)u * 8;
+        store_pieces(v[j], x + to, rest + to);
+    }
+}
+
+// The same of its transpose, 64 x 64 elements a workgroup.
+template <typename T, bool VECTOR>
+__global__ __launch_bounds__(256) void k_orth_pieces_across(const T *g, long long ld, int rows, int columns, const double *sums, int parts, float scale,
+                                                            int m, int n, f16 *x, unsigned char *rest)
 {
     __shared__ float tile[64][65];
-    const double *mine = sums + (long long)blockIdx.z * parts;
-    double sum = 0;
-    for (int i = 0; i < parts; ++i) sum += mine[i];
-    // no number for a matrix that holds none; zeros stay zeros
-    const double by = !(sum < INFINITY) ? (double)NAN : sum > 0 ? scale / __builtin_sqrt(sum) : 0.0;
-    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;   // of X
+    const double by = over_norm(sums + (long long)blockIdx.z * parts, parts, scale);
+    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;   // of X: columns and rows of G
     const T *from = g + (long long)blockIdx.z * rows * ld;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int i = wave; i < 64; i += 4) {
-        const int r = transposed ? c0 + i : r0 + i, c = transposed ? r0 + lane : c0 + lane;
-        float v = 0;
-        if (r < rows && c < columns) v = (float)((double)(float)from[ld * r + c] * by);
-        if (transposed) tile[lane][i] = v; else tile[i][lane] = v;
+    const int piece = threadIdx.x % 8 * 8, line = threadIdx.x / 8;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = line + 32 * h;
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (c0 + i < rows && r0 + piece < columns) load8_any<T, VECTOR>(from + ld * (c0 + i), r0 + piece, columns, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            tile[piece + e][i] = c0 + i < rows && r0 + piece + e < columns ? (float)((double)v[e] * by) : 0.0f;
     }
     __syncthreads();
-    const long long base = (long long)blockIdx.z * m * n;
-    for (int i = wave; i < 64; i += 4) {
-        if (r0 + i >= m || c0 + lane >= n) continue;
-        const float v = tile[i][lane];
-        const f16 h = (f16)v;
-        x[base + (long long)(r0 + i) * n + c0 + lane] = h;
-        rest[base + (long long)(r0 + i) * n + c0 + lane] = (f16)((v - (float)h) * kRest);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = line + 32 * h;
+        if (r0 + i >= m || c0 + piece >= n) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = tile[i][piece + e];
+        const long long to = (long long)blockIdx.z * m * n + (long long)(r0 + i) * n + c0 + piece;
+        store_pieces(v, x + to, rest + to);
     }
 }
 
+// The transposed result out of the pieces.
 template <typename T>
-__global__ __launch_bounds__(256) void k_orth_out(const f16 *x, const f16 *rest, int m, int n, float scale, int transposed, T *out, long long ld,
-                                                  int rows, int columns)
+__global__ __launch_bounds__(256) void k_orth_out_across(const f16 *x, const unsigned char *rest, int m, int n, float scale, T *out, long long ld, int rows,
+                                                         int columns, int wide)
 {
     __shared__ float tile[64][65];
     const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;   // of X
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long base = (long long)blockIdx.z * m * n;
-    for (int i = wave; i < 64; i += 4) {
-        float v = 0;
-        if (r0 + i < m && c0 + lane < n) {
-            const long long at = base + (long long)(r0 + i) * n + c0 + lane;
-            v = __builtin_fmaf((float)rest[at], 1.0f / kRest, (float)x[at]) * scale;
-        }
-        if (transposed) tile[lane][i] = v; else tile[i][lane] = v;
+    const int piece = threadIdx.x % 8 * 8, line = threadIdx.x / 8;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = line + 32 * h;
+        if (r0 + i >= m || c0 + piece >= n) continue;
+        const long long at = (long long)blockIdx.z * m * n + (long long)(r0 + i) * n + c0 + piece;
+        const f16x8 first = *(const f16x8 *)(x + at);
+        const u32x2 left = *(const u32x2 *)(rest + at);
+        float v[8];
+        rest_of(left[0], v);
+        rest_of(left[1], v + 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) tile[piece + e][i] = ((float)first[e] + v[e]) * scale;
     }
     __syncthreads();
-    T *to = out + (long long)blockIdx.z * rows * ld;
-    for (int i = wave; i < 64; i += 4) {
-        const int r = (transposed ? c0 : r0) + i, c = (transposed ? r0 : c0) + lane;
-        if (r < rows && c < columns) to[ld * r + c] = (T)tile[i][lane];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = line + 32 * h;
+        if (c0 + i >= rows || r0 + piece >= columns) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = tile[i][piece + e];
+        store_row<T, 8>(out + ld * ((long long)blockIdx.z * rows + c0 + i), r0 + piece, columns, wide, v);
     }
-}
-
-template <int KIND, int B, int WM, int WN>
-int launch(Product a, hipStream_t s)
-{
-    const long long mt = (a.m + B - 1) / B, nt = (a.n + B - 1) / B, all = a.batch * (KIND == kApply ? mt * nt : mt * (mt + 1) / 2);
-    const long long grid = (all + kXcds - 1) / kXcds * kXcds;
-    if (grid > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "orthogonalize: too many tiles");
-    in_launches(grid, most_workgroups(WM * WN * 64), [&](long long first, long long count) {
-        a.first = (int)first;
-        k_orth<KIND, B, B, WM, WN><<<dim3((unsigned)count), dim3(WM * WN * 64), 0, s>>>(a);
-    });
-    return pfk_internal_launched("k_orth");
 }
 
 template <int KIND>
-int product(const Product &a, hipStream_t s)
+int product(Product a, hipStream_t s)
 {
-    const long long mt = (a.m + 255) / 256, nt = (a.n + 255) / 256, tiles = a.batch * (KIND == kApply ? mt * nt : mt * (mt + 1) / 2);
-    if (tiles >= 256) return launch<KIND, 256, 2, 4>(a, s);
-    return launch<KIND, 128, 2, 2>(a, s);
+    const auto tiles = [&](long long side) {
+        const long long mt = (a.m + side - 1) / side, nt = (a.n + side - 1) / side;
+        return a.batch * (KIND == kApply ? mt * nt : mt * (mt + 1) / 2);
+    };
+    const auto run = [&](auto kernel, long long workgroups, int threads) {
+        if (workgroups > 0x7fffffffLL) return pfk_internal_fail(PF_ERR_UNSUPPORTED, "orthogonalize: too many tiles");
+        in_launches(workgroups, most_workgroups(threads), [&](long long first, long long count) {
+            a.first = (int)first;
+            kernel<<<dim3((unsigned)count), dim3(threads), 0, s>>>(a);
+        });
+        return pfk_internal_launched("k_orth");
+    };
+    const long long large = tiles(256);
+    if (large >= kCus) {
+        const long long over = large % kCus <= kCus / 2 ? large % kCus : 0;
+        a.whole = (int)(large - over);
+        a.parts = (int)(4 * over);
+        return run(k_orth<KIND>, (a.whole + kXcds - 1LL) / kXcds * kXcds + a.parts, 512);
+    }
+    a.whole = (int)tiles(128);
+    return run(k_orth_small<KIND>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 256);
 }
 
 // launch(grid, first matrix) with a workgroup for each 64 x 64 elements of each matrix
@@ -327,24 +527,43 @@ void each_tile(int batch, int m, int n, F launch)
     });
 }
 
+struct Held {
+    int m, n;
+    float scale;
+    f16 *x;
+    unsigned char *rest;
+};
+
 template <typename T>
-void out_of_pieces(const f16 *x, const f16 *rest, int batch, int m, int n, float scale, int transposed, void *out, long long ld, int rows, int columns,
-                   hipStream_t s)
+void into_pieces(const void *from, long long ld, int batch, int rows, int columns, double *sums, const Held &h, hipStream_t s)
 {
-    each_tile(batch, m, n, [&](dim3 grid, long long at) {
-        k_orth_out<T><<<grid, dim3(256), 0, s>>>(x + at * m * n, rest + at * m * n, m, n, scale, transposed, (T *)out + at * rows * ld, ld, rows, columns);
+    const T *g = (const T *)from;
+    const bool vector = (uintptr_t)g % 16 == 0 && ld * sizeof(T) % 16 == 0;
+    const int per = (rows + kParts - 1) / kParts, parts = (rows + per - 1) / per, m = h.m, n = h.n;
+    const auto norm = vector ? k_orth_norm<T, true> : k_orth_norm<T, false>;
+    norm<<<dim3(parts, batch), dim3(256), 0, s>>>(g, ld, rows, columns, per, sums);
+    if (rows > columns) {
+        const auto kernel = vector ? k_orth_pieces_across<T, true> : k_orth_pieces_across<T, false>;
+        each_tile(batch, m, n, [&](dim3 grid, long long at) {
+            kernel<<<grid, dim3(256), 0, s>>>(g + at * rows * ld, ld, rows, columns, sums + at * parts, parts, h.scale, m, n, h.x + at * m * n,
+                                              h.rest + at * m * n);
+        });
+        return;
+    }
+    const auto kernel = vector ? k_orth_pieces<T, true> : k_orth_pieces<T, false>;
+    const long long each = ((long long)m * n / 8 + 1023) / 1024;
+    in_launches(batch, std::max(1LL, most_workgroups(256) / each), [&](long long at, long long count) {
+        kernel<<<dim3((unsigned)each, (unsigned)count), dim3(256), 0, s>>>(g + at * rows * ld, ld, rows, columns, sums + at * parts, parts, h.scale, m, n,
+                                                                          h.x + at * m * n, h.rest + at * m * n);
     });
 }
 
 template <typename T>
-void into_pieces(const void *g, long long ld, int batch, int rows, int columns, int transposed, double *sums, float scale, int m, int n, f16 *x,
-                 f16 *rest, hipStream_t s)
+void out_across(const Held &h, int batch, void *out, long long ld, int rows, int columns, int wide, hipStream_t s)
 {
-    const int per = (rows + kParts - 1) / kParts, parts = (rows + per - 1) / per;
-    k_orth_norm<T><<<dim3(parts, batch), dim3(256), 0, s>>>((const T *)g, ld, rows, columns, per, sums);
-    each_tile(batch, m, n, [&](dim3 grid, long long at) {
-        k_orth_pieces<T><<<grid, dim3(256), 0, s>>>((const T *)g + at * rows * ld, ld, rows, columns, transposed, sums + at * parts, parts, scale, m, n,
-                                                    x + at * m * n, rest + at * m * n);
+    each_tile(batch, h.m, h.n, [&](dim3 grid, long long at) {
+        const long long from = at * h.m * h.n;
+        k_orth_out_across<T><<<grid, dim3(256), 0, s>>>(h.x + from, h.rest + from, h.m, h.n, 1 / h.scale, (T *)out + at * rows * ld, ld, rows, columns, wide);
     });
 }
 
@@ -354,28 +573,63 @@ extern "C" int pfk_orthogonalize(const void *g, long long ld_g, int dtype, int b
                                  long long ld_out, int out_dtype, void *workspace, void *stream)
 {
     hipStream_t s = (hipStream_t)stream;
-    const int transposed = rows > columns;
-    const int m = PFK_ORTH_SIDE(transposed ? columns : rows), n = PFK_ORTH_SIDE(transposed ? rows : columns);
+    const bool across = rows > columns;
+    const int m = PFK_ORTH_SIDE(across ? columns : rows), n = PFK_ORTH_SIDE(across ? rows : columns);
     const long long xs = (long long)batch * m * n, as = (long long)batch * m * m;
-    f16 *x[2] = {(f16 *)workspace, (f16 *)workspace + 2 * xs}, *a = (f16 *)workspace + 4 * xs, *b = a + as;
-    double *sums = (double *)(b + as);
-    float scale = 1;   // X is held times this: elements of about 1, and none over 2^11 where X has none over 2
+    f16 *x = (f16 *)workspace, *a = x + 2 * xs, *b = a + as;
+    unsigned char *rest = (unsigned char *)(b + as);
+    double *sums = (double *)(rest + 2 * xs);
+    float scale = 1;   // X is held times this: elements of about 1, and none over 2^12 where X has none over 4
     while (scale * scale * 4 <= n && scale < 1024) scale *= 2;
-    if (dtype == PF_F32) into_pieces<float>(g, ld_g, batch, rows, columns, transposed, sums, scale, m, n, x[0], x[0] + xs, s);
-    else if (dtype == PF_F16) into_pieces<f16>(g, ld_g, batch, rows, columns, transposed, sums, scale, m, n, x[0], x[0] + xs, s);
-    else into_pieces<bf16>(g, ld_g, batch, rows, columns, transposed, sums, scale, m, n, x[0], x[0] + xs, s);
+    Held from = {m, n, scale, x, rest}, to = {m, n, scale, x + xs, rest + xs};
+    if (dtype == PF_F32) into_pieces<float>(g, ld_g, batch, rows, columns, sums, from, s);
+    else if (dtype == PF_F16) into_pieces<f16>(g, ld_g, batch, rows, columns, sums, from, s);
+    else into_pieces<bf16>(g, ld_g, batch, rows, columns, sums, from, s);
+    const int wide = (uintptr_t)out % 16 == 0 && ld_out % 8 == 0;
     for (int i = 0; i < n_steps; ++i) {
-        f16 *from = x[i & 1], *to = x[~i & 1];
-        Product square = {from, from, m, m, n, batch, 0, 1 / (scale * scale), 0, nullptr, nullptr, a, nullptr};
-        Product poly = {a, a, m, m, m, batch, 0, steps[3 * i + 2], steps[3 * i + 1], a, nullptr, b, nullptr};
-        Product apply = {b, from, m, n, m, batch, 0, 1, steps[3 * i], from, from + xs, to, to + xs};
+        const float *c = steps + 3 * i;
+        Product square = {};
+        square.p = square.q = from.x;
+        square.m = square.n = m;
+        square.k = n;
+        square.batch = batch;
+        square.alpha = 1 / (scale * scale);
+        square.out = a;
+        Product poly = square;
+        poly.p = poly.q = poly.old = a;
+        poly.k = m;
+        poly.alpha = c[2];
+        poly.beta = c[1];
+        poly.gamma = c[0];
+        poly.out = b;
+        Product apply = {};
+        apply.p = b;
+        apply.q = from.x;
+        apply.m = apply.k = m;
+        apply.n = n;
+        apply.batch = batch;
+        apply.alpha = 1 / scale;
+        apply.beta = c[0];
+        apply.old_rest = from.rest;
+        apply.out = to.x;
+        apply.rest = to.rest;
+        if (i == n_steps - 1 && !across) {
+            apply.result = (char *)out;
+            apply.ld_result = ld_out;
+            apply.rows = rows;
+            apply.columns = columns;
+            apply.result_f16 = out_dtype == PF_F16;
+            apply.wide = wide;
+        }
         int st = product<kSquare>(square, s);
         if (st == PF_OK) st = product<kPoly>(poly, s);
         if (st == PF_OK) st = product<kApply>(apply, s);
         if (st != PF_OK) return st;
+        std::swap(from, to);
     }
-    const f16 *last = x[n_steps & 1];
-    if (out_dtype == PF_F16) out_of_pieces<f16>(last, last + xs, batch, m, n, 1 / scale, transposed, out, ld_out, rows, columns, s);
-    else out_of_pieces<bf16>(last, last + xs, batch, m, n, 1 / scale, transposed, out, ld_out, rows, columns, s);
-    return pfk_internal_launched("k_orth_out");
+    if (across) {
+        if (out_dtype == PF_F16) out_across<f16>(from, batch, out, ld_out, rows, columns, wide, s);
+        else out_across<bf16>(from, batch, out, ld_out, rows, columns, wide, s);
+    }
+    return pfk_internal_launched("k_orth_out_across");
 }

@@ -413,7 +413,7 @@ size_t pf_orthogonalize_workspace(int batch, int rows, int columns)
 {
     if (batch < 1 || rows < 1 || columns < 1) return 0;
     const size_t m = PFK_ORTH_SIDE((size_t)std::min(rows, columns)), n = PFK_ORTH_SIDE((size_t)std::max(rows, columns));
-    return batch * (2 * m * (4 * n + 2 * m) + 8 * PFK_ORTH_PARTS);
+    return batch * (m * (6 * n + 4 * m) + 8 * PFK_ORTH_PARTS);
 }
 
 int pf_orthogonalize(const void *g, long long ld_g, int dtype, int batch, int rows, int columns, const float *steps, int n_steps, void *out,
