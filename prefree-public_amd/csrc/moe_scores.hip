@@ -8,6 +8,7 @@ using namespace pfmoe;
 
 struct Scores : Route {
     int score, groups, group_size, kept, best;
+    int group_lanes, need, vector;   // of the choice in 32 bits: lanes a group, experts a lane (0: not for these sizes), 16-byte loads
     const float *bias;
     float scale;
 };
@@ -167,19 +168,284 @@ __device__ __forceinline__ int choose_exactly(const Scores &a, const float (&z)[
     return expert;
 }
 
+// ---- the same choice, nearly always in 32 bits ----------------------------------------------------------------------
+//
+// A score in fixed point, of 24 bits (22 for more than 256 experts), and the expert's number below it are one word: words
+// are sorted in each lane by maxima and minima, the top_k and three more are taken from the lanes' lists by one reduction each,
+// and of equal scores the lowest expert comes first.  A score may be off by `margin` / 2 units, so the order of two is known
+// where they are further apart, or where they have the same logit and bias.  Where neither holds (about one token in 600),
+// the ones taken are put in order by 64 bits; and where that is not enough, all is done by choose_exactly.
+//
+// Lanes: a group of experts has lanes of its own, G / groups (rounded down to a power of two) of them, with `need` experts each.
+
+constexpr int kTaken = 16;   // at most; lane j of a token holds the one taken as number j
+
+// Batcher's sorting by odd-even merges, largest first.
+template <int N>
+__device__ __forceinline__ void sort(unsigned (&v)[N])
+{
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const unsigned a = v[i + j], b = v[i + j + k];
+                        v[i + j] = a > b ? a : b;
+                        v[i + j + k] = a > b ? b : a;
+                    }
+}
+
+__device__ __forceinline__ double shuffled(double v, int lane, int width)
+{
+    return __hiloint2double(__shfl(__double2hiint(v), lane, width), __shfl(__double2loint(v), lane, width));
+}
+
+template <typename T, int G, int PER>
+struct Fast {
+    static constexpr int kNumber = G == 64 ? 10 : 8;    // bits of an expert's number
+    static constexpr unsigned kNumbers = (1u << kNumber) - 1;
+    const Scores &a;
+    const T *row;
+    int lane;            // of the token's
+    bool by_logit;
+    float margin, most, total;   // softmax: the largest logit, and the sum of exponentials less it
+    double total64;
+
+    static __device__ __forceinline__ unsigned units_of(unsigned key) { return key >> kNumber; }
+    static __device__ __forceinline__ int expert_of(unsigned key) { return (int)(kNumbers - (key & kNumbers)); }
+    __device__ __forceinline__ float bias_of(int e) const { return a.bias ? a.bias[e] : 0.0f; }
+
+    // what the choice goes by, in 64 bits
+    __device__ __forceinline__ double exact(unsigned key) const
+    {
+        if (key == 0) return -INFINITY;
+        const int e = expert_of(key);
+        const double z = (double)(float)row[e];
+        if (by_logit) return z;
+        const double s = a.score == PF_SCORE_SOFTMAX ? exp(z - (double)most) / total64 : 1.0 / (1.0 + exp(-z));
+        return s + (double)bias_of(e);
+    }
+    __device__ __forceinline__ void sum_exactly(bool is)
+    {
+        if (a.score != PF_SCORE_SOFTMAX || by_logit) return;
+        double t = 0;
+#pragma unroll 1
+        for (int e = lane; e < a.experts; e += G) t += is ? exp((double)(float)row[e] - (double)most) : 0.0;
+        total64 = sum_of64<G>(t);
+    }
+
+    // Lane j gets the expert taken as number j, or -1; false in `sure` for a token that this cannot decide.
+    __device__ __forceinline__ int choose(bool is, bool &sure)
+    {
+        const int lanes = a.group_lanes, mine = lane / lanes, from = lane % lanes * a.need;
+        const int first = mine * a.group_size + from, have = mine < a.groups ? min(a.need, a.group_size - from) : 0;
+        float z[PER], b[PER];
+        if (a.vector) {
+            constexpr int EACH = 16 / sizeof(T);
+            typedef T piece __attribute__((ext_vector_type(EACH)));
+#pragma unroll
+            for (int i = 0; i < PER; i += EACH) {
+                const piece v = *(const piece *)(row + min(first + i, a.experts - EACH));   // what is not the lane's is loaded too
+#pragma unroll
+                for (int c = 0; c < EACH && i + c < PER; ++c) z[i + c] = is && i + c < have ? (float)v[c] : -INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const float v = (float)row[min(first + i, a.experts - 1)];
+                z[i] = is && i < have ? v : -INFINITY;
+            }
+        }
+        // the largest and the smallest that can be chosen, of the logits and of the biases
+        bool odd = false;
+        float low = INFINITY, high = -INFINITY;
+        most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            odd |= !(z[i] < INFINITY);
+            most = fmaxf(most, z[i]);
+        }
+        if (a.bias) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const float v = a.bias[min(first + i, a.experts - 1)];
+                b[i] = i < have ? v : -INFINITY;
+                odd |= !(b[i] < INFINITY);
+                low = fminf(low, b[i] > -INFINITY ? b[i] : INFINITY);
+                high = fmaxf(high, b[i]);
+            }
+        } else if (by_logit) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) low = fminf(low, z[i] > -INFINITY ? z[i] : INFINITY);
+            high = most;
+        }
+        most = most_of_floats<G>(most);
+        if (!(most > -INFINITY)) most = 0;
+        float scale, shift = 0;
+        constexpr float kUnits = (float)((1 << (32 - kNumber)) - 3);
+        if (a.bias || by_logit) {
+            low = -most_of_floats<G>(-low);
+            high = most_of_floats<G>(high);
+            const float range = high > low ? high - low : 0.0f;
+            odd |= !(range < INFINITY);
+            shift = low;
+            scale = by_logit ? (range > 0 ? kUnits / range : 0.0f) : kUnits / (1.0f + range);
+            odd |= !(scale < INFINITY);
+        } else {
+            scale = kUnits;
+        }
+        constexpr float kLog2e = 0x1.715476p+0f;
+        total = 1;
+        if (a.score == PF_SCORE_SOFTMAX && (!by_logit || !a.normalise)) {
+            float t = 0;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) t += __builtin_amdgcn_exp2f((z[i] - most) * kLog2e);
+            total = sum_of<G>(t);
+        }
+        const float over = total > 0 ? 1.0f / total : 0.0f;
+        unsigned key[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            float v;
+            if (by_logit) {
+                v = z[i] - shift;
+            } else {
+                v = a.score == PF_SCORE_SOFTMAX ? __builtin_amdgcn_exp2f((z[i] - most) * kLog2e) * over
+                                                : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z[i] * -kLog2e));
+                if (a.bias) v += b[i] - shift;
+            }
+            const bool can = z[i] > -INFINITY && (!a.bias || b[i] > -INFINITY);
+            key[i] = can ? ((unsigned)(v * scale) + 1) << kNumber | (kNumbers - (unsigned)(first + i)) : 0;
+        }
+        sort(key);
+        sure = true;
+        if (a.groups > 1) {
+            unsigned one = key[0], two = key[1], three = key[2];
+            const auto merge = [&](unsigned x, unsigned y, unsigned w) {
+                const unsigned t = min(one, x), u = max(two, y);
+                one = max(one, x);
+                two = max(t, u);
+                three = max(min(t, u), max(three, w));
+            };
+#define PF_MERGE(CTRL) merge(pfdev::dpp<CTRL>(one), pfdev::dpp<CTRL>(two), pfdev::dpp<CTRL>(three))
+            if (lanes > 1) PF_MERGE(pfdev::kDppXor1);
+            if (lanes > 2) PF_MERGE(pfdev::kDppXor2);
+            if (lanes > 4) PF_MERGE(pfdev::kDppHalfMirror);
+            if (lanes > 8) PF_MERGE(pfdev::kDppMirror);
+#undef PF_MERGE
+            if constexpr (G == 64) {
+                if (lanes > 16) {
+                    constexpr int kFar = pfdev::swizzle_xor_pattern<16>();
+                    merge((unsigned)__builtin_amdgcn_ds_swizzle((int)one, kFar), (unsigned)__builtin_amdgcn_ds_swizzle((int)two, kFar),
+                          (unsigned)__builtin_amdgcn_ds_swizzle((int)three, kFar));
+                }
+            }
+            // 0 for a group of which nothing can be chosen; where a second score is missing, what a score of 0 has for units
+            unsigned value = one ? (1u << 30) + units_of(one) : 0;
+            if (a.best == 2 && one)
+                value += two ? units_of(two) : (unsigned)((int)fminf(fmaxf(-shift * scale, -0x1p29f), 0x1p29f) + 1);
+            int rank = 0;
+            for (int g = 0; g < a.groups; ++g) {
+                const unsigned other = (unsigned)__shfl((int)value, g * lanes, G);
+                rank += other > value || (other == value && g < mine);
+            }
+            const bool in = mine < a.groups;
+            const unsigned out = most_of<G>(in && rank >= a.kept ? value : 0), least = ~most_of<G>(in && rank < a.kept ? ~value : 0);
+            const bool near = out != 0 && least - out <= 2 * margin;
+            if (__any(near)) {
+                sum_exactly(is);
+                double x = exact(one), y = exact(two), w = exact(three);
+                if (y > x) { const double t = x; x = y; y = t; }
+                if (w > x) { const double t = x; x = w; w = t; }
+                if (w > y) y = w;
+                if (a.best == 2 && y > -INFINITY) x += y;
+                // a fourth may be as near as the third
+                if (near && three != 0 && units_of(a.best == 2 ? two : one) - units_of(three) <= margin) sure = false;
+                int again = 0;
+                for (int g = 0; g < a.groups; ++g) {
+                    const double other = shuffled(x, g * lanes, G);
+                    again += other > x || (other == x && g < mine);
+                }
+                if (near) rank = again;
+            }
+            if (!(in && rank < a.kept)) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) key[i] = 0;
+            }
+        }
+        unsigned taken = 0;
+        const int count = min(a.top_k + 3, kTaken);
+        for (int j = 0; j < count; ++j) {
+            const unsigned best = most_of<G>(key[0]);
+            if (lane == j) taken = best;
+            // by masks: of a choice between two elements the compiler makes one between all
+            const unsigned pop = key[0] == best ? ~0u : 0u;
+#pragma unroll
+            for (int i = 0; i + 1 < PER; ++i) key[i] = (key[i + 1] & pop) | (key[i] & ~pop);
+            key[PER - 1] &= ~pop;
+        }
+        // the one behind each, in the next lane
+        const unsigned next = (unsigned)__builtin_amdgcn_update_dpp(0, (int)taken, 0x101, 0xf, 0xf, true);   // row_shl 1
+        const bool close = taken != 0 && next != 0 && lane + 1 < count && units_of(taken) - units_of(next) <= margin;
+        const unsigned long long all = G == 64 ? ~0ull : ((1ull << G) - 1) << ((threadIdx.x & (kWave - 1)) / G * G);
+        unsigned long long off = __ballot(odd) & all;
+        if (__any(close)) {
+            bool alike = true;
+            if (close) {
+                const int e = expert_of(taken), f = expert_of(next);
+                alike = (float)row[e] == (float)row[f] && bias_of(e) == bias_of(f);
+            }
+            // up to the first gap behind the top_k: what lies behind that gap lies behind all before it
+            const unsigned long long apart = __ballot(lane >= a.top_k - 1 && lane + 1 < count && !close) & all;
+            const unsigned long long unlike = __ballot(!alike) & all & ((apart & (0 - apart)) - 1);
+            if (!apart) off |= all;
+            if (__any(unlike != 0)) {
+                sum_exactly(is);
+                const int e = expert_of(taken);
+                const double x = lane < count ? exact(taken) : -INFINITY;
+                int rank = 0;
+                for (int j = 0; j < count; ++j) {
+                    const double other = shuffled(x, j, G);
+                    const int f = __shfl(e, j, G);
+                    const bool there = __shfl((int)taken, j, G) != 0;
+                    rank += there && (taken == 0 || other > x || (other == x && f < e));
+                }
+                if (taken == 0 || lane >= count) rank = lane;
+                const int base = (threadIdx.x & (kWave - 1)) / G * G;
+                const unsigned moved = (unsigned)__builtin_amdgcn_ds_permute(4 * (base + rank), (int)taken);
+                if (unlike) taken = moved;
+            }
+        }
+        sure = (__ballot(!sure) & all) == 0 && off == 0 && a.top_k < kTaken;
+        return taken != 0 ? expert_of(taken) : -1;
+    }
+};
+
 template <typename T, int G, int PER>
 __device__ __forceinline__ void choose(const Scores &a, int t, bool is, unsigned long long *mask)
 {
     const int lane = threadIdx.x % G, local = t & (kBlock - 1);
-    const T *row = (const T *)a.logits + a.ld * t;
-    float z[PER];
+    const T *row = (const T *)a.logits + a.ld * (is ? t : 0);
+    const bool by_logit = !a.bias && (a.groups == 1 || a.best == 1);
+    Fast<T, G, PER> fast = {a, row, lane, by_logit, by_logit ? 8.0f : a.score == PF_SCORE_SOFTMAX ? 96.0f : 24.0f};
+    bool sure = false;
+    int expert = -1;
+    if (a.need > 0) expert = fast.choose(is, sure);
+    if (__any(is && !sure)) {
+        float z[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int e = lane * PER + i;
-        z[i] = is && e < a.experts ? (float)row[e] : -INFINITY;
+        for (int i = 0; i < PER; ++i) {
+            const int e = lane * PER + i;
+            z[i] = is && e < a.experts ? (float)row[e] : -INFINITY;
+        }
+        const int exactly = choose_exactly<G, PER>(a, z);
+        if (!sure) expert = exactly;
     }
-    const int expert = choose_exactly<G, PER>(a, z);
-    const bool has = is && expert >= 0;
+    const bool has = is && expert >= 0 && lane < a.top_k;
     const float mine = has ? (float)row[expert] : -INFINITY;
     float part, total;
     if (a.score == PF_SCORE_SIGMOID) {
@@ -187,25 +453,33 @@ __device__ __forceinline__ void choose(const Scores &a, int t, bool is, unsigned
         const float m = a.normalise ? fminf(most_of_floats<G>(mine), 0.0f) : 0.0f;
         part = !has ? 0.0f : mine > 0 ? 1.0f / (1.0f + expf(-mine)) : expf(mine - m) / (1.0f + expf(mine));
         total = a.normalise ? sum_of<G>(part) : 1.0f;
-    } else {
-        float m = mine;
-        if (!a.normalise) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) m = fmaxf(m, z[i]);
-        }
-        m = most_of_floats<G>(m);
+    } else if (a.normalise) {
+        const float m = most_of_floats<G>(mine);   // of all lanes, before any parts
         part = has ? expf(mine - m) : 0.0f;
-        total = part;
-        if (!a.normalise) {
-            total = 0;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) total += z[i] > -INFINITY || z[i] != z[i] ? expf(z[i] - m) : 0.0f;
+        total = sum_of<G>(part);
+    } else {
+        float m = -INFINITY;
+        total = 0;
+        if (__any(is && !sure)) {
+#pragma unroll 1
+            for (int e = lane; e < a.experts; e += G) m = is ? fmaxf(m, (float)row[e]) : m;
+            m = most_of_floats<G>(m);
+#pragma unroll 1
+            for (int e = lane; e < a.experts; e += G) {
+                const float z = is ? (float)row[e] : -INFINITY;
+                total += z == -INFINITY ? 0.0f : expf(z - m);
+            }
+            total = sum_of<G>(total);
         }
-        total = sum_of<G>(total);
+        if (sure) {
+            m = fast.most;
+            total = fast.total;
+        }
+        part = has ? expf(mine - m) : 0.0f;
     }
     if (is && lane < a.top_k) {
         const long long at = (long long)t * a.top_k + lane;
-        a.choice[at] = expert;
+        a.choice[at] = has ? expert : -1;
         a.weight[at] = has ? a.scale * (part / total) : 0.0f;
         if (has) atomicOr(mask + expert, 1ull << local);
     }
@@ -309,13 +583,36 @@ template <typename T>
 int route(Scores a, hipStream_t s)
 {
     constexpr int kThreads = 1024;
+    // lanes a token and experts a lane: as few as hold all groups in lanes of their own
+    int g = 0, per = 0, wide = 1;
+    while (wide < a.groups) wide *= 2;
+    const auto holds = [&](int lanes, int each) {
+        const int need = (a.group_size + lanes / wide - 1) / (lanes / wide);
+        if (g || need > each) return;
+        g = lanes;
+        per = each;
+        a.group_lanes = lanes / wide;
+        a.need = need;
+    };
+    holds(16, 4);
+    holds(16, 8);
+    holds(16, 16);
+    holds(64, 8);
+    holds(64, 16);
+    if (!g) {
+        g = 64;
+        per = 16;
+        a.group_lanes = 1;
+    }
+    const int each = 16 / (int)sizeof(T);
+    a.vector = a.need % each == 0 && a.group_size % each == 0 && (uintptr_t)a.logits % 16 == 0 && a.ld % each == 0;
     in_launches(a.blocks, most_workgroups(kThreads), [&](long long first, long long count) {
         const dim3 grid((unsigned)count), block(kThreads);
         a.first = (int)first;
-        if (a.experts <= 64) k_route_scores<T, 16, 4><<<grid, block, 0, s>>>(a);
-        else if (a.experts <= 128) k_route_scores<T, 16, 8><<<grid, block, 0, s>>>(a);
-        else if (a.experts <= 256) k_route_scores<T, 16, 16><<<grid, block, 0, s>>>(a);
-        else if (a.experts <= 512) k_route_scores<T, 64, 8><<<grid, block, 0, s>>>(a);
+        if (per == 4 && g == 16) k_route_scores<T, 16, 4><<<grid, block, 0, s>>>(a);
+        else if (per == 8 && g == 16) k_route_scores<T, 16, 8><<<grid, block, 0, s>>>(a);
+        else if (g == 16) k_route_scores<T, 16, 16><<<grid, block, 0, s>>>(a);
+        else if (per == 8) k_route_scores<T, 64, 8><<<grid, block, 0, s>>>(a);
         else k_route_scores<T, 64, 16><<<grid, block, 0, s>>>(a);
     });
     return a.blocks > 1 ? launch_places(a, s) : pfk_internal_launched("k_route_scores");

@@ -285,3 +285,53 @@ def test_balancing_evens_the_load():
         pf.moe_balance(offsets, experts, 5e-3, bias, bias)
     mean = tokens * k / experts
     assert most[0] > 1.5 * mean and most[-1] < 1.25 * mean
+
+
+def test_equal_and_nearly_equal_at_the_end_of_the_choice():
+    """Behind the last chosen: one with the same logit, then one that 32 bits cannot tell from both and 64 bits put first."""
+    k, experts = 6, 40
+    z = torch.full((64, experts), -4.0, device=DEV)
+    z[:, 30:30 + k - 1] = torch.linspace(2, 1, k - 1, device=DEV)
+    step = 2.0 ** -24                                       # of a logit of 0.5; of its sigmoid a quarter
+    z[:, 3], z[:, 9], z[:, 20] = 0.5, 0.5, 0.5 + 2 * step
+    z[1::2, 21] = 0.5 + step
+    z[2::4, 22:29] = 0.5
+    for bias in (None, torch.zeros(experts, device=DEV), torch.full((experts,), 0.125, device=DEV)):
+        got = check(z, k, bias=bias)
+        assert (got[0][:, k - 1] == 20).all()
+        check(z, k, bias=bias, score="softmax")
+        for groups, kept in ((4, 2), (8, 5), (10, 4)):
+            check(z, k, bias=bias, groups=groups, groups_kept=kept, group_best=1)
+            check(z, k, bias=bias, groups=groups, groups_kept=kept)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("experts,groups,kept", [(255, 3, 2), (256, 8, 4), (96, 16, 3), (1020, 3, 1), (1024, 4, 2), (640, 5, 2), (24, 8, 8), (7, 7, 3)])
+def test_layouts_of_groups_over_lanes(experts, groups, kept, dtype):
+    for top_k in (1, 14, 15, 16):
+        if top_k <= experts:
+            check(logits(70, experts, experts, True), top_k, dtype, biases(experts), groups=groups, groups_kept=kept)
+            check(logits(70, experts, experts), top_k, dtype, groups=groups, groups_kept=kept, group_best=1, score="softmax", normalise=False)
+
+
+def test_wide_biases_and_logits():
+    """Biases far larger than scores, and logits over the whole range of fp32: fixed point with little room between them."""
+    z, g = logits(300, 64, 21), torch.Generator(device=DEV).manual_seed(5)
+    check(z, 8, bias=torch.randn(64, generator=g, device=DEV) * 1e4, groups=8, groups_kept=4)
+    check(z, 8, bias=torch.randint(-2, 3, (64,), generator=g, device=DEV).float() * 1e6, groups=8, groups_kept=4)
+    wild = z * torch.exp2(torch.randint(-60, 60, (300, 64), generator=g, device=DEV).float())
+    check(wild, 8)
+    check(wild, 8, groups=8, groups_kept=2, group_best=1)
+    huge = z.sign() * 3e38
+    check(huge, 8)
+    check(huge, 8, bias=biases(64), groups=4, groups_kept=2)
+
+
+@pytest.mark.parametrize("level", [0.0, -0.3, 0.3, 50.0, -50.0, 3e7, -3e7])
+def test_groups_with_one_expert_left(level):
+    """A group of which one expert can be chosen counts its score alone, above or below the sums of two."""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    z = logits(2000, 32, 13)
+    z[torch.rand(2000, 32, generator=g, device=DEV) < 0.8] = -float("inf")
+    check(z, 4, bias=biases(32) + level, groups=8, groups_kept=3)
+    check(z, 4, bias=biases(32) + level, groups=4, groups_kept=2, score="softmax")
