@@ -105,8 +105,8 @@ __device__ __forceinline__ void store_row(T *row, int c, int columns, bool wide,
     }
 }
 
-// The tile from row m0 and column n0 of a matrix's product.
-template <int KIND, int BM, int BN, int WM, int WN>
+// The tile from row m0 and column n0 of a matrix's product, with STAGES tiles of k in LDS.
+template <int KIND, int BM, int BN, int WM, int WN, int STAGES>
 __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, int n0, char *shared)
 {
     constexpr int THREADS = WM * WN * 64, FM = BM / WM / 16, FN = BN / WN / 16;
@@ -157,8 +157,11 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
     i32x4 x[4], w[2][FN];
-    // Four tiles of k in LDS, as k_mm has them: fragments are read ahead of the products, the columns' of the next tile
-    // beside this one's, and three tiles are on their way.
+    // As in k_mm fragments are read ahead of the products, the columns' of the next tile beside this one's; of the STAGES - 1
+    // tiles on their way all but the last STAGES - 3 have to be there when the waves meet.
+    constexpr int kAhead = STAGES - 1;
+    // LDS reads after the last one of this step's own tile: two fragments of rows, and those of columns behind it
+    constexpr int kNextReads = 2 + (FN - (FM - 3) * FN / FM) * (KIND == kApply ? 2 : 1);
     const auto step = [&](int s, char *__restrict__ fill, const char *__restrict__ here, const char *__restrict__ next) {
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
@@ -173,27 +176,27 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
                 }
                 if (j == FN / 2) {
 #pragma unroll
-                    for (int l = i * LOADS / FM; l < (i + 1) * LOADS / FM; ++l) issue(l, s + 3, fill);
+                    for (int l = i * LOADS / FM; l < (i + 1) * LOADS / FM; ++l) issue(l, s + kAhead, fill);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        wait_and_meet<LOADS>();
+        wait_and_meet<(STAGES - 3) * LOADS, kNextReads>();
         __builtin_amdgcn_sched_barrier(0);
     };
     const int steps = k / 32;
 #pragma unroll
-    for (int s = 0; s < 3; ++s)
+    for (int s = 0; s < kAhead; ++s)
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) issue(i, s, lds(s));
-    wait_and_meet<LOADS>();
+    wait_and_meet<(STAGES - 3) * LOADS>();
 #pragma unroll
     for (int i = 0; i < 2; ++i) x[i] = read_x(lds(0), i);
 #pragma unroll
     for (int j = 0; j < FN; ++j) w[0][j] = read_w(lds(0), j);
 #pragma unroll 1
     for (int s = 0; s < steps; ++s) {
-        step(s, lds((s + 3) & 3), lds(s & 3), lds((s + 1) & 3));
+        step(s, lds((s + kAhead) % STAGES), lds(s % STAGES), lds((s + 1) % STAGES));
 #pragma unroll
         for (int j = 0; j < FN; ++j) w[0][j] = w[1][j];
     }
@@ -313,15 +316,15 @@ __device__ __forceinline__ void find_orth_tile(const Product &a, int at, int &ma
     }
 }
 
-template <int KIND>
-__global__ __launch_bounds__(256) void k_orth_small(const Product a)
+template <int KIND, int WN, int STAGES>
+__global__ __launch_bounds__(128 * WN) void k_orth_small(const Product a)
 {
-    __shared__ __align__(1024) char lds[4 * 256 * 64];
+    __shared__ __align__(1024) char lds[STAGES * 256 * 64];
     const int id = a.first + blockIdx.x, chunk = (a.whole + kXcds - 1) / kXcds, at = id % kXcds * chunk + id / kXcds;
     if (id / kXcds >= chunk || at >= a.whole) return;
     int matrix, m0, n0;
     find_orth_tile<KIND, 128>(a, at, matrix, m0, n0);
-    orth_tile<KIND, 128, 128, 2, 2>(a, matrix, m0, n0, lds);
+    orth_tile<KIND, 128, 128, 2, WN, STAGES>(a, matrix, m0, n0, lds);
 }
 
 template <int KIND>
@@ -335,7 +338,7 @@ __global__ __launch_bounds__(512) void k_orth(const Product a)
         const int at = id % kXcds * (big / kXcds) + id / kXcds;
         if (at >= a.whole) return;
         find_orth_tile<KIND, 256>(a, at, matrix, m0, n0);
-        orth_tile<KIND, 256, 256, 2, 4>(a, matrix, m0, n0, lds);
+        orth_tile<KIND, 256, 256, 2, 4, 4>(a, matrix, m0, n0, lds);
         return;
     }
     if (id - big >= a.parts) return;
@@ -344,7 +347,7 @@ __global__ __launch_bounds__(512) void k_orth(const Product a)
     m0 += (id - big) / 2 % 2 * 128;
     n0 += (id - big) % 2 * 128;
     if (m0 >= a.m || n0 >= a.n || (diagonal && n0 > m0)) return;
-    orth_tile<KIND, 128, 128, 2, 4>(a, matrix, m0, n0, lds);
+    orth_tile<KIND, 128, 128, 2, 4, 8>(a, matrix, m0, n0, lds);
 }
 
 // ---- into the two pieces, and out of them --------------------------------------------------------------------------
@@ -514,7 +517,8 @@ int product(Product a, hipStream_t s)
         return run(k_orth<KIND>, (a.whole + kXcds - 1LL) / kXcds * kXcds + a.parts, 512);
     }
     a.whole = (int)tiles(128);
-    return run(k_orth_small<KIND>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 256);
+    if (a.whole <= kCus) return run(k_orth_small<KIND, 4, 8>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 512);
+    return run(k_orth_small<KIND, 2, 4>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 256);
 }
 
 // launch(grid, first matrix) with a workgroup for each 64 x 64 elements of each matrix

@@ -418,12 +418,12 @@ struct Scales {
     }
 };
 
-// Waits until at most LOADS of this wave's loads to LDS are under way and all its LDS reads are done, then for the
-// other waves.  (__syncthreads() would wait for every load.)
-template <int LOADS>
+// Waits until at most LOADS of this wave's loads to LDS and its last READS LDS reads are under way, then for the other
+// waves.  (__syncthreads() would wait for every load.)
+template <int LOADS, int READS = 0>
 __device__ __forceinline__ void wait_and_meet()
 {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(%1)\n\ts_barrier" ::"n"(LOADS), "n"(READS) : "memory");
 }
 
 // Stores a wave's results: FMV of its FM blocks of 16 rows (every WM-th of the tile's, of which `have` rows exist),
