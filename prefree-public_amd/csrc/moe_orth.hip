@@ -10,13 +10,12 @@
 #include <algorithm>
 #include <utility>
 
+#include "moe_orth.hpp"
 #include "moe_tiles.hpp"
 
 namespace {
 
 using namespace pfmoe;
-
-constexpr float kRest = 2048.0f;   // the second piece is held times this: about as large as the first, whose exponents it has
 
 // One product of all matrices of a batch; they lie one after the other, rows and columns padded with zeros to multiples of 32.
 struct Product {
@@ -39,27 +38,6 @@ struct Product {
 // kApply: X' = P X + beta rest(X): P is B with a on its diagonal, so that a X of the first piece is part of the product.
 //         X is read across its rows.
 enum { kSquare = 0, kPoly = 1, kApply = 2 };
-
-// Transposes 4 x 4 values of 16 bits in each four neighbouring lanes: lane r of them has four values of row r, and gets
-// value r of rows 0 to 3.
-__device__ __forceinline__ void transpose4(unsigned (&h)[2], int lane)
-{
-    const unsigned p0 = (unsigned)pfdev::dpp<pfdev::kDppXor1>(h[0]), p1 = (unsigned)pfdev::dpp<pfdev::kDppXor1>(h[1]);
-    // bytes 0 to 3 are the second argument's, 4 to 7 the first's
-    const unsigned pick = lane & 1 ? 0x03020706 : 0x05040100;
-    const unsigned n0 = __builtin_amdgcn_perm(p0, h[0], pick);
-    const unsigned n1 = __builtin_amdgcn_perm(p1, h[1], pick);
-    const unsigned q0 = (unsigned)pfdev::dpp<pfdev::kDppXor2>(n0), q1 = (unsigned)pfdev::dpp<pfdev::kDppXor2>(n1);
-    h[0] = lane & 2 ? q1 : n0;
-    h[1] = lane & 2 ? n1 : q0;
-}
-
-__device__ __forceinline__ unsigned pair_of(float a, float b)
-{
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    typedef f16 h2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(unsigned, __builtin_convertvector((f2{a, b}), h2));
-}
 
 // Four numbers as their first pieces, and what is left of them in 8 bits (e5m2) each.
 struct Pieces {
@@ -84,27 +62,6 @@ __device__ __forceinline__ void rest_of(unsigned held, float v[4])
     v[3] = hi[1] * (1.0f / kRest);
 }
 
-// N results from column c of a row of the result
-template <typename T, int N>
-__device__ __forceinline__ void store_row(T *row, int c, int columns, bool wide, const float v[N])
-{
-    T h[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) h[i] = (T)v[i];
-    if (wide && c + N <= columns) {
-#pragma unroll
-        for (int i = 0; i < N; i += 8) {
-            i32x4 b;
-            __builtin_memcpy(&b, h + i, 16);
-            *(i32x4 *)(row + c + i) = b;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (c + i < columns) row[c + i] = h[i];
-    }
-}
-
 // The tile from row m0 and column n0 of a matrix's product, with STAGES tiles of k in LDS.
 template <int KIND, int BM, int BN, int WM, int WN, int STAGES>
 __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, int n0, char *shared)
@@ -120,13 +77,13 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
     // the second pieces of what this lane will store; they are long there when the products are
     typedef unsigned Rest __attribute__((ext_vector_type(FN)));
     Rest rest[KIND == kApply ? FM : 1];
-    if constexpr (KIND == kApply) {
+    if constexpr (KIND == kApply) {   // none of the last step's: what they would add is not multiplied any more
         const int c = n0 + wn * FN * 16 + (lane >> 4) * 4 * FN;   // 4 FN columns from here, there as a whole or not at all
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             const int r = m0 + (i * WM + wm) * 16 + (lane & 15);
             rest[i] = Rest{};
-            if (r < a.m && c < a.n) rest[i] = *(const Rest *)(a.old_rest + base + (long long)r * a.n + c);
+            if (a.old_rest && r < a.m && c < a.n) rest[i] = *(const Rest *)(a.old_rest + base + (long long)r * a.n + c);
         }
     }
 
@@ -162,17 +119,18 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
     constexpr int kAhead = STAGES - 1;
     // LDS reads after the last one of this step's own tile: two fragments of rows, and those of columns behind it
     constexpr int kNextReads = 2 + (FN - (FM - 3) * FN / FM) * (KIND == kApply ? 2 : 1);
-    const auto step = [&](int s, char *__restrict__ fill, const char *__restrict__ here, const char *__restrict__ next) {
+    const auto step = [&](auto side, int s, char *__restrict__ fill, const char *__restrict__ here, const char *__restrict__ next) {
+        constexpr int now = decltype(side)::value;   // of w; the next tile's fragments go to the other
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             const char *from = i + 2 < FM ? here : next;
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
-                acc[i][j] = mfma<f16>(w[0][j], x[i % 4], acc[i][j]);
+                acc[i][j] = mfma<f16>(w[now][j], x[i % 4], acc[i][j]);
                 if (j == 0) x[(i + 2) % 4] = read_x(from, (i + 2) % FM);
                 if (j == 1) {
 #pragma unroll
-                    for (int c = i * FN / FM; c < (i + 1) * FN / FM; ++c) w[1][c] = read_w(next, c);
+                    for (int c = i * FN / FM; c < (i + 1) * FN / FM; ++c) w[1 - now][c] = read_w(next, c);
                 }
                 if (j == FN / 2) {
 #pragma unroll
@@ -184,7 +142,7 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
         wait_and_meet<(STAGES - 3) * LOADS, kNextReads>();
         __builtin_amdgcn_sched_barrier(0);
     };
-    const int steps = k / 32;
+    const int steps = k / 32;   // by twos: behind k tiles are zeros
 #pragma unroll
     for (int s = 0; s < kAhead; ++s)
 #pragma unroll
@@ -195,10 +153,9 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
 #pragma unroll
     for (int j = 0; j < FN; ++j) w[0][j] = read_w(lds(0), j);
 #pragma unroll 1
-    for (int s = 0; s < steps; ++s) {
-        step(s, lds((s + kAhead) % STAGES), lds(s % STAGES), lds((s + 1) % STAGES));
-#pragma unroll
-        for (int j = 0; j < FN; ++j) w[0][j] = w[1][j];
+    for (int s = 0; s < steps; s += 2) {
+        step(std::integral_constant<int, 0>(), s, lds((s + kAhead) % STAGES), lds(s % STAGES), lds((s + 1) % STAGES));
+        step(std::integral_constant<int, 1>(), s + 1, lds((s + 1 + kAhead) % STAGES), lds((s + 1) % STAGES), lds((s + 2) % STAGES));
     }
     wait_and_meet<0>();   // nothing may still be on its way to LDS when the workgroup ends
 
@@ -259,7 +216,7 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
                 left[j + 1] = two.rest;
                 *(i32x4 *)(a.out + to + 4 * j) = i32x4{(int)one.first[0], (int)one.first[1], (int)two.first[0], (int)two.first[1]};
             }
-            *(Rest *)(a.rest + to) = left;
+            if (a.rest) *(Rest *)(a.rest + to) = left;
         } else {
             unsigned h[FN][2];
 #pragma unroll
@@ -353,7 +310,6 @@ __global__ __launch_bounds__(512) void k_orth(const Product a)
 // ---- into the two pieces, and out of them --------------------------------------------------------------------------
 
 constexpr int kCus = 256;                // compute units of the card
-constexpr int kParts = PFK_ORTH_PARTS;   // sums of squares of a matrix, at most
 
 // Sums of squares of `per` rows each, in 64 bits: no element is too large or too small for its square.
 template <typename T, bool VECTOR>
@@ -382,16 +338,6 @@ __global__ __launch_bounds__(256) void k_orth_norm(const T *g, long long ld, int
     if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = sum;
     __syncthreads();
     if (threadIdx.x == 0) sums[(long long)blockIdx.y * gridDim.x + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
-}
-
-// scale / |G|; no number for a matrix that holds none, and 0 for one of zeros
-__device__ __forceinline__ double over_norm(const double *sums, int parts, float scale)
-{
-    const int lane = threadIdx.x & (kWave - 1);
-    double sum = lane < parts ? sums[lane] : 0;
-    static_assert(kParts <= kWave, "a lane each");
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-    return !(sum < INFINITY) ? (double)NAN : sum > 0 ? scale / __builtin_sqrt(sum) : 0.0;
 }
 
 __device__ __forceinline__ void store_pieces(const float v[8], f16 *x, unsigned char *rest)
@@ -538,21 +484,23 @@ struct Held {
     unsigned char *rest;
 };
 
+// Squares' sums and, but for narrow matrices, the pieces; returns how many sums a matrix has.
 template <typename T>
-void into_pieces(const void *from, long long ld, int batch, int rows, int columns, double *sums, const Held &h, hipStream_t s)
+int into_pieces(const void *from, long long ld, int batch, int rows, int columns, double *sums, const Held &h, hipStream_t s)
 {
     const T *g = (const T *)from;
     const bool vector = (uintptr_t)g % 16 == 0 && ld * sizeof(T) % 16 == 0;
     const int per = (rows + kParts - 1) / kParts, parts = (rows + per - 1) / per, m = h.m, n = h.n;
     const auto norm = vector ? k_orth_norm<T, true> : k_orth_norm<T, false>;
     norm<<<dim3(parts, batch), dim3(256), 0, s>>>(g, ld, rows, columns, per, sums);
+    if (!h.x) return parts;
     if (rows > columns) {
         const auto kernel = vector ? k_orth_pieces_across<T, true> : k_orth_pieces_across<T, false>;
         each_tile(batch, m, n, [&](dim3 grid, long long at) {
             kernel<<<grid, dim3(256), 0, s>>>(g + at * rows * ld, ld, rows, columns, sums + at * parts, parts, h.scale, m, n, h.x + at * m * n,
                                               h.rest + at * m * n);
         });
-        return;
+        return parts;
     }
     const auto kernel = vector ? k_orth_pieces<T, true> : k_orth_pieces<T, false>;
     const long long each = ((long long)m * n / 8 + 1023) / 1024;
@@ -560,6 +508,7 @@ void into_pieces(const void *from, long long ld, int batch, int rows, int column
         kernel<<<dim3((unsigned)each, (unsigned)count), dim3(256), 0, s>>>(g + at * rows * ld, ld, rows, columns, sums + at * parts, parts, h.scale, m, n,
                                                                           h.x + at * m * n, h.rest + at * m * n);
     });
+    return parts;
 }
 
 template <typename T>
@@ -585,10 +534,15 @@ extern "C" int pfk_orthogonalize(const void *g, long long ld_g, int dtype, int b
     double *sums = (double *)(rest + 2 * xs);
     float scale = 1;   // X is held times this: elements of about 1, and none over 2^12 where X has none over 4
     while (scale * scale * 4 <= n && scale < 1024) scale *= 2;
-    Held from = {m, n, scale, x, rest}, to = {m, n, scale, x + xs, rest + xs};
-    if (dtype == PF_F32) into_pieces<float>(g, ld_g, batch, rows, columns, sums, from, s);
-    else if (dtype == PF_F16) into_pieces<f16>(g, ld_g, batch, rows, columns, sums, from, s);
-    else into_pieces<bf16>(g, ld_g, batch, rows, columns, sums, from, s);
+    const bool narrow = m <= PFK_ORTH_NARROW;
+    if (narrow) sums = (double *)workspace;
+    Held from = {m, n, scale, narrow ? nullptr : x, rest}, to = {m, n, scale, x + xs, rest + xs};
+    const int parts = dtype == PF_F32   ? into_pieces<float>(g, ld_g, batch, rows, columns, sums, from, s)
+                      : dtype == PF_F16 ? into_pieces<f16>(g, ld_g, batch, rows, columns, sums, from, s)
+                                        : into_pieces<bf16>(g, ld_g, batch, rows, columns, sums, from, s);
+    if (narrow)
+        return launch_narrow({g, ld_g, ld_out, dtype, batch, rows, columns, n_steps, out_dtype == PF_F16, steps, scale, sums, parts, out,
+                              (char *)workspace + 8LL * PFK_ORTH_PARTS * batch}, s);
     const int wide = (uintptr_t)out % 16 == 0 && ld_out % 8 == 0;
     for (int i = 0; i < n_steps; ++i) {
         const float *c = steps + 3 * i;
@@ -614,9 +568,9 @@ extern "C" int pfk_orthogonalize(const void *g, long long ld_g, int dtype, int b
         apply.batch = batch;
         apply.alpha = 1 / scale;
         apply.beta = c[0];
-        apply.old_rest = from.rest;
+        apply.old_rest = i == 0 || i < n_steps - 1 ? from.rest : nullptr;
         apply.out = to.x;
-        apply.rest = to.rest;
+        apply.rest = across || i < n_steps - 2 ? to.rest : nullptr;
         if (i == n_steps - 1 && !across) {
             apply.result = (char *)out;
             apply.ld_result = ld_out;
