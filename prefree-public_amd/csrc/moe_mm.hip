@@ -290,6 +290,13 @@ int launch(const Args &a, hipStream_t stream)
 // 1025 -> 1023, 300) 67 / 63, 1536 (32, 2047 -> 2 x 1023, 32) 104 / 97.  It costs up to 16% where the 128 x 128 tiles, two a CU,
 // just fit a round, with 1024 (32, 2047 -> 2 x 511, 64) 89 / 77, or just do not, with 2112 (16, 2047 -> 2047, 200) 156 / 173.
 //
+// 8-bit integers, the rows' kernel, 128 x 128 tiles and k_mm_stream: 64 experts, 2048 -> 2 x 1024, rows 2: 42 / 57 / 61, 8: 56 /
+// 61 / 65, 12: 64 / 61 / 64, 25: - / 63 / 65, 64: - / 82 / 70; 128 experts, 1024 -> 2 x 512, 4: 33 / 37 / 38, 12: 44 / 39 / 39; 16
+// experts, 4096 -> 2048, 8: 35 / 43 / 51, 12: 41 / 42 / 51, 20: 53 / 42 / 51; 32 experts, 2047 -> 2 x 1023, 18: 43 / 34 / 37, 37: 69 /
+// 36 / 38; 2048 -> 2 x 2048, 128: - / 104 / 95.  Where even the 128 x 128 tiles are few the rows' kernel fills the card longer: 12
+// experts, 1111 -> 717, 16: 6 / 12 / 16, 52: 9 / 15 / 21, 100: 13 / 17 / 25; 8 experts, 1024 -> 1024, 32: 8 / 11 / 14, 64: 12 / 12
+// / 15, 96: 16 / 12 / 16; 4 experts, 2048 -> 2 x 512, 50: 9 / 17 / 22.
+//
 // Gradients with 128 x 128 against 256 x 256: 32764 slots of 32 experts, 1023 x 2049, dx 522 / 423, dw 628 / 540; 8000 of 16,
 // 2047 x 2047, dx 243 / 270, dw 377 / 287; 2000 of 16, 1023 x 1025, dx 45 / 72, dw 90 / 91.
 template <typename T, int FORM, int MODE, int ACT, bool ALIGNED>
@@ -300,11 +307,13 @@ int launch_size(const Args &a, hipStream_t stream)
         return (MODE == kDw ? a.experts * ((a.m + side - 1) / side) : a.slots / side + used) * ((a.n * (ACT ? 2LL : 1LL) + side - 1) / side);
     };
     if constexpr (MODE == kFwd) {
-        const bool few = ALIGNED ? rows <= 8 && (tiles(128) < 512 || a.ld_q >= 4000) : rows <= (tiles(128) < 128 ? 24 : 4);
+        const bool few = FORM == kI8 ? rows <= (tiles(128) < 128 ? 60 : 8)
+                         : ALIGNED   ? rows <= 8 && (tiles(128) < 512 || a.ld_q >= 4000)
+                                     : rows <= (tiles(128) < 128 ? 24 : 4);
         if (few) return launch_rows<T, FORM, ACT, ALIGNED>(a, stream);
     }
     if constexpr (ALIGNED) {
-        if (tiles(256) >= (MODE != kDw && rows >= 96 ? 128 : 256)) return launch_stream<T, FORM, MODE, ACT>(a, stream);
+        if (tiles(256) >= (MODE != kDw && rows >= 96 ? 128 : 256) && (FORM != kI8 || rows >= 48)) return launch_stream<T, FORM, MODE, ACT>(a, stream);
     } else if constexpr (MODE == kFwd) {
         if (tiles(64) < 1300) return launch<T, FORM, MODE, ACT, 64, 64, 2, 2, ALIGNED>(a, stream);
     } else {

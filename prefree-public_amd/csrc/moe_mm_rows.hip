@@ -6,7 +6,10 @@ namespace pfmoe {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kPieces = 4;   // 16-byte pieces of a row that a lane takes at a time; four lanes share a row
+// 16-byte pieces of a row that a lane takes at a time; four lanes share a row.  With two, rows of few bytes still give every
+// wave several turns, and more waves fit: 8-bit integers, 16 tokens, 8 of 64 experts, 2048 -> 2 x 1024, in 42 us and not 51, 64
+// tokens of 128, 4096 -> 2 x 512, in 89 and not 103, with one 101.  (The others' order of summation stays as it was.)
+template <int FORM> constexpr int kPiecesOf = FORM == kI8 ? 2 : 4;
 
 // A workgroup computes 16 columns (and the 16 of the gate) of up to 16 rows.  Its waves share k out in blocks of
 // kPieces pieces a lane, the next block's weights on their way while one is multiplied, and add their sums in LDS in a
@@ -17,9 +20,10 @@ constexpr int kPieces = 4;   // 16-byte pieces of a row that a lane takes at a t
 // MB in 107 to 109 us, 5.0 TB/s (a stream that only reads: 6.2, with non-temporal loads 7.0).  With the gate a wave has twice the loads on their way, and two waves a SIMD
 // with their registers do better than three with a spill (118 us); without it two to four are alike.
 template <typename T, int FORM, int ACT, bool ALIGNED>
-__global__ __launch_bounds__(kWaves * kWave, ALIGNED && !ACT ? 4 : 2) void k_mm_rows(const Args a)
+__global__ __launch_bounds__(kWaves * kWave, FORM == kI8 || (ALIGNED && !ACT) ? 4 : 2) void k_mm_rows(const Args a)
 {
     constexpr bool FP4 = FORM == kMx4;
+    constexpr int kPieces = kPiecesOf<FORM>;
     constexpr int NB = ACT ? 2 : 1;
     typedef typename sums_of<FORM>::type SUM;
     typedef typename std::conditional<FORM == kI8, int, float>::type Sum;
@@ -118,8 +122,10 @@ __global__ __launch_bounds__(kWaves * kWave, ALIGNED && !ACT ? 4 : 2) void k_mm_
     const auto multiply = [&](int side, int b) __attribute__((always_inline)) {
         piece(side, b, std::integral_constant<int, 0>());
         piece(side, b, std::integral_constant<int, 1>());
-        piece(side, b, std::integral_constant<int, 2>());
-        piece(side, b, std::integral_constant<int, 3>());
+        if constexpr (kPieces > 2) {
+            piece(side, b, std::integral_constant<int, 2>());
+            piece(side, b, std::integral_constant<int, 3>());
+        }
     };
     int b = wave;
     if (b < blocks) fetch_w(0, b);

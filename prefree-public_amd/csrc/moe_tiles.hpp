@@ -435,9 +435,15 @@ __device__ __forceinline__ void store_blocks(const Args &a, const SUM (&sums)[FM
     asm volatile("" : "+v"(lane));   // addresses are formed here, not kept over the loop before
     constexpr bool SCALED = std::is_same<SUM, i32x4>::value;
     f32x4 unit[SCALED ? FN : 1];
-    if constexpr (SCALED) {
+    float mine[SCALED ? FMV : 1];
+    if constexpr (SCALED) {   // all at once: a row's is behind two loads, one after the other
+        int row[FMV];
+#pragma unroll
+        for (int i = 0; i < FMV; ++i) row[i] = units.row_of(min((i * WM + wm) * 16 + (lane & 15), have - 1));
 #pragma unroll
         for (int j = 0; j < FN; ++j) unit[j] = units.columns(j, lane);
+#pragma unroll
+        for (int i = 0; i < FMV; ++i) mine[i] = a.p_unit[row[i]];
     }
 #pragma unroll
     for (int i = 0; i < FMV; ++i) {
@@ -448,11 +454,10 @@ __device__ __forceinline__ void store_blocks(const Args &a, const SUM (&sums)[FM
         char *out = a.out + a.ld_out * (first + r);
         f32x4 acc[1][FN];
         if constexpr (SCALED) {
-            const float mine = units.row(r, is);
 #pragma unroll
             for (int j = 0; j < FN; ++j)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) acc[0][j][c] = (float)sums[i][j][c] * (mine * unit[j][c]);
+                for (int c = 0; c < 4; ++c) acc[0][j][c] = (float)sums[i][j][c] * (mine[i] * unit[j][c]);
         } else {
 #pragma unroll
             for (int j = 0; j < FN; ++j) acc[0][j] = sums[i][j];
@@ -510,7 +515,7 @@ struct Units {
         for (int c = 0; c < 4; ++c) v[c] = from[n + c < a->n ? n + c : a->n - 1];
         return v;
     }
-    __device__ __forceinline__ float row(int r, bool is) const { return is ? a->p_unit[row_of_slot(*a, (int)(first + r))] : 0.0f; }
+    __device__ __forceinline__ int row_of(int r) const { return row_of_slot(*a, (int)(first + r)); }
 };
 struct NoUnits { };
 
