@@ -244,12 +244,10 @@ __global__ __launch_bounds__(WM * WN * 64) void k_mm(const Args a)
         wait_and_meet<0>();
     }
 
-    const auto units = [&]() {
-        if constexpr (FORM == kI8) return Units<ACT, FN>{&a, a.q_unit + (ACT ? 2LL : 1LL) * a.n * t.e, (long long)t.begin + m0, wn, t.n * OUT_N};
-        else return NoUnits{};
-    };
+    typename std::conditional<FORM == kI8, Units<ACT, FM, FN, WM>, NoUnits>::type units;
+    if constexpr (FORM == kI8) units.load(a, a.q_unit + (ACT ? 2LL : 1LL) * a.n * t.e, wm, wn, t.n * OUT_N, count - m0, slot_row);
     store_results<T, MODE, ACT, FM, FM, FN, WM, OUT_N>(a, acc, wm, wn, MODE == kDw ? (long long)t.e * a.m + m0 : (long long)t.begin + m0,
-                                                MODE == kDw ? a.m - m0 : count - m0, t.n * OUT_N, units());
+                                                MODE == kDw ? a.m - m0 : count - m0, t.n * OUT_N, units);
 }
 
 template <typename T, int FORM, int MODE, int ACT, int BM, int BN, int WM, int WN, bool ALIGNED>

@@ -379,6 +379,10 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
         Work after;
         bool more_after = false;
         const auto all = [&](auto blocks) {
+            // 8-bit integers: there long before the sums are
+            typename std::conditional<FORM == kI8, Units<ACT, decltype(blocks)::value, FN, WM>, NoUnits>::type units;
+            if constexpr (FORM == kI8)
+                units.load(a, a.q_unit + (ACT ? 2LL : 1LL) * a.n * now.e, wm, wn, now.n * OUT_N, have, [&](int r) { return row_of(now, side ^ 1, r); });
             bool fresh = i > 0;
 #pragma unroll 1
             for (int s = 0; s < steps; ++s) {
@@ -392,13 +396,8 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
             // Of the next output tile three tiles of k are on their way.  Stores would end behind them in no order that a
             // counted wait could use, so they have to be there first.
             wait_loads();
-            const auto units = [&]() {
-                if constexpr (FORM == kI8)
-                    return Units<ACT, FN>{&a, a.q_unit + (ACT ? 2LL : 1LL) * a.n * now.e, (long long)now.begin + now.m0, wn, now.n * OUT_N};
-                else return NoUnits{};
-            };
             store_results<T, MODE, ACT, decltype(blocks)::value, FM, FN, WM, OUT_N>(
-                a, acc, wm, wn, MODE == kDw ? (long long)now.e * a.m + now.m0 : (long long)now.begin + now.m0, have, now.n * OUT_N, units());
+                a, acc, wm, wn, MODE == kDw ? (long long)now.e * a.m + now.m0 : (long long)now.begin + now.m0, have, now.n * OUT_N, units);
         };
         if (have > kTile / 2) all(std::integral_constant<int, FM>());
         else all(std::integral_constant<int, FM / 2>());   // half the rows: half the products

@@ -426,6 +426,33 @@ __device__ __forceinline__ void wait_and_meet()
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(%1)\n\ts_barrier" ::"n"(LOADS), "n"(READS) : "memory");
 }
 
+// What 1 of a lane's rows and columns stands for, of 8-bit integers: FM rows, and four columns of each of FN blocks.
+template <int ACT, int FM, int FN, int WM>
+struct Units {
+    float row[FM];
+    f32x4 column[FN];
+
+    // n0: the tile's first column; q: the expert's.  row_of(r): x's row for row r of the tile, of which `have` exist
+    template <typename F>
+    __device__ __forceinline__ void load(const Args &a, const float *q, int wm, int wn, int n0, int have, F row_of)
+    {
+        const int lane = threadIdx.x & (kWave - 1);
+        int of[FM];   // rows first: a unit may be behind a load of its number
+#pragma unroll
+        for (int i = 0; i < FM; ++i) of[i] = row_of(min((i * WM + wm) * 16 + (lane & 15), have - 1));
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int n = ACT ? n0 + (wn * FN + j) / 2 * 16 + (lane >> 4) * 4 : n0 + (wn * FN + j) * 16 + (lane >> 4) * 4;
+            const float *from = q + (ACT && j % 2 ? a.n : 0);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) column[j][c] = from[n + c < a.n ? n + c : a.n - 1];
+        }
+#pragma unroll
+        for (int i = 0; i < FM; ++i) row[i] = a.p_unit[of[i]];
+    }
+};
+struct NoUnits { };
+
 // Stores a wave's results: FMV of its FM blocks of 16 rows (every WM-th of the tile's, of which `have` rows exist),
 // FN blocks of 16 columns.  first: the tile's first row of the output, n0 its first column.
 template <typename T, int MODE, int ACT, bool WHOLE, int FMV, int FM, int FN, int WM, typename SUM, typename U>
@@ -434,17 +461,6 @@ __device__ __forceinline__ void store_blocks(const Args &a, const SUM (&sums)[FM
     int lane = threadIdx.x & (kWave - 1);
     asm volatile("" : "+v"(lane));   // addresses are formed here, not kept over the loop before
     constexpr bool SCALED = std::is_same<SUM, i32x4>::value;
-    f32x4 unit[SCALED ? FN : 1];
-    float mine[SCALED ? FMV : 1];
-    if constexpr (SCALED) {   // all at once: a row's is behind two loads, one after the other
-        int row[FMV];
-#pragma unroll
-        for (int i = 0; i < FMV; ++i) row[i] = units.row_of(min((i * WM + wm) * 16 + (lane & 15), have - 1));
-#pragma unroll
-        for (int j = 0; j < FN; ++j) unit[j] = units.columns(j, lane);
-#pragma unroll
-        for (int i = 0; i < FMV; ++i) mine[i] = a.p_unit[row[i]];
-    }
 #pragma unroll
     for (int i = 0; i < FMV; ++i) {
         __builtin_amdgcn_sched_barrier(0);   // one block's results at a time
@@ -457,7 +473,7 @@ __device__ __forceinline__ void store_blocks(const Args &a, const SUM (&sums)[FM
 #pragma unroll
             for (int j = 0; j < FN; ++j)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) acc[0][j][c] = (float)sums[i][j][c] * (mine[i] * unit[j][c]);
+                for (int c = 0; c < 4; ++c) acc[0][j][c] = (float)sums[i][j][c] * (units.row[i] * units.column[j][c]);
         } else {
 #pragma unroll
             for (int j = 0; j < FN; ++j) acc[0][j] = sums[i][j];
@@ -496,28 +512,6 @@ __device__ __forceinline__ void store_results(const Args &a, const SUM (&acc)[FM
     if (a.wide && n0 + OUT_N <= a.n) store_blocks<T, MODE, ACT, true, FMV, FM, FN, WM>(a, acc, wm, wn, first, have, n0, units);
     else store_blocks<T, MODE, ACT, false, FMV, FM, FN, WM>(a, acc, wm, wn, first, have, n0, units);
 }
-
-// What 1 of a tile's rows and of its columns stands for, of 8-bit integers; for other operands nothing.
-template <int ACT, int FN>
-struct Units {
-    const Args *a;
-    const float *q;        // the expert's
-    long long first;       // slot of the tile's first row
-    int wn, n0;
-
-    // four columns of block j of this wave: those that lane's results are
-    __device__ __forceinline__ f32x4 columns(int j, int lane) const
-    {
-        const int n = ACT ? n0 + (wn * FN + j) / 2 * 16 + (lane >> 4) * 4 : n0 + (wn * FN + j) * 16 + (lane >> 4) * 4;
-        const float *from = q + (ACT && j % 2 ? a->n : 0);
-        f32x4 v;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = from[n + c < a->n ? n + c : a->n - 1];
-        return v;
-    }
-    __device__ __forceinline__ int row_of(int r) const { return row_of_slot(*a, (int)(first + r)); }
-};
-struct NoUnits { };
 
 // The tile of workgroup `id`: expert, tile of rows, tile of columns.  The experts' tiles are counted from the offsets,
 // 64 experts at a time over the lanes, in every wave by itself.  Workgroups reach the 8 XCDs in turn, so each XCD is
