@@ -273,8 +273,12 @@ __device__ __forceinline__ void find_orth_tile(const Product &a, int at, int &ma
     }
 }
 
+// Up to as many tiles as compute units a workgroup each, with eight waves and seven tiles of k on their way; else three a
+// compute unit, of four waves and two tiles on their way, which are one round where two with three would take a second one
+// (12 x 717 x 1111, X': 31 us for 33).  Even and odd tiles of k by half of the waves each, or a tenth tile on its way,
+// changed nothing for the former: beside 10 us of tiles a launch of 18 us starts, and ends with its stores.
 template <int KIND, int WN, int STAGES>
-__global__ __launch_bounds__(128 * WN) void k_orth_small(const Product a)
+__global__ __launch_bounds__(128 * WN, WN == 2 ? 3 : 2) void k_orth_small(const Product a)
 {
     __shared__ __align__(1024) char lds[STAGES * 256 * 64];
     const int id = a.first + blockIdx.x, chunk = (a.whole + kXcds - 1) / kXcds, at = id % kXcds * chunk + id / kXcds;
@@ -311,33 +315,55 @@ __global__ __launch_bounds__(512) void k_orth(const Product a)
 
 constexpr int kCus = 256;                // compute units of the card
 
-// Sums of squares of `per` rows each, in 64 bits: no element is too large or too small for its square.
-template <typename T, bool VECTOR>
-__global__ __launch_bounds__(256) void k_orth_norm(const T *g, long long ld, int rows, int columns, int per, double *sums)
+constexpr int kNormThreads = 256;
+// Sums of squares of every gridDim.x-th row, in 64 bits: no element is too large or too small for its square.  Rows are
+// read in the 16 bytes at multiples of 16 that hold any of them, `pieces` a row, and what is not of the row is left out;
+// WHOLE: they hold nothing else.  16 bytes that reach over the first matrix's begin or the last one's end are not read as
+// such.  (The rows' own eights, shifted out of words: 14 us for 12 x 717 x 1111 in bf16 where this takes 10.)
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(kNormThreads) void k_orth_norm(const T *g, long long ld, int rows, int columns, int pieces, double *sums)
 {
-    __shared__ double part[4];
-    const int begin = blockIdx.x * per, have = min(rows - begin, per);
-    const T *from = g + ((long long)blockIdx.y * rows + begin) * ld;
-    const int pieces = (columns + 7) / 8, units = have * pieces;
+    constexpr int N = 16 / sizeof(T), LOADS = 8;
+    typedef T Piece __attribute__((ext_vector_type(N)));
+    __shared__ double part[kNormThreads / kWave];
+    const int have = (rows - (int)blockIdx.x - 1) / (int)gridDim.x + 1, units = have * pieces;
+    const long long last_row = (long long)gridDim.y * rows - 1;
+    const auto row_at = [&](int i) { return g + ((long long)blockIdx.y * rows + blockIdx.x + (long long)gridDim.x * i) * ld; };
+    const uintptr_t first = (uintptr_t)g, last = (uintptr_t)(g + last_row * ld + columns);
+    const auto outside = [&](uintptr_t p) { return p < first || p + 16 > last; };
+    const auto square = [](T v, double sum) { return __builtin_fma((double)(float)v, (double)(float)v, sum); };
     double sum = 0;
-    for (int u0 = threadIdx.x; u0 < units; u0 += 256 * 4) {
-        float v[4][8];
+    for (int u0 = threadIdx.x; u0 < units; u0 += kNormThreads * LOADS) {
+        Piece v[LOADS];
+        int at[LOADS];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {   // their loads go out together
-            const int u = u0 + 256 * j, r = u / pieces;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[j][i] = 0;
-            if (u < units) load8_any<T, VECTOR>(from + ld * r, (u - r * pieces) * 8, columns, v[j]);
+        for (int j = 0; j < LOADS; ++j) {   // their loads go out together
+            const int u = u0 + kNormThreads * j, r = u / pieces;
+            const uintptr_t row = (uintptr_t)row_at(r), p = (row & ~(uintptr_t)15) + 16LL * (u - r * pieces);
+            at[j] = (int)(long long)(p - row) / (int)sizeof(T);
+            v[j] = Piece{};
+            if (u < units && (WHOLE || !outside(p))) v[j] = *(const Piece *)p;
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < LOADS; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = __builtin_fma((double)v[j][i], (double)v[j][i], sum);
+            for (int i = 0; i < N; ++i) sum = square(WHOLE || (unsigned)(at[j] + i) < (unsigned)columns ? v[j][i] : (T)0, sum);
+    }
+    for (int r = threadIdx.x; !WHOLE && r < have; r += kNormThreads) {   // the few elements of those
+        const T *row = row_at(r);
+        if ((uintptr_t)row - first >= 16 && last - (uintptr_t)(row + columns) >= 16) continue;
+        const auto add = [&](int c) {
+            if (outside((uintptr_t)(row + c) & ~(uintptr_t)15)) sum = square(row[c], sum);
+        };
+        for (int c = 0; c < min(N, columns); ++c) add(c);
+        for (int c = max(columns - N, N); c < columns; ++c) add(c);
     }
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
     if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) sums[(long long)blockIdx.y * gridDim.x + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < kNormThreads / kWave; ++w) sum += part[w];
+    sums[(long long)blockIdx.y * gridDim.x + blockIdx.x] = sum;
 }
 
 __device__ __forceinline__ void store_pieces(const float v[8], f16 *x, unsigned char *rest)
@@ -429,6 +455,12 @@ __global__ __launch_bounds__(256) void k_orth_out_across(const f16 *x, const uns
         for (int e = 0; e < 8; ++e) tile[piece + e][i] = ((float)first[e] + v[e]) * scale;
     }
     __syncthreads();
+    if (!wide) {   // a row a wave, an element a lane: unaligned rows by eight elements a lane took 26 us where this takes 14
+        const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+        for (int i = wave; i < min(64, rows - c0); i += 4)
+            if (r0 + lane < columns) out[ld * ((long long)blockIdx.z * rows + c0 + i) + r0 + lane] = (T)tile[i][lane];
+        return;
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int i = line + 32 * h;
@@ -436,7 +468,7 @@ __global__ __launch_bounds__(256) void k_orth_out_across(const f16 *x, const uns
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = tile[i][piece + e];
-        store_row<T, 8>(out + ld * ((long long)blockIdx.z * rows + c0 + i), r0 + piece, columns, wide, v);
+        store_row<T, 8>(out + ld * ((long long)blockIdx.z * rows + c0 + i), r0 + piece, columns, true, v);
     }
 }
 
@@ -464,7 +496,7 @@ int product(Product a, hipStream_t s)
     }
     a.whole = (int)tiles(128);
     if (a.whole <= kCus) return run(k_orth_small<KIND, 4, 8>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 512);
-    return run(k_orth_small<KIND, 2, 4>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 256);
+    return run(k_orth_small<KIND, 2, 3>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 256);
 }
 
 // launch(grid, first matrix) with a workgroup for each 64 x 64 elements of each matrix
@@ -490,9 +522,11 @@ int into_pieces(const void *from, long long ld, int batch, int rows, int columns
 {
     const T *g = (const T *)from;
     const bool vector = (uintptr_t)g % 16 == 0 && ld * sizeof(T) % 16 == 0;
-    const int per = (rows + kParts - 1) / kParts, parts = (rows + per - 1) / per, m = h.m, n = h.n;
-    const auto norm = vector ? k_orth_norm<T, true> : k_orth_norm<T, false>;
-    norm<<<dim3(parts, batch), dim3(256), 0, s>>>(g, ld, rows, columns, per, sums);
+    const int parts = std::min(rows, kParts), m = h.m, n = h.n;
+    const bool whole = vector && columns * sizeof(T) % 16 == 0;
+    const int pieces = (int)((columns * sizeof(T) + 15) / 16) + !vector;   // a row that starts inside one may reach into one more
+    const auto norm = whole ? k_orth_norm<T, true> : k_orth_norm<T, false>;
+    norm<<<dim3(parts, batch), dim3(kNormThreads), 0, s>>>(g, ld, rows, columns, pieces, sums);
     if (!h.x) return parts;
     if (rows > columns) {
         const auto kernel = vector ? k_orth_pieces_across<T, true> : k_orth_pieces_across<T, false>;

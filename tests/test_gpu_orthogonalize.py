@@ -158,3 +158,13 @@ def test_past_32_bits_of_workspace():
     torch.cuda.synchronize()
     near(out[-1:], reference(g), "bf16")
     assert all(torch.equal(out[i], out[-1]) for i in range(batch))
+
+
+@pytest.mark.parametrize("shift", [0, 1, 3, 8])
+@pytest.mark.parametrize("batch,rows,columns,ld", [(1, 1, 1, 0), (1, 3, 1, 0), (2, 5, 1, 0), (1, 9, 2, 3), (1, 1, 9, 0), (1, 1, 23, 0), (2, 2, 7, 8), (3, 17, 5, 0),
+                                                   (1, 100, 3, 4), (2, 70, 129, 0), (1, 129, 70, 71), (1, 700, 65, 0), (2, 65, 66, 72)])
+def test_length(batch, rows, columns, ld, shift):
+    """One step that changes nothing, of matrices at any address: G / |G|.  Its roundings: the factor and two pieces, under 2^-14."""
+    for dtype, out in (("bf16", "f16"), ("f32", "bf16")):
+        got, held = run(momentum(batch, rows, columns, 5), dtype, out, steps=[(1.0, 0.0, 0.0)], ld=ld, shift=shift, ld_out=ld, shift_out=shift)
+        near(got, reference(held, [(1.0, 0.0, 0.0)]), out, slack=2.0 ** -14)
