@@ -146,8 +146,8 @@ int pf_i8_quantize(const void *x, long long ld_x, int dtype, int rows, int k, vo
 /* Integer times scale, formed in f32 and rounded to dtype. */
 int pf_i8_dequantize(const void *codes, const float *scales, int rows, int k, int dtype, void *y, long long ld_y, void *stream);
 /* pf_moe_mm of such rows: x (x_codes, x_scales) [x_rows][k], w (w_codes, w_scales) [experts][n or 2n][k], a scale for each
- * token and each row of w; y in dtype (f16, bf16).  Sums are exact (k at most 131056); they are scaled, and the activation
- * formed, in f32.  Codes behind a row's k elements are zeros, as pf_i8_quantize writes them; -128 is allowed. */
+ * token and each row of w; y in dtype (f16, bf16).  Sums are exact (k at most 131056); they are scaled, by the token's scale and then by the row's, and
+ * the activation formed, in f32.  Codes behind a row's k elements are zeros, as pf_i8_quantize writes them; -128 is allowed. */
 int pf_moe_mm_i8(const void *x_codes, const float *x_scales, int x_rows, const int *rows, int row_div, const void *w_codes,
                  const float *w_scales, const int *offsets, int experts, int slots, int n, int k, int dtype, int act, void *y,
                  long long ld_y, void *stream);

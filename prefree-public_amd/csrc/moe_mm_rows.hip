@@ -155,7 +155,7 @@ __global__ __launch_bounds__(kWaves * kWave, FORM == kI8 || (ALIGNED && !ACT) ? 
     if constexpr (FORM == kI8) {
         const float mine = a.p_unit[row_of_slot(a, t.begin + s)];
 #pragma unroll
-        for (int j = 0; j < NB; ++j) v[j] *= mine * a.q_unit[(long long)NB * a.n * t.e + (long long)j * a.n + n];
+        for (int j = 0; j < NB; ++j) v[j] = v[j] * mine * a.q_unit[(long long)NB * a.n * t.e + (long long)j * a.n + n];
     }
     T *out = (T *)(a.out + a.ld_out * ((long long)t.begin + s)) + n;
     if constexpr (ACT) {

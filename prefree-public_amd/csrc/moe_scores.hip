@@ -420,7 +420,7 @@ struct Fast {
                 if (unlike) taken = moved;
             }
         }
-        sure = (__ballot(!sure) & all) == 0 && off == 0 && a.top_k < kTaken;
+        sure = (__ballot(!sure) & all) == 0 && off == 0;
         return taken != 0 ? expert_of(taken) : -1;
     }
 };
@@ -605,6 +605,7 @@ int route(Scores a, hipStream_t s)
         a.group_lanes = 1;
     }
     const int each = 16 / (int)sizeof(T);
+    if (a.top_k >= kTaken) a.need = 0;   // there would be none behind the last
     a.vector = a.need % each == 0 && a.group_size % each == 0 && (uintptr_t)a.logits % 16 == 0 && a.ld % each == 0;
     in_launches(a.blocks, most_workgroups(kThreads), [&](long long first, long long count) {
         const dim3 grid((unsigned)count), block(kThreads);

@@ -473,7 +473,7 @@ __device__ __forceinline__ void store_blocks(const Args &a, const SUM (&sums)[FM
 #pragma unroll
             for (int j = 0; j < FN; ++j)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) acc[0][j][c] = (float)sums[i][j][c] * (units.row[i] * units.column[j][c]);
+                for (int c = 0; c < 4; ++c) acc[0][j][c] = (float)sums[i][j][c] * units.row[i] * units.column[j][c];   // never 0 times infinity
         } else {
 #pragma unroll
             for (int j = 0; j < FN; ++j) acc[0][j] = sums[i][j];

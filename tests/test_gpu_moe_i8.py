@@ -212,3 +212,19 @@ def test_rows_outside_and_offsets_that_decrease_stay_inside():
     torch.cuda.synchronize()
     assert y[30:].isnan().all() and y[3].isfinite().all()
     assert torch.equal(y[3].double(), (xq[7].double() @ wq[0].double().t()).bfloat16().double())
+
+
+@pytest.mark.parametrize("slots", [3, 70, 300])
+@pytest.mark.parametrize("x_scale,w_scale", [(2.0 ** 70, 2.0 ** 70), (2.0 ** -90, 2.0 ** -40), (2.0 ** -40, 2.0 ** -90)])
+def test_scales_whose_product_is_no_number(slots, x_scale, w_scale):
+    """Sums of 0 stay 0, and small scales one after the other lose nothing."""
+    n, k = 256, 64
+    xq = torch.randint(-127, 128, (slots, k), generator=gen(slots), device=DEV).to(torch.int8)
+    wq = torch.randint(-127, 128, (n, k), generator=gen(n), device=DEV).to(torch.int8)
+    xq[1], wq[5] = 0, 0
+    xs, ws = torch.full((slots,), x_scale, device=DEV), torch.full((n,), w_scale, device=DEV)
+    y = torch.full((slots, n), NAN, dtype=torch.bfloat16, device=DEV)
+    pf.moe_mm_i8(xq, xs, slots, None, 1, wq, ws, None, 1, slots, n, k, y)
+    torch.cuda.synchronize()
+    ref = (xq.double() @ wq.double().t()) * x_scale * w_scale
+    assert torch.equal(y, ref.float().bfloat16())        # sums under 2^24 and powers of two: one rounding
