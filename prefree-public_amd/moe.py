@@ -1,4 +1,5 @@
-"""Expert-layer operators of the MI355X library: routing, products grouped by expert, 4-bit blocks.
+"""Expert-layer operators of the MI355X library: routing, products grouped by expert, 4-bit blocks, 8-bit integers, and
+orthogonal updates of their weights.
 
 The same calls as include/prefree_moe.h, which says what each computes, on device buffers as in the rest of this
 package: anything with ``data_ptr()``, outputs given by the caller, sizes as numbers, ``stream=None`` the null stream,
