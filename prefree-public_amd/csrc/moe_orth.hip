@@ -62,26 +62,28 @@ __device__ __forceinline__ void rest_of(unsigned held, float v[4])
     v[3] = hi[1] * (1.0f / kRest);
 }
 
-// The tile from row m0 and column n0 of a matrix's product, with STAGES tiles of k in LDS.
-template <int KIND, int BM, int BN, int WM, int WN, int STAGES>
+// The tile from row m0 and column n0 of a matrix's product, by KS times WM x WN waves with STAGES times KS tiles of k in LDS.
+// Each set of waves takes every KS-th tile of k; in the end they add up, and each finishes its share of the rows.
+template <int KIND, int BM, int BN, int WM, int WN, int STAGES, int KS>
 __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, int n0, char *shared)
 {
-    constexpr int THREADS = WM * WN * 64, FM = BM / WM / 16, FN = BN / WN / 16;
+    constexpr int THREADS = WM * WN * KS * 64, FM = BM / WM / 16, FN = BN / WN / 16, DONE = FM / KS;
     typedef Along<BM, THREADS, true> P;
     typedef typename std::conditional<KIND == kApply, Across<BN, THREADS, true>, Along<BN, THREADS, true>>::type Q;
-    constexpr int SLOT = P::kBytes + Q::kBytes, LOADS = P::kLoads + Q::kLoads;
-    const int wave = wave_id(), wm = wave / WN, wn = wave % WN, k = a.k;
+    constexpr int TILE = P::kBytes + Q::kBytes, SLOT = KS * TILE, EACH = P::kLoads + Q::kLoads, LOADS = KS * EACH;
+    const int id = wave_id(), set = KS > 1 ? id / (WM * WN) : 0, wave = KS > 1 ? id % (WM * WN) : id, wm = wave / WN, wn = wave % WN, k = a.k;
+    const auto row_of = [&](int i) { return m0 + ((i + set * DONE) * WM + wm) * 16; };   // of the blocks that this wave finishes
     int lane = threadIdx.x & (kWave - 1);
     const long long base = (long long)matrix * a.m * a.n;
 
     // the second pieces of what this lane will store; they are long there when the products are
     typedef unsigned Rest __attribute__((ext_vector_type(FN)));
-    Rest rest[KIND == kApply ? FM : 1];
+    Rest rest[KIND == kApply ? DONE : 1];
     if constexpr (KIND == kApply) {   // none of the last step's: what they would add is not multiplied any more
         const int c = n0 + wn * FN * 16 + (lane >> 4) * 4 * FN;   // 4 FN columns from here, there as a whole or not at all
 #pragma unroll
-        for (int i = 0; i < FM; ++i) {
-            const int r = m0 + (i * WM + wm) * 16 + (lane & 15);
+        for (int i = 0; i < DONE; ++i) {
+            const int r = row_of(i) + (lane & 15);
             rest[i] = Rest{};
             if (a.old_rest && r < a.m && c < a.n) rest[i] = *(const Rest *)(a.old_rest + base + (long long)r * a.n + c);
         }
@@ -100,13 +102,15 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
         q.init(from, 2ull * a.m * k, 2LL * k, [&](int r) { return min(n0 + r, a.m - 1); }, k, 8);
     }
     const auto lds = [&](int place) { return shared + place * SLOT; };
-    const auto issue = [&](int i, int s, char *to) {
-        if (i < P::kLoads) p.issue(i, s, to);
-        else if constexpr (KIND == kApply) q.template issue<false>(i - P::kLoads, s, to + P::kBytes, 0);
-        else q.issue(i - P::kLoads, s, to + P::kBytes);
+    const auto issue = [&](int l, int s, char *to) {
+        const int i = l % EACH, t = s * KS + l / EACH;
+        to += l / EACH * TILE;
+        if (i < P::kLoads) p.issue(i, t, to);
+        else if constexpr (KIND == kApply) q.template issue<false>(i - P::kLoads, t, to + P::kBytes, 0);
+        else q.issue(i - P::kLoads, t, to + P::kBytes);
     };
-    const auto read_x = [&](const char *from, int i) { return P::fragment(from, (i * WM + wm) * 16); };
-    const auto read_w = [&](const char *from, int j) { return Q::fragment(from + P::kBytes, (wn * FN + j) * 16); };
+    const auto read_x = [&](const char *from, int i) { return P::fragment(from + set * TILE, (i * WM + wm) * 16); };
+    const auto read_w = [&](const char *from, int j) { return Q::fragment(from + set * TILE + P::kBytes, (wn * FN + j) * 16); };
 
     f32x4 acc[FM][FN];
 #pragma unroll
@@ -142,7 +146,7 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
         wait_and_meet<(STAGES - 3) * LOADS, kNextReads>();
         __builtin_amdgcn_sched_barrier(0);
     };
-    const int steps = k / 32;   // by twos: behind k tiles are zeros
+    const int steps = (k / 32 + KS - 1) / KS;   // by twos: behind k tiles are zeros
 #pragma unroll
     for (int s = 0; s < kAhead; ++s)
 #pragma unroll
@@ -158,6 +162,24 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
         step(std::integral_constant<int, 1>(), s + 1, lds((s + 1 + kAhead) % STAGES), lds((s + 1) % STAGES), lds((s + 2) % STAGES));
     }
     wait_and_meet<0>();   // nothing may still be on its way to LDS when the workgroup ends
+    if constexpr (KS > 1) {
+        static_assert(FM * FN * 16 * THREADS <= STAGES * SLOT, "sums of all sets");
+        f32x4 *box = (f32x4 *)shared + threadIdx.x % (THREADS / KS);
+        const auto at = [&](int set, int i, int j) { return ((set * FM + i) * FN + j) * (THREADS / KS); };
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) box[at(set, i, j)] = acc[i][j];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < DONE; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                acc[i][j] = box[at(0, set * DONE + i, j)];
+#pragma unroll
+                for (int other = 1; other < KS; ++other) acc[i][j] += box[at(other, set * DONE + i, j)];
+            }
+    }
 
     // Rows and columns are multiples of 32: blocks of 16 x 16 are there as a whole or not at all.
     asm volatile("" : "+v"(lane));   // addresses are formed here, not kept over the loop before
@@ -166,7 +188,7 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
     f16x4 old[2][FN];   // kPoly: P's, a block of rows ahead
     const auto read_old = [&](int i) {
         if constexpr (KIND == kPoly) {
-            const int r = m0 + (i * WM + wm) * 16 + (lane & 15);
+            const int r = row_of(i) + (lane & 15);
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
                 const int c = c0 + j * 16 + g * 4;
@@ -177,10 +199,10 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
     };
     read_old(0);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        if (i + 1 < FM) read_old(i + 1);
+    for (int i = 0; i < DONE; ++i) {
+        if (i + 1 < DONE) read_old(i + 1);
         __builtin_amdgcn_sched_barrier(0);
-        const int r0 = m0 + (i * WM + wm) * 16, r = r0 + (lane & 15);
+        const int r0 = row_of(i), r = r0 + (lane & 15);
         if (r0 >= a.m) continue;
         if constexpr (KIND == kApply) {
             unsigned v[FN][4];
@@ -253,30 +275,30 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
     }
 }
 
-// Tile `at` of all matrices' tiles of side B.
-template <int KIND, int B>
+// Tile `at` of all matrices' tiles of BM x BN.
+template <int KIND, int BM, int BN>
 __device__ __forceinline__ void find_orth_tile(const Product &a, int at, int &matrix, int &m0, int &n0)
 {
-    const int mt = (a.m + B - 1) / B, nt = (a.n + B - 1) / B, each = KIND == kApply ? mt * nt : mt * (mt + 1) / 2;
+    const int mt = (a.m + BM - 1) / BM, nt = (a.n + BN - 1) / BN, each = KIND == kApply ? mt * nt : mt * (mt + 1) / 2;
     matrix = at / each;
     const int t = at - matrix * each;
     if constexpr (KIND == kApply) {   // eight tiles of rows side by side over the columns
         const int group = t / (8 * nt), side = min(8, mt - group * 8), j = t - group * 8 * nt;
-        m0 = (group * 8 + j % side) * B;
-        n0 = j / side * B;
+        m0 = (group * 8 + j % side) * BM;
+        n0 = j / side * BN;
     } else {
         int tm = (int)((__builtin_sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
         while ((tm + 1) * (tm + 2) / 2 <= t) ++tm;
         while (tm * (tm + 1) / 2 > t) --tm;
-        m0 = tm * B;
-        n0 = (t - tm * (tm + 1) / 2) * B;
+        m0 = tm * BM;
+        n0 = (t - tm * (tm + 1) / 2) * BM;
     }
 }
 
-// Up to as many tiles as compute units a workgroup each, with eight waves and seven tiles of k on their way; else three a
-// compute unit, of four waves and two tiles on their way, which are one round where two with three would take a second one
-// (12 x 717 x 1111, X': 31 us for 33).  Even and odd tiles of k by half of the waves each, or a tenth tile on its way,
-// changed nothing for the former: beside 10 us of tiles a launch of 18 us starts, and ends with its stores.
+// Tiles of 128 x 128.  Up to as many as compute units a workgroup each, with eight waves and seven tiles of k on their way;
+// else three a compute unit, of four waves and two tiles on their way, which are one round where two with three would take a
+// second one (12 x 717 x 1111, X': 31 us for 33).  Even and odd tiles of k by half of the waves each, or two more on their
+// way, changed nothing for the former: beside 10 us of tiles a launch of 18 us starts, and ends with its stores.
 template <int KIND, int WN, int STAGES>
 __global__ __launch_bounds__(128 * WN, WN == 2 ? 3 : 2) void k_orth_small(const Product a)
 {
@@ -284,8 +306,21 @@ __global__ __launch_bounds__(128 * WN, WN == 2 ? 3 : 2) void k_orth_small(const 
     const int id = a.first + blockIdx.x, chunk = (a.whole + kXcds - 1) / kXcds, at = id % kXcds * chunk + id / kXcds;
     if (id / kXcds >= chunk || at >= a.whole) return;
     int matrix, m0, n0;
-    find_orth_tile<KIND, 128>(a, at, matrix, m0, n0);
-    orth_tile<KIND, 128, 128, 2, WN, STAGES>(a, matrix, m0, n0, lds);
+    find_orth_tile<KIND, 128, 128>(a, at, matrix, m0, n0);
+    orth_tile<KIND, 128, 128, 2, WN, STAGES, 1>(a, matrix, m0, n0, lds);
+}
+
+// Tiles of 64 rows, where there are few: a step over a tile of k takes a workgroup some 0.25 us however small it is, so that
+// it is worth to have more of them, and several tiles of k in a step.
+template <int KIND, int BN, int WN, int STAGES, int KS>
+__global__ __launch_bounds__(256) void k_orth_tiny(const Product a)
+{
+    __shared__ __align__(1024) char lds[STAGES * KS * (64 + BN) * 64];
+    const int id = a.first + blockIdx.x, chunk = (a.whole + kXcds - 1) / kXcds, at = id % kXcds * chunk + id / kXcds;
+    if (id / kXcds >= chunk || at >= a.whole) return;
+    int matrix, m0, n0;
+    find_orth_tile<KIND, 64, BN>(a, at, matrix, m0, n0);
+    orth_tile<KIND, 64, BN, 1, WN, STAGES, KS>(a, matrix, m0, n0, lds);
 }
 
 template <int KIND>
@@ -298,17 +333,17 @@ __global__ __launch_bounds__(512) void k_orth(const Product a)
     if (id < big) {
         const int at = id % kXcds * (big / kXcds) + id / kXcds;
         if (at >= a.whole) return;
-        find_orth_tile<KIND, 256>(a, at, matrix, m0, n0);
-        orth_tile<KIND, 256, 256, 2, 4, 4>(a, matrix, m0, n0, lds);
+        find_orth_tile<KIND, 256, 256>(a, at, matrix, m0, n0);
+        orth_tile<KIND, 256, 256, 2, 4, 4, 1>(a, matrix, m0, n0, lds);
         return;
     }
     if (id - big >= a.parts) return;
-    find_orth_tile<KIND, 256>(a, a.whole + (id - big) / 4, matrix, m0, n0);
+    find_orth_tile<KIND, 256, 256>(a, a.whole + (id - big) / 4, matrix, m0, n0);
     const bool diagonal = KIND != kApply && m0 == n0;
     m0 += (id - big) / 2 % 2 * 128;
     n0 += (id - big) % 2 * 128;
     if (m0 >= a.m || n0 >= a.n || (diagonal && n0 > m0)) return;
-    orth_tile<KIND, 128, 128, 2, 4, 8>(a, matrix, m0, n0, lds);
+    orth_tile<KIND, 128, 128, 2, 4, 8, 1>(a, matrix, m0, n0, lds);
 }
 
 // ---- into the two pieces, and out of them --------------------------------------------------------------------------
@@ -475,8 +510,8 @@ __global__ __launch_bounds__(256) void k_orth_out_across(const f16 *x, const uns
 template <int KIND>
 int product(Product a, hipStream_t s)
 {
-    const auto tiles = [&](long long side) {
-        const long long mt = (a.m + side - 1) / side, nt = (a.n + side - 1) / side;
+    const auto tiles = [&](long long side, long long across = 0) {
+        const long long mt = (a.m + side - 1) / side, nt = (a.n + (across ? across : side) - 1) / (across ? across : side);
         return a.batch * (KIND == kApply ? mt * nt : mt * (mt + 1) / 2);
     };
     const auto run = [&](auto kernel, long long workgroups, int threads) {
@@ -493,6 +528,18 @@ int product(Product a, hipStream_t s)
         a.whole = (int)(large - over);
         a.parts = (int)(4 * over);
         return run(k_orth<KIND>, (a.whole + kXcds - 1LL) / kXcds * kXcds + a.parts, 512);
+    }
+    // A, B and X' in us, tiles of 64 rows against 128: 1 x 500 x 1000 8.9, 7.0, 8.9 / 12.4, 10.5, 10.3; 1 x 512 x 4096 19.7, 7.1, 9.5
+    // / 30.8, 10.2, 10.6 (A by twos of tiles of k 24.5); 1 x 1024 x 1024 9.9, 10.1, 12.6 / 12.9, 14.7, 13.4; 12 x 300 x 300 6.1, 7.0,
+    // 7.9 / -, -, 9.1; with more of them than fit at once: 3 x 800 x 800 10.6, 11.5, 13.8 / 12.6, 13.6, 12.7; 2 x 1100 x 1100 12.4,
+    // 13.4, 18.9 / 15.6, 16.7, 16.8; 16 x 500 x 500 12.5, 13.8, 14.2 / 10.7, 11.8, 13.2; 1 x 2048 x 2048 32, 33, 32 / 22, 24, 26.
+    if constexpr (KIND == kApply) {
+        a.whole = (int)tiles(64, 128);
+        if (a.whole <= kCus) return run(k_orth_tiny<KIND, 128, 4, 6, 1>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 256);
+    } else {
+        a.whole = (int)tiles(64);
+        if (a.whole <= kCus && a.k >= 1024) return run(k_orth_tiny<KIND, 64, 1, 4, 4>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 256);
+        if (a.whole <= 2 * kCus) return run(k_orth_tiny<KIND, 64, 2, 4, 2>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 256);
     }
     a.whole = (int)tiles(128);
     if (a.whole <= kCus) return run(k_orth_small<KIND, 4, 8>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 512);

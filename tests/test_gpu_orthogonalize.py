@@ -168,3 +168,12 @@ def test_length(batch, rows, columns, ld, shift):
     for dtype, out in (("bf16", "f16"), ("f32", "bf16")):
         got, held = run(momentum(batch, rows, columns, 5), dtype, out, steps=[(1.0, 0.0, 0.0)], ld=ld, shift=shift, ld_out=ld, shift_out=shift)
         near(got, reference(held, [(1.0, 0.0, 0.0)]), out, slack=2.0 ** -14)
+
+
+# tiles of 64 rows with four, two and one tile of k in a step, of 128 with eight and with four waves, of 256
+@pytest.mark.parametrize("batch,rows,columns", [(1, 66, 1500), (1, 70, 96), (2, 1100, 1100), (3, 800, 833), (16, 500, 520), (9, 860, 1000), (1, 65, 65), (4, 2048, 2050)])
+def test_tiles(batch, rows, columns):
+    for flip in (False, True):
+        g = momentum(batch, rows, columns, 7)
+        got, held = run(g.transpose(1, 2).contiguous() if flip else g, "bf16")
+        near(got, reference(held), "bf16")
