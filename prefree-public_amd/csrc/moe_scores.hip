@@ -526,8 +526,9 @@ __global__ __launch_bounds__(256) void k_scores_backward(const Backward a)
         if ((unsigned)e >= (unsigned)a.experts) e = -1;
         if (e >= 0) { w = a.weight[at]; g = a.dweight[at]; }
     }
-    const float inner = sum_of<16>(w * g);
-    float grad = a.normalise ? w * (g - inner / a.scale) : w * g;
+    // the mean of what the weights get, by shares of 1: where one expert has all of it, it gets exactly 0
+    const float inner = sum_of<16>((a.normalise ? w / a.scale : w) * g);
+    float grad = w * (a.normalise ? g - inner : g);
     if (a.score == PF_SCORE_SIGMOID && e >= 0) {
         const float mine = (float)z[e];   // 1 - s
         grad *= mine > 0 ? expf(-mine) / (1.0f + expf(-mine)) : 1.0f / (1.0f + expf(mine));

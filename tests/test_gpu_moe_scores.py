@@ -335,3 +335,18 @@ def test_groups_with_one_expert_left(level):
     z[torch.rand(2000, 32, generator=g, device=DEV) < 0.8] = -float("inf")
     check(z, 4, bias=biases(32) + level, groups=8, groups_kept=3)
     check(z, 4, bias=biases(32) + level, groups=4, groups_kept=2, score="softmax")
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("scale", [1.0, 2.5, 0.3, 7.7e-5])
+def test_gradient_of_one_expert_is_none(score, scale):
+    """Its weight is the scale, whatever its logit."""
+    tokens, experts = 300, 24
+    z = logits(tokens, experts, 5)
+    (choice, weight, *_), held = route(z, 1, score=score, scale=scale)
+    assert (weight == np.float32(scale)).all()
+    dz = torch.full((tokens, experts), NAN, device=DEV)
+    dweight = torch.randn(tokens, 1, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV)
+    pf.moe_route_scores_backward(held, tokens, experts, 1, torch.from_numpy(choice).to(DEV), torch.from_numpy(weight).to(DEV), dweight, dz, score=score, scale=scale)
+    torch.cuda.synchronize()
+    assert (dz == 0).all()
