@@ -1,10 +1,13 @@
 // moe_orth_narrow.hip — orthogonal updates of matrices with at most 64 rows (or columns) on gfx950: one launch a step.
 //
 // X is held by columns, 64 numbers each, in two f16 pieces; a workgroup takes a share of them.  In a step every workgroup
-// adds the shares' parts of A = X X^T, forms B = a I + b A + c A A (64^3 products, by each of them: less than a launch), X' = B X of its columns, the
-// second piece by way of a I, and its part of the next A.  The matrix cores hand out four rows of a column a lane, and
-// eight of two blocks, in whatever order, are a fragment of the product over columns: X' goes on to A as it comes.
-// 64 x 2048 from fp32 in five steps: 7 launches, 60 us; by tiles of 128 x 128, 17 launches, 152 us.
+// adds the shares' parts of A = X X^T, forms B = a I + b A + c A A (64^3 products, by each of them: less than a launch),
+// X' = B X of its columns and its part of the next A.  The matrix cores hand out four rows of a column a lane, and eight of
+// two blocks, in whatever order, are a fragment of the product over columns: X' goes on to A as it comes.  A launch is
+// loads, meetings and a few hundred products one after the other, not their number: so A and B are in two pieces as well,
+// and of each product all but rest times rest is formed, for results as exact as their type.
+// 64 x 2048 from fp32 in five steps: 7 launches, 63 us (60 with one piece of A, B and the products' X, then 2 10^-3 off; now
+// 2 10^-4 in f16, which is its rounding); by tiles of 128 x 128, 17 launches, 152 us.
 #include "moe_orth.hpp"
 
 namespace {
@@ -35,6 +38,16 @@ struct Step {
 __device__ __forceinline__ f32x4 product(const i32x4 &a, const i32x4 &b, const f32x4 &c)
 {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// four numbers in two pieces
+__device__ __forceinline__ void store_two(f16 *first, f16 *rest, const f32x4 &v)
+{
+    float left[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) left[e] = v[e] - (float)(f16)v[e];
+    *(u32x2 *)first = u32x2{pair_of(v[0], v[1]), pair_of(v[2], v[3])};
+    *(u32x2 *)rest = u32x2{pair_of(left[0], left[1]), pair_of(left[2], left[3])};
 }
 
 // What is not X's is read too, from its last row or column, so that no load has to wait for a branch.
@@ -82,7 +95,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
     constexpr int LD = kSide + 8;
     __shared__ __align__(16) union {
         struct {
-            f16 square[kSide][LD], poly[kSide][LD];   // A and B
+            f16 square[2][kSide][LD], poly[2][kSide][LD];   // A and B, two pieces each
         } s;
         float parts[kWaves][kSide][kSide + 4];   // rows in other banks
     } lds;
@@ -103,7 +116,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
                 l[half][ks] = *(const i32x4 *)(rest + at);
             }
     };
-    i32x4 poly[4][2], unit[2];   // B's columns and a I's, as fragments
+    i32x4 poly[2][4][2];   // B's columns, as fragments
     double by = 0;
     if constexpr (FIRST) {
         by = over_norm(a.sums + (long long)matrix * a.parts, a.parts, a.scale);
@@ -127,7 +140,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
         for (int e = 0; e < 2; ++e) {
             const int at = threadIdx.x * 4 + 2048 * e, r = at / kSide, c = at % kSide;
             sum[e] *= a.over;
-            *(u32x2 *)&lds.s.square[r][c] = u32x2{pair_of(sum[e][0], sum[e][1]), pair_of(sum[e][2], sum[e][3])};
+            store_two(&lds.s.square[0][r][c], &lds.s.square[1][r][c], sum[e]);
         }
         __syncthreads();
         // A is symmetric: its rows are its columns, and what a lane has of a column it stores as a piece of a row
@@ -135,27 +148,28 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
         for (int j = 0; j < 2; ++j) {
             const int rb = wave / 2, cb = wave % 2 * 2 + j;
             f32x4 d = f32x4{0, 0, 0, 0};
+            const auto at = [&](int piece, int block, int ks) { return *(const i32x4 *)&lds.s.square[piece][block * 16 + i16][ks * 32 + g * 8]; };
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-                d = product(*(const i32x4 *)&lds.s.square[rb * 16 + i16][ks * 32 + g * 8], *(const i32x4 *)&lds.s.square[cb * 16 + i16][ks * 32 + g * 8], d);
+            for (int ks = 0; ks < 2; ++ks) {
+                d = product(at(1, rb, ks), at(0, cb, ks), d);
+                d = product(at(0, rb, ks), at(1, cb, ks), d);
+                d = product(at(0, rb, ks), at(0, cb, ks), d);
+            }
             const int c = cb * 16 + i16, r = rb * 16 + g * 4;
-            // b A of the same rounding as A A: near singular values of 1 the two take most of it out of each other
 #pragma unroll
-            for (int e = 0; e < 4; ++e) d[e] = __builtin_fmaf(a.b, (float)lds.s.square[c][r + e], a.c * d[e]) + (r + e == c ? a.a : 0.0f);
-            *(u32x2 *)&lds.s.poly[c][r] = u32x2{pair_of(d[0], d[1]), pair_of(d[2], d[3])};
+            for (int e = 0; e < 4; ++e) {
+                const float same = (float)lds.s.square[0][c][r + e] + (float)lds.s.square[1][c][r + e];
+                d[e] = __builtin_fmaf(a.b, same, a.c * d[e]) + (r + e == c ? a.a : 0.0f);
+            }
+            store_two(&lds.s.poly[0][c][r], &lds.s.poly[1][c][r], d);
         }
         __syncthreads();
 #pragma unroll
-        for (int ib = 0; ib < 4; ++ib)
+        for (int piece = 0; piece < 2; ++piece)
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) poly[ib][ks] = *(const i32x4 *)&lds.s.poly[ib * 16 + i16][ks * 32 + g * 8];
+            for (int ib = 0; ib < 4; ++ib)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            f16x8 v;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (f16)(g * 8 + e == half * 16 + i16 ? a.a / kRest : 0.0f);
-            unit[half] = __builtin_bit_cast(i32x4, v);
-        }
+                for (int ks = 0; ks < 2; ++ks) poly[piece][ib][ks] = *(const i32x4 *)&lds.s.poly[piece][ib * 16 + i16][ks * 32 + g * 8];
     }
 
     f32x4 gram[4][4];
@@ -193,15 +207,24 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
                     }
         } else {
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+            for (int half = 0; half < 2; ++half) {
+                f32x4 d[4];
 #pragma unroll
-                for (int ib = 0; ib < 4; ++ib) {
-                    f32x4 d = product(l[half][ib / 2], unit[ib % 2], f32x4{0, 0, 0, 0});
-                    d = product(h[half][0], poly[ib][0], d);
-                    d = product(h[half][1], poly[ib][1], d);
+                for (int ib = 0; ib < 4; ++ib) d[ib] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) y[ib][half][e] = d[e];
+                for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+                    for (int ib = 0; ib < 4; ++ib) d[ib] = product(l[half][ks], poly[0][ib][ks], d[ib]);
+#pragma unroll
+                    for (int ib = 0; ib < 4; ++ib) d[ib] = product(h[half][ks], poly[1][ib][ks], d[ib]);
+#pragma unroll
+                    for (int ib = 0; ib < 4; ++ib) d[ib] = product(h[half][ks], poly[0][ib][ks], d[ib]);
                 }
+#pragma unroll
+                for (int ib = 0; ib < 4; ++ib)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[ib][half][e] = d[ib][e];
+            }
             if (block + kWaves < a.blocks) fetch(block + kWaves);
         }
         if constexpr (LAST) {
@@ -216,7 +239,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
                     else store_result<bf16>(a, matrix, ib * 16 + i16, n0 + half * 16 + g * 4, v, lane);
                 }
         } else {
-            i32x4 frag[4];
+            i32x4 frag[2][4];
 #pragma unroll
             for (int ib = 0; ib < 4; ++ib)
 #pragma unroll
@@ -224,12 +247,13 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
                     unsigned hi[2], lo[2];
                     float left[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) left[e] = (y[ib][half][e] - (float)(f16)y[ib][half][e]) * kRest;
+                    for (int e = 0; e < 4; ++e) left[e] = y[ib][half][e] - (float)(f16)y[ib][half][e];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         hi[e] = pair_of(y[ib][half][2 * e], y[ib][half][2 * e + 1]);
                         lo[e] = pair_of(left[2 * e], left[2 * e + 1]);
-                        frag[ib][2 * half + e] = (int)hi[e];
+                        frag[0][ib][2 * half + e] = (int)hi[e];
+                        frag[1][ib][2 * half + e] = (int)lo[e];
                     }
                     transpose4(hi, lane);
                     transpose4(lo, lane);
@@ -238,9 +262,11 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
                     *(u32x2 *)(rest + at) = u32x2{lo[0], lo[1]};
                 }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int term = 0; term < 3; ++term)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) gram[i][j] = product(frag[i], frag[j], gram[i][j]);
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) gram[i][j] = product(frag[term == 0][i], frag[term == 1][j], gram[i][j]);
         }
     }
     if constexpr (!LAST) {

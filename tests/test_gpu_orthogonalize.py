@@ -177,3 +177,11 @@ def test_tiles(batch, rows, columns):
         g = momentum(batch, rows, columns, 7)
         got, held = run(g.transpose(1, 2).contiguous() if flip else g, "bf16")
         near(got, reference(held), "bf16")
+
+
+@pytest.mark.parametrize("batch,rows,columns", [(5, 64, 661), (1, 64, 2048), (7, 33, 33), (2, 300, 50), (1, 2, 9)])
+def test_up_to_64_rows_as_exact_as_the_type(batch, rows, columns):
+    """Two pieces hold 2^-22 of a number; 9.4 such roundings a step (see above) and as many of sums in fp32 are under 2^-17, and
+    of five steps, where small singular values may keep all that earlier ones left, under 2^-14."""
+    got, held = run(momentum(batch, rows, columns, 8), out_dtype="f16")
+    near(got, reference(held), "f16", slack=2.0 ** -13)
