@@ -37,7 +37,8 @@ __device__ __forceinline__ u32x2 eight_of(const float v[8], double per)
 constexpr float kLeast = 0x1p-100f;   // of a row's largest magnitude: a scale of its own for smaller ones is not worth a normal number
 
 // G lanes take a row, whole workgroups or waves; each holds PIECES pieces of eight elements, G apart, over both passes: the
-// largest magnitude, then the integers.  Rows that are longer are read again for what does not fit.
+// largest magnitude, then the integers.  Rows that are longer are read again for what does not fit.  32768 x 2048 bf16: 52 to
+// 56 us, as is the way back to fp32: 3.6 and 5.9 TB/s, the copy's bytes between them at 4.8.
 template <typename T, int G, int PIECES, bool VECTOR>
 __global__ __launch_bounds__(256) void k_i8_quantize(const T *x, long long ld, int rows, int k, unsigned char *codes, long long ld_codes,
                                                      float *scales)
