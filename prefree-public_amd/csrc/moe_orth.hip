@@ -324,8 +324,8 @@ __global__ __launch_bounds__(256) void k_orth_tiny(const Product a)
 }
 
 // Tiles of 256 x 256, a workgroup a compute unit, and in quarters those of a last round that is at most half full.  16 x 2048 x
-// 2048: A, B and X' 167, 168 and 271 us, X' at 1.01 PFLOP/s.  The products alone are 197 us of X' (1.39 PFLOP/s, the matrix cores
-// busy 74%); the end of a tile, with nothing beside it, stores 200 MB in the rest.  256 x 128 tiles, two a compute unit: 350.
+// 2048: A, B and X' 167, 168 and 271 us, X' at 1.01 PFLOP/s, the matrix cores busy half of the time.  The products alone are
+// 197 us of X'; the end of a tile, with nothing beside it, stores 200 MB in the rest.  256 x 128 tiles, two a compute unit: 350.
 template <int KIND>
 __global__ __launch_bounds__(512) void k_orth(const Product a)
 {
