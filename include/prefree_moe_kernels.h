@@ -90,7 +90,7 @@ int pfk_moe_mm_i8(const pfk_moe_mm_args *a, void *stream);
 /* Up to PFK_ORTH_NARROW rows (or columns) it holds instead, behind those sums: two pieces of X by columns of PFK_ORTH_NARROW,
  * 2 bytes an element, in shares of whole blocks of 32 columns, and twice a square of 4-byte numbers a share. */
 #define PFK_ORTH_NARROW 64
-#define PFK_ORTH_MOST_SHARES(batch) ((batch) >= 16 ? 16 : 64)
+#define PFK_ORTH_MOST_SHARES(batch) ((batch) >= 256 ? 1 : (batch) <= 4 ? 64 : 256 / (batch))
 #define PFK_ORTH_SHARES(batch, n) (((n) + 255) / 256 < PFK_ORTH_MOST_SHARES(batch) ? ((n) + 255) / 256 : PFK_ORTH_MOST_SHARES(batch))
 #define PFK_ORTH_BLOCKS(batch, n) (((n) + 32 * PFK_ORTH_SHARES(batch, n) - 1) / (32 * PFK_ORTH_SHARES(batch, n)))
 int pfk_orthogonalize(const void *g, long long ld_g, int dtype, int batch, int rows, int columns, const float *steps,
