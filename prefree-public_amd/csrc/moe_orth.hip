@@ -383,9 +383,15 @@ __global__ __launch_bounds__(kNormThreads) void k_orth_norm(const T *g, long lon
             if (u < units && (WHOLE || !outside(p))) v[j] = *(const Piece *)p;
         }
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j)
+        for (int j = 0; j < LOADS; ++j) {
+            if (WHOLE || __all((unsigned)at[j] < (unsigned)max(columns - N + 1, 0))) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum = square(WHOLE || (unsigned)(at[j] + i) < (unsigned)columns ? v[j][i] : (T)0, sum);
+                for (int i = 0; i < N; ++i) sum = square(v[j][i], sum);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum = square((unsigned)(at[j] + i) < (unsigned)columns ? v[j][i] : (T)0, sum);
+            }
+        }
     }
     for (int r = threadIdx.x; !WHOLE && r < have; r += kNormThreads) {   // the few elements of those
         const T *row = row_at(r);
@@ -525,8 +531,15 @@ int product(Product a, hipStream_t s)
         });
         return pfk_internal_launched("k_orth");
     };
-    const long long large = tiles(256);
-    if (large >= kCus) {
+    // X' of 129 to 192 rows, which larger tiles would leave empty by a quarter: 96 x 139 x 2765 72 / 87 (128 x 128) and 80 (256 x 256)
+    if (KIND == kApply && 2 * tiles(64, 128) <= 3 * tiles(128) && tiles(64, 128) > kCus) {
+        a.whole = (int)tiles(64, 128);
+        if constexpr (KIND == kApply) return run(k_orth_tiny<KIND, 128, 4, 4, 1>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 256);
+    }
+    // Tiles of 256 x 256 unless they cover over 1.4 times as much as those of 128 x 128: 128 x 289 x 1567, A and B 82, 33 / 64, 22, X'
+    // alike; 96 x 101 x 3705 X' 81 / 69; 128 x 221 x 3693 X' 199 / 216.
+    const long long large = tiles(256), small = tiles(128);
+    if (large >= kCus && 20 * large <= 7 * small) {
         const long long over = large % kCus <= kCus / 2 ? large % kCus : 0;
         a.whole = (int)(large - over);
         a.parts = (int)(4 * over);
@@ -544,8 +557,9 @@ int product(Product a, hipStream_t s)
         if (a.whole <= kCus && a.k >= 1024) return run(k_orth_tiny<KIND, 64, 1, 4, 4>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 256);
         if (a.whole <= 2 * kCus) return run(k_orth_tiny<KIND, 64, 2, 4, 2>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 256);
     }
-    a.whole = (int)tiles(128);
-    if (a.whole <= kCus) return run(k_orth_small<KIND, 4, 8>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 512);
+    // with a long k also of more tiles one at a time: A of 96 x 139 x 2765 41 / 59, 128 x 221 x 3693 80 / 100, 128 x 1567 64 / 66
+    a.whole = (int)small;
+    if (a.whole <= kCus || (KIND != kApply && a.k >= 1536)) return run(k_orth_small<KIND, 4, 8>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 512);
     return run(k_orth_small<KIND, 2, 3>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 256);
 }
 
@@ -572,7 +586,7 @@ int into_pieces(const void *from, long long ld, int batch, int rows, int columns
 {
     const T *g = (const T *)from;
     const bool vector = (uintptr_t)g % 16 == 0 && ld * sizeof(T) % 16 == 0;
-    const int parts = std::min(rows, kParts), m = h.m, n = h.n;
+    const int parts = std::min(rows, std::min(kParts, std::max(1, 2048 / batch))), m = h.m, n = h.n;   // eight workgroups a compute unit
     const bool whole = vector && columns * sizeof(T) % 16 == 0;
     const int pieces = (int)((columns * sizeof(T) + 15) / 16) + !vector;   // a row that starts inside one may reach into one more
     const auto norm = whole ? k_orth_norm<T, true> : k_orth_norm<T, false>;
