@@ -125,10 +125,13 @@ __global__ __launch_bounds__(256) void k_i8_dequantize(const unsigned char *code
 #pragma unroll
         for (int i = 0; i < EACH; ++i) v[i] = (T)((float)(signed char)(code[j] >> 8 * i) * scale[j]);
         T *out = y + ld * r + at;
-        if (VECTOR && at + EACH <= k) {
-            i32x4 b;
+        typedef T vec_t __attribute__((ext_vector_type(EACH)));
+        typedef vec_t any_t __attribute__((aligned(sizeof(T))));   // one store too, of any address
+        if (at + EACH <= k) {
+            vec_t b;
             __builtin_memcpy(&b, v, 16);
-            *(i32x4 *)out = b;
+            if (VECTOR) *(vec_t *)out = b;
+            else *(any_t *)out = b;
         } else {
 #pragma unroll
             for (int i = 0; i < EACH; ++i)

@@ -297,6 +297,10 @@ int launch(const Args &a, hipStream_t stream)
 //
 // Gradients with 128 x 128 against 256 x 256: 32764 slots of 32 experts, 1023 x 2049, dx 522 / 423, dw 628 / 540; 8000 of 16,
 // 2047 x 2047, dx 243 / 270, dw 377 / 287; 2000 of 16, 1023 x 1025, dx 45 / 72, dw 90 / 91.
+//
+// Figures of results whose rows do not lie in 16 bytes are of when they were stored one element at a time.  By 16 bytes at any
+// address those kernels gain alike: 32764 of 32, 1023 x 2049 dx 325, dw 409; 8192 of 8, 1024 -> 1023 48 to 32; 8-bit integers,
+// 28812 slots of 12, 673 -> 525 78 to 37, 32634 of 24, 1024 -> 549 93 to 46.
 template <typename T, int FORM, int MODE, int ACT, bool ALIGNED>
 int launch_size(const Args &a, hipStream_t stream)
 {

@@ -38,12 +38,15 @@ __device__ __forceinline__ void store_row(T *row, int c, int columns, bool wide,
     T h[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) h[i] = (T)v[i];
-    if (wide && c + N <= columns) {
+    typedef T vec_t __attribute__((ext_vector_type(8)));
+    typedef vec_t any_t __attribute__((aligned(sizeof(T))));   // one store too, of any address
+    if (c + N <= columns) {
 #pragma unroll
         for (int i = 0; i < N; i += 8) {
-            i32x4 b;
+            vec_t b;
             __builtin_memcpy(&b, h + i, 16);
-            *(i32x4 *)(row + c + i) = b;
+            if (wide) *(vec_t *)(row + c + i) = b;
+            else *(any_t *)(row + c + i) = b;
         }
     } else {
 #pragma unroll

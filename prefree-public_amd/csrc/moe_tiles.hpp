@@ -302,12 +302,15 @@ template <typename T, bool WHOLE, int N>
 __device__ __forceinline__ void store(char *row, int n, int have, const T (&v)[N])
 {
     T *out = (T *)row + n;
-    if constexpr (WHOLE) {
-        typedef T vec_t __attribute__((ext_vector_type(N)));
-        vec_t h;
+    typedef T vec_t __attribute__((ext_vector_type(N)));
+    typedef vec_t any_t __attribute__((aligned(sizeof(T))));   // one store too, of any address
+    vec_t h;
 #pragma unroll
-        for (int i = 0; i < N; ++i) h[i] = v[i];
+    for (int i = 0; i < N; ++i) h[i] = v[i];
+    if constexpr (WHOLE) {
         *(vec_t *)out = h;
+    } else if (n + N <= have) {
+        *(any_t *)out = h;
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
