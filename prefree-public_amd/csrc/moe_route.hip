@@ -97,7 +97,8 @@ __global__ __launch_bounds__(256) void k_route_super(const Route a)
 // Offsets and order from the counts: each workgroup sums all blocks' counts, and those before its own.  A thread sums
 // words of four experts' counts, as two pairs of 16 bits: of at most 1024 blocks with 64 tokens each, shared out over
 // the groups of threads (at least four), that is less than 2^16.  256 blocks, 128 experts: 5.4 us, 20 with a byte a load;
-// every workgroup reads all counts out of the L2, which saves a launch and a wait for one workgroup's sums.
+// every workgroup reads all counts out of the L2, which saves a launch and a wait for one workgroup's sums.  No more than 64
+// groups: each adds to its experts' sums in LDS, one after the other (466 blocks, 4 experts: 18 us with 1024 of them).
 __global__ __launch_bounds__(1024) void k_route_place(const Route a)
 {
     extern __shared__ unsigned long long lds[];
@@ -115,7 +116,7 @@ __global__ __launch_bounds__(1024) void k_route_place(const Route a)
         if (e >= 0) atomicOr(mask + e, 1ull << (i / a.top_k));
     }
     // integer sums, so the order in which they are added does not matter
-    const int words = counts_ld(a.experts) / 4, groups = blockDim.x / words, group = threadIdx.x / words, word = threadIdx.x % words;
+    const int words = counts_ld(a.experts) / 4, groups = min((int)blockDim.x / words, 64), group = threadIdx.x / words, word = threadIdx.x % words;
     const int supers = a.super ? a.blocks / kSuper : 0, own = block / kSuper;
     if (group < groups) {
         unsigned all[2] = {0, 0}, prior[2] = {0, 0};
