@@ -87,8 +87,9 @@ int pfk_moe_mm_i8(const pfk_moe_mm_args *a, void *stream);
  * pieces of X, 2 bytes and 1 an element, two squares of its shorter side, 2 bytes, and PFK_ORTH_PARTS sums of 8 bytes a matrix. */
 #define PFK_ORTH_PARTS 64
 #define PFK_ORTH_SIDE(n) (((n) + 31) / 32 * 32)
-/* Up to PFK_ORTH_NARROW rows (or columns) it holds instead, behind those sums: two pieces of X by columns of PFK_ORTH_NARROW,
- * 2 bytes an element, in shares of whole blocks of 32 columns, and twice a square of 4-byte numbers a share. */
+/* Up to PFK_ORTH_NARROW rows (or columns) it holds instead, behind those sums: two pieces of X by columns of at most
+ * PFK_ORTH_NARROW, 2 bytes an element, in shares of whole blocks of 32 columns, about as many as compute units over all matrices,
+ * and twice a square of 4-byte numbers a share. */
 #define PFK_ORTH_NARROW 64
 #define PFK_ORTH_MOST_SHARES(batch) ((batch) >= 256 ? 1 : (batch) <= 4 ? 64 : 256 / (batch))
 #define PFK_ORTH_SHARES(batch, n) (((n) + 255) / 256 < PFK_ORTH_MOST_SHARES(batch) ? ((n) + 255) / 256 : PFK_ORTH_MOST_SHARES(batch))

@@ -1,13 +1,14 @@
 // moe_orth_narrow.hip — orthogonal updates of matrices with at most 64 rows (or columns) on gfx950: one launch a step.
 //
-// X is held by columns, 64 numbers each, in two f16 pieces; a workgroup takes a share of them.  In a step every workgroup
+// X is held by columns, of up to 64 numbers, in two f16 pieces; a workgroup takes a share of them.  In a step every workgroup
 // adds the shares' parts of A = X X^T, forms B = a I + b A + c A A (64^3 products, by each of them: less than a launch),
 // X' = B X of its columns and its part of the next A.  The matrix cores hand out four rows of a column a lane, and eight of
 // two blocks, in whatever order, are a fragment of the product over columns: X' goes on to A as it comes.  A launch is
 // loads, meetings and a few hundred products one after the other, not their number: so A and B are in two pieces as well,
 // and of each product all but rest times rest is formed, for results as exact as their type.
-// 64 x 2048 from fp32 in five steps: 7 launches, 63 us (60 with one piece of A, B and the products' X, then 2 10^-3 off; now
-// 2 10^-4 in f16, which is its rounding); by tiles of 128 x 128, 17 launches, 152 us.
+// 64 x 2048 from fp32 in five steps: 7 launches, 65 us (60 with one piece of A, B and the products' X, then 2 10^-3 off; now
+// 2 10^-4 in f16, which is its rounding); by tiles of 128 x 128, 17 launches, 152 us.  128 x 37 x 3871: 226 us, a
+// share or two a matrix, columns of 40 numbers (734 with 16 shares each and columns of 64).
 #include "moe_orth.hpp"
 
 namespace {
@@ -21,17 +22,17 @@ constexpr int kWaves = 8;   // a wave for each 32 columns of a share of 256
 struct Step {
     const void *g;          // the first launch: X from the matrices
     long long ld_g;
-    int fours;              // rows of four elements at a time
     const double *sums;
     int parts;
     float scale;
     const float *gram;      // else: parts of A, [batch][shares][64][64]
     float over, a, b, c;    // A's factor, the step's triple
-    f16 *x, *rest;          // [batch][n][64]
+    f16 *x, *rest;          // [batch][n][side]
+    int side;               // the rows of X there are, rounded up to a piece of eight
     float *next;            // parts of the next A; the last launch has none
     void *out;              // the last launch: the result
     long long ld_out;
-    int out_f16, wide;      // wide: rows of the result take stores of 8 bytes
+    int out_f16;
     int rows, columns, across, m, n, shares, blocks;   // X is m x n; blocks: of 32 columns a share
 };
 
@@ -59,12 +60,13 @@ __device__ __forceinline__ float element(const Step &a, int matrix, int m, int n
     return (float)((const T *)a.g)[((long long)matrix * a.rows + (a.across ? n : m)) * a.ld_g + (a.across ? m : n)];
 }
 
-// four of a row of the matrices
+// four of a row of the matrices, that are all there, at any address
 template <typename T>
 __device__ __forceinline__ void four_elements(const Step &a, int matrix, int m, int n, float v[4])
 {
     typedef T four __attribute__((ext_vector_type(4)));
-    const four h = *(const four *)((const T *)a.g + ((long long)matrix * a.rows + min(m, a.m - 1)) * a.ld_g + min(n, a.n - 4));
+    typedef four any_t __attribute__((aligned(sizeof(T))));
+    const four h = *(const any_t *)((const T *)a.g + ((long long)matrix * a.rows + min(m, a.m - 1)) * a.ld_g + n);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = (float)h[e];
 }
@@ -78,9 +80,10 @@ __device__ __forceinline__ void store_result(const Step &a, int matrix, int m, i
             if (m < a.m && n + e < a.n) ((T *)a.out)[((long long)matrix * a.rows + n + e) * a.ld_out + m] = (T)v[e];
     } else if (m < a.m) {
         T *to = (T *)a.out + ((long long)matrix * a.rows + m) * a.ld_out + n;
-        if (a.wide && n + 4 <= a.n) {
+        if (n + 4 <= a.n) {
             typedef T four __attribute__((ext_vector_type(4)));
-            *(four *)to = four{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+            typedef four any_t __attribute__((aligned(sizeof(T))));
+            *(any_t *)to = four{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -102,7 +105,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, g = lane >> 4, i16 = lane & 15;
     const int matrix = blockIdx.y, share = blockIdx.x;
     const long long n_held = (long long)a.shares * a.blocks * 32;   // columns of X there is room for
-    f16 *x = a.x + matrix * n_held * kSide, *rest = a.rest + matrix * n_held * kSide;
+    f16 *x = a.x + matrix * n_held * a.side, *rest = a.rest + matrix * n_held * a.side;
 
     i32x4 h[2][2], l[2][2];   // 32 columns' pieces, as fragments
     const auto fetch = [&](int block) {
@@ -111,9 +114,12 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
         for (int half = 0; half < 2; ++half)
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                const long long at = (n0 + half * 16 + i16) * kSide + ks * 32 + g * 8;
-                h[half][ks] = *(const i32x4 *)(x + at);
-                l[half][ks] = *(const i32x4 *)(rest + at);
+                // rows behind the last are not held: some others are loaded, and zeros taken
+                const bool is = ks * 32 + g * 8 < a.side;
+                const long long at = (n0 + half * 16 + i16) * a.side + (is ? ks * 32 + g * 8 : 0);
+                const i32x4 first = *(const i32x4 *)(x + at), second = *(const i32x4 *)(rest + at);
+                h[half][ks] = is ? first : i32x4{0, 0, 0, 0};
+                l[half][ks] = is ? second : i32x4{0, 0, 0, 0};
             }
     };
     i32x4 poly[2][4][2];   // B's columns, as fragments
@@ -182,7 +188,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
         if (n0 >= a.n) break;
         float y[4][2][4];   // row 16 ib + i16; columns n0 + 16 half + 4 g to + 3
         if constexpr (FIRST) {
-            if (a.fours) {
+            if (!a.across && n0 + 32 <= a.n) {
 #pragma unroll
                 for (int ib = 0; ib < 4; ++ib)
 #pragma unroll
@@ -257,7 +263,8 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
                     }
                     transpose4(hi, lane);
                     transpose4(lo, lane);
-                    const long long at = (long long)(n0 + half * 16 + g * 4 + (lane & 3)) * kSide + ib * 16 + (lane & 12);
+                    const long long at = (long long)(n0 + half * 16 + g * 4 + (lane & 3)) * a.side + ib * 16 + (lane & 12);
+                    if (ib * 16 + (lane & 12) >= a.side) continue;
                     *(u32x2 *)(x + at) = u32x2{hi[0], hi[1]};
                     *(u32x2 *)(rest + at) = u32x2{lo[0], lo[1]};
                 }
@@ -307,15 +314,13 @@ int pfmoe::launch_narrow(const Narrow &g, hipStream_t s)
     a.n = a.across ? g.rows : g.columns;
     a.shares = PFK_ORTH_SHARES(g.batch, a.n);
     a.blocks = PFK_ORTH_BLOCKS(g.batch, a.n);
-    const long long held = (long long)g.batch * a.shares * a.blocks * 32 * kSide, gram = (long long)g.batch * a.shares * kSide * kSide;
+    a.side = (a.m + 7) / 8 * 8;
+    const long long held = (long long)g.batch * a.shares * a.blocks * 32 * a.side, gram = (long long)g.batch * a.shares * kSide * kSide;
     a.x = (f16 *)g.workspace;
     a.rest = a.x + held;
     float *parts[2] = {(float *)(a.rest + held), (float *)(a.rest + held) + gram};
     a.out_f16 = g.out_f16;
     a.ld_out = g.ld_out;
-    const size_t four = g.dtype == PF_F32 ? 16 : 8;
-    a.fours = !a.across && a.n % 4 == 0 && (uintptr_t)g.g % four == 0 && g.ld_g % 4 == 0;
-    a.wide = (uintptr_t)g.out % 8 == 0 && g.ld_out % 4 == 0;
     const dim3 grid(a.shares, g.batch), block(kWaves * kWave);
     a.next = parts[0];
     if (g.dtype == PF_F32) k_orth_narrow<true, false, float><<<grid, block, 0, s>>>(a);
