@@ -6,8 +6,8 @@
 // two blocks, in whatever order, are a fragment of the product over columns: X' goes on to A as it comes.  A launch is
 // loads, meetings and a few hundred products one after the other, not their number: so A and B are in two pieces as well,
 // and of each product all but rest times rest is formed, for results as exact as their type.
-// 64 x 2048 from fp32 in five steps: 7 launches, 65 us (60 with one piece of A, B and the products' X, then 2 10^-3 off; now
-// 2 10^-4 in f16, which is its rounding); by tiles of 128 x 128, 17 launches, 152 us.  128 x 37 x 3871: 226 us, a
+// 64 x 2048 from fp32 in five steps: 7 launches, 64 us (60 with one piece of A, B and the products' X, then 2 10^-3 off; now
+// 2 10^-4 in f16, which is its rounding); by tiles of 128 x 128, 17 launches, 152 us.  128 x 37 x 3871: 222 us, a
 // share or two a matrix, columns of 40 numbers (734 with 16 shares each and columns of 64).
 #include "moe_orth.hpp"
 
@@ -92,7 +92,9 @@ __device__ __forceinline__ void store_result(const Step &a, int matrix, int m, i
     }
 }
 
-template <bool FIRST, bool LAST, typename T>   // T: of the matrices, for the first launch
+// T: of the matrices, for the first launch.  SIDE: numbers a column, or 0 where the argument says so (of 64 by the argument, 64 x
+// 2048 takes 68 us and not 64; 33 x 4000 in columns of 64 takes 70 us, of 40 61).
+template <bool FIRST, bool LAST, typename T, int SIDE>
 __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
 {
     constexpr int LD = kSide + 8;
@@ -103,9 +105,9 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
         float parts[kWaves][kSide][kSide + 4];   // rows in other banks
     } lds;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, g = lane >> 4, i16 = lane & 15;
-    const int matrix = blockIdx.y, share = blockIdx.x;
+    const int matrix = blockIdx.y, share = blockIdx.x, side = SIDE ? SIDE : a.side;
     const long long n_held = (long long)a.shares * a.blocks * 32;   // columns of X there is room for
-    f16 *x = a.x + matrix * n_held * a.side, *rest = a.rest + matrix * n_held * a.side;
+    f16 *x = a.x + matrix * n_held * side, *rest = a.rest + matrix * n_held * side;
 
     i32x4 h[2][2], l[2][2];   // 32 columns' pieces, as fragments
     const auto fetch = [&](int block) {
@@ -114,12 +116,10 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
         for (int half = 0; half < 2; ++half)
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                // rows behind the last are not held: some others are loaded, and zeros taken
-                const bool is = ks * 32 + g * 8 < a.side;
-                const long long at = (n0 + half * 16 + i16) * a.side + (is ? ks * 32 + g * 8 : 0);
-                const i32x4 first = *(const i32x4 *)(x + at), second = *(const i32x4 *)(rest + at);
-                h[half][ks] = is ? first : i32x4{0, 0, 0, 0};
-                l[half][ks] = is ? second : i32x4{0, 0, 0, 0};
+                // rows behind the last are not held: the first ones are loaded, and multiplied by zeros
+                const long long at = (n0 + half * 16 + i16) * side + (ks * 32 + g * 8 < side ? ks * 32 + g * 8 : 0);
+                h[half][ks] = *(const i32x4 *)(x + at);
+                l[half][ks] = *(const i32x4 *)(rest + at);
             }
     };
     i32x4 poly[2][4][2];   // B's columns, as fragments
@@ -175,7 +175,10 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
 #pragma unroll
             for (int ib = 0; ib < 4; ++ib)
 #pragma unroll
-                for (int ks = 0; ks < 2; ++ks) poly[piece][ib][ks] = *(const i32x4 *)&lds.s.poly[piece][ib * 16 + i16][ks * 32 + g * 8];
+                for (int ks = 0; ks < 2; ++ks) {
+                    const i32x4 v = *(const i32x4 *)&lds.s.poly[piece][ib * 16 + i16][ks * 32 + g * 8];
+                    poly[piece][ib][ks] = ks * 32 + g * 8 < side ? v : i32x4{0, 0, 0, 0};
+                }
     }
 
     f32x4 gram[4][4];
@@ -263,8 +266,8 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
                     }
                     transpose4(hi, lane);
                     transpose4(lo, lane);
-                    const long long at = (long long)(n0 + half * 16 + g * 4 + (lane & 3)) * a.side + ib * 16 + (lane & 12);
-                    if (ib * 16 + (lane & 12) >= a.side) continue;
+                    const long long at = (long long)(n0 + half * 16 + g * 4 + (lane & 3)) * side + ib * 16 + (lane & 12);
+                    if (ib * 16 + (lane & 12) >= side) continue;
                     *(u32x2 *)(x + at) = u32x2{hi[0], hi[1]};
                     *(u32x2 *)(rest + at) = u32x2{lo[0], lo[1]};
                 }
@@ -296,6 +299,13 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
     }
 }
 
+template <bool FIRST, bool LAST, typename T>
+void run(const Step &a, dim3 grid, hipStream_t s)
+{
+    const auto kernel = a.side == kSide ? k_orth_narrow<FIRST, LAST, T, kSide> : k_orth_narrow<FIRST, LAST, T, 0>;
+    kernel<<<grid, dim3(kWaves * kWave), 0, s>>>(a);
+}
+
 }  // namespace
 
 int pfmoe::launch_narrow(const Narrow &g, hipStream_t s)
@@ -321,11 +331,11 @@ int pfmoe::launch_narrow(const Narrow &g, hipStream_t s)
     float *parts[2] = {(float *)(a.rest + held), (float *)(a.rest + held) + gram};
     a.out_f16 = g.out_f16;
     a.ld_out = g.ld_out;
-    const dim3 grid(a.shares, g.batch), block(kWaves * kWave);
+    const dim3 grid(a.shares, g.batch);
     a.next = parts[0];
-    if (g.dtype == PF_F32) k_orth_narrow<true, false, float><<<grid, block, 0, s>>>(a);
-    else if (g.dtype == PF_F16) k_orth_narrow<true, false, f16><<<grid, block, 0, s>>>(a);
-    else k_orth_narrow<true, false, bf16><<<grid, block, 0, s>>>(a);
+    if (g.dtype == PF_F32) run<true, false, float>(a, grid, s);
+    else if (g.dtype == PF_F16) run<true, false, f16>(a, grid, s);
+    else run<true, false, bf16>(a, grid, s);
     for (int i = 0; i < g.n_steps; ++i) {
         a.gram = parts[i & 1];
         a.next = parts[~i & 1];
@@ -333,8 +343,8 @@ int pfmoe::launch_narrow(const Narrow &g, hipStream_t s)
         a.b = g.steps[3 * i + 1];
         a.c = g.steps[3 * i + 2];
         a.out = g.out;
-        if (i == g.n_steps - 1) k_orth_narrow<false, true, void><<<grid, block, 0, s>>>(a);
-        else k_orth_narrow<false, false, void><<<grid, block, 0, s>>>(a);
+        if (i == g.n_steps - 1) run<false, true, void>(a, grid, s);
+        else run<false, false, void>(a, grid, s);
     }
     return pfk_internal_launched("k_orth_narrow");
 }
