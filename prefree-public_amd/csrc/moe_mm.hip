@@ -291,7 +291,9 @@ int launch(const Args &a, hipStream_t stream)
 // 8-bit integers, the rows' kernel, 128 x 128 tiles and k_mm_stream: 64 experts, 2048 -> 2 x 1024, rows 2: 42 / 57 / 61, 8: 56 /
 // 61 / 65, 12: 64 / 61 / 64, 25: - / 63 / 65, 64: - / 82 / 70; 128 experts, 1024 -> 2 x 512, 4: 33 / 37 / 38, 12: 44 / 39 / 39; 16
 // experts, 4096 -> 2048, 8: 35 / 43 / 51, 12: 41 / 42 / 51, 20: 53 / 42 / 51; 32 experts, 2047 -> 2 x 1023, 18: 43 / 34 / 37, 37: 69 /
-// 36 / 38; 2048 -> 2 x 2048, 128: - / 104 / 95.  Where even the 128 x 128 tiles are few the rows' kernel fills the card longer: 12
+// 36 / 38; 2048 -> 2 x 2048, 128: - / 104 / 95.  Columns that fill less of 256 x 256 tiles by a third or more: 16 experts, 3169 ->
+// 265, 2181: - / 89 / 92; 24, 4013 -> 287, 1460: - / 108 / 113; 96, 3728 -> 304, 350: - / 119 / 135; 12, 1189 -> 317, 3298: - / 46 / 49; 16,
+// 2048 -> 384, 2048: - / 50 / 53; but 2048 -> 768: - / 89 / 65, 1024 -> 640: - / 47 / 42.  Where even the 128 x 128 tiles are few the rows' kernel fills the card longer: 12
 // experts, 1111 -> 717, 16: 6 / 12 / 16, 52: 9 / 15 / 21, 100: 13 / 17 / 25; 8 experts, 1024 -> 1024, 32: 8 / 11 / 14, 64: 12 / 12
 // / 15, 96: 16 / 12 / 16; 4 experts, 2048 -> 2 x 512, 50: 9 / 17 / 22.
 //
@@ -315,7 +317,9 @@ int launch_size(const Args &a, hipStream_t stream)
         if (few) return launch_rows<T, FORM, ACT, ALIGNED>(a, stream);
     }
     if constexpr (ALIGNED) {
-        if (tiles(256) >= (MODE != kDw && rows >= 96 ? 128 : 256) && (FORM != kI8 || rows >= 48)) return launch_stream<T, FORM, MODE, ACT>(a, stream);
+        const long long columns = a.n * (ACT ? 2LL : 1LL);
+        const bool half = FORM == kI8 && (rows < 48 || 20 * ((columns + 255) / 256) >= 13 * ((columns + 127) / 128));   // half empty tiles
+        if (tiles(256) >= (MODE != kDw && rows >= 96 ? 128 : 256) && !half) return launch_stream<T, FORM, MODE, ACT>(a, stream);
     } else if constexpr (MODE == kFwd) {
         if (tiles(64) < 1300) return launch<T, FORM, MODE, ACT, 64, 64, 2, 2, ALIGNED>(a, stream);
     } else {
