@@ -84,7 +84,7 @@ int pfk_moe_mm_mx4(const pfk_moe_mm_args *a, void *stream);
 int pfk_moe_mm_i8(const pfk_moe_mm_args *a, void *stream);
 
 /* Rows or columns of a matrix in the workspace of pfk_orthogonalize, and that workspace's size: two times the
- * pieces of X, 2 bytes and 1 an element, two squares of its shorter side, 2 bytes, and PFK_ORTH_PARTS sums of 8 bytes a matrix. */
+ * two pieces of X, 2 bytes an element, two squares of its shorter side, 2 bytes, and PFK_ORTH_PARTS sums of 8 bytes a matrix. */
 #define PFK_ORTH_PARTS 64
 #define PFK_ORTH_SIDE(n) (((n) + 31) / 32 * 32)
 /* Up to PFK_ORTH_NARROW rows (or columns) it holds instead, behind those sums: two pieces of X by columns of at most

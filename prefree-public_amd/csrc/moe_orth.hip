@@ -1,12 +1,13 @@
 // moe_orth.hip — orthogonal updates on gfx950 (include/prefree_moe.h): X = G / |G|, then a few times
 // X <- a X + (b A + c A A) X with A = X X^T, in 16-bit products on the matrix cores.
 //
-// X is carried in two pieces, f16 and what that leaves in 8 bits (e5m2), of which the products take the first.  What a
-// rounding of X puts where G has nothing is multiplied by a in every step (3.4445^5 = 485), and so are G's small directions
-// with it: in one f16 piece the result of a momentum of rank n / 8 came out 1.5 to 4% off (in bf16 11 to 30%), in two
-// 0.15 to 0.25% (64 to 1024 rows; with 16 bits for the second 0.13 to 0.16).  With a X formed from both pieces the roundings
-// of the first reach X by way of A and of B X alone, and there they are small beside what X has in the same directions.
-// A and B = b A + c A A are one f16 piece.
+// X is carried in two f16 pieces, of which the products take the first.  What a rounding of X puts where G has nothing is
+// multiplied by a in every step (3.4445^5 = 485), and so are G's small directions with it: in one f16 piece the result of a
+// momentum of rank n / 8 came out 1.5 to 4% off (in bf16 11 to 30%), in two 0.14 to 0.17%.  With a second piece of 8 bits
+// (e5m2) those were 0.15 to 0.23%, but of rank 3 0.4 to 0.5%, and of rank 1 0.7%, for 0.15 to 0.21 and 0.2 to 0.28 so.  (Emulated
+// in 64 bits, 96 to 2048 rows.)  With a X formed from both pieces the roundings of the first reach X by way of A and of B X alone,
+// and there they are small beside what X has in the same directions.  A and B = b A + c A A are one f16 piece: where all
+// elements of a matrix are of one magnitude, their roundings are alike and add up, to 1% at the most of 1376 sizes.
 #include <algorithm>
 #include <utility>
 
@@ -25,9 +26,8 @@ struct Product {
     int whole, parts;           // tiles in one piece; quarters of the others
     float alpha, beta, gamma;
     const f16 *old;             // kPoly: A
-    const unsigned char *old_rest;
-    f16 *out;
-    unsigned char *rest;
+    const f16 *old_rest;
+    f16 *out, *rest;
     char *result;               // the last step's, instead of the pieces: [rows][columns], ld_result apart
     long long ld_result;
     int rows, columns, result_f16, wide;
@@ -39,9 +39,9 @@ struct Product {
 //         X is read across its rows.
 enum { kSquare = 0, kPoly = 1, kApply = 2 };
 
-// Four numbers as their first pieces, and what is left of them in 8 bits (e5m2) each.
+// Four numbers as their first pieces, and what is left of them.
 struct Pieces {
-    unsigned first[2], rest;
+    unsigned first[2], rest[2];
     __device__ __forceinline__ explicit Pieces(const float v[4])
     {
         float left[4];
@@ -49,17 +49,18 @@ struct Pieces {
         for (int i = 0; i < 4; ++i) left[i] = (v[i] - (float)(f16)v[i]) * kRest;
         first[0] = pair_of(v[0], v[1]);
         first[1] = pair_of(v[2], v[3]);
-        rest = __builtin_amdgcn_cvt_pk_bf8_f32(left[0], left[1], 0, false);
-        rest = __builtin_amdgcn_cvt_pk_bf8_f32(left[2], left[3], rest, true);
+        rest[0] = pair_of(left[0], left[1]);
+        rest[1] = pair_of(left[2], left[3]);
     }
 };
-__device__ __forceinline__ void rest_of(unsigned held, float v[4])
+__device__ __forceinline__ void rest_of(unsigned lo, unsigned hi, float v[4])
 {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_bf8(held, false), hi = __builtin_amdgcn_cvt_pk_f32_bf8(held, true);
-    v[0] = lo[0] * (1.0f / kRest);
-    v[1] = lo[1] * (1.0f / kRest);
-    v[2] = hi[0] * (1.0f / kRest);
-    v[3] = hi[1] * (1.0f / kRest);
+    typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 a = __builtin_bit_cast(f16x2, lo), b = __builtin_bit_cast(f16x2, hi);
+    v[0] = (float)a[0] * (1.0f / kRest);
+    v[1] = (float)a[1] * (1.0f / kRest);
+    v[2] = (float)b[0] * (1.0f / kRest);
+    v[3] = (float)b[1] * (1.0f / kRest);
 }
 
 // The tile from row m0 and column n0 of a matrix's product, by KS times WM x WN waves with STAGES times KS tiles of k in LDS.
@@ -76,17 +77,19 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
     int lane = threadIdx.x & (kWave - 1);
     const long long base = (long long)matrix * a.m * a.n;
 
-    // the second pieces of what this lane will store; they are long there when the products are
-    typedef unsigned Rest __attribute__((ext_vector_type(FN)));
-    Rest rest[KIND == kApply ? DONE : 1];
-    if constexpr (KIND == kApply) {   // none of the last step's: what they would add is not multiplied any more
-        const int c = n0 + wn * FN * 16 + (lane >> 4) * 4 * FN;   // 4 FN columns from here, there as a whole or not at all
+    // The second pieces of what this lane will store: half of them are long there when the products are, the others follow, each as
+    // the registers of one are free.  None of the last step's: what they would add is not multiplied any more.
+    typedef unsigned Rest __attribute__((ext_vector_type(2 * FN), aligned(16)));
+    constexpr int HELD = KIND == kApply ? DONE / 2 : 1;
+    Rest rest[HELD];
+    const auto read_rest = [&](int i) {
+        const int r = row_of(i) + (lane & 15), c = n0 + wn * FN * 16 + (lane >> 4) * 4 * FN;   // 4 FN columns from there, as a whole or not at all
+        rest[i % HELD] = Rest{};
+        if (a.old_rest && r < a.m && c < a.n) rest[i % HELD] = *(const Rest *)(a.old_rest + base + (long long)r * a.n + c);
+    };
+    if constexpr (KIND == kApply) {
 #pragma unroll
-        for (int i = 0; i < DONE; ++i) {
-            const int r = row_of(i) + (lane & 15);
-            rest[i] = Rest{};
-            if (a.old_rest && r < a.m && c < a.n) rest[i] = *(const Rest *)(a.old_rest + base + (long long)r * a.n + c);
-        }
+        for (int i = 0; i < HELD; ++i) read_rest(i);
     }
 
     P p;
@@ -216,10 +219,11 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
             float y[4 * FN];
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
-                rest_of(rest[i][j], y + 4 * j);
+                rest_of(rest[i % HELD][2 * j], rest[i % HELD][2 * j + 1], y + 4 * j);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[4 * j + e] = __builtin_fmaf(a.beta, y[4 * j + e], __uint_as_float(v[j][e]));
             }
+            if (i + HELD < DONE) read_rest(i + HELD);
             if (a.result) {
                 if (r >= a.rows) continue;
 #pragma unroll
@@ -234,8 +238,11 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
 #pragma unroll
             for (int j = 0; j < FN; j += 2) {
                 const Pieces one(y + 4 * j), two(y + 4 * j + 4);
-                left[j] = one.rest;
-                left[j + 1] = two.rest;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    left[2 * j + e] = one.rest[e];
+                    left[2 * j + 2 + e] = two.rest[e];
+                }
                 *(i32x4 *)(a.out + to + 4 * j) = i32x4{(int)one.first[0], (int)one.first[1], (int)two.first[0], (int)two.first[1]};
             }
             if (a.rest) *(Rest *)(a.rest + to) = left;
@@ -297,8 +304,9 @@ __device__ __forceinline__ void find_orth_tile(const Product &a, int at, int &ma
 
 // Tiles of 128 x 128.  Up to as many as compute units a workgroup each, with eight waves and seven tiles of k on their way;
 // else three a compute unit, of four waves and two tiles on their way, which are one round where two with three would take a
-// second one (12 x 717 x 1111, X': 31 us for 33).  Even and odd tiles of k by half of the waves each, or two more on their
-// way, changed nothing for the former: beside 10 us of tiles a launch of 18 us starts, and ends with its stores.
+// second one (12 x 717 x 1111, X': 34 us; with a second piece of X in 8 bits 31, for 33).  Even and odd tiles of k by half of the
+// waves each, or two more on their way, changed nothing for the former: beside 10 us of tiles a launch of 18 us starts, and ends with
+// its stores.
 template <int KIND, int WN, int STAGES>
 __global__ __launch_bounds__(128 * WN, WN == 2 ? 3 : 2) void k_orth_small(const Product a)
 {
@@ -324,8 +332,8 @@ __global__ __launch_bounds__(256) void k_orth_tiny(const Product a)
 }
 
 // Tiles of 256 x 256, a workgroup a compute unit, and in quarters those of a last round that is at most half full.  16 x 2048 x
-// 2048: A, B and X' 167, 168 and 271 us, X' at 1.01 PFLOP/s, the matrix cores busy half of the time.  The products alone are
-// 197 us of X'; the end of a tile, with nothing beside it, stores 200 MB in the rest.  256 x 128 tiles, two a compute unit: 350.
+// 2048: A, B and X' 173, 177 and 315 us, X' at 0.87 PFLOP/s.  The products alone are some 200 us of X'; the end of a tile, with nothing
+// beside it, reads 134 MB and stores 268 MB in the rest (with a second piece of X in 8 bits 287 us, two thirds of the bytes).
 template <int KIND>
 __global__ __launch_bounds__(512) void k_orth(const Product a)
 {
@@ -410,17 +418,17 @@ __global__ __launch_bounds__(kNormThreads) void k_orth_norm(const T *g, long lon
     sums[(long long)blockIdx.y * gridDim.x + blockIdx.x] = sum;
 }
 
-__device__ __forceinline__ void store_pieces(const float v[8], f16 *x, unsigned char *rest)
+__device__ __forceinline__ void store_pieces(const float v[8], f16 *x, f16 *rest)
 {
     const Pieces one(v), two(v + 4);
     *(i32x4 *)x = i32x4{(int)one.first[0], (int)one.first[1], (int)two.first[0], (int)two.first[1]};
-    *(u32x2 *)rest = u32x2{one.rest, two.rest};
+    *(i32x4 *)rest = i32x4{(int)one.rest[0], (int)one.rest[1], (int)two.rest[0], (int)two.rest[1]};
 }
 
 // The pieces of scale G / |G|, in [m][n] with zeros behind the matrix.
 template <typename T, bool VECTOR>
 __global__ __launch_bounds__(256) void k_orth_pieces(const T *g, long long ld, int rows, int columns, const double *sums, int parts, float scale, int m,
-                                                     int n, f16 *x, unsigned char *rest)
+                                                     int n, f16 *x, f16 *rest)
 {
     const double by = over_norm(sums + (long long)blockIdx.y * parts, parts, scale);
     const T *from = g + (long long)blockIdx.y * rows * ld;
@@ -448,7 +456,7 @@ __global__ __launch_bounds__(256) void k_orth_pieces(const T *g, long long ld, i
 // The same of its transpose, 64 x 64 elements a workgroup.
 template <typename T, bool VECTOR>
 __global__ __launch_bounds__(256) void k_orth_pieces_across(const T *g, long long ld, int rows, int columns, const double *sums, int parts, float scale,
-                                                            int m, int n, f16 *x, unsigned char *rest)
+                                                            int m, int n, f16 *x, f16 *rest)
 {
     __shared__ float tile[64][65];
     const double by = over_norm(sums + (long long)blockIdx.z * parts, parts, scale);
@@ -479,7 +487,7 @@ __global__ __launch_bounds__(256) void k_orth_pieces_across(const T *g, long lon
 
 // The transposed result out of the pieces.
 template <typename T>
-__global__ __launch_bounds__(256) void k_orth_out_across(const f16 *x, const unsigned char *rest, int m, int n, float scale, T *out, long long ld, int rows,
+__global__ __launch_bounds__(256) void k_orth_out_across(const f16 *x, const f16 *rest, int m, int n, float scale, T *out, long long ld, int rows,
                                                          int columns, int wide)
 {
     __shared__ float tile[64][65];
@@ -491,10 +499,10 @@ __global__ __launch_bounds__(256) void k_orth_out_across(const f16 *x, const uns
         if (r0 + i >= m || c0 + piece >= n) continue;
         const long long at = (long long)blockIdx.z * m * n + (long long)(r0 + i) * n + c0 + piece;
         const f16x8 first = *(const f16x8 *)(x + at);
-        const u32x2 left = *(const u32x2 *)(rest + at);
+        const i32x4 left = *(const i32x4 *)(rest + at);
         float v[8];
-        rest_of(left[0], v);
-        rest_of(left[1], v + 4);
+        rest_of(left[0], left[1], v);
+        rest_of(left[2], left[3], v + 4);
 #pragma unroll
         for (int e = 0; e < 8; ++e) tile[piece + e][i] = ((float)first[e] + v[e]) * scale;
     }
@@ -531,13 +539,15 @@ int product(Product a, hipStream_t s)
         });
         return pfk_internal_launched("k_orth");
     };
-    // X' of 129 to 192 rows, which larger tiles would leave empty by a quarter: 96 x 139 x 2765 72 / 87 (128 x 128) and 80 (256 x 256)
+    // X' of 129 to 192 rows, which larger tiles would leave empty by a quarter, in tiles of 64 x 128 / 128 x 128 / 256 x 256, whole calls
+    // in us: 96 x 139 x 2765 734 / 788 / 741, 96 x 160 x 2765 762 / 815 / 773, 64 x 190 x 4000 809 / 826 / 787, 40 x 139 x 1400 179 / 198 /
+    // 174, 32 x 139 x 2765 252 / 273 / 286, 128 x 150 x 1000 339 / 366 / 351, 16 x 170 x 4000 233 / 246 / 232
     if (KIND == kApply && 2 * tiles(64, 128) <= 3 * tiles(128) && tiles(64, 128) > kCus) {
         a.whole = (int)tiles(64, 128);
         if constexpr (KIND == kApply) return run(k_orth_tiny<KIND, 128, 4, 4, 1>, (a.whole + kXcds - 1LL) / kXcds * kXcds, 256);
     }
     // Tiles of 256 x 256 unless they cover over 1.4 times as much as those of 128 x 128: 128 x 289 x 1567, A and B 82, 33 / 64, 22, X'
-    // alike; 96 x 101 x 3705 X' 81 / 69; 128 x 221 x 3693 X' 199 / 216.
+    // 178 / 151; 96 x 101 x 3705 X' 83 / 73; 128 x 221 x 3693 X' 194 / 211.
     const long long large = tiles(256), small = tiles(128);
     if (large >= kCus && 20 * large <= 7 * small) {
         const long long over = large % kCus <= kCus / 2 ? large % kCus : 0;
@@ -545,7 +555,7 @@ int product(Product a, hipStream_t s)
         a.parts = (int)(4 * over);
         return run(k_orth<KIND>, (a.whole + kXcds - 1LL) / kXcds * kXcds + a.parts, 512);
     }
-    // A, B and X' in us, tiles of 64 rows against 128: 1 x 500 x 1000 8.9, 7.0, 8.9 / 12.4, 10.5, 10.3; 1 x 512 x 4096 19.7, 7.1, 9.5
+    // A, B and X' (with a second piece of 8 bits; up to 0.7 more so) in us, tiles of 64 rows against 128: 1 x 500 x 1000 8.9, 7.0, 8.9 / 12.4, 10.5, 10.3; 1 x 512 x 4096 19.7, 7.1, 9.5
     // / 30.8, 10.2, 10.6 (A by twos of tiles of k 24.5); 1 x 1024 x 1024 9.9, 10.1, 12.6 / 12.9, 14.7, 13.4; 12 x 300 x 300 6.1, 7.0,
     // 7.9 / -, -, 9.1; with more of them than fit at once: 3 x 800 x 800 10.6, 11.5, 13.8 / 12.6, 13.6, 12.7; 2 x 1100 x 1100 12.4,
     // 13.4, 18.9 / 15.6, 16.7, 16.8; 16 x 500 x 500 12.5, 13.8, 14.2 / 10.7, 11.8, 13.2; 1 x 2048 x 2048 32, 33, 32 / 22, 24, 26.
@@ -576,8 +586,7 @@ void each_tile(int batch, int m, int n, F launch)
 struct Held {
     int m, n;
     float scale;
-    f16 *x;
-    unsigned char *rest;
+    f16 *x, *rest;
 };
 
 // Squares' sums and, but for narrow matrices, the pieces; returns how many sums a matrix has.
@@ -627,9 +636,8 @@ extern "C" int pfk_orthogonalize(const void *g, long long ld_g, int dtype, int b
     const bool across = rows > columns;
     const int m = PFK_ORTH_SIDE(across ? columns : rows), n = PFK_ORTH_SIDE(across ? rows : columns);
     const long long xs = (long long)batch * m * n, as = (long long)batch * m * m;
-    f16 *x = (f16 *)workspace, *a = x + 2 * xs, *b = a + as;
-    unsigned char *rest = (unsigned char *)(b + as);
-    double *sums = (double *)(rest + 2 * xs);
+    f16 *x = (f16 *)workspace, *rest = x + 2 * xs, *a = rest + 2 * xs, *b = a + as;
+    double *sums = (double *)(b + as);
     float scale = 1;   // X is held times this: elements of about 1, and none over 2^12 where X has none over 4
     while (scale * scale * 4 <= n && scale < 1024) scale *= 2;
     const bool narrow = m <= PFK_ORTH_NARROW;

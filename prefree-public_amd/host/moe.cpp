@@ -417,7 +417,7 @@ size_t pf_orthogonalize_workspace(int batch, int rows, int columns)
         const size_t longer = std::max(rows, columns), shares = PFK_ORTH_SHARES(batch, longer), side = PFK_ORTH_NARROW;
         return batch * (shares * (4 * side * 32 * PFK_ORTH_BLOCKS(batch, longer) + 8 * side * side) + 8 * PFK_ORTH_PARTS);
     }
-    return batch * (m * (6 * n + 4 * m) + 8 * PFK_ORTH_PARTS);
+    return batch * (m * (8 * n + 4 * m) + 8 * PFK_ORTH_PARTS);
 }
 
 int pf_orthogonalize(const void *g, long long ld_g, int dtype, int batch, int rows, int columns, const float *steps, int n_steps, void *out,
