@@ -159,9 +159,10 @@ int pf_moe_mm_i8(const void *x_codes, const float *x_scales, int x_rows, const i
  * becomes a x + b x^3 + c x^5 in each step: with (3.4445, -4.7750, 2.0315) five times those from 0.01 of |g| on come out
  * between 0.7 and 1.2.  out [rows][columns] (f16, bf16).  Matrices follow each other, rows * ld elements apart.
  * Up to 64 rows (or columns) the result is as exact as its type.  Larger matrices: products of f16 values with sums in f32,
- * X held in two f16 pieces, of which the products take the first: within 2^-8 of the formula after up to eight such steps, in the
- * 2-norm over all elements, besides the result's rounding, in f16 too; within 2^-6 where the elements of a matrix are all of
- * one magnitude, and so round alike.  Steps have to keep singular values of 1 and less under 4.  A matrix of zeros gives
+ * X held in two f16 pieces, of which the products take the first: within 2^-8 of the formula, in the 2-norm over all elements,
+ * besides the result's rounding, in f16 too; within 2^-6 where the elements of a matrix are all of one magnitude, and so
+ * round alike.  That is after up to six such steps.  Each further one may multiply it by a: in all of them what rounding puts
+ * where a matrix has nothing grows as its own smallest singular values do.  Steps have to keep singular values of 1 and less under 4.  A matrix of zeros gives
  * zeros, one that holds an infinity or a NaN gives NaN; others of the batch are not touched by it.
  * rows, columns: 1 to 2^20, rows * columns at most 2^29; batch at most 1024; n_steps 1 to 64.
  * workspace: pf_orthogonalize_workspace() bytes, 16-byte aligned; what it holds before and after does not matter. */

@@ -16,7 +16,7 @@ import pytest
 import torch
 
 from moe_util import DEV, ROUND
-from test_gpu_orthogonalize import reference, run
+from test_gpu_orthogonalize import FIVE, reference, run
 
 pytestmark = pytest.mark.gpu
 
@@ -30,6 +30,8 @@ def matrices(kind, batch, rows, columns):
         return randn(batch, rows, 1).sign() * randn(batch, 1, columns).sign() * 0.37
     if kind == "rank 1 and noise":
         return few(1) + 1e-3 * randn(batch, rows, columns)
+    if kind == "all directions":
+        return randn(batch, rows, columns)
     return few({"rank 1": 1, "rank 3": 3, "rank n / 8": max(1, min(rows, columns) // 8)}[kind])
 
 
@@ -49,3 +51,13 @@ def test_few_directions(kind, batch, rows, columns):
 def test_few_directions_up_to_64_rows(kind, batch, rows, columns):
     got, held = run(matrices(kind, batch, rows, columns), "f32", "f16")
     assert off(got, reference(held)) <= 2.0 ** -11 + ROUND["f16"]
+
+
+@pytest.mark.parametrize("n_steps", [6, 7, 8, 10])
+@pytest.mark.parametrize("kind", ["rank 1", "rank n / 8", "one magnitude", "all directions"])
+@pytest.mark.parametrize("batch,rows,columns", [(2, 70, 105), (1, 192, 128), (1, 512, 512), (2, 40, 64), (1, 300, 64)])
+def test_more_steps(kind, batch, rows, columns, n_steps):
+    steps = FIVE[:1] * n_steps
+    got, held = run(matrices(kind, batch, rows, columns), "f32", "f16", steps=steps)
+    bound = 2.0 ** -11 if min(rows, columns) <= 64 else 2.0 ** -6 if kind == "one magnitude" else 2.0 ** -8
+    assert off(got, reference(held, steps)) <= bound * 3.5 ** (n_steps - 6) + ROUND["f16"]
