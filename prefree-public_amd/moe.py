@@ -291,9 +291,10 @@ def orthogonalize(g, batch, rows, columns, out, workspace, dtype="f32", out_dtyp
     d, out_d = dtype_code(dtype), dtype_code(out_dtype)
     if workspace_bytes is None:
         workspace_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    flat = [float(v) for step in steps for v in step]
-    if len(flat) != 3 * len(steps):
+    steps = [tuple(step) for step in steps]
+    if any(len(step) != 3 for step in steps):
         raise ValueError("steps are triples")
+    flat = [float(v) for step in steps for v in step]
     _check(lib().pf_orthogonalize(_buf(g, d, "g"), ld_g, d, int(batch), int(rows), int(columns),
                                   (ctypes.c_float * len(flat))(*flat), len(steps), _buf(out, out_d, "out"), ld_out, out_d,
                                   _buf_checked(workspace, None, "workspace"), int(workspace_bytes), _s(stream)),
