@@ -70,6 +70,8 @@ int pf_moe_route_backward(const void *logits, long long ld_logits, int dtype, in
  * A logit of -infinity and an r of -infinity are never chosen and count in no group.  A NaN counts as larger than any number.
  * r is compared as of 64 bits (and as its logit, where there is no bias and groups count one score: scores that 64 bits
  * do not tell apart are then in the order of their logits).  experts is a multiple of groups; groups: 1 to 16; scale: a positive number.
+ * To leave an expert out use a logit or a bias of -infinity: finite ones far from the others (-1e9, the type's lowest) give the same
+ * choice, but up to 3.5 times as late.
  * offsets, order, slot, workspace: as of pf_moe_route. */
 enum pf_score { PF_SCORE_SOFTMAX = 0, PF_SCORE_SIGMOID = 1 };
 #define PF_MOE_MAX_GROUPS 16
@@ -146,8 +148,8 @@ int pf_i8_quantize(const void *x, long long ld_x, int dtype, int rows, int k, vo
 /* Integer times scale, formed in f32 and rounded to dtype. */
 int pf_i8_dequantize(const void *codes, const float *scales, int rows, int k, int dtype, void *y, long long ld_y, void *stream);
 /* pf_moe_mm of such rows: x (x_codes, x_scales) [x_rows][k], w (w_codes, w_scales) [experts][n or 2n][k], a scale for each
- * token and each row of w; y in dtype (f16, bf16).  Sums are exact (k at most 131056); they are scaled, by the token's scale and then by the row's, and
- * the activation formed, in f32.  Codes behind a row's k elements are zeros, as pf_i8_quantize writes them; -128 is allowed. */
+ * token and each row of w; y in dtype (f16, bf16).  Sums are exact (k at most 131056); they are scaled, by the token's scale and
+ * then by the row's, and the activation formed, in f32.  Codes behind a row's k elements are zeros, as pf_i8_quantize writes them; -128 is allowed. */
 int pf_moe_mm_i8(const void *x_codes, const float *x_scales, int x_rows, const int *rows, int row_div, const void *w_codes,
                  const float *w_scales, const int *offsets, int experts, int slots, int n, int k, int dtype, int act, void *y,
                  long long ld_y, void *stream);
@@ -162,8 +164,9 @@ int pf_moe_mm_i8(const void *x_codes, const float *x_scales, int x_rows, const i
  * X held in two f16 pieces, of which the products take the first: within 2^-8 of the formula, in the 2-norm over all elements,
  * besides the result's rounding, in f16 too; within 2^-6 where the elements of a matrix are all of one magnitude, and so
  * round alike.  That is after up to six such steps.  Each further one may multiply it by a: in all of them what rounding puts
- * where a matrix has nothing grows as its own smallest singular values do.  Steps have to keep singular values of 1 and less under 4.  A matrix of zeros gives
- * zeros, one that holds an infinity or a NaN gives NaN; others of the batch are not touched by it.
+ * where a matrix has nothing grows as its own smallest singular values do.  Steps have to keep singular values of 1 and less
+ * under 4.  A matrix of zeros gives zeros, one that holds an infinity or a NaN gives NaN; others of the batch are not touched by it.
+ * f16 results of larger matrices are no closer than bf16 ones by more than their rounding.
  * rows, columns: 1 to 2^20, rows * columns at most 2^29; batch at most 1024; n_steps 1 to 64.
  * workspace: pf_orthogonalize_workspace() bytes, 16-byte aligned; what it holds before and after does not matter. */
 size_t pf_orthogonalize_workspace(int batch, int rows, int columns);

@@ -171,8 +171,9 @@ int dequantize(const void *codes, const float *scales, int rows, int k, void *y,
     const long long ld_codes = PF_I8_ROW(k);
     in_launches(rows, most_workgroups(256) * 1024 / per_row, [&](long long first, long long count) {
         const long long units = count * per_row;
-        kernel<<<dim3((unsigned)((units + 1023) / 1024)), dim3(256), 0, s>>>((const unsigned char *)codes + ld_codes * first, ld_codes, scales + first,
-                                                                             units, per_row, k, (T *)y + ld * first, ld);
+        const dim3 grid((unsigned)((units + 1023) / 1024));
+        kernel<<<grid, dim3(256), 0, s>>>((const unsigned char *)codes + ld_codes * first, ld_codes, scales + first, units, per_row, k,
+                                          (T *)y + ld * first, ld);
     });
     return pfk_internal_launched("k_i8_dequantize");
 }

@@ -293,9 +293,10 @@ int launch(const Args &a, hipStream_t stream)
 // experts, 4096 -> 2048, 8: 35 / 43 / 51, 12: 41 / 42 / 51, 20: 53 / 42 / 51; 32 experts, 2047 -> 2 x 1023, 18: 43 / 34 / 37, 37: 69 /
 // 36 / 38; 2048 -> 2 x 2048, 128: - / 104 / 95.  Columns that fill less of 256 x 256 tiles by a third or more: 16 experts, 3169 ->
 // 265, 2181: - / 89 / 92; 24, 4013 -> 287, 1460: - / 108 / 113; 96, 3728 -> 304, 350: - / 119 / 135; 12, 1189 -> 317, 3298: - / 46 / 49; 16,
-// 2048 -> 384, 2048: - / 50 / 53; but 2048 -> 768: - / 89 / 65, 1024 -> 640: - / 47 / 42.  Where even the 128 x 128 tiles are few the rows' kernel fills the card longer: 12
-// experts, 1111 -> 717, 16: 6 / 12 / 16, 52: 9 / 15 / 21, 100: 13 / 17 / 25; 8 experts, 1024 -> 1024, 32: 8 / 11 / 14, 64: 12 / 12
-// / 15, 96: 16 / 12 / 16; 4 experts, 2048 -> 2 x 512, 50: 9 / 17 / 22.
+// 2048 -> 384, 2048: - / 50 / 53; but 2048 -> 768: - / 89 / 65, 1024 -> 640: - / 47 / 42.  Where
+// even the 128 x 128 tiles are few the rows' kernel fills the card longer: 12 experts, 1111 -> 717, 16: 6 / 12 / 16, 52: 9 / 15 / 21,
+// 100: 13 / 17 / 25; 8 experts, 1024 -> 1024, 32: 8 / 11 / 14, 64: 12 / 12 / 15, 96: 16 / 12 / 16; 4 experts, 2048 -> 2 x 512, 50:
+// 9 / 17 / 22.  So it ends somewhere between 50 and 100 rows, by the number of tiles: with 60 for all, up to 4 us are lost above.
 //
 // Gradients with 128 x 128 against 256 x 256: 32764 slots of 32 experts, 1023 x 2049, dx 522 / 423, dw 628 / 540; 8000 of 16,
 // 2047 x 2047, dx 243 / 270, dw 377 / 287; 2000 of 16, 1023 x 1025, dx 45 / 72, dw 90 / 91.

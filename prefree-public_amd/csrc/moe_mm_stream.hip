@@ -382,7 +382,8 @@ __global__ __launch_bounds__(kThreads) void k_mm_stream(const Args a)
             // 8-bit integers: there long before the sums are
             typename std::conditional<FORM == kI8, Units<ACT, decltype(blocks)::value, FN, WM>, NoUnits>::type units;
             if constexpr (FORM == kI8)
-                units.load(a, a.q_unit + (ACT ? 2LL : 1LL) * a.n * now.e, wm, wn, now.n * OUT_N, have, [&](int r) { return row_of(now, side ^ 1, r); });
+                units.load(a, a.q_unit + (ACT ? 2LL : 1LL) * a.n * now.e, wm, wn, now.n * OUT_N, have,
+                           [&](int r) { return row_of(now, side ^ 1, r); });
             bool fresh = i > 0;
 #pragma unroll 1
             for (int s = 0; s < steps; ++s) {

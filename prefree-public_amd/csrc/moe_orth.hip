@@ -83,7 +83,7 @@ __device__ __forceinline__ void orth_tile(const Product &a, int matrix, int m0, 
     constexpr int HELD = KIND == kApply ? DONE / 2 : 1;
     Rest rest[HELD];
     const auto read_rest = [&](int i) {
-        const int r = row_of(i) + (lane & 15), c = n0 + wn * FN * 16 + (lane >> 4) * 4 * FN;   // 4 FN columns from there, as a whole or not at all
+        const int r = row_of(i) + (lane & 15), c = n0 + wn * FN * 16 + (lane >> 4) * 4 * FN;   // 4 FN columns, all there or none
         rest[i % HELD] = Rest{};
         if (a.old_rest && r < a.m && c < a.n) rest[i % HELD] = *(const Rest *)(a.old_rest + base + (long long)r * a.n + c);
     };
@@ -555,8 +555,8 @@ int product(Product a, hipStream_t s)
         a.parts = (int)(4 * over);
         return run(k_orth<KIND>, (a.whole + kXcds - 1LL) / kXcds * kXcds + a.parts, 512);
     }
-    // A, B and X' (with a second piece of 8 bits; up to 0.7 more so) in us, tiles of 64 rows against 128: 1 x 500 x 1000 8.9, 7.0, 8.9 / 12.4, 10.5, 10.3; 1 x 512 x 4096 19.7, 7.1, 9.5
-    // / 30.8, 10.2, 10.6 (A by twos of tiles of k 24.5); 1 x 1024 x 1024 9.9, 10.1, 12.6 / 12.9, 14.7, 13.4; 12 x 300 x 300 6.1, 7.0,
+    // A, B and X' (with a second piece of 8 bits; up to 0.7 more so) in us, tiles of 64 rows against 128: 1 x 500 x 1000 8.9, 7.0, 8.9
+    // / 12.4, 10.5, 10.3; 1 x 512 x 4096 19.7, 7.1, 9.5 / 30.8, 10.2, 10.6 (A by twos of tiles of k 24.5); 1 x 1024 x 1024 9.9, 10.1, 12.6 / 12.9, 14.7, 13.4; 12 x 300 x 300 6.1, 7.0,
     // 7.9 / -, -, 9.1; with more of them than fit at once: 3 x 800 x 800 10.6, 11.5, 13.8 / 12.6, 13.6, 12.7; 2 x 1100 x 1100 12.4,
     // 13.4, 18.9 / 15.6, 16.7, 16.8; 16 x 500 x 500 12.5, 13.8, 14.2 / 10.7, 11.8, 13.2; 1 x 2048 x 2048 32, 33, 32 / 22, 24, 26.
     if constexpr (KIND == kApply) {
@@ -623,14 +623,15 @@ void out_across(const Held &h, int batch, void *out, long long ld, int rows, int
 {
     each_tile(batch, h.m, h.n, [&](dim3 grid, long long at) {
         const long long from = at * h.m * h.n;
-        k_orth_out_across<T><<<grid, dim3(256), 0, s>>>(h.x + from, h.rest + from, h.m, h.n, 1 / h.scale, (T *)out + at * rows * ld, ld, rows, columns, wide);
+        k_orth_out_across<T><<<grid, dim3(256), 0, s>>>(h.x + from, h.rest + from, h.m, h.n, 1 / h.scale, (T *)out + at * rows * ld, ld, rows,
+                                                        columns, wide);
     });
 }
 
 }  // namespace
 
-extern "C" int pfk_orthogonalize(const void *g, long long ld_g, int dtype, int batch, int rows, int columns, const float *steps, int n_steps, void *out,
-                                 long long ld_out, int out_dtype, void *workspace, void *stream)
+extern "C" int pfk_orthogonalize(const void *g, long long ld_g, int dtype, int batch, int rows, int columns, const float *steps,
+                                 int n_steps, void *out, long long ld_out, int out_dtype, void *workspace, void *stream)
 {
     hipStream_t s = (hipStream_t)stream;
     const bool across = rows > columns;

@@ -72,7 +72,7 @@ __device__ __forceinline__ void four_elements(const Step &a, int matrix, int m, 
 }
 
 template <typename T>
-__device__ __forceinline__ void store_result(const Step &a, int matrix, int m, int n, const float v[4], int lane)
+__device__ __forceinline__ void store_result(const Step &a, int matrix, int m, int n, const float v[4])
 {
     if (a.across) {   // v: four rows of the result, column m
 #pragma unroll
@@ -244,8 +244,8 @@ __global__ __launch_bounds__(kWaves * kWave) void k_orth_narrow(const Step a)
                     float v[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] = y[ib][half][e] * (1 / a.scale);
-                    if (a.out_f16) store_result<f16>(a, matrix, ib * 16 + i16, n0 + half * 16 + g * 4, v, lane);
-                    else store_result<bf16>(a, matrix, ib * 16 + i16, n0 + half * 16 + g * 4, v, lane);
+                    if (a.out_f16) store_result<f16>(a, matrix, ib * 16 + i16, n0 + half * 16 + g * 4, v);
+                    else store_result<bf16>(a, matrix, ib * 16 + i16, n0 + half * 16 + g * 4, v);
                 }
         } else {
             i32x4 frag[2][4];

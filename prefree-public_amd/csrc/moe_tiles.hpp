@@ -459,7 +459,8 @@ struct NoUnits { };
 // Stores a wave's results: FMV of its FM blocks of 16 rows (every WM-th of the tile's, of which `have` rows exist),
 // FN blocks of 16 columns.  first: the tile's first row of the output, n0 its first column.
 template <typename T, int MODE, int ACT, bool WHOLE, int FMV, int FM, int FN, int WM, typename SUM, typename U>
-__device__ __forceinline__ void store_blocks(const Args &a, const SUM (&sums)[FM][FN], int wm, int wn, long long first, int have, int n0, const U &units)
+__device__ __forceinline__ void store_blocks(const Args &a, const SUM (&sums)[FM][FN], int wm, int wn, long long first, int have, int n0,
+                                             const U &units)
 {
     int lane = threadIdx.x & (kWave - 1);
     asm volatile("" : "+v"(lane));   // addresses are formed here, not kept over the loop before
@@ -510,7 +511,8 @@ __device__ __forceinline__ void store_blocks(const Args &a, const SUM (&sums)[FM
 }
 
 template <typename T, int MODE, int ACT, int FMV, int FM, int FN, int WM, int OUT_N, typename SUM, typename U>
-__device__ __forceinline__ void store_results(const Args &a, const SUM (&acc)[FM][FN], int wm, int wn, long long first, int have, int n0, const U &units)
+__device__ __forceinline__ void store_results(const Args &a, const SUM (&acc)[FM][FN], int wm, int wn, long long first, int have, int n0,
+                                              const U &units)
 {
     if (a.wide && n0 + OUT_N <= a.n) store_blocks<T, MODE, ACT, true, FMV, FM, FN, WM>(a, acc, wm, wn, first, have, n0, units);
     else store_blocks<T, MODE, ACT, false, FMV, FM, FN, WM>(a, acc, wm, wn, first, have, n0, units);

@@ -414,7 +414,8 @@ size_t pf_orthogonalize_workspace(int batch, int rows, int columns)
     if (batch < 1 || rows < 1 || columns < 1) return 0;
     const size_t m = PFK_ORTH_SIDE((size_t)std::min(rows, columns)), n = PFK_ORTH_SIDE((size_t)std::max(rows, columns));
     if (m <= PFK_ORTH_NARROW) {
-        const size_t longer = std::max(rows, columns), shares = PFK_ORTH_SHARES(batch, longer), side = PFK_ORTH_NARROW;
+        const long long longer = std::max(rows, columns);
+        const size_t shares = PFK_ORTH_SHARES(batch, longer), side = PFK_ORTH_NARROW;
         return batch * (shares * (4 * side * 32 * PFK_ORTH_BLOCKS(batch, longer) + 8 * side * side) + 8 * PFK_ORTH_PARTS);
     }
     return batch * (m * (8 * n + 4 * m) + 8 * PFK_ORTH_PARTS);
