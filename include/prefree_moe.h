@@ -166,7 +166,7 @@ int pf_moe_mm_i8(const void *x_codes, const float *x_scales, int x_rows, const i
  * round alike.  That is after up to six such steps.  Each further one may multiply it by a: in all of them what rounding puts
  * where a matrix has nothing grows as its own smallest singular values do.  Steps have to keep singular values of 1 and less
  * under 4.  A matrix of zeros gives zeros, one that holds an infinity or a NaN gives NaN; others of the batch are not touched by it.
- * f16 results of larger matrices are no closer than bf16 ones by more than their rounding.
+ * Of larger matrices f16 results are rounded more finely than bf16 ones, and are no closer to the formula otherwise.
  * rows, columns: 1 to 2^20, rows * columns at most 2^29; batch at most 1024; n_steps 1 to 64.
  * workspace: pf_orthogonalize_workspace() bytes, 16-byte aligned; what it holds before and after does not matter. */
 size_t pf_orthogonalize_workspace(int batch, int rows, int columns);

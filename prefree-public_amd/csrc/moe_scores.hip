@@ -303,7 +303,8 @@ struct Fast {
             shift = low;
             scale = by_logit ? (range > 0 ? kUnits / range : 0.0f) : kUnits / (1.0f + range);
             odd |= !(scale < INFINITY);
-            // around a level this far, sums of 64 bits may be equal where units are not: 4 levels 2^-52 reach 2 margins of 24 units
+            // around a far level sums of 64 bits may be equal where scores are not: two groups' sums are off by up to 4 levels 2^-52,
+            // which stays under the 2 margins of 24 units that tell them apart
             if (!by_logit) odd |= fmaxf(fabsf(low), fabsf(high)) > 0x1p30f * (1.0f + range);
         } else {
             scale = kUnits;
